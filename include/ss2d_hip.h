@@ -658,6 +658,113 @@ int64_t ss2d_product_f32_workspace_bytes(int64_t M, int N, int64_t K, int a_by_c
 int ss2d_product_f32(const float *a, const float *b, const float *bias, const float *other, float *out, float *out2, int64_t M, int N, int64_t K,
                      int a_by_columns, int b_by_columns, int mode, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * Linear attention with a decay for each head, of sequences (batch, token, head, dim): with a state S of key_dim x value_dim values per head,
+ *   S_t = exp(decay_t) S_(t-1) + k_t v_t^T,   out_t = scale q_t^T S_t,   S_0 = initial_state or 0.
+ * The selective scan with one decay for the whole of a matrix state, chunked (classification/models/mamba2/ssd_minimal.py:144).
+ *   q (batch, seqlen, q_heads, key_dim), k (.., k_heads, key_dim), v (.., v_heads, value_dim): dtype, the last dimension dense, other strides in
+ *   elements; head h of `heads` reads head h / (heads / q_heads) of q, and so on: each divides `heads`.
+ *   decay (batch, seqlen, heads) by its strides, (heads) with strides 0 for batch and token, or NULL (no decay): the LOGARITHM of the
+ *   factor, SS2D_F32 or dtype (decay_dtype); -infinity forgets all that came before.
+ *   cu_seqlens NULL, or n_seqs + 1 ascending places (device memory): sequence i is tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of batch 1.  Places
+ *   outside 0 .. seqlen are moved into it, a descending one is taken as the one before it; rows of no sequence get zeros.
+ *   initial_state, final_state (n_seqs or batch, heads, key_dim, value_dim) fp32, dense, either or both NULL; of a sequence without
+ *   tokens the final state is the initial one.  out (batch, seqlen, heads, value_dim) dtype, dense.
+ * Dimensions up to 256 (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a
+ * negative status), 16-byte aligned.
+ */
+typedef struct ss2d_linear_attention_params {
+    int32_t batch, seqlen, heads, q_heads, k_heads, v_heads, key_dim, value_dim;
+    int32_t dtype, decay_dtype, n_seqs;
+    float scale;
+    const void *q, *k, *v, *decay;
+    const int32_t *cu_seqlens;
+    const float *initial_state;
+    void *out;
+    float *final_state;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    int64_t decay_batch_stride, decay_token_stride, decay_head_stride;
+} ss2d_linear_attention_params;
+
+int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params *params);
+int ss2d_linear_attention_fwd(const ss2d_linear_attention_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, from the inputs again (fwd.out and fwd.final_state are not looked at): dout (batch, seqlen, heads, value_dim) dtype by its strides,
+ * dfinal_state as final_state or NULL.  dq, dk, dv: dtype, dense, in the shapes of q, k and v; heads that share are summed in fp32.
+ * ddecay: decay_dtype, dense, (batch, seqlen, heads), with decay_per_head (heads); or NULL.  dinitial_state fp32 or NULL.
+ * No atomics: the same bits every time.  Rows of no sequence get zeros.
+ */
+typedef struct ss2d_linear_attention_bwd_params {
+    ss2d_linear_attention_params fwd;
+    const void *dout;
+    const float *dfinal_state;
+    void *dq, *dk, *dv, *ddecay;
+    float *dinitial_state;
+    int64_t dout_batch_stride, dout_token_stride, dout_head_stride;
+    int32_t decay_per_head, reserved;
+} ss2d_linear_attention_bwd_params;
+
+int64_t ss2d_linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params *params);
+int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * One token for each of `batch` sequences: state = exp(decay) state + k v^T in place, out = scale q^T state (the recurrence itself,
+ * classification/models/mamba2/ssd_minimal.py:144 with one position).  q (batch, q_heads, key_dim), k, v: dtype, the last dimension dense; decay
+ * (batch, heads) by its strides (0 for one that the batch shares) or NULL; state (batch, heads, key_dim, value_dim) fp32, dense but
+ * for the batch's stride, which keeps the states apart; out (batch, heads, value_dim) dtype, dense.
+ */
+typedef struct ss2d_linear_attention_step_params {
+    int32_t batch, heads, q_heads, k_heads, v_heads, key_dim, value_dim;
+    int32_t dtype, decay_dtype;
+    float scale;
+    const void *q, *k, *v, *decay;
+    float *state;
+    void *out;
+    int64_t q_batch_stride, q_head_stride, k_batch_stride, k_head_stride, v_batch_stride, v_head_stride;
+    int64_t decay_batch_stride, decay_head_stride, state_batch_stride;
+} ss2d_linear_attention_step_params;
+
+int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *params, void *stream);
+
+/*
+ * Norm of each head of queries and keys, and their rotation by position, in one pass:
+ *   n = x / sqrt(mean(x^2) + eps) * weight;  of the first 2 * axes * per_axis values, pair i = (axis, f) is turned by position[axis] * frequency[axis][f]:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), the pair being values (i, i + axes * per_axis), with `interleaved` (2 i, 2 i + 1).
+ * q (batch, seqlen, q_heads, dim), k (.., k_heads, dim): dtype, the last dimension dense, either with 0 heads; q_out, k_out dense; weights (dim) of
+ * weight_dtype (SS2D_F32 or dtype) or NULL (1); positions int32 or int64 (batch, seqlen, axes) by strides, or NULL (no rotation); frequencies
+ * (axes, per_axis) float or double, dense.  Angles are 64-bit products.  The LayerNorm of a row without centring
+ * (classification/models/vmamba.py:52-57 is the framework's norm of a map's channels).  dim up to 512 (SS2D_ENOTSUP beyond).
+ */
+typedef struct ss2d_qk_norm_rotate_params {
+    int32_t batch, seqlen, q_heads, k_heads, dim;
+    int32_t dtype, weight_dtype, axes, per_axis, interleaved, positions_int64, frequencies_float64;
+    float eps;
+    int32_t reserved;
+    const void *q, *k, *q_weight, *k_weight, *positions, *frequencies;
+    void *q_out, *k_out;
+    int64_t q_batch_stride, q_token_stride, q_head_stride, k_batch_stride, k_token_stride, k_head_stride;
+    int64_t position_batch_stride, position_token_stride, position_axis_stride;
+} ss2d_qk_norm_rotate_params;
+
+int ss2d_qk_norm_rotate(const ss2d_qk_norm_rotate_params *params, void *stream);
+
+/*
+ * Its gradients, from the inputs again (fwd.q_out and fwd.k_out are not looked at): dq_out, dk_out by strides -> dq, dk dense; dq_weight, dk_weight
+ * weight_dtype, either or both NULL.  workspace (for the weights'): ..._workspace_bytes(dim) bytes, 16-byte aligned.  No atomics.
+ */
+typedef struct ss2d_qk_norm_rotate_bwd_params {
+    ss2d_qk_norm_rotate_params fwd;
+    const void *dq_out, *dk_out;
+    void *dq, *dk, *dq_weight, *dk_weight;
+    int64_t dq_batch_stride, dq_token_stride, dq_head_stride, dk_batch_stride, dk_token_stride, dk_head_stride;
+} ss2d_qk_norm_rotate_bwd_params;
+
+int64_t ss2d_qk_norm_rotate_bwd_workspace_bytes(int dim);
+int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,7 +27,9 @@ EXPORTS = ("ss2d_abi_version", "ss2d_strerror", "ss2d_cross_scan", "ss2d_cross_m
            "ss2d_dwconv3x3_silu_f32", "ss2d_dwconv3x3_silu_bwd", "ss2d_dwconv3x3_silu_bwd_workspace_bytes", "ss2d_cross_scan_1b1", "ss2d_core_fwd",
            "ss2d_core_workspace_bytes", "ss2d_core_fwd_ws", "ss2d_forward_core", "ss2d_forward_core_workspace_bytes", "ss2d_block_fwd", "ss2d_block_workspace_bytes", "ss2d_few_rows_bytes", "ss2d_few_applies", "ss2d_x_proj_few", "ss2d_core_few", "ss2d_core_mask_pads", "ss2d_core_embed_maps",
            "ss2d_x_proj", "ss2d_x_proj_applies", "ss2d_x_proj_f32", "ss2d_dt_proj", "ss2d_dt_proj_f32", "ss2d_dt_proj_masked", "ss2d_cross_scan_flex", "ss2d_cross_scan_flex_ws", "ss2d_cross_scan_flex_static", "ss2d_cross_merge_flex",
-           "ss2d_selective_scan_bwd", "ss2d_selective_scan_bwd_kernel", "ss2d_clear", "ss2d_round_pair", "ss2d_transpose_bcl", "ss2d_mlp_fused", "ss2d_linear_cl", "ss2d_linear_rows", "ss2d_linear_tiles", "ss2d_conv3x3s2_cl", "ss2d_linear_dw_f32", "ss2d_layer_norm_bwd_f32", "ss2d_layer_norm_bwd_f32_workspace_bytes", "ss2d_column_sums_f32", "ss2d_column_sums_f32_workspace_bytes", "ss2d_product_f32", "ss2d_product_f32_workspace_bytes", "ss2d_linear_dw_f32_workspace_bytes", "ss2d_linear_cf_ln", "ss2d_stem_conv_ln_gelu", "ss2d_stem_conv2_ln", "ss2d_mean_pool_cl")
+           "ss2d_selective_scan_bwd", "ss2d_selective_scan_bwd_kernel", "ss2d_clear", "ss2d_round_pair", "ss2d_transpose_bcl", "ss2d_mlp_fused", "ss2d_linear_cl", "ss2d_linear_rows", "ss2d_linear_tiles", "ss2d_conv3x3s2_cl", "ss2d_linear_dw_f32", "ss2d_layer_norm_bwd_f32", "ss2d_layer_norm_bwd_f32_workspace_bytes", "ss2d_column_sums_f32", "ss2d_column_sums_f32_workspace_bytes", "ss2d_product_f32", "ss2d_product_f32_workspace_bytes", "ss2d_linear_dw_f32_workspace_bytes", "ss2d_linear_cf_ln", "ss2d_stem_conv_ln_gelu", "ss2d_stem_conv2_ln", "ss2d_mean_pool_cl",
+           "ss2d_linear_attention_workspace_bytes", "ss2d_linear_attention_fwd", "ss2d_linear_attention_bwd_workspace_bytes", "ss2d_linear_attention_bwd",
+           "ss2d_linear_attention_step", "ss2d_qk_norm_rotate", "ss2d_qk_norm_rotate_bwd_workspace_bytes", "ss2d_qk_norm_rotate_bwd")
 
 
 class ScanParams(ctypes.Structure):
@@ -88,6 +90,54 @@ class BlockParams(ctypes.Structure):
         + [(n, ctypes.c_void_p) for n in ("x", "residual", "norm_weight", "norm_bias", "in_proj_weight", "in_proj_bias", "conv_weight", "conv_bias",
                                           "out_proj_weight", "out_proj_bias", "norm2_weight", "norm2_bias", "fc1_weight", "fc1_bias",
                                           "fc2_weight", "fc2_bias", "out")]
+    )
+
+
+class LinearAttentionParams(ctypes.Structure):
+    """struct ss2d_linear_attention_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "seqlen", "heads", "q_heads", "k_heads", "v_heads", "key_dim", "value_dim", "dtype", "decay_dtype", "n_seqs")]
+        + [("scale", ctypes.c_float)]
+        + [(n, ctypes.c_void_p) for n in ("q", "k", "v", "decay", "cu_seqlens", "initial_state", "out", "final_state")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("q", "k", "v", "decay") for axis in ("batch", "token", "head")]
+    )
+
+
+class LinearAttentionBwdParams(ctypes.Structure):
+    """struct ss2d_linear_attention_bwd_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [("fwd", LinearAttentionParams)] + [(n, ctypes.c_void_p) for n in ("dout", "dfinal_state", "dq", "dk", "dv", "ddecay", "dinitial_state")]
+        + [(f"dout_{axis}_stride", ctypes.c_int64) for axis in ("batch", "token", "head")]
+        + [(n, ctypes.c_int32) for n in ("decay_per_head", "reserved")]
+    )
+
+
+class LinearAttentionStepParams(ctypes.Structure):
+    """struct ss2d_linear_attention_step_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "heads", "q_heads", "k_heads", "v_heads", "key_dim", "value_dim", "dtype", "decay_dtype")]
+        + [("scale", ctypes.c_float)] + [(n, ctypes.c_void_p) for n in ("q", "k", "v", "decay", "state", "out")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("q", "k", "v", "decay") for axis in ("batch", "head")] + [("state_batch_stride", ctypes.c_int64)]
+    )
+
+
+class QkNormRotateParams(ctypes.Structure):
+    """struct ss2d_qk_norm_rotate_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "seqlen", "q_heads", "k_heads", "dim", "dtype", "weight_dtype", "axes", "per_axis", "interleaved",
+                                       "positions_int64", "frequencies_float64")]
+        + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+        + [(n, ctypes.c_void_p) for n in ("q", "k", "q_weight", "k_weight", "positions", "frequencies", "q_out", "k_out")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("q", "k") for axis in ("batch", "token", "head")]
+        + [(f"position_{axis}_stride", ctypes.c_int64) for axis in ("batch", "token", "axis")]
+    )
+
+
+class QkNormRotateBwdParams(ctypes.Structure):
+    """struct ss2d_qk_norm_rotate_bwd_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [("fwd", QkNormRotateParams)] + [(n, ctypes.c_void_p) for n in ("dq_out", "dk_out", "dq", "dk", "dq_weight", "dk_weight")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("dq", "dk") for axis in ("batch", "token", "head")]
     )
 
 
@@ -251,6 +301,16 @@ def lib():
                                         [ctypes.c_int] * 5 + [ctypes.c_void_p])
         L.ss2d_mean_pool_cl.restype = ctypes.c_int
         L.ss2d_mean_pool_cl.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+        for name, params in (("ss2d_linear_attention", LinearAttentionParams), ("ss2d_linear_attention_bwd", LinearAttentionBwdParams)):
+            getattr(L, name + "_workspace_bytes").restype, getattr(L, name + "_workspace_bytes").argtypes = ctypes.c_int64, [ctypes.POINTER(params)]
+        for name, params in (("ss2d_linear_attention_fwd", LinearAttentionParams), ("ss2d_linear_attention_bwd", LinearAttentionBwdParams),
+                             ("ss2d_qk_norm_rotate_bwd", QkNormRotateBwdParams)):
+            getattr(L, name).restype = ctypes.c_int
+            getattr(L, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+        for name, params in (("ss2d_linear_attention_step", LinearAttentionStepParams), ("ss2d_qk_norm_rotate", QkNormRotateParams)):
+            getattr(L, name).restype, getattr(L, name).argtypes = ctypes.c_int, [ctypes.POINTER(params), ctypes.c_void_p]
+        L.ss2d_qk_norm_rotate_bwd_workspace_bytes.restype = ctypes.c_int64
+        L.ss2d_qk_norm_rotate_bwd_workspace_bytes.argtypes = [ctypes.c_int]
         if L.ss2d_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.ss2d_abi_version()} != expected {ABI_VERSION}; rebuild")
         _lib = L

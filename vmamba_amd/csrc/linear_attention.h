@@ -1,0 +1,183 @@
+// Linear attention with a decay for each head, what its kernels share: per head a state S of Dk x Dv values,
+//     S_t = exp(g_t) S_(t-1) + k_t v_t^T,   o_t = scale q_t^T S_t
+// -- the selective scan with a matrix for a state and one decay for all of it, which makes its products matrix products.  A sequence
+// is cut into chunks of C tokens.  With G_t the sum of the chunk's g up to and with t, and S the state before the chunk,
+//     o_t = scale sum_(s <= t) exp(G_t - G_s) (q_t . k_s) v_s + scale exp(G_t) q_t^T S,
+//     S after = exp(G_C) S + sum_s exp(G_C - G_s) k_s v_s^T,
+// so only the states are walked from chunk to chunk (linear_attention.hip); outputs (same file) and gradients (linear_attention_bwd.hip) of all
+// chunks are independent of one another.  Everything that is a sum of g stands as a pair of floats from a sum in 64 bits and
+// goes through exp as a difference first: a decay of -inf (a reset) or a long sum loses nothing.
+//
+// Operands.  bf16 goes to the 16-bit matrix cores as it is; what is computed on the way (weights of pairs, states) is rounded to bf16
+// where it becomes an operand of a product that is itself rounded to bf16 at its end, and split into two bf16 values where its
+// result is kept in 32 bits (states, single precision decays' gradients).  fp16 and fp32 go to the fp32 matrix cores: the states' and
+// weights' range is not fp16's.
+#pragma once
+#include <float.h>
+
+#include "ss2d_common.h"
+
+namespace ss2d {
+
+constexpr int kLaMaxDim = 256;       // of a key or value
+constexpr int kLaTile = 64;          // sides of the piece of a state that a workgroup walks
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct LaSide {                      // q, k, v, out or a gradient: (batch, token, head, dim), the last one dense
+    void *p;
+    int64_t batch, token, head;      // strides in elements
+    int32_t div;                     // heads of the state to one of this
+    int32_t dim;
+    int32_t aligned;                 // base and strides are multiples of 16 bytes
+};
+
+struct LaArgs {
+    LaSide q, k, v, out, dout, dq, dk, dv;
+    const void *decay;               // (batch, token, head) or (head) or NULL
+    void *ddecay;
+    int64_t decay_batch, decay_token, decay_head;
+    int32_t decay_dtype, ddecay_f32;
+    const int32_t *cu;               // packed sequences: n_seqs + 1 places, or NULL
+    int32_t batch, tokens, heads, n_seqs;
+    int32_t per_seq;                 // chunks of a sequence that is not packed
+    int32_t max_chunks, seg_chunks, max_segs, segs_per_seq;
+    float scale;
+    const float *initial, *dfinal;   // (n_seqs, heads, Dk, Dv), dense
+    float *final, *dinitial;
+    // workspace
+    int4 *chunks;                    // {batch, first token, tokens, sequence}; no tokens: unused; sequence -1: rows of no sequence
+    int4 *seqs;                      // packed: {start, end, first chunk, first segment}, and {rows before, rows' end, chunks, segments} behind them
+    float2 *cum;                     // [chunk][head][C]: G in log2 units, high and low part
+    void *states, *dstates, *dstates_t;
+    int64_t low;                     // elements from a state's bf16 value to what the rounding left, 0: not kept
+    float *local;                    // [segment][head][tile][4096] and behind it [segment][head] decays
+};
+
+// ---- operands of the matrix cores --------------------------------------------------------------------------------------------
+// rows(): the lane's part of 16 rows of a tile that is dense along the sum (k); cols(): of 16 columns of a tile that is dense across it.
+// A lane holds the same k for A and B, so the order inside a step is free.
+struct OperandF32 {
+    using E = float;
+    using Frag = floatx4_t;
+    static constexpr int kStep = 16, kChunk = 32, kPad = 4;
+    static __device__ __forceinline__ Frag rows(const E *tile, int pitch, int row0, int k0, int lane) {
+        return *reinterpret_cast<const Frag *>(tile + (row0 + (lane & 15)) * pitch + k0 + 4 * (lane >> 4));
+    }
+    static __device__ __forceinline__ Frag cols(const E *tile, int pitch, int col0, int k0, int lane) {
+        const E *p = tile + (k0 + 4 * (lane >> 4)) * pitch + col0 + (lane & 15);
+        return Frag{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
+    }
+    static __device__ __forceinline__ floatx4_t mma(Frag a, Frag b, floatx4_t c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ void put4(E *p, floatx4_t v) { *reinterpret_cast<floatx4_t *>(p) = v; }
+};
+
+struct OperandBf16 {
+    using E = bf16_t;
+    using Frag = u32x4_t;
+    static constexpr int kStep = 32, kChunk = 64, kPad = 8;
+    static __device__ __forceinline__ Frag rows(const E *tile, int pitch, int row0, int k0, int lane) {
+        return *reinterpret_cast<const Frag *>(tile + (row0 + (lane & 15)) * pitch + k0 + 8 * (lane >> 4));
+    }
+    // ds_read_b64_tr_b16: of the four rows that a group of 16 lanes names, 8 bytes to a lane, a lane gets its column
+    static __device__ __forceinline__ Frag cols(const E *tile, int pitch, int col0, int k0, int lane) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        using Lds = __attribute__((address_space(3))) s16x4;
+        const E *p = tile + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * pitch + col0 + 4 * (lane & 3);
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)p));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(p + 4 * pitch)));
+        return Frag{lo[0], lo[1], hi[0], hi[1]};
+    }
+    static __device__ __forceinline__ floatx4_t mma(Frag a, Frag b, floatx4_t c) { return mfma_16x16x32(bf16_t{}, a, b, c); }
+    static __device__ __forceinline__ void put4(E *p, floatx4_t v) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_from_f32<bf16_t>(v[0], v[1]), pack2_from_f32<bf16_t>(v[2], v[3]));
+    }
+};
+
+// ---- tiles ------------------------------------------------------------------------------------------------------------------------
+template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
+
+// 16 bytes' worth of a row from column c on: in one load where they are aligned and inside the row, else element by element
+template <typename T> __device__ __forceinline__ u32x4_t load_piece(const T *row, int c, int cols, bool aligned) {
+    if (aligned && c + kVecOf<T> <= cols) return *reinterpret_cast<const u32x4_t *>(row + c);
+    union { T e[kVecOf<T>]; u32x4_t w; } u;
+    u.w = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kVecOf<T>; ++i)
+        if (c + i < cols) u.e[i] = row[c + i];
+    return u.w;
+}
+
+template <typename T> __device__ __forceinline__ float piece_at(u32x4_t w, int i) {
+    if constexpr (sizeof(T) == 4) return bits_to_f32(w[i]);
+    else return i % 2 ? unpack_hi<T>(w[i / 2]) : unpack_lo<T>(w[i / 2]);
+}
+
+// Whether one of the piece's values is infinite or NaN
+template <typename T> __device__ __forceinline__ bool piece_bad(u32x4_t w) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
+        else {
+            constexpr uint32_t m = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+            bad |= (w[i] & m) == m || (w[i] & (m << 16)) == (m << 16);
+        }
+    }
+    return bad;
+}
+
+template <typename T, typename E> __device__ __forceinline__ void put_piece(E *lds, u32x4_t w) {
+    if constexpr (sizeof(T) == sizeof(E)) *reinterpret_cast<u32x4_t *>(lds) = w;
+    else {
+#pragma unroll
+        for (int i = 0; i < kVecOf<T>; i += 4)
+            *reinterpret_cast<floatx4_t *>(lds + i) = floatx4_t{piece_at<T>(w, i), piece_at<T>(w, i + 1), piece_at<T>(w, i + 2), piece_at<T>(w, i + 3)};
+    }
+}
+
+// Four neighbouring results of one token to memory, `left` of them inside the row
+template <typename T> __device__ __forceinline__ void store4(T *p, floatx4_t v, int left, bool aligned) {
+    if (aligned && left >= 4) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<floatx4_t *>(p) = v;
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_from_f32<T>(v[0], v[1]), pack2_from_f32<T>(v[2], v[3]));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < left) p[i] = from_f32<T>(v[i]);
+}
+
+inline __host__ __device__ int la_up(int n, int m) { return (n + m - 1) / m * m; }
+// Rows of a state stand at a pitch that every operand's step divides, with zeros behind them
+inline __host__ __device__ int la_state_dim(int d) { return la_up(d, 32); }
+
+__device__ __forceinline__ float load_decay(const void *p, int64_t at, int dtype) {
+    return dtype == SS2D_F32 ? reinterpret_cast<const float *>(p)[at] : dtype == SS2D_BF16 ? to_f32(reinterpret_cast<const bf16_t *>(p)[at])
+                                                                                          : to_f32(reinterpret_cast<const f16_t *>(p)[at]);
+}
+
+// A sequence's {start, end, first chunk, first segment}, whichever way the sequences stand
+__device__ __forceinline__ int4 la_sequence(const LaArgs &p, int n) {
+    return p.cu ? p.seqs[n] : make_int4(0, p.tokens, n * p.per_seq, n * p.segs_per_seq);
+}
+
+// The walks over the states that linear_attention.hip offers to both directions: a and b are (k, v), (v, k), (do, q)
+struct LaWalk {
+    LaSide a, b;                     // M = sum of w a b^T, stored as rows of b's dimension, dense in a's
+    void *out, *out_t;               // [chunk][head][Db][Da] and, where wanted, [chunk][head][Da][Db]
+    int64_t low;                     // as LaArgs::low, of out
+    const float *from;               // the state to begin with, element (ia, ib) at ia * from_a + ib * from_b; NULL: zero
+    float *to;                       // the state to end with, or NULL
+    int32_t from_a, from_b;
+    int32_t reverse;                 // from the last chunk to the first, weights scale exp(G_t) instead of exp(G_C - G_s)
+};
+int la_plan(LaArgs &p, int chunk);                                                     // sizes of the tables and segments
+int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
+template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream);
+
+}  // namespace ss2d

@@ -1,0 +1,460 @@
+// Gradients of linear attention with a decay for each head.  With E the gradient of the state behind a chunk, S the state before it,
+// P_ts = scale exp(G_t - G_s) q_t . k_s and D_ts = scale exp(G_t - G_s) do_t . v_s for s <= t, 0 behind:
+//     dq_t = sum_s D_ts k_s + scale exp(G_t) S do_t,     dk_s = sum_t D_ts q_t + exp(G_C - G_s) E v_s,
+//     dv_s = sum_t P_ts do_t + exp(G_C - G_s) E^T k_s,   E before = exp(G_C) E + sum_t scale exp(G_t) q_t do_t^T.
+// A decay g_t stands in every pair of a key before t and a query from t on, wherever the two are:
+//     dg_t = sum_(s < t <= t') P_t's do_t' . v_s + sum_(t' >= t) scale exp(G_t') q_t' . (S do_t') + sum_(s < t) exp(G_C - G_s) k_s . (E v_s) + exp(G_C) <S, E>
+// -- sums over the chunk alone.  (The shorter form, the sum of q . dq - k . dk from t to the sequence's end, is a small difference of
+// long sums.)  S and E of all chunks come from two walks, and every chunk is then on its own.
+#include "linear_attention.h"
+
+namespace ss2d {
+
+// Sums over the lanes that hold the same column (four groups of 16), and over 16 columns
+__device__ __forceinline__ float sum_groups(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
+__device__ __forceinline__ float sum_columns(float v) {
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+
+__device__ __forceinline__ float dot_frags(floatx4_t a, floatx4_t b) { return fmaf(a[0], b[0], a[1] * b[1]) + fmaf(a[2], b[2], a[3] * b[3]); }
+__device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fmaf(unpack_lo<bf16_t>(a[i]), unpack_lo<bf16_t>(b[i]), fmaf(unpack_hi<bf16_t>(a[i]), unpack_hi<bf16_t>(b[i]), sum));
+    return sum;
+}
+
+// A workgroup owns a chunk of one head: weights of its pairs to LDS, then 16 columns of dq and dk, and of dv, to a wavefront at a time, as the
+// outputs' kernel does (transposed products, states straight from memory).  kLow: dq's and dk's share of the states with
+// what their rounding to bf16 left, for a decay's gradient in single precision.
+template <typename Op, typename T, bool kLow>
+__global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
+    using E = typename Op::E;
+    using Frag = typename Op::Frag;
+    constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad;
+    extern __shared__ __align__(16) char lds[];
+    const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), pitch_k = dk + Op::kPad, pitch_v = dv + Op::kPad;
+    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * pitch_k, *vt = kt + kC * pitch_k, *ot = vt + kC * pitch_v;
+    E *pt = ot + kC * pitch_v, *dt = pt + kC * kPitchP;              // P and D, as rows of a key's token
+    float2 *cum = reinterpret_cast<float2 *>(dt + kC * kPitchP);
+    float *of_queries = reinterpret_cast<float *>(cum + kC), *of_keys = of_queries + kM * kC;        // sums of the pairs' products, [16 keys / queries][token]
+    float *with_s = of_keys + kM * kC, *with_e = with_s + 4 * kC, *both = with_e + 4 * kC;           // [wavefront][token], [wavefront]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
+    const uint32_t id = xcd_contiguous_id(blockIdx.x, total);
+    const int c = id / (uint32_t)p.heads, h = id - (uint32_t)c * (uint32_t)p.heads;
+    const int4 e = p.chunks[c];
+    const int64_t entry = (int64_t)c * p.heads + h;
+    if (e.z <= 0 || e.w < 0) {
+        if (head_sums && tid == 0) head_sums[entry] = 0.0f;
+        if (e.z <= 0) return;
+    }
+    const int64_t row0 = (int64_t)e.x * p.tokens + e.y;
+    auto put = [&](const LaSide &side, int t, int d, floatx4_t v) {  // four values of a gradient, in single precision where heads are still to be summed
+        const int64_t at = e.x * side.batch + (int64_t)(e.y + t) * side.token + (int64_t)h * side.head + d;
+        if (side.div > 1) store4(reinterpret_cast<float *>(side.p) + at, v, side.dim - d, side.aligned);
+        else store4(reinterpret_cast<T *>(side.p) + at, v, side.dim - d, side.aligned);
+    };
+    auto put_decay = [&](int t, float v) {
+        const int64_t at = (row0 + t) * p.heads + h;
+        if (p.ddecay_f32) reinterpret_cast<float *>(p.ddecay)[at] = v;
+        else reinterpret_cast<T *>(p.ddecay)[at] = from_f32<T>(v);
+    };
+    if (e.w < 0) {                                                   // rows of no sequence
+        const floatx4_t none = {0, 0, 0, 0};
+        for (int i = tid; i < e.z * (kLaMaxDim / 4); i += kBlock) {
+            const int t = i / (kLaMaxDim / 4), d = i % (kLaMaxDim / 4) * 4;
+            if (d < p.k.dim) { put(p.dq, t, d, none); put(p.dk, t, d, none); }
+            if (d < p.v.dim) put(p.dv, t, d, none);
+        }
+        if (p.ddecay && !head_sums && tid < e.z) put_decay(tid, 0.0f);
+        return;
+    }
+    auto load = [&](const LaSide &side, E *tile, int pitch, const FastDiv &per_row) {
+        const T *src = reinterpret_cast<const T *>(side.p) + e.x * side.batch + (int64_t)e.y * side.token + (int64_t)(h / side.div) * side.head;
+        bool bad = false;
+        for (uint32_t i = tid; i < kC * per_row.d; i += 4 * kBlock) {
+            u32x4_t piece[4];
+            uint32_t row[4], at[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                divmod(i + j * kBlock, per_row, row[j], at[j]);
+                piece[j] = u32x4_t{0, 0, 0, 0};
+                if ((int)row[j] < e.z) piece[j] = load_piece(src + (int64_t)row[j] * side.token, at[j] * kVec, side.dim, side.aligned);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (row[j] < kC) {
+                    put_piece<T, E>(tile + row[j] * pitch + at[j] * kVec, piece[j]);
+                    bad |= piece_bad<T>(piece[j]);
+                }
+        }
+        return bad;
+    };
+    if (tid < kC) cum[tid] = p.cum[entry * kC + tid];
+    bool bad = load(p.q, qt, pitch_k, per_key);
+    bad |= load(p.k, kt, pitch_k, per_key);
+    bad |= load(p.dout, ot, pitch_v, per_value);
+    load(p.v, vt, pitch_v, per_value);
+    bad = __syncthreads_or(bad);
+
+#pragma unroll
+    for (int i = 0; i < kM * kM / 4; ++i) {
+        const int tt = wave % kM, ts = wave / kM + i * (4 / kM);
+        floatx4_t weights = {0, 0, 0, 0}, through = {0, 0, 0, 0}, product = {0, 0, 0, 0};
+        const int t = 16 * tt + quad, s = 16 * ts + col;
+        if (ts <= tt) {
+            for (int k0 = 0; k0 < dk; k0 += Op::kStep)
+                weights = Op::mma(Op::rows(qt, pitch_k, 16 * tt, k0, lane), Op::rows(kt, pitch_k, 16 * ts, k0, lane), weights);
+            for (int k0 = 0; k0 < dv; k0 += Op::kStep)
+                through = Op::mma(Op::rows(ot, pitch_v, 16 * tt, k0, lane), Op::rows(vt, pitch_v, 16 * ts, k0, lane), through);
+            const float2 gs = cum[s];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float2 gt = cum[t + v];
+                const float decay = exp2f((gt.x - gs.x) + (gt.y - gs.y)) * p.scale;
+                weights[v] = s <= t + v ? weights[v] * decay : 0.0f;
+                product[v] = s < t + v ? weights[v] * through[v] : 0.0f;         // (a pair of one token has no decay between)
+                through[v] = s <= t + v ? through[v] * decay : 0.0f;
+            }
+        }
+        Op::put4(pt + s * kPitchP + t, weights);
+        Op::put4(dt + s * kPitchP + t, through);
+        // of these 16 x 16 pairs: sums for each query and each key; on the diagonal, for each token the pairs that it stands between
+        const float of_key = sum_groups((product[0] + product[1]) + (product[2] + product[3]));
+        if (lane < 16) of_keys[tt * kC + s] = ts < tt ? of_key : 0.0f;
+        if (ts == tt) {
+            product[2] += product[3];                                // from a query on
+            product[1] += product[2];
+            product[0] += product[1];
+            const float next = __shfl_down(product[0], 16), third = __shfl_down(product[0], 32), fourth = __shfl_down(product[0], 48);
+            const float behind = (lane < 48 ? next : 0.0f) + (lane < 32 ? third : 0.0f) + (lane < 16 ? fourth : 0.0f);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) product[v] = col < quad + v ? product[v] + behind : 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const float of_query = sum_columns(product[v]);
+            if (col == 0) of_queries[ts * kC + t + v] = of_query;
+        }
+    }
+    __syncthreads();
+
+    const int4 seq = la_sequence(p, e.w);
+    const bool has_s = e.y != seq.x || p.initial, has_e = e.y + e.z < seq.y || p.dfinal;
+    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim);
+    const E *states = reinterpret_cast<const E *>(p.states) + entry * sk * sv, *dstates = reinterpret_cast<const E *>(p.dstates) + entry * sk * sv;
+    const E *dstates_t = reinterpret_cast<const E *>(p.dstates_t) + entry * sk * sv;
+    const float2 end = cum[kC - 1];
+    float q_dot[kM], k_dot[kM], se = 0.0f, in[kM], out[kM];          // of a token: the decay from what came in, to what goes out
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+        const float2 g = cum[16 * m + col];
+        q_dot[m] = k_dot[m] = 0.0f;
+        in[m] = p.scale * exp2f(g.x + g.y);
+        out[m] = exp2f((end.x - g.x) + (end.y - g.y));
+    }
+    for (int n = wave; 16 * n < p.k.dim; n += 4) {
+        floatx4_t dq[kM], dkey[kM];
+#pragma unroll
+        for (int m = 0; m < kM; ++m) dq[m] = dkey[m] = floatx4_t{0, 0, 0, 0};
+        for (int k0 = 0; k0 < dv && (has_s || has_e); k0 += Op::kStep) {
+            Frag s, d, sl, dl;
+            if (has_s) s = Op::rows(states, sv, 16 * n, k0, lane);
+            if (has_e) d = Op::rows(dstates, sv, 16 * n, k0, lane);
+            if constexpr (kLow) {
+                if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
+                if (has_e) dl = Op::rows(dstates + p.low, sv, 16 * n, k0, lane);
+            }
+            if (has_s)
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    const Frag o = Op::rows(ot, pitch_v, 16 * m, k0, lane);
+                    dq[m] = Op::mma(s, o, dq[m]);
+                    if constexpr (kLow) dq[m] = Op::mma(sl, o, dq[m]);
+                }
+            if (has_e)
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    const Frag v = Op::rows(vt, pitch_v, 16 * m, k0, lane);
+                    dkey[m] = Op::mma(d, v, dkey[m]);
+                    if constexpr (kLow) dkey[m] = Op::mma(dl, v, dkey[m]);
+                }
+            if (has_s && has_e) {
+                se += dot_frags(s, d);
+                if constexpr (kLow) se += dot_frags(s, dl) + dot_frags(sl, d);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+            const E *q = qt + (16 * m + col) * pitch_k + 16 * n + quad, *k = kt + (16 * m + col) * pitch_k + 16 * n + quad;
+            dq[m] *= in[m];
+            dkey[m] *= out[m];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                q_dot[m] = fmaf(dq[m][v], to_f32(q[v]), q_dot[m]);
+                k_dot[m] = fmaf(dkey[m][v], to_f32(k[v]), k_dot[m]);
+            }
+        }
+        if (!bad) {
+#pragma unroll
+            for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
+                const Frag k = Op::cols(kt, pitch_k, 16 * n, k0, lane), q = Op::cols(qt, pitch_k, 16 * n, k0, lane);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    if (16 * m >= k0) dq[m] = Op::mma(k, Op::cols(dt, kPitchP, 16 * m, k0, lane), dq[m]);
+                    if (16 * m < k0 + Op::kStep) dkey[m] = Op::mma(q, Op::rows(dt, kPitchP, 16 * m, k0, lane), dkey[m]);
+                }
+            }
+        } else {                                                     // as in the outputs' kernel: nothing from behind the diagonal
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                const int own = 16 * m + col;
+                for (int r = 0; r < kC; ++r)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + 16 * n + quad + v]);
+                        if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + 16 * n + quad + v]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+            if (16 * m + col < e.z) {
+                put(p.dq, 16 * m + col, 16 * n + quad, dq[m]);
+                put(p.dk, 16 * m + col, 16 * n + quad, dkey[m]);
+            }
+    }
+    for (int n = wave; 16 * n < p.v.dim; n += 4) {
+        floatx4_t acc[kM];
+#pragma unroll
+        for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
+        if (has_e) {
+            for (int k0 = 0; k0 < dk; k0 += Op::kStep) {
+                const Frag a = Op::rows(dstates_t, sk, 16 * n, k0, lane);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::rows(kt, pitch_k, 16 * m, k0, lane), acc[m]);
+            }
+#pragma unroll
+            for (int m = 0; m < kM; ++m) acc[m] *= out[m];
+        }
+        if (!bad) {
+#pragma unroll
+            for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
+                const Frag o = Op::cols(ot, pitch_v, 16 * n, k0, lane);
+#pragma unroll
+                for (int m = 0; m < kM; ++m)
+                    if (16 * m < k0 + Op::kStep) acc[m] = Op::mma(o, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+                for (int r = 16 * m + col; r < kC; ++r)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + col) * kPitchP + r]) * to_f32(ot[r * pitch_v + 16 * n + quad + v]);
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+            if (16 * m + col < e.z) put(p.dv, 16 * m + col, 16 * n + quad, acc[m]);
+    }
+    if (!p.ddecay) return;
+
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+        const float a = sum_groups(q_dot[m]), b = sum_groups(k_dot[m]);
+        if (lane < 16) {
+            with_s[wave * kC + 16 * m + col] = a;
+            with_e[wave * kC + 16 * m + col] = b;
+        }
+    }
+    se = sum_groups(sum_columns(se));
+    if (lane == 0) both[wave] = se;
+    __syncthreads();
+    if (wave != 0) return;
+    // The pairs that a token t stands between: of its own 16 tokens, of those with earlier keys (from t on), of those with later queries (before t), of
+    // earlier keys and later queries; then those of what came in (from t on) and of what goes out (before t).
+    float between = 0.0f, from = 0.0f, until = 0.0f, after = 0.0f, before = 0.0f;
+    const int own = lane / 16;
+    if (lane < kC) {
+        between = of_queries[own * kC + lane];
+        for (int i = 0; i < own; ++i) from += of_queries[i * kC + lane];
+        for (int i = own + 1; i < kM; ++i) until += of_keys[i * kC + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            after += with_s[i * kC + lane];
+            before += with_e[i * kC + lane];
+        }
+    }
+#pragma unroll
+    for (int m = 1; m + 1 < kM; ++m) {
+        float over = 0.0f;
+        if (own < m)
+            for (int i = m + 1; i < kM; ++i) over += of_keys[i * kC + lane];
+        over = sum_groups(sum_columns(over));
+        if (own == m) between += over;
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        const float a = __shfl_down(from, d), b = __shfl_up(until, d);
+        if (col + d < 16) from += a;
+        if (col >= d) until += b;
+    }
+#pragma unroll
+    for (int d = 1; d < kC; d *= 2) {
+        const float a = __shfl_down(after, d), b = __shfl_up(before, d);
+        if (lane + d < kC) after += a;
+        if (lane >= d) before += b;
+    }
+    const float until_t = __shfl_up(until, 1), before_t = __shfl_up(before, 1);      // (a token's key is not before it)
+    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + exp2f(end.x + end.y) * ((both[0] + both[1]) + (both[2] + both[3]));
+    if (head_sums) {
+        dg = sum_groups(sum_columns(lane < e.z ? dg : 0.0f));
+        if (lane == 0) head_sums[entry] = dg;
+    } else if (lane < e.z) put_decay(lane, dg);
+}
+
+// Gradients of what several heads share: the heads' sum, of `per` neighbouring values in single precision, dim apart
+template <typename T> __global__ __launch_bounds__(kBlock) void la_sum_heads_kernel(const float *x, T *out, int64_t total, int dim, int per) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i >= total) return;
+    const int64_t group = i / dim;
+    const float *at = x + group * per * dim + (i - group * dim);
+    float sum = 0.0f;
+    for (int k = 0; k < per; ++k) sum += at[(int64_t)k * dim];
+    out[i] = from_f32<T>(sum);
+}
+
+// A learnt decay's gradient: the chunks' sums of its head, a workgroup to a head
+template <typename T> __global__ __launch_bounds__(kBlock) void la_sum_decays_kernel(const float *sums, void *out, int chunks, int heads, int f32) {
+    __shared__ double part[kBlock];
+    const int h = blockIdx.x, tid = threadIdx.x;
+    double sum = 0.0;
+    for (int c = tid; c < chunks; c += kBlock) sum += (double)sums[(int64_t)c * heads + h];
+    part[tid] = sum;
+    for (int d = kBlock / 2; d >= 1; d /= 2) {
+        __syncthreads();
+        if (tid < d) part[tid] += part[tid + d];
+    }
+    if (tid != 0) return;
+    if (f32) reinterpret_cast<float *>(out)[h] = (float)part[0];
+    else reinterpret_cast<T *>(out)[h] = from_f32<T>((float)part[0]);
+}
+
+struct LaBackward {
+    LaArgs a;
+    bool low;
+    float *head_sums;
+    void *dq, *dk, *dv;              // where the heads' sums go
+};
+
+template <typename Op, typename T> static int la_backward(const LaBackward &b, float *dinitial, void *stream) {
+    const LaArgs &p = b.a;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    int rc = la_tables(p, Op::kChunk, stream);
+    if (rc != SS2D_OK) return rc;
+    LaWalk w = {};
+    w.from_a = 1; w.from_b = p.v.dim;
+    const bool one = !p.cu && p.per_seq <= 1;                        // a chunk to a sequence: nothing comes in but what the caller gives
+    if (!one || p.initial) {
+        w.a = p.v; w.b = p.k;
+        w.out = p.states; w.low = p.low;
+        w.from = p.initial;
+        if ((rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
+    }
+    if (!one || p.dfinal || dinitial) {
+        w.a = p.dout; w.b = p.q;
+        w.out = p.dstates; w.out_t = p.dstates_t; w.low = p.low;
+        w.from = p.dfinal; w.to = dinitial;
+        w.reverse = 1;
+        if ((rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
+    }
+    const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
+    if (total > 0) {
+        const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), c = Op::kChunk, m = c / 16;
+        const size_t bytes = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad)) + sizeof(float2) * c +
+                             sizeof(float) * (2 * m * c + 8 * c + 4);
+        auto go = [&](auto kernel) {
+            // (up to 155 KB of LDS: this runtime asks for no attribute above 64)
+            kernel<<<total, kBlock, bytes, st>>>(p, b.head_sums, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
+            return launch_status();
+        };
+        if constexpr (sizeof(typename Op::E) == 2) rc = b.low ? go(la_bwd_kernel<Op, T, true>) : go(la_bwd_kernel<Op, T, false>);
+        else rc = go(la_bwd_kernel<Op, T, false>);
+        if (rc != SS2D_OK) return rc;
+        auto sum = [&](const LaSide &side, void *out) {
+            if (side.div <= 1) return;
+            const int64_t n = (int64_t)p.batch * p.tokens * (p.heads / side.div) * side.dim;
+            la_sum_heads_kernel<T><<<(uint32_t)((n + kBlock - 1) / kBlock), kBlock, 0, st>>>(reinterpret_cast<const float *>(side.p), reinterpret_cast<T *>(out), n, side.dim, side.div);
+        };
+        sum(p.dq, b.dq);
+        sum(p.dk, b.dk);
+        sum(p.dv, b.dv);
+    }
+    if (b.head_sums) la_sum_decays_kernel<T><<<p.heads, kBlock, 0, st>>>(b.head_sums, p.ddecay, p.max_chunks, p.heads, p.ddecay_f32);
+    return launch_status();
+}
+
+LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size, int bytes);
+int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty);
+int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low);
+
+// Everything of a backward call, its workspace laid out from `base` on; the bytes that takes, or a status.
+static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, LaBackward &b, bool &empty, char *base) {
+    empty = false;
+    if (!params) return SS2D_EINVAL;
+    const ss2d_linear_attention_params &f = params->fwd;
+    const int rc = la_arguments(&f, b.a, empty);
+    if (rc != SS2D_OK || empty) return rc;
+    LaArgs &a = b.a;
+    const int size = f.dtype == SS2D_F32 ? 4 : 2;
+    if (params->ddecay && !f.decay) return SS2D_EINVAL;
+    b.low = f.dtype == SS2D_BF16 && params->ddecay && f.decay_dtype == SS2D_F32;
+    a.dout = la_side(params->dout, params->dout_batch_stride, params->dout_token_stride, params->dout_head_stride, f.heads, f.heads, f.value_dim, size, 16);
+    a.dfinal = params->dfinal_state;
+    a.ddecay = params->ddecay;
+    a.ddecay_f32 = f.decay_dtype == SS2D_F32;
+    int64_t at = la_carve(a, f.dtype, base, true, b.low);
+    auto gradient = [&](LaSide &side, void *&to, void *ptr, int own, int dim) {
+        const bool shared = own != f.heads;
+        to = ptr;
+        const int64_t row = (int64_t)f.heads * dim;
+        side = la_side(shared ? base + at : ptr, row * f.seqlen, row, dim, f.heads, own, dim, shared ? 4 : size, shared ? 16 : 4 * size);
+        if (shared) at += (4 * row * f.seqlen * f.batch + 255) / 256 * 256;
+    };
+    gradient(a.dq, b.dq, params->dq, f.q_heads, f.key_dim);
+    gradient(a.dk, b.dk, params->dk, f.k_heads, f.key_dim);
+    gradient(a.dv, b.dv, params->dv, f.v_heads, f.value_dim);
+    b.head_sums = nullptr;
+    if (params->ddecay && params->decay_per_head) {
+        b.head_sums = reinterpret_cast<float *>(base + at);
+        at += ((int64_t)4 * a.max_chunks * a.heads + 255) / 256 * 256;
+    }
+    return at;
+}
+
+}  // namespace ss2d
+
+using namespace ss2d;
+
+extern "C" int64_t ss2d_linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params *params) {
+    LaBackward b;
+    bool empty;
+    return la_backward_plan(params, b, empty, nullptr);
+}
+
+extern "C" int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
+    LaBackward b;
+    bool empty;
+    const int64_t need = la_backward_plan(params, b, empty, reinterpret_cast<char *>(workspace));
+    if (need < 0) return (int)need;
+    if (empty) return SS2D_OK;
+    if (b.a.tokens > 0 && (!params->dout || !params->dq || !params->dk || !params->dv)) return SS2D_EINVAL;
+    if (!workspace || (uintptr_t)workspace % 16 != 0) return SS2D_EINVAL;
+    if (workspace_bytes < need) return SS2D_ENOMEM;
+    switch (params->fwd.dtype) {
+    case SS2D_F32: return la_backward<OperandF32, float>(b, params->dinitial_state, stream);
+    case SS2D_F16: return la_backward<OperandF32, f16_t>(b, params->dinitial_state, stream);
+    default: return la_backward<OperandBf16, bf16_t>(b, params->dinitial_state, stream);
+    }
+}
