@@ -238,7 +238,7 @@ def test_layouts(dtype):
             assert torch.equal(got[name], dense[name]), (how, name)
     # a head and a batch that are expanded, and the gradient of such a broadcast
     one = k[:1, :, :1].detach().requires_grad_()
-    out = linear_attention_fn(q, one.expand(B, T, H, dk), v, g)
+    out, _ = linear_attention_fn(q, one.expand(B, T, H, dk), v, g, output_final_state=True)
     dk_one, = torch.autograd.grad(out, one, dout)
     shared = run_all(q, k[:1, :, :1].expand(B, T, 1, dk), v, g, None, dout, None)
     assert torch.equal(out, shared["out"])

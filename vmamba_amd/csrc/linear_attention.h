@@ -28,7 +28,7 @@ struct LaSide {                      // q, k, v, out or a gradient: (batch, toke
     int64_t batch, token, head;      // strides in elements
     int32_t div;                     // heads of the state to one of this
     int32_t dim;
-    int32_t aligned;                 // base and strides are multiples of 16 bytes
+    int32_t aligned;                 // base and strides are multiples of 16 bytes (outputs: of four values), and rows of whole pieces
 };
 
 struct LaArgs {
@@ -73,6 +73,14 @@ struct OperandF32 {
         return c;
     }
     static __device__ __forceinline__ void put4(E *p, floatx4_t v) { *reinterpret_cast<floatx4_t *>(p) = v; }
+    // Accumulators of kStep rows (the sum's) as an operand of the next product, and rows() in the order of k that this gives
+    static __device__ __forceinline__ Frag from_acc(const floatx4_t *acc) { return acc[0]; }
+    static __device__ __forceinline__ Frag rows_acc(const E *tile, int pitch, int row0, int k0, int lane) { return rows(tile, pitch, row0, k0, lane); }
+    // The operand's values times their tokens' weights (weight: of token k0 on), in kParts operands whose sum it is
+    static constexpr int kMostParts = 1;
+    template <int kParts> static __device__ __forceinline__ void weigh(Frag f, const float *weight, int lane, Frag (&parts)[kParts]) {
+        parts[0] = f * *reinterpret_cast<const floatx4_t *>(weight + 4 * (lane >> 4));
+    }
 };
 
 struct OperandBf16 {
@@ -96,20 +104,57 @@ struct OperandBf16 {
     static __device__ __forceinline__ void put4(E *p, floatx4_t v) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_from_f32<bf16_t>(v[0], v[1]), pack2_from_f32<bf16_t>(v[2], v[3]));
     }
+    static __device__ __forceinline__ Frag from_acc(const floatx4_t *acc) {
+        return Frag{pack2_from_f32<bf16_t>(acc[0][0], acc[0][1]), pack2_from_f32<bf16_t>(acc[0][2], acc[0][3]), pack2_from_f32<bf16_t>(acc[1][0], acc[1][1]),
+                    pack2_from_f32<bf16_t>(acc[1][2], acc[1][3])};
+    }
+    static __device__ __forceinline__ Frag rows_acc(const E *tile, int pitch, int row0, int k0, int lane) {
+        const E *p = tile + (row0 + (lane & 15)) * pitch + k0 + 4 * (lane >> 4);
+        const uint2 lo = *reinterpret_cast<const uint2 *>(p), hi = *reinterpret_cast<const uint2 *>(p + 16);
+        return Frag{lo.x, lo.y, hi.x, hi.y};
+    }
+    // (bf16 of the value, of what that left, and of what that left: 24 bits)
+    static constexpr int kMostParts = 3;
+    template <int kParts> static __device__ __forceinline__ void weigh(Frag f, const float *weight, int lane, Frag (&parts)[kParts]) {
+        const floatx4_t w[2] = {*reinterpret_cast<const floatx4_t *>(weight + 8 * (lane >> 4)), *reinterpret_cast<const floatx4_t *>(weight + 8 * (lane >> 4) + 4)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x = unpack_lo<bf16_t>(f[i]) * w[i / 2][2 * i % 4], y = unpack_hi<bf16_t>(f[i]) * w[i / 2][2 * i % 4 + 1];
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) {
+                parts[k][i] = pack2_from_f32<bf16_t>(x, y);
+                if (k + 1 == kParts) break;
+                const float xh = unpack_lo<bf16_t>(parts[k][i]), yh = unpack_hi<bf16_t>(parts[k][i]);
+                const float xl = x - xh, yl = y - yh;
+                x = fabsf(xh) <= FLT_MAX ? xl : 0.0f;
+                y = fabsf(yh) <= FLT_MAX ? yl : 0.0f;
+            }
+        }
+    }
 };
 
 // ---- tiles ------------------------------------------------------------------------------------------------------------------------
 template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 
-// 16 bytes' worth of a row from column c on: in one load where they are aligned and inside the row, else element by element
-template <typename T> __device__ __forceinline__ u32x4_t load_piece(const T *row, int c, int cols, bool aligned) {
-    if (aligned && c + kVecOf<T> <= cols) return *reinterpret_cast<const u32x4_t *>(row + c);
+// 16 bytes' worth of row `row` of `rows` (one at least), from column c on.  kFast: the side is aligned and its dimension a multiple of a piece; the load
+// is then unconditional -- a row or column that is not there repeats another -- so that nothing waits for it before it is used, and held_piece() makes
+// zeros of it there.  Otherwise element by element, zeros for what is not there.
+template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(const T *base, int64_t stride, int row, int rows, int c, int cols) {
+    if constexpr (kFast) return *reinterpret_cast<const u32x4_t *>(base + min(row, rows - 1) * stride + (c < cols ? c : 0));
     union { T e[kVecOf<T>]; u32x4_t w; } u;
     u.w = u32x4_t{0, 0, 0, 0};
+    if (row < rows)
 #pragma unroll
-    for (int i = 0; i < kVecOf<T>; ++i)
-        if (c + i < cols) u.e[i] = row[c + i];
+        for (int i = 0; i < kVecOf<T>; ++i)
+            if (c + i < cols) u.e[i] = base[row * stride + c + i];
     return u.w;
+}
+template <bool kFast> __device__ __forceinline__ u32x4_t held_piece(u32x4_t piece, bool in) {
+    if constexpr (kFast) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) piece[i] = in ? piece[i] : 0u;
+    }
+    return piece;
 }
 
 template <typename T> __device__ __forceinline__ float piece_at(u32x4_t w, int i) {
@@ -152,6 +197,12 @@ template <typename T> __device__ __forceinline__ void store4(T *p, floatx4_t v, 
         if (i < left) p[i] = from_f32<T>(v[i]);
 }
 
+// The value, as if it were made here: what follows from it is not computed ahead of a branch that is hardly ever taken
+__device__ __forceinline__ int la_here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 inline __host__ __device__ int la_up(int n, int m) { return (n + m - 1) / m * m; }
 // Rows of a state stand at a pitch that every operand's step divides, with zeros behind them
 inline __host__ __device__ int la_state_dim(int d) { return la_up(d, 32); }
@@ -175,9 +226,11 @@ struct LaWalk {
     float *to;                       // the state to end with, or NULL
     int32_t from_a, from_b;
     int32_t reverse;                 // from the last chunk to the first, weights scale exp(G_t) instead of exp(G_C - G_s)
+    int32_t exact;                   // the states are kept in 32 bits: three parts to a weighted 16-bit operand instead of two
 };
-int la_plan(LaArgs &p, int chunk);                                                     // sizes of the tables and segments
+int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest);                        // sizes of the tables and segments, for `tiles` workgroups a head
 int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
-template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream);
+template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream);        // states before all chunks
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }            // (what is below 2^-126 is 0)
 
 }  // namespace ss2d

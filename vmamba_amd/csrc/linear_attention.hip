@@ -1,5 +1,7 @@
 // Linear attention with a decay for each head: tables of the chunks, the walk over the states, outputs (the mathematics is in
 // linear_attention.h).
+#include <type_traits>
+
 #include "linear_attention.h"
 
 namespace ss2d {
@@ -97,43 +99,63 @@ __global__ __launch_bounds__(kBlock) void la_chunks_kernel(const LaArgs p, int64
 }
 
 // ---- the walk over the states ------------------------------------------------------------------------------------------------------
-// A workgroup owns a 64 x 64 piece of one head's state, in accumulators (wavefront w rows 16 w .. of a's dimension), and walks a segment of
-// a sequence's chunks.  kLocal: a segment's own sum alone, from zero, and its decay, so that la_join_kernel can tell every segment
-// what comes in.  The next chunk's rows are on their way while this one is added.
-// For 16-bit operands the weighted one is split into two bf16 values: states are good to 2^-17.
-template <typename Op, typename T, bool kLocal>
-__global__ __launch_bounds__(kBlock) void la_walk_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
-    using E = typename Op::E;
-    using Frag = typename Op::Frag;
-    constexpr int kC = Op::kChunk, kPitch = kLaTile + Op::kPad, kVec = kVecOf<T>, kPerRow = kLaTile / kVec, kN = kC * kPerRow / kBlock;
-    constexpr bool kSplit = sizeof(E) == 2;
-    __shared__ __align__(16) E at[kC * kPitch], al[kSplit ? kC * kPitch : 1], bt[kC * kPitch];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
-    const uint32_t id = xcd_contiguous_id(blockIdx.x, total);
-    const int tile = id % (uint32_t)tiles, h = id / (uint32_t)tiles % (uint32_t)p.heads, seg = id / (uint32_t)tiles / (uint32_t)p.heads;
-    const int a0 = tile % tiles_a * kLaTile, b0 = tile / tiles_a * kLaTile;
-    int n;
+// Which piece of which head, and which segment of which sequence, a workgroup walks.
+struct LaPlace {
+    int n, h, seg, tile;
+    int4 s;                          // the sequence
+    int begin, count, chunks;        // of the segment, in chunks; of the sequence
+};
+__device__ __forceinline__ bool la_place(const LaArgs &p, uint32_t id, int tiles, int chunk, LaPlace &at) {
+    at.tile = id % (uint32_t)tiles;
+    at.h = id / (uint32_t)tiles % (uint32_t)p.heads;
+    at.seg = id / (uint32_t)tiles / (uint32_t)p.heads;
     if (p.cu) {
-        if (seg >= p.seqs[p.n_seqs].w) return;
+        if (at.seg >= p.seqs[p.n_seqs].w) return false;
         int lo = 0, hi = p.n_seqs;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (p.seqs[mid].w <= seg) lo = mid; else hi = mid;
+            if (p.seqs[mid].w <= at.seg) lo = mid; else hi = mid;
         }
-        n = lo;
-    } else n = seg / p.segs_per_seq;
-    const int4 s = la_sequence(p, n);
-    const int n_chunks = (s.y - s.x + kC - 1) / kC, begin = (seg - s.w) * p.seg_chunks, count = min(p.seg_chunks, n_chunks - begin);
-    const bool lone = n_chunks <= p.seg_chunks;                      // the sequence has this one segment
-    const bool last = w.reverse ? begin == 0 : begin + count >= n_chunks;
+        at.n = lo;
+    } else at.n = at.seg / p.segs_per_seq;
+    at.s = la_sequence(p, at.n);
+    at.chunks = (at.s.y - at.s.x + chunk - 1) / chunk;
+    at.begin = (at.seg - at.s.w) * p.seg_chunks;
+    at.count = min(p.seg_chunks, at.chunks - at.begin);
+    return true;
+}
+
+// Element (ia, ib) of the state of sequence n and head h that the caller gives or gets
+__device__ __forceinline__ int64_t la_state_at(const LaArgs &p, const LaWalk &w, int n, int h, int ia, int ib) {
+    return ((int64_t)n * p.heads + h) * p.k.dim * p.v.dim + ia * w.from_a + ib * w.from_b;
+}
+
+// A workgroup owns a 64 x 64 piece of one head's state, in accumulators (wavefront w rows 16 w .. of a's dimension), and walks a segment of
+// a sequence's chunks.  kLocal: a segment's own sum alone, from zero, and its decay, so that la_join_kernel can tell every segment
+// what comes in.  The next chunk's rows are on their way while this one is added.
+template <typename Op, typename T, bool kLocal, int kParts, bool kFast>
+__global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
+    using E = typename Op::E;
+    using Frag = typename Op::Frag;
+    constexpr int kC = Op::kChunk, kPitch = kLaTile + Op::kPad, kVec = kVecOf<T>, kPerRow = kLaTile / kVec, kN = kC * kPerRow / kBlock;
+    __shared__ __align__(16) E at[kC * kPitch], bt[kC * kPitch];
+    __shared__ __align__(16) float weights[kC];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
+    LaPlace here;
+    if (!la_place(p, xcd_contiguous_id(blockIdx.x, total), tiles, kC, here)) return;
+    const int a0 = here.tile % tiles_a * kLaTile, b0 = here.tile / tiles_a * kLaTile, h = here.h, n = here.n;
+    const int4 s = here.s;
+    const bool lone = here.chunks <= p.seg_chunks;                   // the sequence has this one segment
+    const bool last = w.reverse ? here.begin == 0 : here.begin + here.count >= here.chunks;
+    if (kLocal && lone) return;
     const int64_t b = p.cu ? 0 : n;
     const T *pa = reinterpret_cast<const T *>(w.a.p) + b * w.a.batch + (int64_t)(h / w.a.div) * w.a.head + a0;
     const T *pb = reinterpret_cast<const T *>(w.b.p) + b * w.b.batch + (int64_t)(h / w.b.div) * w.b.head + b0;
 
     floatx4_t acc[4];                                                // element (16 wave + 4 (lane / 16) + v, 16 i + lane % 16)
     const int ia = a0 + 16 * wave + 4 * (lane >> 4), ib = b0 + (lane & 15);
-    float *local = p.local + (((int64_t)seg * p.heads + h) * tiles + tile) * (kLaTile * kLaTile);
+    float *local = p.local + (((int64_t)here.seg * p.heads + h) * tiles + here.tile) * (kLaTile * kLaTile);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         acc[i] = floatx4_t{0, 0, 0, 0};
@@ -142,96 +164,84 @@ __global__ __launch_bounds__(kBlock) void la_walk_kernel(const LaArgs p, const L
             else if (w.from)
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
-                    if (ia + v < w.a.dim && ib + 16 * i < w.b.dim)
-                        acc[i][v] = w.from[((int64_t)n * p.heads + h) * p.k.dim * p.v.dim + (ia + v) * w.from_a + (ib + 16 * i) * w.from_b];
+                    if (ia + v < w.a.dim && ib + 16 * i < w.b.dim) acc[i][v] = w.from[la_state_at(p, w, n, h, ia + v, ib + 16 * i)];
         }
     }
-    if (kLocal && lone) return;
 
     u32x4_t ra[kN], rb[kN];
-    float weight[kN], decay = 1.0f;
+    float weight = 0.0f, decay = 1.0f;
     double sum = 0.0;
     auto fetch = [&](int i) {                                        // the i-th chunk of the walk
-        const int c = begin + (w.reverse ? count - 1 - i : i), t0 = s.x + c * kC, len = min(kC, s.y - t0);
+        const int c = here.begin + (w.reverse ? here.count - 1 - i : i), t0 = s.x + c * kC, len = min(kC, s.y - t0);
         const float2 *cum = p.cum + ((int64_t)(s.z + c) * p.heads + h) * kC;
         const float2 end = cum[kC - 1];
         if constexpr (kLocal) sum += (double)end.x + (double)end.y;
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const int at_ = tid + j * kBlock, row = at_ / kPerRow, col = at_ % kPerRow * kVec;
-            ra[j] = rb[j] = u32x4_t{0, 0, 0, 0};
-            if (row < len) {
-                ra[j] = load_piece(pa + (int64_t)(t0 + row) * w.a.token, col, w.a.dim - a0, w.a.aligned);
-                rb[j] = load_piece(pb + (int64_t)(t0 + row) * w.b.token, col, w.b.dim - b0, w.b.aligned);
-            }
-            const float2 g = cum[row];
-            weight[j] = w.reverse ? p.scale * exp2f(g.x + g.y) : exp2f((end.x - g.x) + (end.y - g.y));
+            ra[j] = load_piece<kFast>(pa + (int64_t)t0 * w.a.token, w.a.token, row, len, col, w.a.dim - a0);
+            rb[j] = load_piece<kFast>(pb + (int64_t)t0 * w.b.token, w.b.token, row, len, col, w.b.dim - b0);
         }
-        decay = exp2f(end.x + end.y);
+        if (tid < kC) {
+            const float2 g = cum[tid];
+            weight = w.reverse ? p.scale * fast_exp2(g.x + g.y) : fast_exp2((end.x - g.x) + (end.y - g.y));
+        }
+        decay = fast_exp2(end.x + end.y);
     };
-    if (count > 0) fetch(0);
-    for (int i = 0; i < count; ++i) {
-        const int64_t at_chunk = (int64_t)(s.z + begin + (w.reverse ? count - 1 - i : i)) * p.heads + h;
+    if (here.count > 0) fetch(0);
+    for (int i = 0; i < here.count; ++i) {
+        const int c = here.begin + (w.reverse ? here.count - 1 - i : i), len = min(kC, s.y - s.x - c * kC);
+        const int64_t at_chunk = (int64_t)(s.z + c) * p.heads + h;
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const int at_ = tid + j * kBlock, row = at_ / kPerRow, col = at_ % kPerRow * kVec;
-            put_piece<T, E>(bt + row * kPitch + col, rb[j]);
-            if constexpr (kSplit) {
-                u32x4_t hi, lo;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float x = unpack_lo<T>(ra[j][q]) * weight[j], y = unpack_hi<T>(ra[j][q]) * weight[j];
-                    hi[q] = pack2_from_f32<bf16_t>(x, y);
-                    const float xh = unpack_lo<bf16_t>(hi[q]), yh = unpack_hi<bf16_t>(hi[q]);
-                    lo[q] = pack2_from_f32<bf16_t>(fabsf(xh) <= FLT_MAX ? x - xh : 0.0f, fabsf(yh) <= FLT_MAX ? y - yh : 0.0f);
-                }
-                *reinterpret_cast<u32x4_t *>(at + row * kPitch + col) = hi;
-                *reinterpret_cast<u32x4_t *>(al + row * kPitch + col) = lo;
-            } else {
-#pragma unroll
-                for (int q = 0; q < kVec; q += 4)
-                    *reinterpret_cast<floatx4_t *>(at + row * kPitch + col + q) =
-                        floatx4_t{piece_at<T>(ra[j], q), piece_at<T>(ra[j], q + 1), piece_at<T>(ra[j], q + 2), piece_at<T>(ra[j], q + 3)} * weight[j];
-            }
+            put_piece<T, E>(at + row * kPitch + col, held_piece<kFast>(ra[j], row < len && col < w.a.dim - a0));
+            put_piece<T, E>(bt + row * kPitch + col, held_piece<kFast>(rb[j], row < len && col < w.b.dim - b0));
         }
+        if (tid < kC) weights[tid] = weight;
         const float keep = decay;
         __syncthreads();
-        if (i + 1 < count) fetch(i + 1);
+        if (i + 1 < here.count) fetch(i + 1);
         if constexpr (!kLocal) {                                     // the state as the chunk finds it
             const int da = la_state_dim(w.a.dim), db = la_state_dim(w.b.dim);
-            E *out = reinterpret_cast<E *>(w.out) + at_chunk * da * db, *out_t = reinterpret_cast<E *>(w.out_t) + at_chunk * da * db;
+            const int64_t base = at_chunk * da * db;
+            E *out = reinterpret_cast<E *>(w.out) + base + (int64_t)ib * da + ia, *out_t = reinterpret_cast<E *>(w.out_t) + base + (int64_t)ia * db + ib;
+            if (ia < da) {
+                const int left = (db - ib + 15) / 16;                // columns of 16 that there are
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (w.out && ia < da && ib + 16 * j < db) {
-                    E *o = out + (int64_t)(ib + 16 * j) * da + ia;
-                    Op::put4(o, acc[j]);
-                    if constexpr (kSplit)
-                        if (w.low) {
+                for (int j = 0; j < 4; ++j)
+                    if (j < left) Op::put4(out + (int64_t)16 * j * da, acc[j]);
+                if (sizeof(E) == 2 && w.low)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < left) {
                             floatx4_t rest;
 #pragma unroll
                             for (int v = 0; v < 4; ++v) {
-                                const float high = to_f32(from_f32<bf16_t>(acc[j][v]));
-                                rest[v] = fabsf(high) <= FLT_MAX ? acc[j][v] - high : 0.0f;
+                                const float high = to_f32(from_f32<bf16_t>(acc[j][v])), under = acc[j][v] - high;
+                                rest[v] = fabsf(high) <= FLT_MAX ? under : 0.0f;
                             }
-                            Op::put4(o + w.low, rest);
+                            Op::put4(out + (int64_t)16 * j * da + w.low, rest);
                         }
-                    if (w.out_t)
+                if (w.out_t)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) out_t[(int64_t)(ia + v) * db + ib + 16 * j] = from_f32<E>(acc[j][v]);
-                }
+                    for (int j = 0; j < 4; ++j)
+                        if (j < left)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) out_t[(int64_t)v * db + 16 * j] = from_f32<E>(acc[j][v]);
+            }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] *= keep;
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-            const Frag fa = Op::cols(at, kPitch, 16 * wave, k0, lane);
-            Frag fl;
-            if constexpr (kSplit) fl = Op::cols(al, kPitch, 16 * wave, k0, lane);
+            Frag fa[kParts];
+            Op::template weigh<kParts>(Op::cols(at, kPitch, 16 * wave, k0, lane), weights + k0, lane, fa);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const Frag fb = Op::cols(bt, kPitch, 16 * j, k0, lane);
-                acc[j] = Op::mma(fa, fb, acc[j]);
-                if constexpr (kSplit) acc[j] = Op::mma(fl, fb, acc[j]);
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) acc[j] = Op::mma(fa[q], fb, acc[j]);
             }
         }
         __syncthreads();
@@ -239,53 +249,79 @@ __global__ __launch_bounds__(kBlock) void la_walk_kernel(const LaArgs p, const L
     if constexpr (kLocal) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4_t *>(local + i * 4 * kBlock + 4 * tid) = acc[i];
-        if (tile == 0 && tid == 0) p.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)seg * p.heads + h] = exp2f((float)sum);
+        if (here.tile == 0 && tid == 0)
+            p.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)here.seg * p.heads + h] = exp2f((float)sum);
     } else if (w.to && last) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int v = 0; v < 4; ++v)
-                if (ia + v < w.a.dim && ib + 16 * i < w.b.dim)
-                    w.to[((int64_t)n * p.heads + h) * p.k.dim * p.v.dim + (ia + v) * w.from_a + (ib + 16 * i) * w.from_b] = acc[i][v];
+                if (ia + v < w.a.dim && ib + 16 * i < w.b.dim) w.to[la_state_at(p, w, n, h, ia + v, ib + 16 * i)] = acc[i][v];
     }
 }
 
-// What comes into each segment of a sequence, from the segments' own sums: in their place.
+// What comes into each segment of a sequence, from the segments' own sums: in their place.  A workgroup takes 16 columns of a piece; the sums of
+// eight segments are on their way at once.
 __global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w, int chunk) {
+    constexpr int kAhead = 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
-    const int tile = blockIdx.x % (uint32_t)tiles, h = blockIdx.x / (uint32_t)tiles % (uint32_t)p.heads, n = blockIdx.x / (uint32_t)tiles / (uint32_t)p.heads;
+    const uint32_t id = blockIdx.x / 4;
+    const int i = blockIdx.x % 4, tile = id % (uint32_t)tiles, h = id / (uint32_t)tiles % (uint32_t)p.heads, n = id / (uint32_t)tiles / (uint32_t)p.heads;
     const int4 s = la_sequence(p, n);
     const int n_chunks = (s.y - s.x + chunk - 1) / chunk, segs = (n_chunks + p.seg_chunks - 1) / p.seg_chunks;
     if (segs <= 1) return;
-    const int ia = tile % tiles_a * kLaTile + 16 * wave + 4 * (lane >> 4), ib = tile / tiles_a * kLaTile + (lane & 15);
+    const int ia = tile % tiles_a * kLaTile + 16 * wave + 4 * (lane >> 4), ib = tile / tiles_a * kLaTile + 16 * i + (lane & 15);
     const float *decays = p.local + (int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile);
-    for (int i = 0; i < 4; ++i) {
-        floatx4_t state = {0, 0, 0, 0};
-        if (w.from)
-            for (int v = 0; v < 4; ++v)
-                if (ia + v < w.a.dim && ib + 16 * i < w.b.dim)
-                    state[v] = w.from[((int64_t)n * p.heads + h) * p.k.dim * p.v.dim + (ia + v) * w.from_a + (ib + 16 * i) * w.from_b];
-        for (int q = 0; q < segs; ++q) {
-            const int64_t seg = s.w + (w.reverse ? segs - 1 - q : q);
-            floatx4_t *at = reinterpret_cast<floatx4_t *>(p.local + ((seg * p.heads + h) * tiles + tile) * (kLaTile * kLaTile) + i * 4 * kBlock + 4 * tid);
-            const floatx4_t own = *at;
-            *at = state;
-            state = state * decays[seg * p.heads + h] + own;
+    floatx4_t state = {0, 0, 0, 0};
+    if (w.from)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            if (ia + v < w.a.dim && ib < w.b.dim) state[v] = w.from[la_state_at(p, w, n, h, ia + v, ib)];
+    auto place = [&](int q) { return ((int64_t)s.w + (w.reverse ? segs - 1 - q : q)) * p.heads + h; };
+    auto at = [&](int q) { return reinterpret_cast<floatx4_t *>(p.local + (place(q) * tiles + tile) * (kLaTile * kLaTile) + i * 4 * kBlock + 4 * tid); };
+    for (int q0 = 0; q0 < segs; q0 += kAhead) {
+        floatx4_t own[kAhead];
+        float decay[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int safe = min(q0 + q, segs - 1);
+            own[q] = *at(safe);
+            decay[q] = decays[place(safe)];
         }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q)
+            if (q0 + q < segs) {
+                *at(q0 + q) = state;
+                state = state * decay[q] + own[q];
+            }
     }
+}
+
+static int64_t la_tiles(const LaArgs &p) { return (int64_t)((p.k.dim + kLaTile - 1) / kLaTile) * ((p.v.dim + kLaTile - 1) / kLaTile); }
+
+template <typename Op, typename T, bool kLocal> static void la_walk_launch(const LaArgs &p, const LaWalk &w, uint32_t total, hipStream_t st) {
+    constexpr int kMost = Op::kMostParts, kLess = kMost < 2 ? kMost : 2;
+    const bool fast = w.a.aligned && w.b.aligned;
+    if (w.exact) fast ? la_walk_kernel<Op, T, kLocal, kMost, true><<<total, kBlock, 0, st>>>(p, w, total) : la_walk_kernel<Op, T, kLocal, kMost, false><<<total, kBlock, 0, st>>>(p, w, total);
+    else fast ? la_walk_kernel<Op, T, kLocal, kLess, true><<<total, kBlock, 0, st>>>(p, w, total) : la_walk_kernel<Op, T, kLocal, kLess, false><<<total, kBlock, 0, st>>>(p, w, total);
+}
+
+// What comes into the segments
+template <typename Op, typename T> static int la_segments(const LaArgs &p, const LaWalk &w, hipStream_t st) {
+    if (p.max_segs <= p.n_seqs) return SS2D_OK;
+    const int64_t tiles = la_tiles(p), total = (int64_t)p.max_segs * p.heads * tiles;
+    la_walk_launch<Op, T, true>(p, w, (uint32_t)total, st);
+    la_join_kernel<<<(uint32_t)((int64_t)p.n_seqs * p.heads * tiles * 4), kBlock, 0, st>>>(p, w, Op::kChunk);
+    return launch_status();
 }
 
 template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream) {
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int64_t tiles = (int64_t)((w.a.dim + kLaTile - 1) / kLaTile) * ((w.b.dim + kLaTile - 1) / kLaTile);
-    const int64_t total = (int64_t)p.max_segs * p.heads * tiles;
-    if (total > 0x7fffffff) return SS2D_EINVAL;
-    if (p.max_segs > p.n_seqs) {
-        la_walk_kernel<Op, T, true><<<(uint32_t)total, kBlock, 0, st>>>(p, w, (uint32_t)total);
-        la_join_kernel<<<(uint32_t)((int64_t)p.n_seqs * p.heads * tiles), kBlock, 0, st>>>(p, w, Op::kChunk);
-    }
-    la_walk_kernel<Op, T, false><<<(uint32_t)total, kBlock, 0, st>>>(p, w, (uint32_t)total);
+    const int64_t total = (int64_t)p.max_segs * p.heads * la_tiles(p);
+    const int rc = la_segments<Op, T>(p, w, st);
+    if (rc != SS2D_OK) return rc;
+    la_walk_launch<Op, T, false>(p, w, (uint32_t)total, st);
     return launch_status();
 }
 template int la_walk<OperandF32, float>(const LaArgs &, const LaWalk &, void *);
@@ -293,142 +329,225 @@ template int la_walk<OperandF32, f16_t>(const LaArgs &, const LaWalk &, void *);
 template int la_walk<OperandBf16, bf16_t>(const LaArgs &, const LaWalk &, void *);
 
 // ---- outputs -----------------------------------------------------------------------------------------------------------------------
-// A workgroup owns a chunk of one head.  Its wavefronts take the weights of the chunk's pairs 16 tokens each, then the output's columns 16 each: the
-// states are read from memory straight into operands, each value once.  Products come out transposed (lane: one token, four
-// neighbouring values), so that what a token has to be multiplied with is one value of the lane and stores are 8 or 16 bytes.
+// A workgroup owns 64 values' columns of one head and walks a segment of chunks: the state stays in accumulators, 16 columns for all kTiles * 16 keys
+// to a wavefront, and is turned into an operand of the outputs' product where it lies (an accumulator's rows are the next product's sum).
+// Nothing but q, k, v and the outputs passes through memory.  Per chunk: weights of its pairs, 16 tokens to a wavefront, through LDS; out = state and
+// pairs; then the state with the chunk's keys and weighted values.  Products come out transposed (lane: one token, four
+// neighbouring values), so that what a token has to be multiplied with is one value of the lane.
 // The weights behind the diagonal are zeros; a product of zero with what is infinite or NaN would reach tokens in front of it, so a
 // chunk that holds such a value sums its pairs one by one.
-template <typename Op, typename T>
-__global__ __launch_bounds__(kBlock) void la_out_kernel(const LaArgs p, uint32_t total, FastDiv per_key, FastDiv per_value) {
+template <typename Op, typename T, int kTiles, int kParts, bool kFast>
+__global__ __launch_bounds__(kBlock, 2) void la_out_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
-    constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad;
+    constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kKeys = 16 * kTiles, kPitchK = kKeys + Op::kPad, kPitchV = kLaTile + Op::kPad, kPitchP = kC + Op::kPad;
+    constexpr int kPerKey = kKeys / kVec, kPerValue = kLaTile / kVec, kNk = (kC * kPerKey + kBlock - 1) / kBlock, kNv = kC * kPerValue / kBlock;
+    constexpr int kJoin = Op::kStep / 16;                            // accumulators to an operand
     extern __shared__ __align__(16) char lds[];
-    const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, 16), pitch_k = dk + Op::kPad, pitch_v = dv + Op::kPad;
-    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * pitch_k, *vt = kt + kC * pitch_k, *pt = vt + kC * pitch_v;
-    float2 *cum = reinterpret_cast<float2 *>(pt + kC * kPitchP);
+    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * kPitchK, *vt = kt + kC * kPitchK, *pt = vt + kC * kPitchV;
+    float *weights = reinterpret_cast<float *>(pt + kC * kPitchP);   // of a token's value in the state behind the chunk
+    float2 *cum = reinterpret_cast<float2 *>(weights + kC);
+    int *bad = reinterpret_cast<int *>(cum + kC);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
-    const uint32_t id = xcd_contiguous_id(blockIdx.x, total);
-    const int c = id / (uint32_t)p.heads, h = id - (uint32_t)c * (uint32_t)p.heads;
-    const int4 e = p.chunks[c];
-    if (e.z <= 0) return;
-    T *out = reinterpret_cast<T *>(p.out.p) + e.x * p.out.batch + (int64_t)e.y * p.out.token + (int64_t)h * p.out.head;
-    if (e.w < 0) {                                                   // rows of no sequence
-        for (int i = tid; i < e.z * p.v.dim; i += kBlock) out[i / p.v.dim * p.out.token + i % p.v.dim] = from_f32<T>(0.0f);
-        return;
-    }
-    auto load = [&](const LaSide &side, E *tile, int pitch, const FastDiv &per_row) {
-        const T *src = reinterpret_cast<const T *>(side.p) + e.x * side.batch + (int64_t)e.y * side.token + (int64_t)(h / side.div) * side.head;
-        bool bad = false;
-        for (uint32_t i = tid; i < kC * per_row.d; i += 4 * kBlock) {
-            u32x4_t piece[4];
-            uint32_t row[4], at[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                divmod(i + j * kBlock, per_row, row[j], at[j]);
-                piece[j] = u32x4_t{0, 0, 0, 0};
-                if ((int)row[j] < e.z) piece[j] = load_piece(src + (int64_t)row[j] * side.token, at[j] * kVec, side.dim, side.aligned);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (row[j] < kC) {
-                    put_piece<T, E>(tile + row[j] * pitch + at[j] * kVec, piece[j]);
-                    bad |= piece_bad<T>(piece[j]);
-                }
-        }
-        return bad;
-    };
-    if (tid < kC) cum[tid] = p.cum[((int64_t)c * p.heads + h) * kC + tid];
-    load(p.q, qt, pitch_k, per_key);
-    load(p.k, kt, pitch_k, per_key);
-    const bool bad = __syncthreads_or(load(p.v, vt, pitch_v, per_value));
+    const int tiles = (p.v.dim + kLaTile - 1) / kLaTile;
+    LaPlace here;
+    if (!la_place(p, xcd_contiguous_id(blockIdx.x, total), tiles, kC, here)) return;
+    const int v0 = here.tile * kLaTile, h = here.h, n = here.n;
+    const int4 s = here.s;
+    const bool lone = here.chunks <= p.seg_chunks, last = here.begin + here.count >= here.chunks;
+    const int64_t b = p.cu ? 0 : n;
+    const T *pq = reinterpret_cast<const T *>(p.q.p) + b * p.q.batch + (int64_t)(h / p.q.div) * p.q.head;
+    const T *pk = reinterpret_cast<const T *>(p.k.p) + b * p.k.batch + (int64_t)(h / p.k.div) * p.k.head;
+    const T *pv = reinterpret_cast<const T *>(p.v.p) + b * p.v.batch + (int64_t)(h / p.v.div) * p.v.head + v0;
+    T *out = reinterpret_cast<T *>(p.out.p) + b * p.out.batch + (int64_t)h * p.out.head + v0;
 
-    // weights of the pairs, P[t][s]
+    floatx4_t state[kTiles];                                         // key 16 d + quad + v, value v0 + 16 wave + col
+    const int value = v0 + 16 * wave + col;
+    const int tiles_a = (p.k.dim + kLaTile - 1) / kLaTile;
 #pragma unroll
-    for (int i = 0; i < kM * kM / 4; ++i) {
-        const int tt = wave % kM, ts = wave / kM + i * (4 / kM);
-        floatx4_t acc = {0, 0, 0, 0};
-        if (ts <= tt) {
-            for (int k0 = 0; k0 < dk; k0 += Op::kStep)
-                acc = Op::mma(Op::rows(kt, pitch_k, 16 * ts, k0, lane), Op::rows(qt, pitch_k, 16 * tt, k0, lane), acc);
-            const int t = 16 * tt + col, s = 16 * ts + quad;
+    for (int d = 0; d < kTiles; ++d) {
+        state[d] = floatx4_t{0, 0, 0, 0};
+        if (!lone) {
+            if (d / 4 < tiles_a)
+                state[d] = *reinterpret_cast<const floatx4_t *>(p.local + (((int64_t)here.seg * p.heads + h) * tiles_a * tiles + here.tile * tiles_a + d / 4) * (kLaTile * kLaTile) +
+                                                                wave * 4 * kBlock + 4 * (d % 4 * kWave + lane));
+        } else if (w.from)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (16 * d + quad + v < p.k.dim && value < p.v.dim) state[d][v] = w.from[la_state_at(p, w, n, h, 16 * d + quad + v, value)];
+    }
+    bool carried = here.begin > 0 || w.from;                         // a state has come in
+
+    u32x4_t rq[kNk], rk[kNk], rv[kNv];
+    float2 rc = make_float2(0.0f, 0.0f), re = rc;
+    auto fetch = [&](int i) {
+        const int c = here.begin + i, t0 = s.x + c * kC, len = min(kC, s.y - t0);
+#pragma unroll
+        for (int j = 0; j < kNk; ++j) {
+            const int at = tid + j * kBlock, row = at / kPerKey, d = at % kPerKey * kVec;
+            rq[j] = load_piece<kFast>(pq + (int64_t)t0 * p.q.token, p.q.token, row, len, d, p.k.dim);
+            rk[j] = load_piece<kFast>(pk + (int64_t)t0 * p.k.token, p.k.token, row, len, d, p.k.dim);
+        }
+#pragma unroll
+        for (int j = 0; j < kNv; ++j) {
+            const int at = tid + j * kBlock, row = at / kPerValue, d = at % kPerValue * kVec;
+            rv[j] = load_piece<kFast>(pv + (int64_t)t0 * p.v.token, p.v.token, row, len, d, p.v.dim - v0);
+        }
+        if (tid < kC) {
+            const float2 *at = p.cum + ((int64_t)(s.z + c) * p.heads + h) * kC;
+            rc = at[tid];
+            re = at[kC - 1];
+        }
+    };
+    if (here.count > 0) fetch(0);
+    for (int i = tid; i < kC * kPitchP; i += kBlock) pt[i] = E{};    // (behind the diagonal they stay)
+    if (tid < 2) bad[tid] = 0;
+    __syncthreads();
+    for (int i = 0; i < here.count; ++i) {
+        const int t0 = s.x + (here.begin + i) * kC, len = min(kC, s.y - t0);
+        bool none = false;
+#pragma unroll
+        for (int j = 0; j < kNk; ++j) {
+            const int at = tid + j * kBlock, row = at / kPerKey, d = at % kPerKey * kVec;
+            if (kC * kPerKey % kBlock == 0 || row < kC) {
+                put_piece<T, E>(qt + row * kPitchK + d, held_piece<kFast>(rq[j], row < len && d < p.k.dim));
+                put_piece<T, E>(kt + row * kPitchK + d, held_piece<kFast>(rk[j], row < len && d < p.k.dim));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kNv; ++j) {
+            const int at = tid + j * kBlock, row = at / kPerValue, d = at % kPerValue * kVec;
+            const u32x4_t piece = held_piece<kFast>(rv[j], row < len && d < p.v.dim - v0);
+            put_piece<T, E>(vt + row * kPitchV + d, piece);
+            none |= piece_bad<T>(piece);
+        }
+        if (none) bad[i & 1] = 1;
+        if (tid < kC) {
+            cum[tid] = rc;
+            weights[tid] = fast_exp2((re.x - rc.x) + (re.y - rc.y));
+        }
+        __syncthreads();
+        if (i + 1 < here.count) fetch(i + 1);
+        if (tid == 0) bad[(i + 1) & 1] = 0;
+
+        // weights of the pairs, P[t][s]
+#pragma unroll
+        for (int k = 0; k < kM * kM / 4; ++k) {
+            const int tt = wave % kM, ts = wave / kM + k * (4 / kM);
+            if (ts > tt) continue;
+            floatx4_t acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int k0 = 0; k0 < kKeys; k0 += Op::kStep)
+                acc = Op::mma(Op::rows(kt, kPitchK, 16 * ts, k0, lane), Op::rows(qt, kPitchK, 16 * tt, k0, lane), acc);
+            const int t = 16 * tt + col, r = 16 * ts + quad;
             const float2 gt = cum[t];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float2 gs = cum[s + v];
-                acc[v] = s + v <= t ? acc[v] * exp2f((gt.x - gs.x) + (gt.y - gs.y)) : 0.0f;
+                const float2 gs = cum[r + v];
+                const float weight = acc[v] * fast_exp2((gt.x - gs.x) + (gt.y - gs.y));
+                acc[v] = r + v <= t ? weight : 0.0f;
             }
+            Op::put4(pt + t * kPitchP + r, acc);
         }
-        Op::put4(pt + (16 * tt + col) * kPitchP + 16 * ts + quad, acc);
-    }
-    __syncthreads();
-
-    const int4 s = la_sequence(p, e.w);
-    const bool carried = e.y != s.x || p.initial;                    // a state comes in
-    const int da = la_state_dim(p.k.dim), db = la_state_dim(p.v.dim);
-    const E *states = reinterpret_cast<const E *>(p.states) + ((int64_t)c * p.heads + h) * da * db;
-    for (int n = wave; 16 * n < dv; n += 4) {
         floatx4_t acc[kM];
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
         if (carried) {
-            for (int k0 = 0; k0 < dk; k0 += Op::kStep) {
-                const Frag a = Op::rows(states, da, 16 * n, k0, lane);
 #pragma unroll
-                for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::rows(qt, pitch_k, 16 * m, k0, lane), acc[m]);
+            for (int k = 0; k < kTiles / kJoin; ++k) {
+                const Frag a = Op::from_acc(state + k * kJoin);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::rows_acc(qt, kPitchK, 16 * m, k * Op::kStep, lane), acc[m]);
             }
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
                 const float2 g = cum[16 * m + col];
-                acc[m] *= exp2f(g.x + g.y);
+                acc[m] *= fast_exp2(g.x + g.y);
             }
         }
-        if (!bad) {
+        Frag values[kC / Op::kStep];
 #pragma unroll
-            for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-                const Frag a = Op::cols(vt, pitch_v, 16 * n, k0, lane);
+        for (int k = 0; k < kC / Op::kStep; ++k) values[k] = Op::cols(vt, kPitchV, 16 * wave, k * Op::kStep, lane);
+        __syncthreads();
+        if (!bad[i & 1]) {
 #pragma unroll
-                for (int m = k0 / 16; m < kM; ++m) acc[m] = Op::mma(a, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
-            }
+            for (int k = 0; k < kC / Op::kStep; ++k)
+#pragma unroll
+                for (int m = k * Op::kStep / 16; m < kM; ++m) acc[m] = Op::mma(values[k], Op::rows(pt, kPitchP, 16 * m, k * Op::kStep, lane), acc[m]);
         } else {
+            const int t = la_here(col), d = la_here(16 * wave + quad);
 #pragma unroll
             for (int m = 0; m < kM; ++m)
-                for (int r = 0; r <= 16 * m + col; ++r) {
-                    const float weight = to_f32(pt[(16 * m + col) * kPitchP + r]);
+                for (int r = 0; r <= 16 * m + t; ++r) {
+                    const float weight = to_f32(pt[(16 * m + t) * kPitchP + r]);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][v] += weight * to_f32(vt[r * pitch_v + 16 * n + quad + v]);
+                    for (int v = 0; v < 4; ++v) acc[m][v] += weight * to_f32(vt[r * kPitchV + d + v]);
                 }
         }
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
             const int t = 16 * m + col;
-            if (t < e.z) store4(out + (int64_t)t * p.out.token + 16 * n + quad, acc[m] * p.scale, p.v.dim - 16 * n - quad, p.out.aligned);
+            if (t < len) store4(out + (int64_t)(t0 + t) * p.out.token + 16 * wave + quad, acc[m] * p.scale, p.v.dim - v0 - 16 * wave - quad, p.out.aligned);
         }
+        if (i + 1 < here.count || (last && w.to)) {                  // somebody wants the state behind this chunk
+            const float2 end = cum[kC - 1];
+            const float keep = fast_exp2(end.x + end.y);
+#pragma unroll
+            for (int d = 0; d < kTiles; ++d) state[d] *= keep;
+#pragma unroll
+            for (int k = 0; k < kC / Op::kStep; ++k) {
+                Frag parts[kParts];
+                Op::template weigh<kParts>(values[k], weights + k * Op::kStep, lane, parts);
+#pragma unroll
+                for (int d = 0; d < kTiles; ++d) {
+                    const Frag a = Op::cols(kt, kPitchK, 16 * d, k * Op::kStep, lane);
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) state[d] = Op::mma(a, parts[q], state[d]);
+                }
+            }
+        }
+        carried = true;
+        __syncthreads();
+    }
+    if (!w.to || !last) return;
+#pragma unroll
+    for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            if (16 * d + quad + v < p.k.dim && value < p.v.dim) w.to[la_state_at(p, w, n, h, 16 * d + quad + v, value)] = state[d][v];
+}
+
+// Rows of no sequence
+template <typename T> __global__ __launch_bounds__(kBlock) void la_nobody_kernel(const LaArgs p) {
+    const int4 all = p.seqs[p.n_seqs];
+    const int64_t rows = (int64_t)all.x + (p.tokens - all.y), row = (int64_t)p.heads * p.v.dim;
+    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < rows * row; i += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = i / row;
+        reinterpret_cast<T *>(p.out.p)[(r < all.x ? r : all.y + (r - all.x)) * row + (i - r * row)] = from_f32<T>(0.0f);
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
-// Segments: where the sequences alone do not give the chip its workgroups, each is cut so that they do, into eight chunks at least:
-// a segment is walked twice.
-int la_plan(LaArgs &p, int chunk) {
-    const int64_t tiles = (int64_t)((p.k.dim + kLaTile - 1) / kLaTile) * ((p.v.dim + kLaTile - 1) / kLaTile);
-    const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= 512 ? 1 : (1024 + p.heads * tiles - 1) / (p.heads * tiles);
+// Segments: where the sequences alone do not give the chip its workgroups (two to a CU, of `tiles` for a head), each is cut so that they do, into
+// `shortest` chunks at least: a segment is walked twice.
+int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
+    const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= 192 ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk;
     int64_t chunks, segs, seg_chunks;
     if (p.cu) {
         chunks = (int64_t)p.tokens / chunk + p.n_seqs + 2;
         seg_chunks = want == 1 ? per_seq : (per_seq + want - 1) / want;
-        seg_chunks = seg_chunks < 8 ? 8 : seg_chunks;
+        seg_chunks = seg_chunks < shortest ? shortest : seg_chunks;
         segs = per_seq <= seg_chunks ? p.n_seqs : chunks / seg_chunks + p.n_seqs;
     } else {
         chunks = per_seq * p.n_seqs;
         const int64_t each = (want + p.n_seqs - 1) / p.n_seqs;
         seg_chunks = (per_seq + each - 1) / each;
-        seg_chunks = seg_chunks < 8 ? 8 : seg_chunks;
+        seg_chunks = seg_chunks < shortest ? shortest : seg_chunks;
         p.segs_per_seq = per_seq <= seg_chunks ? 1 : (int)((per_seq + seg_chunks - 1) / seg_chunks);
         segs = (int64_t)p.segs_per_seq * p.n_seqs;
     }
-    if (chunks * p.heads > 0x7fffffff / 4 || segs * p.heads * tiles > 0x7fffffff) return SS2D_EINVAL;
+    if (chunks * p.heads > 0x7fffffff / 4 || segs * p.heads * la_tiles(p) > 0x7fffffff / 4) return SS2D_EINVAL;
     p.per_seq = (int)per_seq;
     p.max_chunks = (int)chunks;
     p.seg_chunks = (int)seg_chunks;
@@ -448,22 +567,32 @@ int la_tables(const LaArgs &p, int chunk, void *stream) {
 }
 
 template <typename Op, typename T> static int la_forward(const LaArgs &p, void *stream) {
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     int rc = la_tables(p, Op::kChunk, stream);
     if (rc != SS2D_OK) return rc;
-    // with one chunk to a sequence the states that come in are none, or the initial ones, which the walk lays out
     LaWalk w = {};
     w.a = p.k; w.b = p.v;
-    w.out = p.states;
     w.from = p.initial; w.to = p.final;
     w.from_a = p.v.dim; w.from_b = 1;
-    const bool skip = !p.cu && p.per_seq <= 1 && !p.initial && !p.final;
-    if (!skip && (rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
-    const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
-    if (total == 0) return SS2D_OK;
-    const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, 16), c = Op::kChunk;
-    const size_t bytes = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + dv + Op::kPad + c + Op::kPad) + sizeof(float2) * c;
-    // (up to 104 KB of LDS: this runtime asks for no attribute above 64)
-    la_out_kernel<Op, T><<<total, kBlock, bytes, reinterpret_cast<hipStream_t>(stream)>>>(p, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
+    w.exact = p.final != nullptr;
+    if ((rc = la_segments<Op, T>(p, w, st)) != SS2D_OK) return rc;
+    const uint32_t total = (uint32_t)((int64_t)p.max_segs * p.heads * ((p.v.dim + kLaTile - 1) / kLaTile));
+    auto go = [&](auto kernel, int keys) {
+        constexpr int c = Op::kChunk;
+        const size_t bytes = sizeof(typename Op::E) * c * (2 * (keys + Op::kPad) + kLaTile + Op::kPad + c + Op::kPad) + c * (sizeof(float) + sizeof(float2)) + 16;
+        kernel<<<total, kBlock, bytes, st>>>(p, w, total);           // (up to 88 KB of LDS: this runtime asks for no attribute above 64)
+    };
+    const bool fast = p.q.aligned && p.k.aligned && p.v.aligned;
+    auto sized = [&](auto tiles) {
+        constexpr int kTiles = decltype(tiles)::value, kMost = Op::kMostParts, kLess = kMost < 2 ? kMost : 2;
+        if (w.exact) fast ? go(la_out_kernel<Op, T, kTiles, kMost, true>, 16 * kTiles) : go(la_out_kernel<Op, T, kTiles, kMost, false>, 16 * kTiles);
+        else fast ? go(la_out_kernel<Op, T, kTiles, kLess, true>, 16 * kTiles) : go(la_out_kernel<Op, T, kTiles, kLess, false>, 16 * kTiles);
+    };
+    if (p.k.dim <= 32) sized(std::integral_constant<int, 2>{});
+    else if (p.k.dim <= 64) sized(std::integral_constant<int, 4>{});
+    else if (p.k.dim <= 128) sized(std::integral_constant<int, 8>{});
+    else sized(std::integral_constant<int, 16>{});
+    if (p.cu && p.tokens > 0) la_nobody_kernel<T><<<256, kBlock, 0, st>>>(p);
     return launch_status();
 }
 
@@ -477,9 +606,11 @@ LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int 
     s.batch = batch; s.token = token; s.head = head;
     s.div = own_heads > 0 ? heads / own_heads : 1;
     s.dim = dim;
-    s.aligned = la_aligned(ptr, batch, token, head, bytes, size);
+    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0;
     return s;
 }
+
+int la_chunk(int dtype) { return dtype == SS2D_BF16 ? OperandBf16::kChunk : OperandF32::kChunk; }
 
 // The arguments of a call, checked; *empty where there is nothing to do at all.
 int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) {
@@ -509,17 +640,21 @@ int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) 
     if (a.heads == 0 || a.n_seqs == 0) { empty = true; return SS2D_OK; }
     const bool rows = a.tokens > 0;
     if (rows && (!p->q || !p->k || !p->v)) return SS2D_EINVAL;
-    return la_plan(a, p->dtype == SS2D_BF16 ? OperandBf16::kChunk : OperandF32::kChunk);
+    return SS2D_OK;
+}
+
+static int la_forward_plan(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) {
+    const int rc = la_arguments(p, a, empty);
+    return rc != SS2D_OK || empty ? rc : la_plan(a, la_chunk(p->dtype), (a.v.dim + kLaTile - 1) / kLaTile, 2);
 }
 
 static int64_t la_round(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Lays a call's workspace out from `base` on and says how long it is.  layouts: of states at all, of E across too; halves: 2 where what the rounding
-// of states leaves is kept.
+// Lays a call's workspace out from `base` on and says how long it is.  low: what the rounding of states leaves is kept.
 int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
-    const int chunk = dtype == SS2D_BF16 ? OperandBf16::kChunk : OperandF32::kChunk, size = dtype == SS2D_BF16 ? 2 : 4;
+    const int chunk = la_chunk(dtype), size = dtype == SS2D_BF16 ? 2 : 4;
     const int64_t entries = (int64_t)p.max_chunks * p.heads, state = (int64_t)la_state_dim(p.k.dim) * la_state_dim(p.v.dim);
-    const int64_t tiles = (int64_t)((p.k.dim + kLaTile - 1) / kLaTile) * ((p.v.dim + kLaTile - 1) / kLaTile);
+    const int64_t tiles = la_tiles(p);
     int64_t at = 0;
     auto take = [&](auto *&ptr, int64_t bytes) {
         ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + at);
@@ -529,8 +664,8 @@ int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
     take(p.seqs, p.cu ? sizeof(int4) * ((int64_t)p.n_seqs + 1) : 0);
     take(p.cum, sizeof(float2) * entries * chunk);
     p.low = low ? entries * state : 0;
-    take(p.states, (low ? 2 : 1) * size * entries * state);
     if (backward) {
+        take(p.states, (low ? 2 : 1) * size * entries * state);
         take(p.dstates, (low ? 2 : 1) * size * entries * state);
         take(p.dstates_t, size * entries * state);
     }
@@ -545,7 +680,7 @@ using namespace ss2d;
 extern "C" int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params *params) {
     LaArgs a;
     bool empty;
-    const int rc = la_arguments(params, a, empty);
+    const int rc = la_forward_plan(params, a, empty);
     if (rc != SS2D_OK || empty) return rc;
     return la_carve(a, params->dtype, nullptr, false, false);
 }
@@ -553,7 +688,7 @@ extern "C" int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_atten
 extern "C" int ss2d_linear_attention_fwd(const ss2d_linear_attention_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
     LaArgs a;
     bool empty;
-    const int rc = la_arguments(params, a, empty);
+    const int rc = la_forward_plan(params, a, empty);
     if (rc != SS2D_OK || empty) return rc;
     if (a.tokens > 0 && !params->out) return SS2D_EINVAL;
     if (!workspace || (uintptr_t)workspace % 16 != 0) return SS2D_EINVAL;

@@ -29,8 +29,8 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
 // A workgroup owns a chunk of one head: weights of its pairs to LDS, then 16 columns of dq and dk, and of dv, to a wavefront at a time, as the
 // outputs' kernel does (transposed products, states straight from memory).  kLow: dq's and dk's share of the states with
 // what their rounding to bf16 left, for a decay's gradient in single precision.
-template <typename Op, typename T, bool kLow>
-__global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
+template <typename Op, typename T, bool kLow, bool kFast>
+__global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
     constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad;
@@ -80,12 +80,12 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 divmod(i + j * kBlock, per_row, row[j], at[j]);
-                piece[j] = u32x4_t{0, 0, 0, 0};
-                if ((int)row[j] < e.z) piece[j] = load_piece(src + (int64_t)row[j] * side.token, at[j] * kVec, side.dim, side.aligned);
+                piece[j] = load_piece<kFast>(src, side.token, (int)row[j], e.z, at[j] * kVec, side.dim);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (row[j] < kC) {
+                    piece[j] = held_piece<kFast>(piece[j], (int)row[j] < e.z && (int)at[j] * kVec < side.dim);
                     put_piece<T, E>(tile + row[j] * pitch + at[j] * kVec, piece[j]);
                     bad |= piece_bad<T>(piece[j]);
                 }
@@ -113,10 +113,11 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const float2 gt = cum[t + v];
-                const float decay = exp2f((gt.x - gs.x) + (gt.y - gs.y)) * p.scale;
-                weights[v] = s <= t + v ? weights[v] * decay : 0.0f;
-                product[v] = s < t + v ? weights[v] * through[v] : 0.0f;         // (a pair of one token has no decay between)
-                through[v] = s <= t + v ? through[v] * decay : 0.0f;
+                const float decay = fast_exp2((gt.x - gs.x) + (gt.y - gs.y)) * p.scale, weight = weights[v] * decay, both = weight * through[v],
+                            back = through[v] * decay;
+                weights[v] = s <= t + v ? weight : 0.0f;
+                product[v] = s < t + v ? both : 0.0f;                // (a pair of one token has no decay between)
+                through[v] = s <= t + v ? back : 0.0f;
             }
         }
         Op::put4(pt + s * kPitchP + t, weights);
@@ -152,8 +153,8 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
     for (int m = 0; m < kM; ++m) {
         const float2 g = cum[16 * m + col];
         q_dot[m] = k_dot[m] = 0.0f;
-        in[m] = p.scale * exp2f(g.x + g.y);
-        out[m] = exp2f((end.x - g.x) + (end.y - g.y));
+        in[m] = p.scale * fast_exp2(g.x + g.y);
+        out[m] = fast_exp2((end.x - g.x) + (end.y - g.y));
     }
     for (int n = wave; 16 * n < p.k.dim; n += 4) {
         floatx4_t dq[kM], dkey[kM];
@@ -208,14 +209,15 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
                 }
             }
         } else {                                                     // as in the outputs' kernel: nothing from behind the diagonal
+            const int c0 = la_here(col), d0 = la_here(16 * n + quad);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                const int own = 16 * m + col;
+                const int own = 16 * m + c0;
                 for (int r = 0; r < kC; ++r)
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + 16 * n + quad + v]);
-                        if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + 16 * n + quad + v]);
+                        if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + d0 + v]);
+                        if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + d0 + v]);
                     }
             }
         }
@@ -248,11 +250,12 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
                     if (16 * m < k0 + Op::kStep) acc[m] = Op::mma(o, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
             }
         } else {
+            const int c0 = la_here(col), d0 = la_here(16 * n + quad);
 #pragma unroll
             for (int m = 0; m < kM; ++m)
-                for (int r = 16 * m + col; r < kC; ++r)
+                for (int r = 16 * m + c0; r < kC; ++r)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + col) * kPitchP + r]) * to_f32(ot[r * pitch_v + 16 * n + quad + v]);
+                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + r]) * to_f32(ot[r * pitch_v + d0 + v]);
         }
 #pragma unroll
         for (int m = 0; m < kM; ++m)
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(kBlock) void la_bwd_kernel(const LaArgs p, float *h
         if (lane >= d) before += b;
     }
     const float until_t = __shfl_up(until, 1), before_t = __shfl_up(before, 1);      // (a token's key is not before it)
-    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + exp2f(end.x + end.y) * ((both[0] + both[1]) + (both[2] + both[3]));
+    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + fast_exp2(end.x + end.y) * ((both[0] + both[1]) + (both[2] + both[3]));
     if (head_sums) {
         dg = sum_groups(sum_columns(lane < e.z ? dg : 0.0f));
         if (lane == 0) head_sums[entry] = dg;
@@ -355,6 +358,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (rc != SS2D_OK) return rc;
     LaWalk w = {};
     w.from_a = 1; w.from_b = p.v.dim;
+    w.exact = p.low != 0;
     const bool one = !p.cu && p.per_seq <= 1;                        // a chunk to a sequence: nothing comes in but what the caller gives
     if (!one || p.initial) {
         w.a = p.v; w.b = p.k;
@@ -366,6 +370,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
         w.a = p.dout; w.b = p.q;
         w.out = p.dstates; w.out_t = p.dstates_t; w.low = p.low;
         w.from = p.dfinal; w.to = dinitial;
+        if (dinitial) w.exact = 1;
         w.reverse = 1;
         if ((rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
     }
@@ -379,8 +384,11 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
             kernel<<<total, kBlock, bytes, st>>>(p, b.head_sums, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
             return launch_status();
         };
-        if constexpr (sizeof(typename Op::E) == 2) rc = b.low ? go(la_bwd_kernel<Op, T, true>) : go(la_bwd_kernel<Op, T, false>);
-        else rc = go(la_bwd_kernel<Op, T, false>);
+        const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
+        if (sizeof(typename Op::E) == 2 && b.low) {
+            constexpr bool kLow = sizeof(typename Op::E) == 2;
+            rc = fast ? go(la_bwd_kernel<Op, T, kLow, true>) : go(la_bwd_kernel<Op, T, kLow, false>);
+        } else rc = fast ? go(la_bwd_kernel<Op, T, false, true>) : go(la_bwd_kernel<Op, T, false, false>);
         if (rc != SS2D_OK) return rc;
         auto sum = [&](const LaSide &side, void *out) {
             if (side.div <= 1) return;
@@ -397,6 +405,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
 
 LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size, int bytes);
 int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty);
+int la_chunk(int dtype);
 int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low);
 
 // Everything of a backward call, its workspace laid out from `base` on; the bytes that takes, or a status.
@@ -407,6 +416,8 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
     const int rc = la_arguments(&f, b.a, empty);
     if (rc != SS2D_OK || empty) return rc;
     LaArgs &a = b.a;
+    const int planned = la_plan(a, la_chunk(f.dtype), (int64_t)((f.key_dim + kLaTile - 1) / kLaTile) * ((f.value_dim + kLaTile - 1) / kLaTile), 8);
+    if (planned != SS2D_OK) return planned;
     const int size = f.dtype == SS2D_F32 ? 4 : 2;
     if (params->ddecay && !f.decay) return SS2D_EINVAL;
     b.low = f.dtype == SS2D_BF16 && params->ddecay && f.decay_dtype == SS2D_F32;

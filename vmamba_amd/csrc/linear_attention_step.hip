@@ -43,12 +43,9 @@ __global__ __launch_bounds__(kBlock) void la_step_kernel(const LaStepArgs p, int
         v[i] = in ? to_f32(reinterpret_cast<const T *>(p.v.p)[b * p.v.batch + (int64_t)(h / p.v.div) * p.v.head + c + i]) : 0.0f;
         sum[i] = 0.0f;
     }
-    auto fetch = [&](int r0, vec_t (&s)[kStepRows]) {
+    auto fetch = [&](int r0, vec_t (&s)[kStepRows]) {                // (rows past the last repeat it, columns past theirs the first; nobody stores them)
 #pragma unroll
-        for (int i = 0; i < kStepRows; ++i) {
-            const int r = r0 + slot + i * kSlots;
-            if (in && r < dk) s[i] = *reinterpret_cast<const vec_t *>(state + (int64_t)r * dv);
-        }
+        for (int i = 0; i < kStepRows; ++i) s[i] = load_streaming(reinterpret_cast<const vec_t *>(state + (in ? 0 : -c) + (int64_t)min(r0 + slot + i * kSlots, dk - 1) * dv));
     };
     vec_t s[kStepRows];
     fetch(0, s);
@@ -58,9 +55,10 @@ __global__ __launch_bounds__(kBlock) void la_step_kernel(const LaStepArgs p, int
 #pragma unroll
         for (int i = 0; i < kStepRows; ++i) {
             const int r = r0 + slot + i * kSlots;
+            const float key = r < dk ? ks[r] : 0.0f;
+            s[i] = s[i] * decay + v * key;
             if (in && r < dk) {
-                s[i] = s[i] * decay + v * ks[r];
-                *reinterpret_cast<vec_t *>(state + (int64_t)r * dv) = s[i];
+                store_streaming(reinterpret_cast<vec_t *>(state + (int64_t)r * dv), s[i]);
                 sum += s[i] * qs[r];
             }
         }

@@ -12,7 +12,7 @@ namespace ss2d {
 
 constexpr int kQnMaxDim = 512;       // 64 lanes x 8
 constexpr int kQnTokens = 16;        // of one round of a workgroup, at most
-constexpr int kQnPairs = 4096;       // angles in LDS
+constexpr int kQnPairs = 1024;       // angles in LDS
 
 struct QnSide {
     const void *x, *dy;              // (batch, token, head, dim) by strides, the last dimension dense
@@ -30,6 +30,7 @@ struct QnArgs {
     int32_t pos64, freq64, axes, per_axis, pairs;                    // pairs = axes * per_axis
     int32_t batch, tokens, dim, w_dtype, interleaved, round, has_w;  // round: tokens of a workgroup's round
     int64_t rounds;
+    FastDiv by_heads, by_pairs;
     float eps;
     float *partial;                  // backward: [workgroup][side][dim]
 };
@@ -39,16 +40,17 @@ __device__ __forceinline__ float qn_weight(const void *w, int at, int dtype) {
                      : dtype == SS2D_BF16 ? to_f32(reinterpret_cast<const bf16_t *>(w)[at]) : to_f32(reinterpret_cast<const f16_t *>(w)[at]);
 }
 
-// (cos, sin) of one pair of a token
-__device__ __forceinline__ float2 qn_angle(const QnArgs &p, int64_t token, int pair) {
-    const int64_t b = token / p.tokens, t = token - b * p.tokens;
-    const int axis = pair / p.per_axis;
+// (cos, sin) of one pair of a token.  For results in 16 bits the hardware's sine and cosine of a part of a turn do: off by 1.3e-7 at most.
+template <typename T> __device__ __forceinline__ float2 qn_angle(const QnArgs &p, int b, int t, int pair) {
+    const int axis = p.axes == 1 ? 0 : pair / p.per_axis;
     const int64_t at = b * p.pos_batch + t * p.pos_token + axis * p.pos_axis;
     const double pos = p.pos64 ? (double)reinterpret_cast<const int64_t *>(p.positions)[at] : (double)reinterpret_cast<const int32_t *>(p.positions)[at];
     const double f = p.freq64 ? reinterpret_cast<const double *>(p.frequencies)[pair] : (double)reinterpret_cast<const float *>(p.frequencies)[pair];
     const double turns = pos * f * 0.15915494309189535;              // 1 / (2 pi)
+    const float part = (float)(turns - rint(turns));
+    if constexpr (sizeof(T) == 2) return make_float2(__builtin_amdgcn_cosf(part), __builtin_amdgcn_sinf(part));
     float s, c;
-    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+    sincospif(2.0f * part, &s, &c);
     return make_float2(c, s);
 }
 
@@ -92,7 +94,7 @@ template <int kLanes> __device__ __forceinline__ float qn_sum(float v) {
 // kLanes lanes to a row.  A workgroup takes rounds of p.round tokens, all heads of both sides.
 template <typename T, int kLanes, bool kBack>
 __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) {
-    constexpr int kSlots = kBlock / kLanes;
+    constexpr int kSlots = kBlock / kLanes, kAhead = kBack ? 2 : 4;
     __shared__ float2 angles[kQnPairs];
     __shared__ float sums[kBack ? kBlock * 8 : 1];
     const int tid = threadIdx.x, slot = tid / kLanes, unit = tid % kLanes;
@@ -112,59 +114,86 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
     for (int64_t round = blockIdx.x; round < p.rounds; round += gridDim.x) {
         const int64_t token0 = round * p.round;
         const int n_tokens = (int)(all - token0 < p.round ? all - token0 : p.round), rows = n_tokens * heads;
+        const int b0 = (int)(token0 / p.tokens), t0 = (int)(token0 - (int64_t)b0 * p.tokens);
+        auto place = [&](int t, int &b, int &at) {                   // the round's t-th token
+            b = b0;
+            at = t0 + t;
+            while (at >= p.tokens) { at -= p.tokens; ++b; }
+        };
         if (p.positions) {
             if (round != blockIdx.x) __syncthreads();
-            for (int i = tid; i < n_tokens * p.pairs; i += kBlock) angles[i] = qn_angle(p, token0 + i / p.pairs, i % p.pairs);
+            for (int i = tid; i < n_tokens * p.pairs; i += kBlock) {
+                uint32_t t, pair;
+                int b, at;
+                divmod((uint32_t)i, p.by_pairs, t, pair);
+                place((int)t, b, at);
+                angles[i] = qn_angle<T>(p, b, at, (int)pair);
+            }
             __syncthreads();
         }
-        for (int row = slot; row < rows; row += kSlots) {            // (a row's lanes are together here)
-            const int t = row / heads, h = row - t * heads;
-            const bool key = h >= p.side[0].heads;
-            const QnSide &s = p.side[key];
-            const int head = key ? h - p.side[0].heads : h;
-            const int64_t token = token0 + t, b = token / p.tokens, tt = token - b * p.tokens;
-            const T *x = reinterpret_cast<const T *>(s.x) + b * s.batch + tt * s.token + head * s.head;
-            float v[8], d[8];
+        // kAhead rows of a lane on their way at once (a row's lanes are together here); past the last row that one again
+        for (int row0 = slot; row0 < rows; row0 += kAhead * kSlots) {
+            float v[kAhead][8], d[kBack ? kAhead : 1][8];
+            T *to[kAhead];
+            bool key[kAhead];
+            int token[kAhead];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = d[i] = 0.0f;
-            if (in) {
-                qn_load4(x + first, v);
-                qn_load4(x + second, v + 4);
+            for (int a = 0; a < kAhead; ++a) {
+                uint32_t t, h;
+                int b, at;
+                divmod((uint32_t)min(row0 + a * kSlots, rows - 1), p.by_heads, t, h);
+                place((int)t, b, at);
+                key[a] = (int)h >= p.side[0].heads;
+                const QnSide &s = p.side[key[a]];
+                const int head = key[a] ? (int)h - p.side[0].heads : (int)h;
+                const T *x = reinterpret_cast<const T *>(s.x) + b * s.batch + at * s.token + head * s.head;
+                token[a] = (int)t;
+                to[a] = reinterpret_cast<T *>(s.y) + ((token0 + t) * s.heads + head) * p.dim;
+                qn_load4(x + (in ? first : 0), v[a]);
+                qn_load4(x + (in ? second : 4), v[a] + 4);
                 if constexpr (kBack) {
-                    const T *dy = reinterpret_cast<const T *>(s.dy) + b * s.dy_batch + tt * s.dy_token + head * s.dy_head;
-                    qn_load4(dy + first, d);
-                    qn_load4(dy + second, d + 4);
+                    const T *dy = reinterpret_cast<const T *>(s.dy) + b * s.dy_batch + at * s.dy_token + head * s.dy_head;
+                    qn_load4(dy + (in ? first : 0), d[a]);
+                    qn_load4(dy + (in ? second : 4), d[a] + 4);
                 }
             }
-            float q = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
-            const float r = rsqrtf(qn_sum<kLanes>(q) * inv_d + p.eps);
-            const float2 *cs = angles + t * p.pairs + 4 * unit;
-            if constexpr (!kBack) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * r * (key ? w[1][i] : w[0][i]);
-                if (turned) qn_turn8(v, cs, p.interleaved, false);
-            } else {
-                if (turned) qn_turn8(d, cs, p.interleaved, true);
-                float m = 0.0f;
+            for (int a = 0; a < kAhead; ++a) {
+                const bool live = in && row0 + a * kSlots < rows;
+                float q = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    v[i] *= r;
-                    const float g = d[i] * v[i];
-                    dw[0][i] += key ? 0.0f : g;
-                    dw[1][i] += key ? g : 0.0f;
-                    d[i] *= key ? w[1][i] : w[0][i];
-                    m = fmaf(d[i], v[i], m);
+                    v[a][i] = in ? v[a][i] : 0.0f;
+                    q = fmaf(v[a][i], v[a][i], q);
                 }
-                m = qn_sum<kLanes>(m) * inv_d;
+                const float r = rsqrtf(qn_sum<kLanes>(q) * inv_d + p.eps);
+                const float2 *cs = angles + token[a] * p.pairs + 4 * unit;
+                if constexpr (!kBack) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = (d[i] - v[i] * m) * r;
-            }
-            if (in) {
-                T *y = reinterpret_cast<T *>(s.y) + (token * s.heads + head) * p.dim;
-                qn_store4(y + first, v);
-                qn_store4(y + second, v + 4);
+                    for (int i = 0; i < 8; ++i) v[a][i] = v[a][i] * r * (key[a] ? w[1][i] : w[0][i]);
+                    if (turned) qn_turn8(v[a], cs, p.interleaved, false);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[a][i] = live ? d[a][i] : 0.0f;
+                    if (turned) qn_turn8(d[a], cs, p.interleaved, true);
+                    float m = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[a][i] *= r;
+                        const float g = live ? d[a][i] * v[a][i] : 0.0f;
+                        dw[0][i] += key[a] ? 0.0f : g;
+                        dw[1][i] += key[a] ? g : 0.0f;
+                        d[a][i] *= key[a] ? w[1][i] : w[0][i];
+                        m = fmaf(d[a][i], v[a][i], m);
+                    }
+                    m = qn_sum<kLanes>(m) * inv_d;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[a][i] = (d[a][i] - v[a][i] * m) * r;
+                }
+                if (live) {
+                    qn_store4(to[a] + first, v[a]);
+                    qn_store4(to[a] + second, v[a] + 4);
+                }
             }
         }
     }
@@ -211,7 +240,10 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_any_kernel(const QnArgs
         const int n_tokens = (int)(all - token0 < p.round ? all - token0 : p.round), rows = n_tokens * heads;
         if (p.positions) {
             if (round != blockIdx.x) __syncthreads();
-            for (int i = tid; i < n_tokens * p.pairs; i += kBlock) angles[i] = qn_angle(p, token0 + i / p.pairs, i % p.pairs);
+            for (int i = tid; i < n_tokens * p.pairs; i += kBlock) {
+                const int64_t token = token0 + i / p.pairs, b = token / p.tokens;
+                angles[i] = qn_angle<T>(p, (int)b, (int)(token - b * p.tokens), i % p.pairs);
+            }
             __syncthreads();
         }
         for (int row = slot; row < rows; row += kSlots) {
@@ -292,23 +324,26 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_any_kernel(const QnArgs
     }
 }
 
-// The workgroups' sums of the weights' gradients: 32 columns to a workgroup, an eighth of the shares to each of its 8 slots
-__global__ __launch_bounds__(kBlock) void qn_weights_kernel(const float *partial, void *dqw, void *dkw, int shares, int dim, int dtype) {
-    __shared__ float sums[8][32];
-    const int slot = threadIdx.x / 32, col = blockIdx.x * 32 + threadIdx.x % 32;
+// The workgroups' sums of the weights' gradients: 16 columns to a workgroup, the shares dealt out to its 64 slots
+__global__ __launch_bounds__(1024) void qn_weights_kernel(const float *partial, void *dqw, void *dkw, int shares, int dim, int dtype) {
+    __shared__ float sums[64][17];
+    const int slot = threadIdx.x / 16, at = threadIdx.x % 16, col = blockIdx.x * 16 + at, safe = min(col, 2 * dim - 1);
     float total = 0.0f;
-    if (col < 2 * dim)
-        for (int s = slot; s < shares; s += 8) total += partial[(int64_t)s * 2 * dim + col];
-    sums[slot][threadIdx.x % 32] = total;
-    __syncthreads();
+#pragma unroll 4
+    for (int s = slot; s < shares; s += 64) total += partial[(int64_t)s * 2 * dim + safe];
+    sums[slot][at] = total;
+    for (int d = 32; d >= 1; d /= 2) {
+        __syncthreads();
+        if (slot < d) sums[slot][at] += sums[slot + d][at];
+    }
     if (slot != 0 || col >= 2 * dim) return;
-    for (int s = 1; s < 8; ++s) total += sums[s][threadIdx.x % 32];
+    total = sums[0][at];
     void *out = col < dim ? dqw : dkw;
-    const int at = col < dim ? col : col - dim;
+    const int place = col < dim ? col : col - dim;
     if (!out) return;
-    if (dtype == SS2D_F32) reinterpret_cast<float *>(out)[at] = total;
-    else if (dtype == SS2D_BF16) reinterpret_cast<bf16_t *>(out)[at] = from_f32<bf16_t>(total);
-    else reinterpret_cast<f16_t *>(out)[at] = from_f32<f16_t>(total);
+    if (dtype == SS2D_F32) reinterpret_cast<float *>(out)[place] = total;
+    else if (dtype == SS2D_BF16) reinterpret_cast<bf16_t *>(out)[place] = from_f32<bf16_t>(total);
+    else reinterpret_cast<f16_t *>(out)[place] = from_f32<f16_t>(total);
 }
 
 static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &vec, bool back, const ss2d_qk_norm_rotate_bwd_params *g) {
@@ -351,6 +386,8 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
     if (a.pairs > 0 && round > kQnPairs / a.pairs) round = kQnPairs / a.pairs;
     while (round > 1 && all / round < 1024) round /= 2;
     a.round = (int)round;
+    a.by_heads = make_fastdiv((uint32_t)(heads > 0 ? heads : 1));
+    a.by_pairs = make_fastdiv((uint32_t)(a.pairs > 0 ? a.pairs : 1));
     a.rounds = all > 0 && heads > 0 ? (all + round - 1) / round : 0;
     return SS2D_OK;
 }
@@ -414,6 +451,6 @@ extern "C" int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *g, 
         }
         if (status != SS2D_OK) return status;
     }
-    if (weights) qn_weights_kernel<<<(2 * p->dim + 31) / 32, kBlock, 0, st>>>(a.partial, g->dq_weight, g->dk_weight, (int)grid, p->dim, p->weight_dtype);
+    if (weights) qn_weights_kernel<<<(2 * p->dim + 15) / 16, 1024, 0, st>>>(a.partial, g->dq_weight, g->dk_weight, (int)grid, p->dim, p->weight_dtype);
     return launch_status();
 }
