@@ -13,8 +13,6 @@
 // result is kept in 32 bits (states, single precision decays' gradients).  fp16 and fp32 go to the fp32 matrix cores: the states' and
 // weights' range is not fp16's.
 #pragma once
-#include <float.h>
-
 #include "ss2d_common.h"
 
 namespace ss2d {
@@ -28,7 +26,7 @@ struct LaSide {                      // q, k, v, out or a gradient: (batch, toke
     int64_t batch, token, head;      // strides in elements
     int32_t div;                     // heads of the state to one of this
     int32_t dim;
-    int32_t aligned;                 // base and strides are multiples of 16 bytes (outputs: of four values), and rows of whole pieces
+    int32_t aligned;                 // base and strides are multiples of 16 bytes (outputs: of four values), and rows of whole pieces, at strides below 2^24 bytes
 };
 
 struct LaArgs {
@@ -73,10 +71,12 @@ struct OperandF32 {
         return c;
     }
     static __device__ __forceinline__ void put4(E *p, floatx4_t v) { *reinterpret_cast<floatx4_t *>(p) = v; }
-    // Accumulators of kStep rows (the sum's) as an operand of the next product, and rows() in the order of k that this gives
-    static __device__ __forceinline__ Frag from_acc(const floatx4_t *acc) { return acc[0]; }
-    static __device__ __forceinline__ Frag rows_acc(const E *tile, int pitch, int row0, int k0, int lane) { return rows(tile, pitch, row0, k0, lane); }
-    // The operand's values times their tokens' weights (weight: of token k0 on), in kParts operands whose sum it is
+    // Where a product sums over rows of a tile (cols()), what rows() reads against it stands in cols()'s order of k: place() of k inside the row,
+    // put4_places() four neighbours from a multiple of 4 on.
+    static __device__ __forceinline__ int place(int k) { return k; }
+    static __device__ __forceinline__ void put4_places(E *row, int k, floatx4_t v) { put4(row + k, v); }
+    static __device__ __forceinline__ Frag in_places(Frag f) { return f; }          // of rows() that stand as they are
+    // The operand's values times their tokens' weights (weight: of token k0 on, in places), in kParts operands whose sum it is
     static constexpr int kMostParts = 1;
     template <int kParts> static __device__ __forceinline__ void weigh(Frag f, const float *weight, int lane, Frag (&parts)[kParts]) {
         parts[0] = f * *reinterpret_cast<const floatx4_t *>(weight + 4 * (lane >> 4));
@@ -90,30 +90,33 @@ struct OperandBf16 {
     static __device__ __forceinline__ Frag rows(const E *tile, int pitch, int row0, int k0, int lane) {
         return *reinterpret_cast<const Frag *>(tile + (row0 + (lane & 15)) * pitch + k0 + 8 * (lane >> 4));
     }
-    // ds_read_b64_tr_b16: of the four rows that a group of 16 lanes names, 8 bytes to a lane, a lane gets its column
+    // ds_read_b64_tr_b16: of the four rows that a group of 16 lanes names, 8 bytes to a lane, a lane gets its column.  A group takes the even rows of
+    // eight, then the odd ones: at these tiles' pitches (36 and 68 dwords, modulo 64) four neighbouring rows would share banks.
     static __device__ __forceinline__ Frag cols(const E *tile, int pitch, int col0, int k0, int lane) {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         using Lds = __attribute__((address_space(3))) s16x4;
-        const E *p = tile + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * pitch + col0 + 4 * (lane & 3);
+        const E *p = tile + (k0 + 8 * (lane >> 4) + 2 * ((lane & 15) >> 2)) * pitch + col0 + 4 * (lane & 3);
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)p));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(p + 4 * pitch)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds *)(p + pitch)));
         return Frag{lo[0], lo[1], hi[0], hi[1]};
+    }
+    static __device__ __forceinline__ int place(int k) { return (k & ~7) + 4 * (k & 1) + ((k & 7) >> 1); }
+    static __device__ __forceinline__ void put4_places(E *row, int k, floatx4_t v) {
+        uint32_t *p = reinterpret_cast<uint32_t *>(row + (k & ~7) + ((k & 4) >> 1));
+        p[0] = pack2_from_f32<bf16_t>(v[0], v[2]);
+        p[2] = pack2_from_f32<bf16_t>(v[1], v[3]);
+    }
+    static __device__ __forceinline__ Frag in_places(Frag f) {
+        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;  // of two dwords the low halves, the high ones
+        return Frag{__builtin_amdgcn_perm(f[1], f[0], kLow), __builtin_amdgcn_perm(f[3], f[2], kLow), __builtin_amdgcn_perm(f[1], f[0], kHigh),
+                    __builtin_amdgcn_perm(f[3], f[2], kHigh)};
     }
     static __device__ __forceinline__ floatx4_t mma(Frag a, Frag b, floatx4_t c) { return mfma_16x16x32(bf16_t{}, a, b, c); }
     static __device__ __forceinline__ void put4(E *p, floatx4_t v) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_from_f32<bf16_t>(v[0], v[1]), pack2_from_f32<bf16_t>(v[2], v[3]));
     }
-    static __device__ __forceinline__ Frag from_acc(const floatx4_t *acc) {
-        return Frag{pack2_from_f32<bf16_t>(acc[0][0], acc[0][1]), pack2_from_f32<bf16_t>(acc[0][2], acc[0][3]), pack2_from_f32<bf16_t>(acc[1][0], acc[1][1]),
-                    pack2_from_f32<bf16_t>(acc[1][2], acc[1][3])};
-    }
-    static __device__ __forceinline__ Frag rows_acc(const E *tile, int pitch, int row0, int k0, int lane) {
-        const E *p = tile + (row0 + (lane & 15)) * pitch + k0 + 4 * (lane >> 4);
-        const uint2 lo = *reinterpret_cast<const uint2 *>(p), hi = *reinterpret_cast<const uint2 *>(p + 16);
-        return Frag{lo.x, lo.y, hi.x, hi.y};
-    }
-    // (bf16 of the value, of what that left, and of what that left: 24 bits)
+    // (bf16 of the value, of what that left, and of what that left: 24 bits.  Of an infinity it is NaN that is left: a state with one is of no use.)
     static constexpr int kMostParts = 3;
     template <int kParts> static __device__ __forceinline__ void weigh(Frag f, const float *weight, int lane, Frag (&parts)[kParts]) {
         const floatx4_t w[2] = {*reinterpret_cast<const floatx4_t *>(weight + 8 * (lane >> 4)), *reinterpret_cast<const floatx4_t *>(weight + 8 * (lane >> 4) + 4)};
@@ -124,10 +127,8 @@ struct OperandBf16 {
             for (int k = 0; k < kParts; ++k) {
                 parts[k][i] = pack2_from_f32<bf16_t>(x, y);
                 if (k + 1 == kParts) break;
-                const float xh = unpack_lo<bf16_t>(parts[k][i]), yh = unpack_hi<bf16_t>(parts[k][i]);
-                const float xl = x - xh, yl = y - yh;
-                x = fabsf(xh) <= FLT_MAX ? xl : 0.0f;
-                y = fabsf(yh) <= FLT_MAX ? yl : 0.0f;
+                x -= unpack_lo<bf16_t>(parts[k][i]);
+                y -= unpack_hi<bf16_t>(parts[k][i]);
             }
         }
     }
@@ -136,11 +137,14 @@ struct OperandBf16 {
 // ---- tiles ------------------------------------------------------------------------------------------------------------------------
 template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 
-// 16 bytes' worth of row `row` of `rows` (one at least), from column c on.  kFast: the side is aligned and its dimension a multiple of a piece; the load
-// is then unconditional -- a row or column that is not there repeats another -- so that nothing waits for it before it is used, and held_piece() makes
-// zeros of it there.  Otherwise element by element, zeros for what is not there.
+// 16 bytes' worth of row `row` of `rows` (one at least), from column c on.  kFast: the side is aligned, its dimension a multiple of a piece and a chunk's
+// offsets fit 32 bits; the load is then unconditional -- a row or column that is not there repeats another -- so that nothing waits for it before
+// it is used, and held_piece() makes zeros of it there.  Otherwise element by element, zeros for what is not there.
 template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(const T *base, int64_t stride, int row, int rows, int c, int cols) {
-    if constexpr (kFast) return *reinterpret_cast<const u32x4_t *>(base + min(row, rows - 1) * stride + (c < cols ? c : 0));
+    if constexpr (kFast) {
+        const uint32_t at = (uint32_t)min(row, rows - 1) * (uint32_t)stride + (uint32_t)(c < cols ? c : 0);
+        return *reinterpret_cast<const u32x4_t *>(reinterpret_cast<const char *>(base) + at * (uint32_t)sizeof(T));
+    }
     union { T e[kVecOf<T>]; u32x4_t w; } u;
     u.w = u32x4_t{0, 0, 0, 0};
     if (row < rows)

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
             put_piece<T, E>(at + row * kPitch + col, held_piece<kFast>(ra[j], row < len && col < w.a.dim - a0));
             put_piece<T, E>(bt + row * kPitch + col, held_piece<kFast>(rb[j], row < len && col < w.b.dim - b0));
         }
-        if (tid < kC) weights[tid] = weight;
+        if (tid < kC) weights[Op::place(tid)] = weight;
         const float keep = decay;
         __syncthreads();
         if (i + 1 < here.count) fetch(i + 1);
@@ -217,10 +217,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
                         if (j < left) {
                             floatx4_t rest;
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) {
-                                const float high = to_f32(from_f32<bf16_t>(acc[j][v])), under = acc[j][v] - high;
-                                rest[v] = fabsf(high) <= FLT_MAX ? under : 0.0f;
-                            }
+                            for (int v = 0; v < 4; ++v) rest[v] = acc[j][v] - to_f32(from_f32<bf16_t>(acc[j][v]));
                             Op::put4(out + (int64_t)16 * j * da + w.low, rest);
                         }
                 if (w.out_t)
@@ -235,14 +232,16 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
         for (int j = 0; j < 4; ++j) acc[j] *= keep;
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-            Frag fa[kParts];
+            Frag fa[kParts], fb[4];
             Op::template weigh<kParts>(Op::cols(at, kPitch, 16 * wave, k0, lane), weights + k0, lane, fa);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const Frag fb = Op::cols(bt, kPitch, 16 * j, k0, lane);
-#pragma unroll
-                for (int q = 0; q < kParts; ++q) acc[j] = Op::mma(fa[q], fb, acc[j]);
+                fb[j] = Op::cols(bt, kPitch, 16 * j, k0, lane);
             }
+#pragma unroll
+            for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = Op::mma(fa[q], fb[j], acc[j]);
         }
         __syncthreads();
     }
@@ -329,117 +328,141 @@ template int la_walk<OperandF32, f16_t>(const LaArgs &, const LaWalk &, void *);
 template int la_walk<OperandBf16, bf16_t>(const LaArgs &, const LaWalk &, void *);
 
 // ---- outputs -----------------------------------------------------------------------------------------------------------------------
-// A workgroup owns 64 values' columns of one head and walks a segment of chunks: the state stays in accumulators, 16 columns for all kTiles * 16 keys
-// to a wavefront, and is turned into an operand of the outputs' product where it lies (an accumulator's rows are the next product's sum).
-// Nothing but q, k, v and the outputs passes through memory.  Per chunk: weights of its pairs, 16 tokens to a wavefront, through LDS; out = state and
-// pairs; then the state with the chunk's keys and weighted values.  Products come out transposed (lane: one token, four
-// neighbouring values), so that what a token has to be multiplied with is one value of the lane.
+// A workgroup owns 64 values' columns of one head and walks a segment of chunks with their states, so that nothing but q, k, v and the outputs passes
+// through memory.  Its eight wavefronts are two to 16 columns: of a chunk's outputs each makes half of the tokens', of the state (in
+// accumulators, 32 bits) half of the keys', and the state as an operand goes from one to the other through LDS.  Per chunk: weights of its pairs,
+// 16 x 16 tokens to a wavefront at a time, through LDS; out = state and pairs; then the state with the chunk's keys and weighted values.  Products come
+// out transposed (lane: one token, four neighbouring values), so that what a token has to be multiplied with is one value of the lane.
 // The weights behind the diagonal are zeros; a product of zero with what is infinite or NaN would reach tokens in front of it, so a
 // chunk that holds such a value sums its pairs one by one.
+constexpr int kLaThreads = 512, kLaWaves = kLaThreads / kWave;
+
 template <typename Op, typename T, int kTiles, int kParts, bool kFast>
-__global__ __launch_bounds__(kBlock, 2) void la_out_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
+__global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
     constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kKeys = 16 * kTiles, kPitchK = kKeys + Op::kPad, kPitchV = kLaTile + Op::kPad, kPitchP = kC + Op::kPad;
-    constexpr int kPerKey = kKeys / kVec, kPerValue = kLaTile / kVec, kNk = (kC * kPerKey + kBlock - 1) / kBlock, kNv = kC * kPerValue / kBlock;
-    constexpr int kJoin = Op::kStep / 16;                            // accumulators to an operand
+    constexpr int kPerKey = kKeys / kVec, kPerValue = kLaTile / kVec, kNk = (kC * kPerKey + kLaThreads - 1) / kLaThreads, kNv = (kC * kPerValue + kLaThreads - 1) / kLaThreads;
+    constexpr int kHalfM = kM / 2, kHalf = kTiles / 2, kSteps = kC / Op::kStep, kPairTiles = kM * (kM + 1) / 2;
     extern __shared__ __align__(16) char lds[];
-    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * kPitchK, *vt = kt + kC * kPitchK, *pt = vt + kC * kPitchV;
+    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * kPitchK, *st = kt + kC * kPitchK, *vt = st + kLaTile * kPitchK, *pt = vt + kC * kPitchV;
     float *weights = reinterpret_cast<float *>(pt + kC * kPitchP);   // of a token's value in the state behind the chunk
     float2 *cum = reinterpret_cast<float2 *>(weights + kC);
     int *bad = reinterpret_cast<int *>(cum + kC);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
+    const int mine = wave % 4, half = wave / 4;                      // columns 16 mine .., tokens and keys of this half
     const int tiles = (p.v.dim + kLaTile - 1) / kLaTile;
     LaPlace here;
     if (!la_place(p, xcd_contiguous_id(blockIdx.x, total), tiles, kC, here)) return;
     const int v0 = here.tile * kLaTile, h = here.h, n = here.n;
     const int4 s = here.s;
-    const bool lone = here.chunks <= p.seg_chunks, last = here.begin + here.count >= here.chunks;
+    const bool lone = here.chunks <= p.seg_chunks, last = here.begin + here.count >= here.chunks, live = v0 + 16 * mine < p.v.dim;
     const int64_t b = p.cu ? 0 : n;
     const T *pq = reinterpret_cast<const T *>(p.q.p) + b * p.q.batch + (int64_t)(h / p.q.div) * p.q.head;
     const T *pk = reinterpret_cast<const T *>(p.k.p) + b * p.k.batch + (int64_t)(h / p.k.div) * p.k.head;
     const T *pv = reinterpret_cast<const T *>(p.v.p) + b * p.v.batch + (int64_t)(h / p.v.div) * p.v.head + v0;
-    T *out = reinterpret_cast<T *>(p.out.p) + b * p.out.batch + (int64_t)h * p.out.head + v0;
-
-    floatx4_t state[kTiles];                                         // key 16 d + quad + v, value v0 + 16 wave + col
-    const int value = v0 + 16 * wave + col;
-    const int tiles_a = (p.k.dim + kLaTile - 1) / kLaTile;
-#pragma unroll
-    for (int d = 0; d < kTiles; ++d) {
-        state[d] = floatx4_t{0, 0, 0, 0};
-        if (!lone) {
-            if (d / 4 < tiles_a)
-                state[d] = *reinterpret_cast<const floatx4_t *>(p.local + (((int64_t)here.seg * p.heads + h) * tiles_a * tiles + here.tile * tiles_a + d / 4) * (kLaTile * kLaTile) +
-                                                                wave * 4 * kBlock + 4 * (d % 4 * kWave + lane));
-        } else if (w.from)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-                if (16 * d + quad + v < p.k.dim && value < p.v.dim) state[d][v] = w.from[la_state_at(p, w, n, h, 16 * d + quad + v, value)];
-    }
-    bool carried = here.begin > 0 || w.from;                         // a state has come in
+    T *out = reinterpret_cast<T *>(p.out.p) + b * p.out.batch + (s.x + (int64_t)here.begin * kC) * p.out.token + (int64_t)h * p.out.head + v0 + 16 * mine + quad;
+    pq += (s.x + (int64_t)here.begin * kC) * p.q.token;              // (these walk along: of the next chunk to be fetched)
+    pk += (s.x + (int64_t)here.begin * kC) * p.k.token;
+    pv += (s.x + (int64_t)here.begin * kC) * p.v.token;
+    const float2 *pc = p.cum + ((int64_t)(s.z + here.begin) * p.heads + h) * kC;
+    const int ms[2] = {half ? kM / 4 + (kM < 4) : 0, half ? kM / 2 : kM - 1};        // its tokens: of the four 16s the first and the last, or the others
 
     u32x4_t rq[kNk], rk[kNk], rv[kNv];
     float2 rc = make_float2(0.0f, 0.0f), re = rc;
     auto fetch = [&](int i) {
-        const int c = here.begin + i, t0 = s.x + c * kC, len = min(kC, s.y - t0);
+        const int len = min(kC, s.y - s.x - (here.begin + i) * kC);
 #pragma unroll
         for (int j = 0; j < kNk; ++j) {
-            const int at = tid + j * kBlock, row = at / kPerKey, d = at % kPerKey * kVec;
-            rq[j] = load_piece<kFast>(pq + (int64_t)t0 * p.q.token, p.q.token, row, len, d, p.k.dim);
-            rk[j] = load_piece<kFast>(pk + (int64_t)t0 * p.k.token, p.k.token, row, len, d, p.k.dim);
+            const int at = tid + j * kLaThreads, row = at / kPerKey, d = at % kPerKey * kVec;
+            rq[j] = load_piece<kFast>(pq, p.q.token, row, len, d, p.k.dim);
+            rk[j] = load_piece<kFast>(pk, p.k.token, row, len, d, p.k.dim);
         }
 #pragma unroll
         for (int j = 0; j < kNv; ++j) {
-            const int at = tid + j * kBlock, row = at / kPerValue, d = at % kPerValue * kVec;
-            rv[j] = load_piece<kFast>(pv + (int64_t)t0 * p.v.token, p.v.token, row, len, d, p.v.dim - v0);
+            const int at = tid + j * kLaThreads, row = at / kPerValue, d = at % kPerValue * kVec;
+            rv[j] = load_piece<kFast>(pv, p.v.token, row, len, d, p.v.dim - v0);
         }
         if (tid < kC) {
-            const float2 *at = p.cum + ((int64_t)(s.z + c) * p.heads + h) * kC;
-            rc = at[tid];
-            re = at[kC - 1];
+            rc = pc[tid];
+            re = pc[kC - 1];
         }
+        pq += kC * p.q.token;
+        pk += kC * p.k.token;
+        pv += kC * p.v.token;
+        pc += (int64_t)p.heads * kC;
     };
     if (here.count > 0) fetch(0);
-    for (int i = tid; i < kC * kPitchP; i += kBlock) pt[i] = E{};    // (behind the diagonal they stay)
+
+    floatx4_t state[kHalf];                                          // key 16 (kHalf half + d) + quad + v, value v0 + 16 mine + col
+    const int value = v0 + 16 * mine + col, key0 = 16 * kHalf * half;
+    const int tiles_a = (p.k.dim + kLaTile - 1) / kLaTile;
+    E *own = st + (16 * mine + col) * kPitchK + key0 + quad;         // its place as an operand
+#pragma unroll
+    for (int d = 0; d < kHalf; ++d) {
+        const int at = kHalf * half + d;
+        state[d] = floatx4_t{0, 0, 0, 0};
+        if (!lone) {
+            if (at / 4 < tiles_a)
+                state[d] = *reinterpret_cast<const floatx4_t *>(p.local + (((int64_t)here.seg * p.heads + h) * tiles_a * tiles + here.tile * tiles_a + at / 4) * (kLaTile * kLaTile) +
+                                                                mine * 4 * kBlock + 4 * (at % 4 * kWave + lane));
+        } else if (w.from)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (key0 + 16 * d + quad + v < p.k.dim && value < p.v.dim) state[d][v] = w.from[la_state_at(p, w, n, h, key0 + 16 * d + quad + v, value)];
+        Op::put4(own + 16 * d, state[d]);
+    }
+    bool carried = here.begin > 0 || w.from;                         // a state has come in
+    const bool whole = p.k.dim == kKeys && p.v.dim - v0 >= kLaTile;  // the tiles' columns are all there
+    for (int i = tid; i < kC * kPitchP; i += kLaThreads) pt[i] = E{};        // (behind the diagonal they stay)
     if (tid < 2) bad[tid] = 0;
     __syncthreads();
     for (int i = 0; i < here.count; ++i) {
-        const int t0 = s.x + (here.begin + i) * kC, len = min(kC, s.y - t0);
+        const int len = min(kC, s.y - s.x - (here.begin + i) * kC);
         bool none = false;
+        if (len < kC || !whole) {
+#pragma unroll
+            for (int j = 0; j < kNk; ++j) {
+                const int at = tid + j * kLaThreads, row = at / kPerKey, d = at % kPerKey * kVec;
+                rq[j] = held_piece<kFast>(rq[j], row < len && d < p.k.dim);
+                rk[j] = held_piece<kFast>(rk[j], row < len && d < p.k.dim);
+            }
+#pragma unroll
+            for (int j = 0; j < kNv; ++j) {
+                const int at = tid + j * kLaThreads, row = at / kPerValue, d = at % kPerValue * kVec;
+                rv[j] = held_piece<kFast>(rv[j], row < len && d < p.v.dim - v0);
+            }
+        }
 #pragma unroll
         for (int j = 0; j < kNk; ++j) {
-            const int at = tid + j * kBlock, row = at / kPerKey, d = at % kPerKey * kVec;
-            if (kC * kPerKey % kBlock == 0 || row < kC) {
-                put_piece<T, E>(qt + row * kPitchK + d, held_piece<kFast>(rq[j], row < len && d < p.k.dim));
-                put_piece<T, E>(kt + row * kPitchK + d, held_piece<kFast>(rk[j], row < len && d < p.k.dim));
+            const int at = tid + j * kLaThreads, row = at / kPerKey, d = at % kPerKey * kVec;
+            if (kC * kPerKey % kLaThreads == 0 || row < kC) {
+                put_piece<T, E>(qt + row * kPitchK + d, rq[j]);
+                put_piece<T, E>(kt + row * kPitchK + d, rk[j]);
             }
         }
 #pragma unroll
         for (int j = 0; j < kNv; ++j) {
-            const int at = tid + j * kBlock, row = at / kPerValue, d = at % kPerValue * kVec;
-            const u32x4_t piece = held_piece<kFast>(rv[j], row < len && d < p.v.dim - v0);
-            put_piece<T, E>(vt + row * kPitchV + d, piece);
-            none |= piece_bad<T>(piece);
+            const int at = tid + j * kLaThreads, row = at / kPerValue, d = at % kPerValue * kVec;
+            if (kC * kPerValue % kLaThreads == 0 || row < kC) put_piece<T, E>(vt + row * kPitchV + d, rv[j]);
+            none |= piece_bad<T>(rv[j]);
         }
         if (none) bad[i & 1] = 1;
         if (tid < kC) {
             cum[tid] = rc;
-            weights[tid] = fast_exp2((re.x - rc.x) + (re.y - rc.y));
+            weights[Op::place(tid)] = fast_exp2((re.x - rc.x) + (re.y - rc.y));
         }
         __syncthreads();
         if (i + 1 < here.count) fetch(i + 1);
         if (tid == 0) bad[(i + 1) & 1] = 0;
 
-        // weights of the pairs, P[t][s]
-#pragma unroll
-        for (int k = 0; k < kM * kM / 4; ++k) {
-            const int tt = wave % kM, ts = wave / kM + k * (4 / kM);
-            if (ts > tt) continue;
+        // weights of the pairs, P[t][s]: tiles on and below the diagonal, the k-th of them in row tt, column ts
+        for (int k = wave; k < kPairTiles; k += kLaWaves) {
+            const int tt = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, ts = k - tt * (tt + 1) / 2, t = 16 * tt + col, r = 16 * ts + quad;
             floatx4_t acc = {0, 0, 0, 0};
 #pragma unroll
             for (int k0 = 0; k0 < kKeys; k0 += Op::kStep)
                 acc = Op::mma(Op::rows(kt, kPitchK, 16 * ts, k0, lane), Op::rows(qt, kPitchK, 16 * tt, k0, lane), acc);
-            const int t = 16 * tt + col, r = 16 * ts + quad;
             const float2 gt = cum[t];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -447,74 +470,81 @@ __global__ __launch_bounds__(kBlock, 2) void la_out_kernel(const LaArgs p, const
                 const float weight = acc[v] * fast_exp2((gt.x - gs.x) + (gt.y - gs.y));
                 acc[v] = r + v <= t ? weight : 0.0f;
             }
-            Op::put4(pt + t * kPitchP + r, acc);
+            Op::put4_places(pt + t * kPitchP, r, acc);
         }
-        floatx4_t acc[kM];
+        floatx4_t acc[kHalfM];
+        Frag values[kSteps];
+        if (live) {
 #pragma unroll
-        for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
-        if (carried) {
+            for (int m = 0; m < kHalfM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
+            if (carried) {
 #pragma unroll
-            for (int k = 0; k < kTiles / kJoin; ++k) {
-                const Frag a = Op::from_acc(state + k * kJoin);
+                for (int k0 = 0; k0 < kKeys; k0 += Op::kStep) {
+                    const Frag a = Op::rows(st, kPitchK, 16 * mine, k0, lane);
 #pragma unroll
-                for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::rows_acc(qt, kPitchK, 16 * m, k * Op::kStep, lane), acc[m]);
+                    for (int m = 0; m < kHalfM; ++m) acc[m] = Op::mma(a, Op::rows(qt, kPitchK, 16 * ms[m], k0, lane), acc[m]);
+                }
+#pragma unroll
+                for (int m = 0; m < kHalfM; ++m) {
+                    const float2 g = cum[16 * ms[m] + col];
+                    acc[m] *= fast_exp2(g.x + g.y);
+                }
             }
 #pragma unroll
-            for (int m = 0; m < kM; ++m) {
-                const float2 g = cum[16 * m + col];
-                acc[m] *= fast_exp2(g.x + g.y);
-            }
+            for (int k = 0; k < kSteps; ++k) values[k] = Op::cols(vt, kPitchV, 16 * mine, k * Op::kStep, lane);
         }
-        Frag values[kC / Op::kStep];
-#pragma unroll
-        for (int k = 0; k < kC / Op::kStep; ++k) values[k] = Op::cols(vt, kPitchV, 16 * wave, k * Op::kStep, lane);
         __syncthreads();
-        if (!bad[i & 1]) {
+        if (live) {
+            if (!bad[i & 1]) {
 #pragma unroll
-            for (int k = 0; k < kC / Op::kStep; ++k)
+                for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int m = k * Op::kStep / 16; m < kM; ++m) acc[m] = Op::mma(values[k], Op::rows(pt, kPitchP, 16 * m, k * Op::kStep, lane), acc[m]);
-        } else {
-            const int t = la_here(col), d = la_here(16 * wave + quad);
+                    for (int m = 0; m < kHalfM; ++m) acc[m] = Op::mma(values[k], Op::rows(pt, kPitchP, 16 * ms[m], k * Op::kStep, lane), acc[m]);
+            } else {
+                const int t = la_here(col), d = la_here(16 * mine + quad);
 #pragma unroll
-            for (int m = 0; m < kM; ++m)
-                for (int r = 0; r <= 16 * m + t; ++r) {
-                    const float weight = to_f32(pt[(16 * m + t) * kPitchP + r]);
+                for (int m = 0; m < kHalfM; ++m)
+                    for (int r = 0; r <= 16 * ms[m] + t; ++r) {
+                        const float weight = to_f32(pt[(16 * ms[m] + t) * kPitchP + Op::place(r)]);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][v] += weight * to_f32(vt[r * kPitchV + d + v]);
+                        for (int v = 0; v < 4; ++v) acc[m][v] += weight * to_f32(vt[r * kPitchV + d + v]);
+                    }
+            }
+#pragma unroll
+            for (int m = 0; m < kHalfM; ++m) {
+                const int t = 16 * ms[m] + col;
+                if (t < len) store4(out + (int64_t)t * p.out.token, acc[m] * p.scale, p.v.dim - value + col - quad, p.out.aligned);
+            }
+            if (i + 1 < here.count || (last && w.to)) {              // somebody wants the state behind this chunk
+                const float2 end = cum[kC - 1];
+                const float keep = fast_exp2(end.x + end.y);
+#pragma unroll
+                for (int d = 0; d < kHalf; ++d) state[d] *= keep;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    Frag parts[kParts], keys[kHalf];
+                    Op::template weigh<kParts>(values[k], weights + k * Op::kStep, lane, parts);
+#pragma unroll
+                    for (int d = 0; d < kHalf; ++d) keys[d] = Op::cols(kt, kPitchK, key0 + 16 * d, k * Op::kStep, lane);
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                        for (int d = 0; d < kHalf; ++d) state[d] = Op::mma(keys[d], parts[q], state[d]);
                 }
-        }
 #pragma unroll
-        for (int m = 0; m < kM; ++m) {
-            const int t = 16 * m + col;
-            if (t < len) store4(out + (int64_t)(t0 + t) * p.out.token + 16 * wave + quad, acc[m] * p.scale, p.v.dim - v0 - 16 * wave - quad, p.out.aligned);
-        }
-        if (i + 1 < here.count || (last && w.to)) {                  // somebody wants the state behind this chunk
-            const float2 end = cum[kC - 1];
-            const float keep = fast_exp2(end.x + end.y);
-#pragma unroll
-            for (int d = 0; d < kTiles; ++d) state[d] *= keep;
-#pragma unroll
-            for (int k = 0; k < kC / Op::kStep; ++k) {
-                Frag parts[kParts];
-                Op::template weigh<kParts>(values[k], weights + k * Op::kStep, lane, parts);
-#pragma unroll
-                for (int d = 0; d < kTiles; ++d) {
-                    const Frag a = Op::cols(kt, kPitchK, 16 * d, k * Op::kStep, lane);
-#pragma unroll
-                    for (int q = 0; q < kParts; ++q) state[d] = Op::mma(a, parts[q], state[d]);
-                }
+                for (int d = 0; d < kHalf; ++d) Op::put4(own + 16 * d, state[d]);
             }
         }
+        out += kC * p.out.token;
         carried = true;
         __syncthreads();
     }
     if (!w.to || !last) return;
 #pragma unroll
-    for (int d = 0; d < kTiles; ++d)
+    for (int d = 0; d < kHalf; ++d)
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-            if (16 * d + quad + v < p.k.dim && value < p.v.dim) w.to[la_state_at(p, w, n, h, 16 * d + quad + v, value)] = state[d][v];
+            if (key0 + 16 * d + quad + v < p.k.dim && value < p.v.dim) w.to[la_state_at(p, w, n, h, key0 + 16 * d + quad + v, value)] = state[d][v];
 }
 
 // Rows of no sequence
@@ -536,7 +566,7 @@ int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
     int64_t chunks, segs, seg_chunks;
     if (p.cu) {
         chunks = (int64_t)p.tokens / chunk + p.n_seqs + 2;
-        seg_chunks = want == 1 ? per_seq : (per_seq + want - 1) / want;
+        seg_chunks = (per_seq * p.heads * tiles + 767) / 768;        // whatever the longest of them is
         seg_chunks = seg_chunks < shortest ? shortest : seg_chunks;
         segs = per_seq <= seg_chunks ? p.n_seqs : chunks / seg_chunks + p.n_seqs;
     } else {
@@ -579,8 +609,8 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
     const uint32_t total = (uint32_t)((int64_t)p.max_segs * p.heads * ((p.v.dim + kLaTile - 1) / kLaTile));
     auto go = [&](auto kernel, int keys) {
         constexpr int c = Op::kChunk;
-        const size_t bytes = sizeof(typename Op::E) * c * (2 * (keys + Op::kPad) + kLaTile + Op::kPad + c + Op::kPad) + c * (sizeof(float) + sizeof(float2)) + 16;
-        kernel<<<total, kBlock, bytes, st>>>(p, w, total);           // (up to 88 KB of LDS: this runtime asks for no attribute above 64)
+        const size_t bytes = sizeof(typename Op::E) * ((2 * c + kLaTile) * (keys + Op::kPad) + c * (kLaTile + Op::kPad + c + Op::kPad)) + c * (sizeof(float) + sizeof(float2)) + 16;
+        kernel<<<total, kLaThreads, bytes, st>>>(p, w, total);       // (up to 146 KB of LDS: this runtime asks for no attribute above 64)
     };
     const bool fast = p.q.aligned && p.k.aligned && p.v.aligned;
     auto sized = [&](auto tiles) {
@@ -606,7 +636,7 @@ LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int 
     s.batch = batch; s.token = token; s.head = head;
     s.div = own_heads > 0 ? heads / own_heads : 1;
     s.dim = dim;
-    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0;
+    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0 && token * size < (1 << 24);
     return s;
 }
 

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
                 through[v] = s <= t + v ? back : 0.0f;
             }
         }
-        Op::put4(pt + s * kPitchP + t, weights);
+        Op::put4_places(pt + s * kPitchP, t, weights);
         Op::put4(dt + s * kPitchP + t, through);
         // of these 16 x 16 pairs: sums for each query and each key; on the diagonal, for each token the pairs that it stands between
         const float of_key = sum_groups((product[0] + product[1]) + (product[2] + product[3]));
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
                     if (16 * m >= k0) dq[m] = Op::mma(k, Op::cols(dt, kPitchP, 16 * m, k0, lane), dq[m]);
-                    if (16 * m < k0 + Op::kStep) dkey[m] = Op::mma(q, Op::rows(dt, kPitchP, 16 * m, k0, lane), dkey[m]);
+                    if (16 * m < k0 + Op::kStep) dkey[m] = Op::mma(q, Op::in_places(Op::rows(dt, kPitchP, 16 * m, k0, lane)), dkey[m]);
                 }
             }
         } else {                                                     // as in the outputs' kernel: nothing from behind the diagonal
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
             for (int m = 0; m < kM; ++m)
                 for (int r = 16 * m + c0; r < kC; ++r)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + r]) * to_f32(ot[r * pitch_v + d0 + v]);
+                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + Op::place(r)]) * to_f32(ot[r * pitch_v + d0 + v]);
         }
 #pragma unroll
         for (int m = 0; m < kM; ++m)
