@@ -48,7 +48,8 @@ struct LaArgs {
     float2 *cum;                     // [chunk][head][C]: G in log2 units, high and low part
     void *states, *dstates, *dstates_t;
     int64_t low;                     // elements from a state's bf16 value to what the rounding left, 0: not kept
-    float *local;                    // [segment][head][tile][4096] and behind it [segment][head] decays
+    float *local;                    // [segment][head][tile][4096] and behind it [segment][head] decays; for the backward twice
+    int64_t local_floats;
 };
 
 // ---- operands of the matrix cores --------------------------------------------------------------------------------------------
@@ -225,16 +226,17 @@ __device__ __forceinline__ int4 la_sequence(const LaArgs &p, int n) {
 struct LaWalk {
     LaSide a, b;                     // M = sum of w a b^T, stored as rows of b's dimension, dense in a's
     void *out, *out_t;               // [chunk][head][Db][Da] and, where wanted, [chunk][head][Da][Db]
-    int64_t low;                     // as LaArgs::low, of out
     const float *from;               // the state to begin with, element (ia, ib) at ia * from_a + ib * from_b; NULL: zero
     float *to;                       // the state to end with, or NULL
+    float *local;                    // as LaArgs::local
+    int64_t low;                     // as LaArgs::low, of out
     int32_t from_a, from_b;
     int32_t reverse;                 // from the last chunk to the first, weights scale exp(G_t) instead of exp(G_C - G_s)
     int32_t exact;                   // the states are kept in 32 bits: three parts to a weighted 16-bit operand instead of two
 };
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest);                        // sizes of the tables and segments, for `tiles` workgroups a head
 int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
-template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream);        // states before all chunks
+template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w, int n, void *stream);        // states before all chunks, one walk or two side by side
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }            // (what is below 2^-126 is 0)
 
 }  // namespace ss2d

@@ -132,124 +132,168 @@ __device__ __forceinline__ int64_t la_state_at(const LaArgs &p, const LaWalk &w,
 
 // A workgroup owns a 64 x 64 piece of one head's state, in accumulators (wavefront w rows 16 w .. of a's dimension), and walks a segment of
 // a sequence's chunks.  kLocal: a segment's own sum alone, from zero, and its decay, so that la_join_kernel can tell every segment
-// what comes in.  The next chunk's rows are on their way while this one is added.
-template <typename Op, typename T, bool kLocal, int kParts, bool kFast>
-__global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
+// what comes in.  The next two chunks' rows are on their way while this one is added.  Where states are wanted in both orders (kBoth) the products are made
+// twice, with their operands exchanged: an accumulator then is four neighbours of either.  Two walks may share a launch.
+template <typename Op, typename T, bool kLocal, int kParts, bool kFast, bool kBoth>
+__global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, uint32_t total) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
     constexpr int kC = Op::kChunk, kPitch = kLaTile + Op::kPad, kVec = kVecOf<T>, kPerRow = kLaTile / kVec, kN = kC * kPerRow / kBlock;
-    __shared__ __align__(16) E at[kC * kPitch], bt[kC * kPitch];
+    constexpr int kTile = kLaTile * kPitch;
+    constexpr bool kStaged = !kLocal && sizeof(E) == 2;              // (four floats of a lane are 16 bytes as they are)
+    __shared__ __align__(16) E at[kC * kPitch], bt[kC * kPitch], st[kStaged ? (kBoth ? 4 : 2) * kTile : 1];
     __shared__ __align__(16) float weights[kC];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool second = blockIdx.x >= total;
+    const LaWalk w = second ? w1 : w0;
     const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
     LaPlace here;
-    if (!la_place(p, xcd_contiguous_id(blockIdx.x, total), tiles, kC, here)) return;
+    if (!la_place(p, xcd_contiguous_id(second ? blockIdx.x - total : blockIdx.x, total), tiles, kC, here)) return;
     const int a0 = here.tile % tiles_a * kLaTile, b0 = here.tile / tiles_a * kLaTile, h = here.h, n = here.n;
     const int4 s = here.s;
     const bool lone = here.chunks <= p.seg_chunks;                   // the sequence has this one segment
     const bool last = w.reverse ? here.begin == 0 : here.begin + here.count >= here.chunks;
-    if (kLocal && lone) return;
+    if (kLocal && (lone || last)) return;                            // (nobody asks for the last one's sum)
     const int64_t b = p.cu ? 0 : n;
     const T *pa = reinterpret_cast<const T *>(w.a.p) + b * w.a.batch + (int64_t)(h / w.a.div) * w.a.head + a0;
     const T *pb = reinterpret_cast<const T *>(w.b.p) + b * w.b.batch + (int64_t)(h / w.b.div) * w.b.head + b0;
 
-    floatx4_t acc[4];                                                // element (16 wave + 4 (lane / 16) + v, 16 i + lane % 16)
-    const int ia = a0 + 16 * wave + 4 * (lane >> 4), ib = b0 + (lane & 15);
-    float *local = p.local + (((int64_t)here.seg * p.heads + h) * tiles + here.tile) * (kLaTile * kLaTile);
+    floatx4_t acc[4], turned[kBoth ? 4 : 1];                         // element (16 wave + 4 (lane / 16) + v, 16 i + lane % 16); (16 wave + lane % 16, 16 i + 4 (lane / 16) + v)
+    const int quad = 4 * (lane >> 4), col = lane & 15, ia = a0 + 16 * wave + quad, ib = b0 + col, ja = a0 + 16 * wave + col, jb = b0 + quad;
+    float *local = w.local + (((int64_t)here.seg * p.heads + h) * tiles + here.tile) * (kLaTile * kLaTile);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         acc[i] = floatx4_t{0, 0, 0, 0};
+        if constexpr (kBoth) turned[i] = floatx4_t{0, 0, 0, 0};
         if constexpr (!kLocal) {
-            if (!lone) acc[i] = *reinterpret_cast<const floatx4_t *>(local + i * 4 * kBlock + 4 * tid);
-            else if (w.from)
+            if (!lone) {
+                acc[i] = *reinterpret_cast<const floatx4_t *>(local + i * 4 * kBlock + 4 * tid);
+                if constexpr (kBoth)
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
+                    for (int v = 0; v < 4; ++v) turned[i][v] = local[i * 4 * kBlock + 4 * (wave * kWave + 16 * (col >> 2) + quad + v) + (col & 3)];
+            } else if (w.from)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
                     if (ia + v < w.a.dim && ib + 16 * i < w.b.dim) acc[i][v] = w.from[la_state_at(p, w, n, h, ia + v, ib + 16 * i)];
+                    if constexpr (kBoth)
+                        if (ja < w.a.dim && jb + 16 * i + v < w.b.dim) turned[i][v] = w.from[la_state_at(p, w, n, h, ja, jb + 16 * i + v)];
+                }
         }
     }
 
-    u32x4_t ra[kN], rb[kN];
-    float weight = 0.0f, decay = 1.0f;
+    struct Rows {
+        u32x4_t a[kN], b[kN];
+        float weight, decay;
+    } ring[2];
     double sum = 0.0;
-    auto fetch = [&](int i) {                                        // the i-th chunk of the walk
+    auto fetch = [&](int i, Rows &r) {                               // the i-th chunk of the walk
         const int c = here.begin + (w.reverse ? here.count - 1 - i : i), t0 = s.x + c * kC, len = min(kC, s.y - t0);
         const float2 *cum = p.cum + ((int64_t)(s.z + c) * p.heads + h) * kC;
         const float2 end = cum[kC - 1];
         if constexpr (kLocal) sum += (double)end.x + (double)end.y;
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
-            const int at_ = tid + j * kBlock, row = at_ / kPerRow, col = at_ % kPerRow * kVec;
-            ra[j] = load_piece<kFast>(pa + (int64_t)t0 * w.a.token, w.a.token, row, len, col, w.a.dim - a0);
-            rb[j] = load_piece<kFast>(pb + (int64_t)t0 * w.b.token, w.b.token, row, len, col, w.b.dim - b0);
+            const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
+            r.a[j] = load_piece<kFast>(pa + (int64_t)t0 * w.a.token, w.a.token, row, len, c0, w.a.dim - a0);
+            r.b[j] = load_piece<kFast>(pb + (int64_t)t0 * w.b.token, w.b.token, row, len, c0, w.b.dim - b0);
         }
         if (tid < kC) {
             const float2 g = cum[tid];
-            weight = w.reverse ? p.scale * fast_exp2(g.x + g.y) : fast_exp2((end.x - g.x) + (end.y - g.y));
+            r.weight = w.reverse ? p.scale * fast_exp2(g.x + g.y) : fast_exp2((end.x - g.x) + (end.y - g.y));
         }
-        decay = fast_exp2(end.x + end.y);
+        r.decay = fast_exp2(end.x + end.y);
     };
-    if (here.count > 0) fetch(0);
-    for (int i = 0; i < here.count; ++i) {
+    auto stage = [&](int i) {                                        // the piece before chunk i, for the stores of that chunk's step
+        if constexpr (kStaged) {
+            E *to = st + (i & 1) * kTile;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                Op::put4(to + (16 * j + col) * kPitch + 16 * wave + quad, acc[j]);
+                if constexpr (kBoth) Op::put4(to + 2 * kTile + (16 * wave + col) * kPitch + 16 * j + quad, turned[j]);
+            }
+        }
+    };
+    auto step = [&](int i, Rows &r) {
         const int c = here.begin + (w.reverse ? here.count - 1 - i : i), len = min(kC, s.y - s.x - c * kC);
         const int64_t at_chunk = (int64_t)(s.z + c) * p.heads + h;
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
-            const int at_ = tid + j * kBlock, row = at_ / kPerRow, col = at_ % kPerRow * kVec;
-            put_piece<T, E>(at + row * kPitch + col, held_piece<kFast>(ra[j], row < len && col < w.a.dim - a0));
-            put_piece<T, E>(bt + row * kPitch + col, held_piece<kFast>(rb[j], row < len && col < w.b.dim - b0));
+            const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
+            put_piece<T, E>(at + row * kPitch + c0, held_piece<kFast>(r.a[j], row < len && c0 < w.a.dim - a0));
+            put_piece<T, E>(bt + row * kPitch + c0, held_piece<kFast>(r.b[j], row < len && c0 < w.b.dim - b0));
         }
-        if (tid < kC) weights[Op::place(tid)] = weight;
-        const float keep = decay;
+        if (tid < kC) weights[Op::place(tid)] = r.weight;
+        const float keep = r.decay;
         __syncthreads();
-        if (i + 1 < here.count) fetch(i + 1);
-        if constexpr (!kLocal) {                                     // the state as the chunk finds it
+        if (i + 2 < here.count) fetch(i + 2, r);
+        if constexpr (!kLocal) {                                     // the state as the chunk finds it, whole rows of the piece at a time
             const int da = la_state_dim(w.a.dim), db = la_state_dim(w.b.dim);
             const int64_t base = at_chunk * da * db;
-            E *out = reinterpret_cast<E *>(w.out) + base + (int64_t)ib * da + ia, *out_t = reinterpret_cast<E *>(w.out_t) + base + (int64_t)ia * db + ib;
-            if (ia < da) {
-                const int left = (db - ib + 15) / 16;                // columns of 16 that there are
+            if constexpr (kStaged) {
+                constexpr int kPieces = 16 / (int)sizeof(E), kRow = kLaTile / kPieces;
+                const E *from = st + (i & 1) * kTile;
+#pragma unroll
+                for (int j = 0; j < kLaTile * kRow / kBlock; ++j) {
+                    const int at_ = tid + j * kBlock, row = at_ / kRow, c0 = at_ % kRow * kPieces;
+                    if (b0 + row < db && a0 + c0 < da)
+                        *reinterpret_cast<u32x4_t *>(reinterpret_cast<E *>(w.out) + base + (int64_t)(b0 + row) * da + a0 + c0) = *reinterpret_cast<const u32x4_t *>(from + row * kPitch + c0);
+                    if constexpr (kBoth)
+                        if (w.out_t && a0 + row < da && b0 + c0 < db)
+                            *reinterpret_cast<u32x4_t *>(reinterpret_cast<E *>(w.out_t) + base + (int64_t)(a0 + row) * db + b0 + c0) =
+                                *reinterpret_cast<const u32x4_t *>(from + 2 * kTile + row * kPitch + c0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (ia < da && ib + 16 * j < db) Op::put4(reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia, acc[j]);
+                    if constexpr (kBoth)
+                        if (w.out_t && ja < da && jb + 16 * j < db) Op::put4(reinterpret_cast<E *>(w.out_t) + base + (int64_t)ja * db + jb + 16 * j, turned[j]);
+                }
+            }
+            if (sizeof(E) == 2 && w.low && ia < da)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j < left) Op::put4(out + (int64_t)16 * j * da, acc[j]);
-                if (sizeof(E) == 2 && w.low)
+                    if (ib + 16 * j < db) {
+                        floatx4_t rest;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < left) {
-                            floatx4_t rest;
-#pragma unroll
-                            for (int v = 0; v < 4; ++v) rest[v] = acc[j][v] - to_f32(from_f32<bf16_t>(acc[j][v]));
-                            Op::put4(out + (int64_t)16 * j * da + w.low, rest);
-                        }
-                if (w.out_t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < left)
-#pragma unroll
-                            for (int v = 0; v < 4; ++v) out_t[(int64_t)v * db + 16 * j] = from_f32<E>(acc[j][v]);
-            }
+                        for (int v = 0; v < 4; ++v) rest[v] = acc[j][v] - to_f32(from_f32<bf16_t>(acc[j][v]));
+                        Op::put4(reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia + w.low, rest);
+                    }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] *= keep;
+        for (int j = 0; j < 4; ++j) {
+            acc[j] *= keep;
+            if constexpr (kBoth) turned[j] *= keep;
+        }
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
             Frag fa[kParts], fb[4];
             Op::template weigh<kParts>(Op::cols(at, kPitch, 16 * wave, k0, lane), weights + k0, lane, fa);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                fb[j] = Op::cols(bt, kPitch, 16 * j, k0, lane);
-            }
+            for (int j = 0; j < 4; ++j) fb[j] = Op::cols(bt, kPitch, 16 * j, k0, lane);
 #pragma unroll
             for (int q = 0; q < kParts; ++q)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = Op::mma(fa[q], fb[j], acc[j]);
+                for (int j = 0; j < 4; ++j) {
+                    acc[j] = Op::mma(fa[q], fb[j], acc[j]);
+                    if constexpr (kBoth) turned[j] = Op::mma(fb[j], fa[q], turned[j]);
+                }
         }
+        stage(i + 1);
         __syncthreads();
+    };
+    if (here.count > 0) fetch(0, ring[0]);
+    if (here.count > 1) fetch(1, ring[1]);
+    stage(0);
+    for (int i = 0; i < here.count; i += 2) {
+        step(i, ring[0]);
+        if (i + 1 < here.count) step(i + 1, ring[1]);
     }
     if constexpr (kLocal) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4_t *>(local + i * 4 * kBlock + 4 * tid) = acc[i];
         if (here.tile == 0 && tid == 0)
-            p.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)here.seg * p.heads + h] = exp2f((float)sum);
+            w.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)here.seg * p.heads + h] = exp2f((float)sum);
     } else if (w.to && last) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -261,30 +305,32 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 
 // What comes into each segment of a sequence, from the segments' own sums: in their place.  A workgroup takes 16 columns of a piece; the sums of
 // eight segments are on their way at once.
-__global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w, int chunk) {
+__global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, int chunk, uint32_t total) {
     constexpr int kAhead = 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool second = blockIdx.x >= total;
+    const LaWalk w = second ? w1 : w0;
     const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
-    const uint32_t id = blockIdx.x / 4;
-    const int i = blockIdx.x % 4, tile = id % (uint32_t)tiles, h = id / (uint32_t)tiles % (uint32_t)p.heads, n = id / (uint32_t)tiles / (uint32_t)p.heads;
+    const uint32_t block = second ? blockIdx.x - total : blockIdx.x, id = block / 4;
+    const int i = block % 4, tile = id % (uint32_t)tiles, h = id / (uint32_t)tiles % (uint32_t)p.heads, n = id / (uint32_t)tiles / (uint32_t)p.heads;
     const int4 s = la_sequence(p, n);
     const int n_chunks = (s.y - s.x + chunk - 1) / chunk, segs = (n_chunks + p.seg_chunks - 1) / p.seg_chunks;
     if (segs <= 1) return;
     const int ia = tile % tiles_a * kLaTile + 16 * wave + 4 * (lane >> 4), ib = tile / tiles_a * kLaTile + 16 * i + (lane & 15);
-    const float *decays = p.local + (int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile);
+    const float *decays = w.local + (int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile);
     floatx4_t state = {0, 0, 0, 0};
     if (w.from)
 #pragma unroll
         for (int v = 0; v < 4; ++v)
             if (ia + v < w.a.dim && ib < w.b.dim) state[v] = w.from[la_state_at(p, w, n, h, ia + v, ib)];
     auto place = [&](int q) { return ((int64_t)s.w + (w.reverse ? segs - 1 - q : q)) * p.heads + h; };
-    auto at = [&](int q) { return reinterpret_cast<floatx4_t *>(p.local + (place(q) * tiles + tile) * (kLaTile * kLaTile) + i * 4 * kBlock + 4 * tid); };
+    auto at = [&](int q) { return reinterpret_cast<floatx4_t *>(w.local + (place(q) * tiles + tile) * (kLaTile * kLaTile) + i * 4 * kBlock + 4 * tid); };
     for (int q0 = 0; q0 < segs; q0 += kAhead) {
         floatx4_t own[kAhead];
         float decay[kAhead];
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
-            const int safe = min(q0 + q, segs - 1);
+            const int safe = min(q0 + q, segs - 2);                  // (the last one's sum is none)
             own[q] = *at(safe);
             decay[q] = decays[place(safe)];
         }
@@ -299,33 +345,40 @@ __global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const L
 
 static int64_t la_tiles(const LaArgs &p) { return (int64_t)((p.k.dim + kLaTile - 1) / kLaTile) * ((p.v.dim + kLaTile - 1) / kLaTile); }
 
-template <typename Op, typename T, bool kLocal> static void la_walk_launch(const LaArgs &p, const LaWalk &w, uint32_t total, hipStream_t st) {
+template <typename Op, typename T, bool kLocal, bool kBoth> static void la_walk_launch(const LaArgs &p, const LaWalk *w, int n, hipStream_t st) {
     constexpr int kMost = Op::kMostParts, kLess = kMost < 2 ? kMost : 2;
-    const bool fast = w.a.aligned && w.b.aligned;
-    if (w.exact) fast ? la_walk_kernel<Op, T, kLocal, kMost, true><<<total, kBlock, 0, st>>>(p, w, total) : la_walk_kernel<Op, T, kLocal, kMost, false><<<total, kBlock, 0, st>>>(p, w, total);
-    else fast ? la_walk_kernel<Op, T, kLocal, kLess, true><<<total, kBlock, 0, st>>>(p, w, total) : la_walk_kernel<Op, T, kLocal, kLess, false><<<total, kBlock, 0, st>>>(p, w, total);
+    const LaWalk &w0 = w[0], &w1 = w[n - 1];
+    const bool fast = w0.a.aligned && w0.b.aligned && w1.a.aligned && w1.b.aligned;
+    const uint32_t total = (uint32_t)((int64_t)p.max_segs * p.heads * la_tiles(p)), grid = total * (uint32_t)n;
+    if (w0.exact || w1.exact) {
+        if (fast) la_walk_kernel<Op, T, kLocal, kMost, true, kBoth><<<grid, kBlock, 0, st>>>(p, w0, w1, total);
+        else la_walk_kernel<Op, T, kLocal, kMost, false, kBoth><<<grid, kBlock, 0, st>>>(p, w0, w1, total);
+    } else {
+        if (fast) la_walk_kernel<Op, T, kLocal, kLess, true, kBoth><<<grid, kBlock, 0, st>>>(p, w0, w1, total);
+        else la_walk_kernel<Op, T, kLocal, kLess, false, kBoth><<<grid, kBlock, 0, st>>>(p, w0, w1, total);
+    }
 }
 
 // What comes into the segments
-template <typename Op, typename T> static int la_segments(const LaArgs &p, const LaWalk &w, hipStream_t st) {
+template <typename Op, typename T> static int la_segments(const LaArgs &p, const LaWalk *w, int n, hipStream_t st) {
     if (p.max_segs <= p.n_seqs) return SS2D_OK;
-    const int64_t tiles = la_tiles(p), total = (int64_t)p.max_segs * p.heads * tiles;
-    la_walk_launch<Op, T, true>(p, w, (uint32_t)total, st);
-    la_join_kernel<<<(uint32_t)((int64_t)p.n_seqs * p.heads * tiles * 4), kBlock, 0, st>>>(p, w, Op::kChunk);
+    la_walk_launch<Op, T, true, false>(p, w, n, st);
+    const uint32_t total = (uint32_t)((int64_t)p.n_seqs * p.heads * la_tiles(p) * 4);
+    la_join_kernel<<<total * (uint32_t)n, kBlock, 0, st>>>(p, w[0], w[n - 1], Op::kChunk, total);
     return launch_status();
 }
 
-template <typename Op, typename T> int la_walk(const LaArgs &p, const LaWalk &w, void *stream) {
+template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w, int n, void *stream) {
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int64_t total = (int64_t)p.max_segs * p.heads * la_tiles(p);
-    const int rc = la_segments<Op, T>(p, w, st);
+    const int rc = la_segments<Op, T>(p, w, n, st);
     if (rc != SS2D_OK) return rc;
-    la_walk_launch<Op, T, false>(p, w, (uint32_t)total, st);
+    if (w[0].out_t || w[n - 1].out_t) la_walk_launch<Op, T, false, true>(p, w, n, st);
+    else la_walk_launch<Op, T, false, false>(p, w, n, st);
     return launch_status();
 }
-template int la_walk<OperandF32, float>(const LaArgs &, const LaWalk &, void *);
-template int la_walk<OperandF32, f16_t>(const LaArgs &, const LaWalk &, void *);
-template int la_walk<OperandBf16, bf16_t>(const LaArgs &, const LaWalk &, void *);
+template int la_walks<OperandF32, float>(const LaArgs &, const LaWalk *, int, void *);
+template int la_walks<OperandF32, f16_t>(const LaArgs &, const LaWalk *, int, void *);
+template int la_walks<OperandBf16, bf16_t>(const LaArgs &, const LaWalk *, int, void *);
 
 // ---- outputs -----------------------------------------------------------------------------------------------------------------------
 // A workgroup owns 64 values' columns of one head and walks a segment of chunks with their states, so that nothing but q, k, v and the outputs passes
@@ -404,7 +457,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
         state[d] = floatx4_t{0, 0, 0, 0};
         if (!lone) {
             if (at / 4 < tiles_a)
-                state[d] = *reinterpret_cast<const floatx4_t *>(p.local + (((int64_t)here.seg * p.heads + h) * tiles_a * tiles + here.tile * tiles_a + at / 4) * (kLaTile * kLaTile) +
+                state[d] = *reinterpret_cast<const floatx4_t *>(w.local + (((int64_t)here.seg * p.heads + h) * tiles_a * tiles + here.tile * tiles_a + at / 4) * (kLaTile * kLaTile) +
                                                                 mine * 4 * kBlock + 4 * (at % 4 * kWave + lane));
         } else if (w.from)
 #pragma unroll
@@ -561,7 +614,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void la_nobody_kernel
 // Segments: where the sequences alone do not give the chip its workgroups (two to a CU, of `tiles` for a head), each is cut so that they do, into
 // `shortest` chunks at least: a segment is walked twice.
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
-    const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= 192 ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
+    const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= (tiles > (p.v.dim + kLaTile - 1) / kLaTile ? 384 : 192) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk;
     int64_t chunks, segs, seg_chunks;
     if (p.cu) {
@@ -577,7 +630,7 @@ int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
         p.segs_per_seq = per_seq <= seg_chunks ? 1 : (int)((per_seq + seg_chunks - 1) / seg_chunks);
         segs = (int64_t)p.segs_per_seq * p.n_seqs;
     }
-    if (chunks * p.heads > 0x7fffffff / 4 || segs * p.heads * la_tiles(p) > 0x7fffffff / 4) return SS2D_EINVAL;
+    if (chunks * p.heads > 0x7fffffff / 4 || segs * p.heads * la_tiles(p) > 0x7fffffff / 16) return SS2D_EINVAL;
     p.per_seq = (int)per_seq;
     p.max_chunks = (int)chunks;
     p.seg_chunks = (int)seg_chunks;
@@ -604,8 +657,9 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
     w.a = p.k; w.b = p.v;
     w.from = p.initial; w.to = p.final;
     w.from_a = p.v.dim; w.from_b = 1;
+    w.local = p.local;
     w.exact = p.final != nullptr;
-    if ((rc = la_segments<Op, T>(p, w, st)) != SS2D_OK) return rc;
+    if ((rc = la_segments<Op, T>(p, &w, 1, st)) != SS2D_OK) return rc;
     const uint32_t total = (uint32_t)((int64_t)p.max_segs * p.heads * ((p.v.dim + kLaTile - 1) / kLaTile));
     auto go = [&](auto kernel, int keys) {
         constexpr int c = Op::kChunk;
@@ -699,7 +753,8 @@ int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
         take(p.dstates, (low ? 2 : 1) * size * entries * state);
         take(p.dstates_t, size * entries * state);
     }
-    take(p.local, p.max_segs > p.n_seqs ? 4 * (int64_t)p.max_segs * p.heads * (tiles * kLaTile * kLaTile + 1) : 0);
+    p.local_floats = p.max_segs > p.n_seqs ? (la_round(4 * (int64_t)p.max_segs * p.heads * (tiles * kLaTile * kLaTile + 1)) / 4) : 0;
+    take(p.local, 4 * p.local_floats * (backward ? 2 : 1));
     return at < 256 ? 256 : at;                                      // (a caller has an address to give)
 }
 

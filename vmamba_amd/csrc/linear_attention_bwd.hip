@@ -6,6 +6,8 @@
 //     dg_t = sum_(s < t <= t') P_t's do_t' . v_s + sum_(t' >= t) scale exp(G_t') q_t' . (S do_t') + sum_(s < t) exp(G_C - G_s) k_s . (E v_s) + exp(G_C) <S, E>
 // -- sums over the chunk alone.  (The shorter form, the sum of q . dq - k . dk from t to the sequence's end, is a small difference of
 // long sums.)  S and E of all chunks come from two walks, and every chunk is then on its own.
+#include <type_traits>
+
 #include "linear_attention.h"
 
 namespace ss2d {
@@ -26,21 +28,21 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
     return sum;
 }
 
-// A workgroup owns a chunk of one head: weights of its pairs to LDS, then 16 columns of dq and dk, and of dv, to a wavefront at a time, as the
-// outputs' kernel does (transposed products, states straight from memory).  kLow: dq's and dk's share of the states with
-// what their rounding to bf16 left, for a decay's gradient in single precision.
-template <typename Op, typename T, bool kLow, bool kFast>
-__global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
+// A workgroup owns a chunk of one head: weights of its pairs to LDS, then its wavefronts take 16 columns of dq and dk, or of dv, at a time, as the
+// outputs' kernel does (transposed products, states straight from memory; those of a wavefront's first columns are on their way from the start).
+// kLow: dq's and dk's share of the states with what their rounding to bf16 left, for a decay's gradient in single precision.
+template <typename Op, typename T, int kWaves, bool kLow, bool kFast>
+__global__ __launch_bounds__(kWaves * kWave, kWaves == 4 ? 3 : 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
-    constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad;
+    constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad, kAhead = 4, kThreads = kWaves * kWave, kLower = kM * (kM + 1) / 2;
     extern __shared__ __align__(16) char lds[];
     const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), pitch_k = dk + Op::kPad, pitch_v = dv + Op::kPad;
     E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * pitch_k, *vt = kt + kC * pitch_k, *ot = vt + kC * pitch_v;
     E *pt = ot + kC * pitch_v, *dt = pt + kC * kPitchP;              // P and D, as rows of a key's token
     float2 *cum = reinterpret_cast<float2 *>(dt + kC * kPitchP);
     float *of_queries = reinterpret_cast<float *>(cum + kC), *of_keys = of_queries + kM * kC;        // sums of the pairs' products, [16 keys / queries][token]
-    float *with_s = of_keys + kM * kC, *with_e = with_s + 4 * kC, *both = with_e + 4 * kC;           // [wavefront][token], [wavefront]
+    float *with_s = of_keys + kM * kC, *with_e = with_s + kWaves * kC, *both = with_e + kWaves * kC;     // [wavefront][token], [wavefront]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
     const uint32_t id = xcd_contiguous_id(blockIdx.x, total);
     const int c = id / (uint32_t)p.heads, h = id - (uint32_t)c * (uint32_t)p.heads;
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
     };
     if (e.w < 0) {                                                   // rows of no sequence
         const floatx4_t none = {0, 0, 0, 0};
-        for (int i = tid; i < e.z * (kLaMaxDim / 4); i += kBlock) {
+        for (int i = tid; i < e.z * (kLaMaxDim / 4); i += kThreads) {
             const int t = i / (kLaMaxDim / 4), d = i % (kLaMaxDim / 4) * 4;
             if (d < p.k.dim) { put(p.dq, t, d, none); put(p.dk, t, d, none); }
             if (d < p.v.dim) put(p.dv, t, d, none);
@@ -71,37 +73,75 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
         if (p.ddecay && !head_sums && tid < e.z) put_decay(tid, 0.0f);
         return;
     }
-    auto load = [&](const LaSide &side, E *tile, int pitch, const FastDiv &per_row) {
-        const T *src = reinterpret_cast<const T *>(side.p) + e.x * side.batch + (int64_t)e.y * side.token + (int64_t)(h / side.div) * side.head;
-        bool bad = false;
-        for (uint32_t i = tid; i < kC * per_row.d; i += 4 * kBlock) {
-            u32x4_t piece[4];
-            uint32_t row[4], at[4];
+    // tasks of 16 columns: of dq and dk, then of dv
+    const int key_tasks = (p.k.dim + 15) / 16, tasks = key_tasks + (p.v.dim + 15) / 16;
+    const int4 seq = la_sequence(p, e.w);
+    const bool has_s = e.y != seq.x || p.initial, has_e = e.y + e.z < seq.y || p.dfinal;
+    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim);
+    const E *states = reinterpret_cast<const E *>(p.states) + entry * sk * sv, *dstates = reinterpret_cast<const E *>(p.dstates) + entry * sk * sv;
+    const E *dstates_t = reinterpret_cast<const E *>(p.dstates_t) + entry * sk * sv;
+    Frag s_ahead[kAhead], e_ahead[kAhead];                           // kAhead steps of a task's states
+    auto fetch = [&](int task, int k0) {                             // (steps past the last repeat it, nobody uses them)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                divmod(i + j * kBlock, per_row, row[j], at[j]);
-                piece[j] = load_piece<kFast>(src, side.token, (int)row[j], e.z, at[j] * kVec, side.dim);
+        for (int k = 0; k < kAhead; ++k) {
+            if (task < key_tasks) {
+                const int at = min(k0 + k * Op::kStep, dv - Op::kStep);
+                if (has_s) s_ahead[k] = Op::rows(states, sv, 16 * task, at, lane);
+                if (has_e) e_ahead[k] = Op::rows(dstates, sv, 16 * task, at, lane);
+            } else if (has_e) e_ahead[k] = Op::rows(dstates_t, sk, 16 * (task - key_tasks), min(k0 + k * Op::kStep, dk - Op::kStep), lane);
+        }
+    };
+
+    {
+        constexpr int kN = 16 / kWaves;
+        const LaSide *sides[4] = {&p.q, &p.k, &p.dout, &p.v};
+        E *tiles[4] = {qt, kt, ot, vt};
+        bool bad = false;
+        if (tid < kC) cum[tid] = p.cum[entry * kC + tid];
+        const uint32_t most = kC * (per_key.d > per_value.d ? per_key.d : per_value.d);
+        for (uint32_t i = 0; i < most; i += kN * kThreads) {
+            u32x4_t piece[4][kN];
+            uint32_t row[2][kN], at[2][kN];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                divmod(i + tid + j * kThreads, per_key, row[0][j], at[0][j]);
+                divmod(i + tid + j * kThreads, per_value, row[1][j], at[1][j]);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (row[j] < kC) {
-                    piece[j] = held_piece<kFast>(piece[j], (int)row[j] < e.z && (int)at[j] * kVec < side.dim);
-                    put_piece<T, E>(tile + row[j] * pitch + at[j] * kVec, piece[j]);
-                    bad |= piece_bad<T>(piece[j]);
+            for (int side = 0; side < 4; ++side) {
+                const LaSide &from = *sides[side];
+                const T *src = reinterpret_cast<const T *>(from.p) + e.x * from.batch + (int64_t)e.y * from.token + (int64_t)(h / from.div) * from.head;
+#pragma unroll
+                for (int j = 0; j < kN; ++j)
+                    if (!kFast || i + j * kThreads < kC * (side < 2 ? per_key.d : per_value.d))
+                        piece[side][j] = load_piece<kFast>(src, from.token, (int)row[side / 2][j], e.z, at[side / 2][j] * kVec, from.dim);
+            }
+            if (i == 0 && wave < tasks) fetch(wave, 0);
+#pragma unroll
+            for (int side = 0; side < 4; ++side)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    const uint32_t r = row[side / 2][j], d = at[side / 2][j] * kVec;
+                    if (r < kC) {
+                        const u32x4_t held = held_piece<kFast>(piece[side][j], (int)r < e.z && (int)d < sides[side]->dim);
+                        put_piece<T, E>(tiles[side] + r * (side < 2 ? pitch_k : pitch_v) + d, held);
+                        if (side < 3) bad |= piece_bad<T>(held);
+                    }
                 }
         }
-        return bad;
-    };
-    if (tid < kC) cum[tid] = p.cum[entry * kC + tid];
-    bool bad = load(p.q, qt, pitch_k, per_key);
-    bad |= load(p.k, kt, pitch_k, per_key);
-    bad |= load(p.dout, ot, pitch_v, per_value);
-    load(p.v, vt, pitch_v, per_value);
-    bad = __syncthreads_or(bad);
+        if (tid == 0) both[kWaves] = 0.0f;
+        __syncthreads();
+        if (bad) both[kWaves] = 1.0f;
+    }
 
-#pragma unroll
-    for (int i = 0; i < kM * kM / 4; ++i) {
-        const int tt = wave % kM, ts = wave / kM + i * (4 / kM);
+    // weights of the pairs: tiles of 16 x 16 below and on the diagonal first, then zeros
+    for (int k = wave; k < kM * kM; k += kWaves) {
+        int tt = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, ts = k - tt * (tt + 1) / 2;
+        if (k >= kLower) {
+            const int u = k - kLower;
+            ts = u < 1 ? 1 : u < 3 ? 2 : 3;
+            tt = u - ts * (ts - 1) / 2;
+        }
         floatx4_t weights = {0, 0, 0, 0}, through = {0, 0, 0, 0}, product = {0, 0, 0, 0};
         const int t = 16 * tt + quad, s = 16 * ts + col;
         if (ts <= tt) {
@@ -113,15 +153,16 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const float2 gt = cum[t + v];
-                const float decay = fast_exp2((gt.x - gs.x) + (gt.y - gs.y)) * p.scale, weight = weights[v] * decay, both = weight * through[v],
+                const float decay = fast_exp2((gt.x - gs.x) + (gt.y - gs.y)) * p.scale, weight = weights[v] * decay, pair = weight * through[v],
                             back = through[v] * decay;
                 weights[v] = s <= t + v ? weight : 0.0f;
-                product[v] = s < t + v ? both : 0.0f;                // (a pair of one token has no decay between)
+                product[v] = s < t + v ? pair : 0.0f;                // (a pair of one token has no decay between)
                 through[v] = s <= t + v ? back : 0.0f;
             }
         }
         Op::put4_places(pt + s * kPitchP, t, weights);
         Op::put4(dt + s * kPitchP + t, through);
+        if (!p.ddecay) continue;
         // of these 16 x 16 pairs: sums for each query and each key; on the diagonal, for each token the pairs that it stands between
         const float of_key = sum_groups((product[0] + product[1]) + (product[2] + product[3]));
         if (lane < 16) of_keys[tt * kC + s] = ts < tt ? of_key : 0.0f;
@@ -142,11 +183,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
     }
     __syncthreads();
 
-    const int4 seq = la_sequence(p, e.w);
-    const bool has_s = e.y != seq.x || p.initial, has_e = e.y + e.z < seq.y || p.dfinal;
-    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim);
-    const E *states = reinterpret_cast<const E *>(p.states) + entry * sk * sv, *dstates = reinterpret_cast<const E *>(p.dstates) + entry * sk * sv;
-    const E *dstates_t = reinterpret_cast<const E *>(p.dstates_t) + entry * sk * sv;
+    const bool bad = both[kWaves] != 0.0f;
     const float2 end = cum[kC - 1];
     float q_dot[kM], k_dot[kM], se = 0.0f, in[kM], out[kM];          // of a token: the decay from what came in, to what goes out
 #pragma unroll
@@ -156,110 +193,120 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
         in[m] = p.scale * fast_exp2(g.x + g.y);
         out[m] = fast_exp2((end.x - g.x) + (end.y - g.y));
     }
-    for (int n = wave; 16 * n < p.k.dim; n += 4) {
-        floatx4_t dq[kM], dkey[kM];
+    for (int task = wave; task < tasks; task += kWaves) {
+        if (task < key_tasks) {
+            const int n = task;
+            floatx4_t dq[kM], dkey[kM];
 #pragma unroll
-        for (int m = 0; m < kM; ++m) dq[m] = dkey[m] = floatx4_t{0, 0, 0, 0};
-        for (int k0 = 0; k0 < dv && (has_s || has_e); k0 += Op::kStep) {
-            Frag s, d, sl, dl;
-            if (has_s) s = Op::rows(states, sv, 16 * n, k0, lane);
-            if (has_e) d = Op::rows(dstates, sv, 16 * n, k0, lane);
-            if constexpr (kLow) {
-                if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
-                if (has_e) dl = Op::rows(dstates + p.low, sv, 16 * n, k0, lane);
-            }
-            if (has_s)
+            for (int m = 0; m < kM; ++m) dq[m] = dkey[m] = floatx4_t{0, 0, 0, 0};
+            for (int g = 0; g < dv && (has_s || has_e); g += kAhead * Op::kStep) {
+                if (g) fetch(task, g);                               // (the first ones: from the start, or from the task before)
 #pragma unroll
-                for (int m = 0; m < kM; ++m) {
-                    const Frag o = Op::rows(ot, pitch_v, 16 * m, k0, lane);
-                    dq[m] = Op::mma(s, o, dq[m]);
-                    if constexpr (kLow) dq[m] = Op::mma(sl, o, dq[m]);
-                }
-            if (has_e)
+                for (int k = 0; k < kAhead; ++k) {
+                    const int k0 = g + k * Op::kStep;
+                    if (k0 >= dv) break;
+                    Frag sl, dl;
+                    if constexpr (kLow) {
+                        if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
+                        if (has_e) dl = Op::rows(dstates + p.low, sv, 16 * n, k0, lane);
+                    }
+                    if (has_s)
 #pragma unroll
-                for (int m = 0; m < kM; ++m) {
-                    const Frag v = Op::rows(vt, pitch_v, 16 * m, k0, lane);
-                    dkey[m] = Op::mma(d, v, dkey[m]);
-                    if constexpr (kLow) dkey[m] = Op::mma(dl, v, dkey[m]);
-                }
-            if (has_s && has_e) {
-                se += dot_frags(s, d);
-                if constexpr (kLow) se += dot_frags(s, dl) + dot_frags(sl, d);
-            }
-        }
+                        for (int m = 0; m < kM; ++m) {
+                            const Frag o = Op::rows(ot, pitch_v, 16 * m, k0, lane);
+                            dq[m] = Op::mma(s_ahead[k], o, dq[m]);
+                            if constexpr (kLow) dq[m] = Op::mma(sl, o, dq[m]);
+                        }
+                    if (has_e)
 #pragma unroll
-        for (int m = 0; m < kM; ++m) {
-            const E *q = qt + (16 * m + col) * pitch_k + 16 * n + quad, *k = kt + (16 * m + col) * pitch_k + 16 * n + quad;
-            dq[m] *= in[m];
-            dkey[m] *= out[m];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                q_dot[m] = fmaf(dq[m][v], to_f32(q[v]), q_dot[m]);
-                k_dot[m] = fmaf(dkey[m][v], to_f32(k[v]), k_dot[m]);
-            }
-        }
-        if (!bad) {
-#pragma unroll
-            for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-                const Frag k = Op::cols(kt, pitch_k, 16 * n, k0, lane), q = Op::cols(qt, pitch_k, 16 * n, k0, lane);
-#pragma unroll
-                for (int m = 0; m < kM; ++m) {
-                    if (16 * m >= k0) dq[m] = Op::mma(k, Op::cols(dt, kPitchP, 16 * m, k0, lane), dq[m]);
-                    if (16 * m < k0 + Op::kStep) dkey[m] = Op::mma(q, Op::in_places(Op::rows(dt, kPitchP, 16 * m, k0, lane)), dkey[m]);
+                        for (int m = 0; m < kM; ++m) {
+                            const Frag v = Op::rows(vt, pitch_v, 16 * m, k0, lane);
+                            dkey[m] = Op::mma(e_ahead[k], v, dkey[m]);
+                            if constexpr (kLow) dkey[m] = Op::mma(dl, v, dkey[m]);
+                        }
+                    if (has_s && has_e && p.ddecay) {
+                        se += dot_frags(s_ahead[k], e_ahead[k]);
+                        if constexpr (kLow) se += dot_frags(s_ahead[k], dl) + dot_frags(sl, e_ahead[k]);
+                    }
                 }
             }
-        } else {                                                     // as in the outputs' kernel: nothing from behind the diagonal
-            const int c0 = la_here(col), d0 = la_here(16 * n + quad);
+            if (task + kWaves < tasks) fetch(task + kWaves, 0);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                const int own = 16 * m + c0;
-                for (int r = 0; r < kC; ++r)
+                const E *q = qt + (16 * m + col) * pitch_k + 16 * n + quad, *k = kt + (16 * m + col) * pitch_k + 16 * n + quad;
+                dq[m] *= in[m];
+                dkey[m] *= out[m];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + d0 + v]);
-                        if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + d0 + v]);
+                for (int v = 0; v < 4; ++v) {
+                    q_dot[m] = fmaf(dq[m][v], to_f32(q[v]), q_dot[m]);
+                    k_dot[m] = fmaf(dkey[m][v], to_f32(k[v]), k_dot[m]);
+                }
+            }
+            if (!bad) {
+#pragma unroll
+                for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
+                    const Frag k = Op::cols(kt, pitch_k, 16 * n, k0, lane), q = Op::cols(qt, pitch_k, 16 * n, k0, lane);
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) {
+                        if (16 * m >= k0) dq[m] = Op::mma(k, Op::cols(dt, kPitchP, 16 * m, k0, lane), dq[m]);
+                        if (16 * m < k0 + Op::kStep) dkey[m] = Op::mma(q, Op::in_places(Op::rows(dt, kPitchP, 16 * m, k0, lane)), dkey[m]);
                     }
+                }
+            } else {                                                 // as in the outputs' kernel: nothing from behind the diagonal
+                const int c0 = la_here(col), d0 = la_here(16 * n + quad);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    const int own = 16 * m + c0;
+                    for (int r = 0; r < kC; ++r)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + d0 + v]);
+                            if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + d0 + v]);
+                        }
+                }
             }
-        }
 #pragma unroll
-        for (int m = 0; m < kM; ++m)
-            if (16 * m + col < e.z) {
-                put(p.dq, 16 * m + col, 16 * n + quad, dq[m]);
-                put(p.dk, 16 * m + col, 16 * n + quad, dkey[m]);
-            }
-    }
-    for (int n = wave; 16 * n < p.v.dim; n += 4) {
-        floatx4_t acc[kM];
+            for (int m = 0; m < kM; ++m)
+                if (16 * m + col < e.z) {
+                    put(p.dq, 16 * m + col, 16 * n + quad, dq[m]);
+                    put(p.dk, 16 * m + col, 16 * n + quad, dkey[m]);
+                }
+        } else {
+            const int n = task - key_tasks;
+            floatx4_t acc[kM];
 #pragma unroll
-        for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
-        if (has_e) {
-            for (int k0 = 0; k0 < dk; k0 += Op::kStep) {
-                const Frag a = Op::rows(dstates_t, sk, 16 * n, k0, lane);
+            for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
+            for (int g = 0; g < dk && has_e; g += kAhead * Op::kStep) {
+                if (g || (task != wave && task - kWaves >= key_tasks)) fetch(task, g);
 #pragma unroll
-                for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::rows(kt, pitch_k, 16 * m, k0, lane), acc[m]);
+                for (int k = 0; k < kAhead; ++k) {
+                    if (g + k * Op::kStep >= dk) break;
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(e_ahead[k], Op::rows(kt, pitch_k, 16 * m, g + k * Op::kStep, lane), acc[m]);
+                }
             }
 #pragma unroll
             for (int m = 0; m < kM; ++m) acc[m] *= out[m];
-        }
-        if (!bad) {
+            if (!bad) {
 #pragma unroll
-            for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-                const Frag o = Op::cols(ot, pitch_v, 16 * n, k0, lane);
+                for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
+                    const Frag o = Op::cols(ot, pitch_v, 16 * n, k0, lane);
+#pragma unroll
+                    for (int m = 0; m < kM; ++m)
+                        if (16 * m < k0 + Op::kStep) acc[m] = Op::mma(o, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
+                }
+            } else {
+                const int c0 = la_here(col), d0 = la_here(16 * n + quad);
 #pragma unroll
                 for (int m = 0; m < kM; ++m)
-                    if (16 * m < k0 + Op::kStep) acc[m] = Op::mma(o, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
+                    for (int r = 16 * m + c0; r < kC; ++r)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + Op::place(r)]) * to_f32(ot[r * pitch_v + d0 + v]);
             }
-        } else {
-            const int c0 = la_here(col), d0 = la_here(16 * n + quad);
 #pragma unroll
             for (int m = 0; m < kM; ++m)
-                for (int r = 16 * m + c0; r < kC; ++r)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + Op::place(r)]) * to_f32(ot[r * pitch_v + d0 + v]);
+                if (16 * m + col < e.z) put(p.dv, 16 * m + col, 16 * n + quad, acc[m]);
         }
-#pragma unroll
-        for (int m = 0; m < kM; ++m)
-            if (16 * m + col < e.z) put(p.dv, 16 * m + col, 16 * n + quad, acc[m]);
     }
     if (!p.ddecay) return;
 
@@ -277,18 +324,20 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
     if (wave != 0) return;
     // The pairs that a token t stands between: of its own 16 tokens, of those with earlier keys (from t on), of those with later queries (before t), of
     // earlier keys and later queries; then those of what came in (from t on) and of what goes out (before t).
-    float between = 0.0f, from = 0.0f, until = 0.0f, after = 0.0f, before = 0.0f;
+    float between = 0.0f, from = 0.0f, until = 0.0f, after = 0.0f, before = 0.0f, states_both = 0.0f;
     const int own = lane / 16;
     if (lane < kC) {
         between = of_queries[own * kC + lane];
         for (int i = 0; i < own; ++i) from += of_queries[i * kC + lane];
         for (int i = own + 1; i < kM; ++i) until += of_keys[i * kC + lane];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kWaves; ++i) {
             after += with_s[i * kC + lane];
             before += with_e[i * kC + lane];
         }
     }
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) states_both += both[i];
 #pragma unroll
     for (int m = 1; m + 1 < kM; ++m) {
         float over = 0.0f;
@@ -310,7 +359,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_bwd_kernel(const LaArgs p, float
         if (lane >= d) before += b;
     }
     const float until_t = __shfl_up(until, 1), before_t = __shfl_up(before, 1);      // (a token's key is not before it)
-    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + fast_exp2(end.x + end.y) * ((both[0] + both[1]) + (both[2] + both[3]));
+    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + fast_exp2(end.x + end.y) * states_both;
     if (head_sums) {
         dg = sum_groups(sum_columns(lane < e.z ? dg : 0.0f));
         if (lane == 0) head_sums[entry] = dg;
@@ -356,39 +405,51 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     int rc = la_tables(p, Op::kChunk, stream);
     if (rc != SS2D_OK) return rc;
-    LaWalk w = {};
-    w.from_a = 1; w.from_b = p.v.dim;
-    w.exact = p.low != 0;
+    // S by keys, dense along values; E the same way, and for dv by values, dense along keys
+    LaWalk w[2] = {};
+    int n = 0;
     const bool one = !p.cu && p.per_seq <= 1;                        // a chunk to a sequence: nothing comes in but what the caller gives
     if (!one || p.initial) {
-        w.a = p.v; w.b = p.k;
-        w.out = p.states; w.low = p.low;
-        w.from = p.initial;
-        if ((rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
+        LaWalk &s = w[n];
+        s.a = p.v; s.b = p.k;
+        s.out = p.states; s.low = p.low;
+        s.from = p.initial;
+        s.local = p.local + n++ * p.local_floats;
     }
     if (!one || p.dfinal || dinitial) {
-        w.a = p.dout; w.b = p.q;
-        w.out = p.dstates; w.out_t = p.dstates_t; w.low = p.low;
-        w.from = p.dfinal; w.to = dinitial;
-        if (dinitial) w.exact = 1;
-        w.reverse = 1;
-        if ((rc = la_walk<Op, T>(p, w, stream)) != SS2D_OK) return rc;
+        LaWalk &s = w[n];
+        s.a = p.dout; s.b = p.q;
+        s.out = p.dstates; s.out_t = p.dstates_t; s.low = p.low;
+        s.from = p.dfinal; s.to = dinitial;
+        s.reverse = 1;
+        s.exact = dinitial != nullptr;
+        s.local = p.local + n++ * p.local_floats;
     }
+    for (LaWalk &s : w) {
+        s.from_a = 1; s.from_b = p.v.dim;
+        s.exact = s.exact || p.low != 0;
+    }
+    if (n && (rc = la_walks<Op, T>(p, w, n, stream)) != SS2D_OK) return rc;
     const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
     if (total > 0) {
         const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), c = Op::kChunk, m = c / 16;
-        const size_t bytes = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad)) + sizeof(float2) * c +
-                             sizeof(float) * (2 * m * c + 8 * c + 4);
+        const size_t tiles = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad));
+        // eight wavefronts where a workgroup has a CU to itself, four where two or more share it
+        const int waves = tiles > 72 * 1024 ? 8 : 4;
+        const size_t bytes = tiles + sizeof(float2) * c + sizeof(float) * (2 * m * c + 2 * waves * c + waves + 1);
         auto go = [&](auto kernel) {
-            // (up to 155 KB of LDS: this runtime asks for no attribute above 64)
-            kernel<<<total, kBlock, bytes, st>>>(p, b.head_sums, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
+            // (up to 157 KB of LDS: this runtime asks for no attribute above 64)
+            kernel<<<total, waves * kWave, bytes, st>>>(p, b.head_sums, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
             return launch_status();
         };
         const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
-        if (sizeof(typename Op::E) == 2 && b.low) {
+        auto sized = [&](auto count) {
+            constexpr int kWaves = decltype(count)::value;
             constexpr bool kLow = sizeof(typename Op::E) == 2;
-            rc = fast ? go(la_bwd_kernel<Op, T, kLow, true>) : go(la_bwd_kernel<Op, T, kLow, false>);
-        } else rc = fast ? go(la_bwd_kernel<Op, T, false, true>) : go(la_bwd_kernel<Op, T, false, false>);
+            if (kLow && b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, kLow, true>) : go(la_bwd_kernel<Op, T, kWaves, kLow, false>);
+            return fast ? go(la_bwd_kernel<Op, T, kWaves, false, true>) : go(la_bwd_kernel<Op, T, kWaves, false, false>);
+        };
+        rc = waves == 8 ? sized(std::integral_constant<int, 8>{}) : sized(std::integral_constant<int, 4>{});
         if (rc != SS2D_OK) return rc;
         auto sum = [&](const LaSide &side, void *out) {
             if (side.div <= 1) return;
@@ -416,7 +477,7 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
     const int rc = la_arguments(&f, b.a, empty);
     if (rc != SS2D_OK || empty) return rc;
     LaArgs &a = b.a;
-    const int planned = la_plan(a, la_chunk(f.dtype), (int64_t)((f.key_dim + kLaTile - 1) / kLaTile) * ((f.value_dim + kLaTile - 1) / kLaTile), 8);
+    const int planned = la_plan(a, la_chunk(f.dtype), (int64_t)((f.key_dim + kLaTile - 1) / kLaTile) * ((f.value_dim + kLaTile - 1) / kLaTile) * 2, 4);
     if (planned != SS2D_OK) return planned;
     const int size = f.dtype == SS2D_F32 ? 4 : 2;
     if (params->ddecay && !f.decay) return SS2D_EINVAL;
