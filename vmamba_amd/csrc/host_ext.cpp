@@ -278,6 +278,8 @@ static py::object cross_merge(const py::tuple &kinds, const py::object &y_in) {
     return rc != SS2D_OK ? py::object(py::int_(rc)) : py::cast(out);
 }
 
+#include "host_attention.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("forward_core", &forward_core);
     m.def("block", &block);
@@ -285,4 +287,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("scan_bwd", &scan_bwd);
     m.def("cross_scan", &cross_scan);
     m.def("cross_merge", &cross_merge);
+    m.def("linear_attention", &attention::linear_attention);
+    m.def("linear_attention_step", &attention::linear_attention_step);
+    m.def("qk_norm_rotate", &attention::qk_norm_rotate);
 }

@@ -32,7 +32,7 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
 // outputs' kernel does (transposed products, states straight from memory; those of a wavefront's first columns are on their way from the start).
 // kLow: dq's and dk's share of the states with what their rounding to bf16 left, for a decay's gradient in single precision.
 template <typename Op, typename T, int kWaves, bool kLow, bool kFast>
-__global__ __launch_bounds__(kWaves * kWave, kWaves == 4 ? 3 : 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
+__global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::E) == 4 ? 3 : 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
     constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad, kAhead = 4, kThreads = kWaves * kWave, kLower = kM * (kM + 1) / 2;

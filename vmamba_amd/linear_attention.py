@@ -10,7 +10,7 @@ here.  Arguments are checked as csms6s.py does and fail with RuntimeError.
 import torch
 
 from . import _lib
-from .norm import TENSOR_KINDS
+from .norm import TENSOR_KINDS, native_stands
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
 MAX_HEAD_DIM = 256
@@ -170,6 +170,10 @@ def linear_attention_fn(q, k, v, log_decay=None, scale=None, initial_state=None,
     Returns out (batch, tokens, heads, value_dim) in q's dtype, with ``output_final_state`` (out, final_state): the states behind the last tokens,
     float32, which linear_attention_step_fn carries on."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
+    if native_stands(q):
+        native = _lib.host().linear_attention(TENSOR_KINDS, q, k, v, log_decay, initial_state, cu_seqlens, scale, bool(output_final_state))
+        if native is not None:
+            return native
     heads = _check_sides(q, k, v, "linear_attention_fn", 4)
     _check_decay(log_decay, q, heads, (q.shape[0], q.shape[1], heads))
     n_seqs = q.shape[0]
@@ -194,6 +198,10 @@ def linear_attention_step_fn(q, k, v, log_decay, state, scale=None):
     be dense but for the batch's stride, which keeps them apart.  For inference: it refuses tensors that require a gradient while
     gradients are recorded."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
+    if native_stands(q):
+        native = _lib.host().linear_attention_step(TENSOR_KINDS, q, k, v, log_decay, state, scale)
+        if native is not None:
+            return _lib.result(native, "ss2d_linear_attention_step")
     heads = _check_sides(q, k, v, "linear_attention_step_fn", 3)
     _check_decay(log_decay, q, heads, (q.shape[0], heads))
     shape = (q.shape[0], heads, q.shape[2], v.shape[2])
@@ -216,5 +224,6 @@ def linear_attention_step_fn(q, k, v, log_decay, state, scale=None):
     p.k_batch_stride, p.k_head_stride = k.stride()[:2]
     p.v_batch_stride, p.v_head_stride = v.stride()[:2]
     p.state_batch_stride = state.stride(0) if state.shape[0] > 1 else per_sequence
+    torch.autograd.graph.increment_version(state)                # (written in place, behind autograd's back)
     _lib.check(_lib.launch(q, _lib.lib().ss2d_linear_attention_step, p), "ss2d_linear_attention_step")
     return out

@@ -10,6 +10,7 @@ import torch
 
 from . import _lib
 from .linear_attention import _check, _dense_last, _ptr, check_plain
+from .norm import TENSOR_KINDS, native_stands
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
 MAX_DIM = 512
@@ -77,6 +78,10 @@ def qk_norm_rotate_fn(q, k, q_weight=None, k_weight=None, positions=None, freque
     i is values (i, i + R / 2) of the first R = 2 * frequencies.numel() values of a head, with ``interleaved`` values (2 i, 2 i + 1); what is behind them is
     not turned.  Without positions nothing is."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
+    if native_stands(q):
+        native = _lib.host().qk_norm_rotate(TENSOR_KINDS, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
+        if native is not None:
+            return native
     check_plain(q, q=q, k=k, q_weight=q_weight, k_weight=k_weight, positions=positions, frequencies=frequencies)
     _check(q.dtype in _DTYPE_CODE, f"qk_norm_rotate_fn not implemented for input type '{q.dtype}'")
     _check(k is not None and k.dtype == q.dtype, "k must have q's dtype")
