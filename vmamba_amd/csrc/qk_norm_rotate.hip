@@ -30,7 +30,7 @@ struct QnArgs {
     int32_t pos64, freq64, axes, per_axis, pairs;                    // pairs = axes * per_axis
     int32_t batch, tokens, dim, w_dtype, interleaved, round, has_w;  // round: tokens of a workgroup's round
     int64_t rounds;
-    FastDiv by_heads, by_pairs;
+    FastDiv by_heads[2], by_pairs;
     float eps;
     float *partial;                  // backward: [workgroup][side][dim]
 };
@@ -85,23 +85,28 @@ __device__ __forceinline__ void qn_turn8(float (&v)[8], const float2 *cs, bool i
     }
 }
 
+// Sum over the kLanes lanes of a row, in each of them: neighbours, pairs, the other four, the other eight by lane moves inside the addition
 template <int kLanes> __device__ __forceinline__ float qn_sum(float v) {
-#pragma unroll
-    for (int m = kLanes / 2; m >= 1; m /= 2) v += __shfl_xor(v, m);
+    v += dpp_move<0xB1>(0.0f, v);
+    v += dpp_move<0x4E>(0.0f, v);
+    if constexpr (kLanes >= 8) v += dpp_move<0x141>(0.0f, v);
+    if constexpr (kLanes >= 16) v += dpp_move<0x140>(0.0f, v);
+    if constexpr (kLanes >= 32) v += __shfl_xor(v, 16);
+    if constexpr (kLanes >= 64) v += __shfl_xor(v, 32);
     return v;
 }
 
-// kLanes lanes to a row.  A workgroup takes rounds of p.round tokens, all heads of both sides.
+// kLanes lanes to a row.  A workgroup takes rounds of p.round tokens: their angles and places, then all heads of queries, then of keys.
 template <typename T, int kLanes, bool kBack>
 __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) {
     constexpr int kSlots = kBlock / kLanes, kAhead = kBack ? 2 : 4;
     __shared__ float2 angles[kQnPairs];
+    __shared__ int64_t places[4][kQnTokens];                         // of a token's first head: x of queries and of keys, dy of both
     __shared__ float sums[kBack ? kBlock * 8 : 1];
     const int tid = threadIdx.x, slot = tid / kLanes, unit = tid % kLanes;
     const bool in = 8 * unit < p.dim, turned = 4 * unit < p.pairs && p.positions;
-    const int first = turned && !p.interleaved ? 4 * unit : 8 * unit, second = turned && !p.interleaved ? p.pairs + 4 * unit : 8 * unit + 4;
+    const int first = !in ? 0 : turned && !p.interleaved ? 4 * unit : 8 * unit, second = !in ? 4 : turned && !p.interleaved ? p.pairs + 4 * unit : 8 * unit + 4;
     const float inv_d = 1.0f / (float)p.dim;
-    const int heads = p.side[0].heads + p.side[1].heads;
     const int64_t all = (int64_t)p.batch * p.tokens;
     float w[2][8], dw[2][8];
 #pragma unroll
@@ -113,15 +118,22 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
         }
     for (int64_t round = blockIdx.x; round < p.rounds; round += gridDim.x) {
         const int64_t token0 = round * p.round;
-        const int n_tokens = (int)(all - token0 < p.round ? all - token0 : p.round), rows = n_tokens * heads;
+        const int n_tokens = (int)(all - token0 < p.round ? all - token0 : p.round);
         const int b0 = (int)(token0 / p.tokens), t0 = (int)(token0 - (int64_t)b0 * p.tokens);
         auto place = [&](int t, int &b, int &at) {                   // the round's t-th token
             b = b0;
             at = t0 + t;
             while (at >= p.tokens) { at -= p.tokens; ++b; }
         };
-        if (p.positions) {
-            if (round != blockIdx.x) __syncthreads();
+        if (round != blockIdx.x) __syncthreads();
+        if (tid < 4 * kQnTokens && tid % kQnTokens < n_tokens) {
+            const int what = tid / kQnTokens;
+            const QnSide &s = p.side[what % 2];
+            int b, at;
+            place(tid % kQnTokens, b, at);
+            places[what][tid % kQnTokens] = what < 2 ? b * s.batch + at * s.token : b * s.dy_batch + at * s.dy_token;
+        }
+        if (p.positions)
             for (int i = tid; i < n_tokens * p.pairs; i += kBlock) {
                 uint32_t t, pair;
                 int b, at;
@@ -129,70 +141,62 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
                 place((int)t, b, at);
                 angles[i] = qn_angle<T>(p, b, at, (int)pair);
             }
-            __syncthreads();
-        }
-        // kAhead rows of a lane on their way at once (a row's lanes are together here); past the last row that one again
-        for (int row0 = slot; row0 < rows; row0 += kAhead * kSlots) {
-            float v[kAhead][8], d[kBack ? kAhead : 1][8];
-            T *to[kAhead];
-            bool key[kAhead];
-            int token[kAhead];
+        __syncthreads();
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                uint32_t t, h;
-                int b, at;
-                divmod((uint32_t)min(row0 + a * kSlots, rows - 1), p.by_heads, t, h);
-                place((int)t, b, at);
-                key[a] = (int)h >= p.side[0].heads;
-                const QnSide &s = p.side[key[a]];
-                const int head = key[a] ? (int)h - p.side[0].heads : (int)h;
-                const T *x = reinterpret_cast<const T *>(s.x) + b * s.batch + at * s.token + head * s.head;
-                token[a] = (int)t;
-                to[a] = reinterpret_cast<T *>(s.y) + ((token0 + t) * s.heads + head) * p.dim;
-                qn_load4(x + (in ? first : 0), v[a]);
-                qn_load4(x + (in ? second : 4), v[a] + 4);
-                if constexpr (kBack) {
-                    const T *dy = reinterpret_cast<const T *>(s.dy) + b * s.dy_batch + at * s.dy_token + head * s.dy_head;
-                    qn_load4(dy + (in ? first : 0), d[a]);
-                    qn_load4(dy + (in ? second : 4), d[a] + 4);
-                }
-            }
+        for (int side = 0; side < 2; ++side) {
+            const QnSide &s = p.side[side];
+            const int rows = n_tokens * s.heads;
+            const T *x = reinterpret_cast<const T *>(s.x), *dy = reinterpret_cast<const T *>(s.dy);
+            T *y = reinterpret_cast<T *>(s.y) + token0 * s.heads * p.dim;
+            // kAhead rows of a lane on their way at once (a row's lanes are together here); past the last row that one again
+            for (int row0 = slot; row0 < rows; row0 += kAhead * kSlots) {
+                float v[kAhead][8], d[kBack ? kAhead : 1][8];
+                uint32_t token[kAhead];
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                const bool live = in && row0 + a * kSlots < rows;
-                float q = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[a][i] = in ? v[a][i] : 0.0f;
-                    q = fmaf(v[a][i], v[a][i], q);
-                }
-                const float r = rsqrtf(qn_sum<kLanes>(q) * inv_d + p.eps);
-                const float2 *cs = angles + token[a] * p.pairs + 4 * unit;
-                if constexpr (!kBack) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[a][i] = v[a][i] * r * (key[a] ? w[1][i] : w[0][i]);
-                    if (turned) qn_turn8(v[a], cs, p.interleaved, false);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) d[a][i] = live ? d[a][i] : 0.0f;
-                    if (turned) qn_turn8(d[a], cs, p.interleaved, true);
-                    float m = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[a][i] *= r;
-                        const float g = live ? d[a][i] * v[a][i] : 0.0f;
-                        dw[0][i] += key[a] ? 0.0f : g;
-                        dw[1][i] += key[a] ? g : 0.0f;
-                        d[a][i] *= key[a] ? w[1][i] : w[0][i];
-                        m = fmaf(d[a][i], v[a][i], m);
+                for (int a = 0; a < kAhead; ++a) {
+                    uint32_t h;
+                    divmod((uint32_t)min(row0 + a * kSlots, rows - 1), p.by_heads[side], token[a], h);
+                    const T *from = x + places[side][token[a]] + (int64_t)h * s.head;
+                    qn_load4(from + first, v[a]);
+                    qn_load4(from + second, v[a] + 4);
+                    if constexpr (kBack) {
+                        const T *back = dy + places[2 + side][token[a]] + (int64_t)h * s.dy_head;
+                        qn_load4(back + first, d[a]);
+                        qn_load4(back + second, d[a] + 4);
                     }
-                    m = qn_sum<kLanes>(m) * inv_d;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[a][i] = (d[a][i] - v[a][i] * m) * r;
                 }
-                if (live) {
-                    qn_store4(to[a] + first, v[a]);
-                    qn_store4(to[a] + second, v[a] + 4);
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const bool live = in && row0 + a * kSlots < rows;
+                    float q = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) q = fmaf(v[a][i], v[a][i], q);
+                    const float r = rsqrtf(qn_sum<kLanes>(in ? q : 0.0f) * inv_d + p.eps);
+                    const float2 *cs = angles + token[a] * p.pairs + 4 * unit;
+                    if constexpr (!kBack) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[a][i] = v[a][i] * r * w[side][i];
+                        if (turned) qn_turn8(v[a], cs, p.interleaved, false);
+                    } else {
+                        if (turned) qn_turn8(d[a], cs, p.interleaved, true);
+                        float m = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[a][i] *= r;
+                            const float g = d[a][i] * v[a][i];
+                            dw[side][i] += live ? g : 0.0f;
+                            d[a][i] *= w[side][i];
+                            m = fmaf(d[a][i], v[a][i], m);
+                        }
+                        m = qn_sum<kLanes>(in ? m : 0.0f) * inv_d;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[a][i] = (d[a][i] - v[a][i] * m) * r;
+                    }
+                    if (live) {
+                        T *to = y + (int64_t)(row0 + a * kSlots) * p.dim;
+                        qn_store4(to + first, v[a]);
+                        qn_store4(to + second, v[a] + 4);
+                    }
                 }
             }
         }
@@ -376,17 +380,25 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
         vec = vec && bits % (4 * size) == 0;
     }
     const int64_t all = (int64_t)a.batch * a.tokens, heads = (int64_t)p->q_heads + p->k_heads;
-    if (heads > 0x7fffffff / kQnTokens) return SS2D_EINVAL;
-    // A round of four rows to a group of lanes, where that leaves a thousand workgroups
+    if (heads > 0x7fffffff / kQnTokens / kQnMaxDim) return SS2D_EINVAL;
+    // A round's rows come to a group of lanes `ahead` at a time: as many tokens as make these full on both sides, while a thousand workgroups remain
     int lanes = 4;
     while (8 * lanes < p->dim) lanes *= 2;
-    if (!vec) lanes = kWave;
-    int64_t round = heads > 0 ? (4 * (kBlock / lanes) + heads - 1) / heads : 1;
-    if (round > kQnTokens) round = kQnTokens;
-    if (a.pairs > 0 && round > kQnPairs / a.pairs) round = kQnPairs / a.pairs;
-    while (round > 1 && all / round < 1024) round /= 2;
+    const int64_t step = (int64_t)(kBlock / (vec ? lanes : kWave)) * (!vec ? 1 : back ? 2 : 4);
+    int64_t most = kQnTokens, round = 1;
+    if (a.pairs > 0 && most > kQnPairs / a.pairs) most = kQnPairs / a.pairs;
+    double best = 0.0;
+    for (int64_t n = 1; n <= most && (n == 1 || all / n >= 1024); ++n) {
+        double rows = 0.0, taken = 0.0;
+        for (const QnSide &s : a.side) {
+            rows += (double)(n * s.heads);
+            taken += (double)((n * s.heads + step - 1) / step * step);
+        }
+        const double full = rows / (taken + step);                   // (and a step's worth for the angles)
+        if (full > best) { best = full; round = n; }
+    }
     a.round = (int)round;
-    a.by_heads = make_fastdiv((uint32_t)(heads > 0 ? heads : 1));
+    for (int i = 0; i < 2; ++i) a.by_heads[i] = make_fastdiv((uint32_t)(a.side[i].heads > 0 ? a.side[i].heads : 1));
     a.by_pairs = make_fastdiv((uint32_t)(a.pairs > 0 ? a.pairs : 1));
     a.rounds = all > 0 && heads > 0 ? (all + round - 1) / round : 0;
     return SS2D_OK;
