@@ -132,8 +132,8 @@ __device__ __forceinline__ int64_t la_state_at(const LaArgs &p, const LaWalk &w,
 
 // A workgroup owns a 64 x 64 piece of one head's state, in accumulators (wavefront w rows 16 w .. of a's dimension), and walks a segment of
 // a sequence's chunks.  kLocal: a segment's own sum alone, from zero, and its decay, so that la_join_kernel can tell every segment
-// what comes in.  The next two chunks' rows are on their way while this one is added.  Where states are wanted in both orders (kBoth) the products are made
-// twice, with their operands exchanged: an accumulator then is four neighbours of either.  Two walks may share a launch.
+// what comes in.  The next two chunks' rows are on their way while this one is added.  Where 16-bit states are wanted in both orders (kBoth) the products are
+// made twice, with their operands exchanged: an accumulator then is four neighbours of either.  Two walks may share a launch.
 template <typename Op, typename T, bool kLocal, int kParts, bool kFast, bool kBoth>
 __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, uint32_t total) {
     using E = typename Op::E;
@@ -244,11 +244,13 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (ia < da && ib + 16 * j < db) Op::put4(reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia, acc[j]);
-                    if constexpr (kBoth)
-                        if (w.out_t && ja < da && jb + 16 * j < db) Op::put4(reinterpret_cast<E *>(w.out_t) + base + (int64_t)ja * db + jb + 16 * j, turned[j]);
-                }
+                for (int j = 0; j < 4; ++j)
+                    if (ia < da && ib + 16 * j < db) {
+                        Op::put4(reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia, acc[j]);
+                        if (w.out_t)                                 // (16 lanes are 64 bytes of a row as they are)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) reinterpret_cast<E *>(w.out_t)[base + (int64_t)(ia + v) * db + ib + 16 * j] = from_f32<E>(acc[j][v]);
+                    }
             }
             if (sizeof(E) == 2 && w.low && ia < da)
 #pragma unroll
@@ -275,6 +277,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
             for (int q = 0; q < kParts; ++q)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    if (!kBoth && j >= 2 && w.b.dim - b0 <= 32) break;       // (nothing there)
                     acc[j] = Op::mma(fa[q], fb[j], acc[j]);
                     if constexpr (kBoth) turned[j] = Op::mma(fb[j], fa[q], turned[j]);
                 }
@@ -304,9 +307,9 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 }
 
 // What comes into each segment of a sequence, from the segments' own sums: in their place.  A workgroup takes 16 columns of a piece; the sums of
-// eight segments are on their way at once.
+// sixteen segments are on their way at once.
 __global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, int chunk, uint32_t total) {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool second = blockIdx.x >= total;
     const LaWalk w = second ? w1 : w0;
@@ -372,7 +375,8 @@ template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int rc = la_segments<Op, T>(p, w, n, st);
     if (rc != SS2D_OK) return rc;
-    if (w[0].out_t || w[n - 1].out_t) la_walk_launch<Op, T, false, true>(p, w, n, st);
+    constexpr bool kTurn = sizeof(typename Op::E) == 2;
+    if (kTurn && (w[0].out_t || w[n - 1].out_t)) la_walk_launch<Op, T, false, kTurn>(p, w, n, st);
     else la_walk_launch<Op, T, false, false>(p, w, n, st);
     return launch_status();
 }
