@@ -30,8 +30,9 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
 
 // A workgroup owns a chunk of one head: weights of its pairs to LDS, then its wavefronts take 16 columns of dq and dk, or of dv, at a time, as the
 // outputs' kernel does (transposed products, states straight from memory; those of a wavefront's first columns are on their way from the start).
+// kTile: E comes through LDS, where dk reads its rows and dv its columns; otherwise memory holds it both ways.
 // kLow: dq's and dk's share of the states with what their rounding to bf16 left, for a decay's gradient in single precision.
-template <typename Op, typename T, int kWaves, bool kLow, bool kFast>
+template <typename Op, typename T, int kWaves, bool kTile, bool kLow, bool kFast>
 __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::E) == 4 ? 3 : 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
@@ -40,7 +41,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
     const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), pitch_k = dk + Op::kPad, pitch_v = dv + Op::kPad;
     E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * pitch_k, *vt = kt + kC * pitch_k, *ot = vt + kC * pitch_v;
     E *pt = ot + kC * pitch_v, *dt = pt + kC * kPitchP;              // P and D, as rows of a key's token
-    float2 *cum = reinterpret_cast<float2 *>(dt + kC * kPitchP);
+    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim), pitch_e = sv + Op::kPad;
+    E *et = dt + kC * kPitchP;
+    float2 *cum = reinterpret_cast<float2 *>(et + (kTile ? sk * pitch_e : 0));
     float *of_queries = reinterpret_cast<float *>(cum + kC), *of_keys = of_queries + kM * kC;        // sums of the pairs' products, [16 keys / queries][token]
     float *with_s = of_keys + kM * kC, *with_e = with_s + kWaves * kC, *both = with_e + kWaves * kC;     // [wavefront][token], [wavefront]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
@@ -77,7 +80,6 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
     const int key_tasks = (p.k.dim + 15) / 16, tasks = key_tasks + (p.v.dim + 15) / 16;
     const int4 seq = la_sequence(p, e.w);
     const bool has_s = e.y != seq.x || p.initial, has_e = e.y + e.z < seq.y || p.dfinal;
-    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim);
     const E *states = reinterpret_cast<const E *>(p.states) + entry * sk * sv, *dstates = reinterpret_cast<const E *>(p.dstates) + entry * sk * sv;
     const E *dstates_t = reinterpret_cast<const E *>(p.dstates_t) + entry * sk * sv;
     Frag s_ahead[kAhead], e_ahead[kAhead];                           // kAhead steps of a task's states
@@ -87,8 +89,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             if (task < key_tasks) {
                 const int at = min(k0 + k * Op::kStep, dv - Op::kStep);
                 if (has_s) s_ahead[k] = Op::rows(states, sv, 16 * task, at, lane);
-                if (has_e) e_ahead[k] = Op::rows(dstates, sv, 16 * task, at, lane);
-            } else if (has_e) e_ahead[k] = Op::rows(dstates_t, sk, 16 * (task - key_tasks), min(k0 + k * Op::kStep, dk - Op::kStep), lane);
+                if (!kTile && has_e) e_ahead[k] = Op::rows(dstates, sv, 16 * task, at, lane);
+            } else if (!kTile && has_e) e_ahead[k] = Op::rows(dstates_t, sk, 16 * (task - key_tasks), min(k0 + k * Op::kStep, dk - Op::kStep), lane);
         }
     };
 
@@ -99,6 +101,21 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
         bool bad = false;
         if (tid < kC) cum[tid] = p.cum[entry * kC + tid];
         const uint32_t most = kC * (per_key.d > per_value.d ? per_key.d : per_value.d);
+        // (E is 16-bit and dense: kE pieces of 8 to a thread and pass)
+        constexpr int kE = 4;
+        const int e_row = sv / 8, e_pieces = sk * e_row;
+        u32x4_t e_piece[kE];
+        auto load_e = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < kE; ++j) e_piece[j] = reinterpret_cast<const u32x4_t *>(dstates)[min(i + tid + j * kThreads, e_pieces - 1)];
+        };
+        auto put_e = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < kE; ++j) {
+                const int at = i + tid + j * kThreads, row = at / e_row;
+                if (at < e_pieces) *reinterpret_cast<u32x4_t *>(et + row * pitch_e + (at - row * e_row) * 8) = e_piece[j];
+            }
+        };
         for (uint32_t i = 0; i < most; i += kN * kThreads) {
             u32x4_t piece[4][kN];
             uint32_t row[2][kN], at[2][kN];
@@ -116,7 +133,10 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                     if (!kFast || i + j * kThreads < kC * (side < 2 ? per_key.d : per_value.d))
                         piece[side][j] = load_piece<kFast>(src, from.token, (int)row[side / 2][j], e.z, at[side / 2][j] * kVec, from.dim);
             }
-            if (i == 0 && wave < tasks) fetch(wave, 0);
+            if (i == 0) {
+                if (kTile && has_e) load_e(0);
+                if (wave < tasks) fetch(wave, 0);
+            }
 #pragma unroll
             for (int side = 0; side < 4; ++side)
 #pragma unroll
@@ -128,6 +148,13 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                         if (side < 3) bad |= piece_bad<T>(held);
                     }
                 }
+        }
+        if (kTile && has_e) {
+            put_e(0);
+            for (int i = kE * kThreads; i < e_pieces; i += kE * kThreads) {
+                load_e(i);
+                put_e(i);
+            }
         }
         if (tid == 0) both[kWaves] = 0.0f;
         __syncthreads();
@@ -205,6 +232,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                 for (int k = 0; k < kAhead; ++k) {
                     const int k0 = g + k * Op::kStep;
                     if (k0 >= dv) break;
+                    if (kTile && has_e) e_ahead[k] = Op::rows(et, pitch_e, 16 * n, k0, lane);
                     Frag sl, dl;
                     if constexpr (kLow) {
                         if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
@@ -276,7 +304,14 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             floatx4_t acc[kM];
 #pragma unroll
             for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
-            for (int g = 0; g < dk && has_e; g += kAhead * Op::kStep) {
+            if (kTile && has_e) {
+                for (int k0 = 0; k0 < dk; k0 += Op::kStep) {
+                    const Frag a = Op::cols(et, pitch_e, 16 * n, k0, lane);
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::in_places(Op::rows(kt, pitch_k, 16 * m, k0, lane)), acc[m]);
+                }
+            }
+            for (int g = 0; !kTile && g < dk && has_e; g += kAhead * Op::kStep) {
                 if (g || (task != wave && task - kWaves >= key_tasks)) fetch(task, g);
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
@@ -400,6 +435,9 @@ struct LaBackward {
     void *dq, *dk, *dv;              // where the heads' sums go
 };
 
+// 16-bit E goes through LDS where a piece of it fits there beside the rows
+template <typename Op> static bool la_tiled(const LaArgs &p) { return sizeof(typename Op::E) == 2 && p.k.dim <= 128 && p.v.dim <= 128; }
+
 template <typename Op, typename T> static int la_backward(const LaBackward &b, float *dinitial, void *stream) {
     const LaArgs &p = b.a;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -419,7 +457,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (!one || p.dfinal || dinitial) {
         LaWalk &s = w[n];
         s.a = p.dout; s.b = p.q;
-        s.out = p.dstates; s.out_t = p.dstates_t; s.low = p.low;
+        s.out = p.dstates; s.out_t = la_tiled<Op>(p) ? nullptr : p.dstates_t; s.low = p.low;
         s.from = p.dfinal; s.to = dinitial;
         s.reverse = 1;
         s.exact = dinitial != nullptr;
@@ -433,8 +471,10 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
     if (total > 0) {
         const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), c = Op::kChunk, m = c / 16;
-        const size_t tiles = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad));
+        size_t tiles = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad));
         // eight wavefronts where a workgroup has a CU to itself, four where two or more share it
+        const bool tiled = la_tiled<Op>(p);
+        if (tiled) tiles += sizeof(typename Op::E) * la_state_dim(p.k.dim) * (la_state_dim(p.v.dim) + Op::kPad);
         const int waves = tiles > 72 * 1024 ? 8 : 4;
         const size_t bytes = tiles + sizeof(float2) * c + sizeof(float) * (2 * m * c + 2 * waves * c + waves + 1);
         auto go = [&](auto kernel) {
@@ -445,9 +485,13 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
         const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
         auto sized = [&](auto count) {
             constexpr int kWaves = decltype(count)::value;
-            constexpr bool kLow = sizeof(typename Op::E) == 2;
-            if (kLow && b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, kLow, true>) : go(la_bwd_kernel<Op, T, kWaves, kLow, false>);
-            return fast ? go(la_bwd_kernel<Op, T, kWaves, false, true>) : go(la_bwd_kernel<Op, T, kWaves, false, false>);
+            constexpr bool k16 = sizeof(typename Op::E) == 2;
+            if (k16 && tiled) {
+                if (b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, k16, k16, true>) : go(la_bwd_kernel<Op, T, kWaves, k16, k16, false>);
+                return fast ? go(la_bwd_kernel<Op, T, kWaves, k16, false, true>) : go(la_bwd_kernel<Op, T, kWaves, k16, false, false>);
+            }
+            if (k16 && b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, false, k16, true>) : go(la_bwd_kernel<Op, T, kWaves, false, k16, false>);
+            return fast ? go(la_bwd_kernel<Op, T, kWaves, false, false, true>) : go(la_bwd_kernel<Op, T, kWaves, false, false, false>);
         };
         rc = waves == 8 ? sized(std::integral_constant<int, 8>{}) : sized(std::integral_constant<int, 4>{});
         if (rc != SS2D_OK) return rc;
