@@ -28,22 +28,36 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
     return sum;
 }
 
+// Eight wavefronts where a workgroup has a CU's LDS to itself, four where two or more share it
+template <typename Op, int kDim> struct LaBwdShape {
+    static constexpr bool kTile = sizeof(typename Op::E) == 2 && kDim <= 128;
+    static constexpr int kC = Op::kChunk, kPitch = kDim + Op::kPad, kM = kC / 16;
+    static constexpr int kTiles = (int)sizeof(typename Op::E) * (4 * kC * kPitch + 2 * kC * (kC + Op::kPad) + (kTile ? kDim * kPitch : 0));
+    static constexpr int kWaves = kTiles > 78 * 1024 ? 8 : 4;
+    static constexpr int kBytes = kTiles + (int)sizeof(float2) * kC + (int)sizeof(float) * (2 * kM * kC + 2 * kWaves * kC + kWaves + 1);
+    static_assert(kBytes <= 160 * 1024, "LDS of a CU");
+};
+
 // A workgroup owns a chunk of one head: weights of its pairs to LDS, then its wavefronts take 16 columns of dq and dk, or of dv, at a time, as the
 // outputs' kernel does (transposed products, states straight from memory; those of a wavefront's first columns are on their way from the start).
 // kTile: E comes through LDS, where dk reads its rows and dv its columns; otherwise memory holds it both ways.
 // kLow: dq's and dk's share of the states with what their rounding to bf16 left, for a decay's gradient in single precision.
-template <typename Op, typename T, int kWaves, bool kTile, bool kLow, bool kFast>
-__global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::E) == 4 ? 3 : 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total, FastDiv per_key, FastDiv per_value) {
+// kDim: what both dimensions fit; the rows' pitch in LDS hangs on it, so that operands are read at fixed distances.
+template <typename Op, typename T, int kDim, bool kLow, bool kFast>
+__global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total) {
     using E = typename Op::E;
     using Frag = typename Op::Frag;
+    using Shape = LaBwdShape<Op, kDim>;
+    constexpr bool kTile = Shape::kTile;
+    constexpr int kWaves = Shape::kWaves, kPitch = Shape::kPitch, kPerRow = kDim / kVecOf<T>;
     constexpr int kC = Op::kChunk, kM = kC / 16, kVec = kVecOf<T>, kPitchP = kC + Op::kPad, kAhead = 4, kThreads = kWaves * kWave, kLower = kM * (kM + 1) / 2;
     extern __shared__ __align__(16) char lds[];
-    const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), pitch_k = dk + Op::kPad, pitch_v = dv + Op::kPad;
-    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * pitch_k, *vt = kt + kC * pitch_k, *ot = vt + kC * pitch_v;
-    E *pt = ot + kC * pitch_v, *dt = pt + kC * kPitchP;              // P and D, as rows of a key's token
-    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim), pitch_e = sv + Op::kPad;
+    const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep);
+    E *qt = reinterpret_cast<E *>(lds), *kt = qt + kC * kPitch, *vt = kt + kC * kPitch, *ot = vt + kC * kPitch;
+    E *pt = ot + kC * kPitch, *dt = pt + kC * kPitchP;              // P and D, as rows of a key's token
+    const int sk = la_state_dim(p.k.dim), sv = la_state_dim(p.v.dim);
     E *et = dt + kC * kPitchP;
-    float2 *cum = reinterpret_cast<float2 *>(et + (kTile ? sk * pitch_e : 0));
+    float2 *cum = reinterpret_cast<float2 *>(et + (kTile ? kDim * kPitch : 0));
     float *of_queries = reinterpret_cast<float *>(cum + kC), *of_keys = of_queries + kM * kC;        // sums of the pairs' products, [16 keys / queries][token]
     float *with_s = of_keys + kM * kC, *with_e = with_s + kWaves * kC, *both = with_e + kWaves * kC;     // [wavefront][token], [wavefront]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
@@ -57,7 +71,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
     }
     const int64_t row0 = (int64_t)e.x * p.tokens + e.y;
     auto put = [&](const LaSide &side, int t, int d, floatx4_t v) {  // four values of a gradient, in single precision where heads are still to be summed
-        const int64_t at = e.x * side.batch + (int64_t)(e.y + t) * side.token + (int64_t)h * side.head + d;
+        const int64_t at = e.x * side.batch + (int64_t)(e.y + la_here(t)) * side.token + (int64_t)h * side.head + d;
         if (side.div > 1) store4(reinterpret_cast<float *>(side.p) + at, v, side.dim - d, side.aligned);
         else store4(reinterpret_cast<T *>(side.p) + at, v, side.dim - d, side.aligned);
     };
@@ -95,12 +109,11 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
     };
 
     {
-        constexpr int kN = 16 / kWaves;
+        constexpr int kPieces = kC * kPerRow, kN = kPieces / kThreads < 1 ? 1 : kPieces / kThreads < 16 / kWaves ? kPieces / kThreads : 16 / kWaves;
         const LaSide *sides[4] = {&p.q, &p.k, &p.dout, &p.v};
         E *tiles[4] = {qt, kt, ot, vt};
         bool bad = false;
         if (tid < kC) cum[tid] = p.cum[entry * kC + tid];
-        const uint32_t most = kC * (per_key.d > per_value.d ? per_key.d : per_value.d);
         // (E is 16-bit and dense: kE pieces of 8 to a thread and pass)
         constexpr int kE = 4;
         const int e_row = sv / 8, e_pieces = sk * e_row;
@@ -113,25 +126,21 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
 #pragma unroll
             for (int j = 0; j < kE; ++j) {
                 const int at = i + tid + j * kThreads, row = at / e_row;
-                if (at < e_pieces) *reinterpret_cast<u32x4_t *>(et + row * pitch_e + (at - row * e_row) * 8) = e_piece[j];
+                if (at < e_pieces) *reinterpret_cast<u32x4_t *>(et + row * kPitch + (at - row * e_row) * 8) = e_piece[j];
             }
         };
-        for (uint32_t i = 0; i < most; i += kN * kThreads) {
-            u32x4_t piece[4][kN];
-            uint32_t row[2][kN], at[2][kN];
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                divmod(i + tid + j * kThreads, per_key, row[0][j], at[0][j]);
-                divmod(i + tid + j * kThreads, per_value, row[1][j], at[1][j]);
-            }
+        for (int i = 0; i < kPieces; i += kN * kThreads) {
+            u32x4_t piece[4][kN];
 #pragma unroll
             for (int side = 0; side < 4; ++side) {
                 const LaSide &from = *sides[side];
                 const T *src = reinterpret_cast<const T *>(from.p) + e.x * from.batch + (int64_t)e.y * from.token + (int64_t)(h / from.div) * from.head;
 #pragma unroll
-                for (int j = 0; j < kN; ++j)
-                    if (!kFast || i + j * kThreads < kC * (side < 2 ? per_key.d : per_value.d))
-                        piece[side][j] = load_piece<kFast>(src, from.token, (int)row[side / 2][j], e.z, at[side / 2][j] * kVec, from.dim);
+                for (int j = 0; j < kN; ++j) {
+                    const int at = i + tid + j * kThreads;
+                    piece[side][j] = load_piece<kFast>(src, from.token, at / kPerRow, e.z, at % kPerRow * kVec, from.dim);
+                }
             }
             if (i == 0) {
                 if (kTile && has_e) load_e(0);
@@ -141,10 +150,10 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             for (int side = 0; side < 4; ++side)
 #pragma unroll
                 for (int j = 0; j < kN; ++j) {
-                    const uint32_t r = row[side / 2][j], d = at[side / 2][j] * kVec;
-                    if (r < kC) {
-                        const u32x4_t held = held_piece<kFast>(piece[side][j], (int)r < e.z && (int)d < sides[side]->dim);
-                        put_piece<T, E>(tiles[side] + r * (side < 2 ? pitch_k : pitch_v) + d, held);
+                    const int at = i + tid + j * kThreads, r = at / kPerRow, d = at % kPerRow * kVec;
+                    if (kPieces % (kN * kThreads) == 0 || r < kC) {
+                        const u32x4_t held = held_piece<kFast>(piece[side][j], r < e.z && d < sides[side]->dim);
+                        put_piece<T, E>(tiles[side] + r * kPitch + d, held);
                         if (side < 3) bad |= piece_bad<T>(held);
                     }
                 }
@@ -173,9 +182,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
         const int t = 16 * tt + quad, s = 16 * ts + col;
         if (ts <= tt) {
             for (int k0 = 0; k0 < dk; k0 += Op::kStep)
-                weights = Op::mma(Op::rows(qt, pitch_k, 16 * tt, k0, lane), Op::rows(kt, pitch_k, 16 * ts, k0, lane), weights);
+                weights = Op::mma(Op::rows(qt, kPitch, 16 * tt, k0, lane), Op::rows(kt, kPitch, 16 * ts, k0, lane), weights);
             for (int k0 = 0; k0 < dv; k0 += Op::kStep)
-                through = Op::mma(Op::rows(ot, pitch_v, 16 * tt, k0, lane), Op::rows(vt, pitch_v, 16 * ts, k0, lane), through);
+                through = Op::mma(Op::rows(ot, kPitch, 16 * tt, k0, lane), Op::rows(vt, kPitch, 16 * ts, k0, lane), through);
             const float2 gs = cum[s];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -232,7 +241,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                 for (int k = 0; k < kAhead; ++k) {
                     const int k0 = g + k * Op::kStep;
                     if (k0 >= dv) break;
-                    if (kTile && has_e) e_ahead[k] = Op::rows(et, pitch_e, 16 * n, k0, lane);
+                    if (kTile && has_e) e_ahead[k] = Op::rows(et, kPitch, 16 * n, k0, lane);
                     Frag sl, dl;
                     if constexpr (kLow) {
                         if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
@@ -241,14 +250,14 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                     if (has_s)
 #pragma unroll
                         for (int m = 0; m < kM; ++m) {
-                            const Frag o = Op::rows(ot, pitch_v, 16 * m, k0, lane);
+                            const Frag o = Op::rows(ot, kPitch, 16 * m, k0, lane);
                             dq[m] = Op::mma(s_ahead[k], o, dq[m]);
                             if constexpr (kLow) dq[m] = Op::mma(sl, o, dq[m]);
                         }
                     if (has_e)
 #pragma unroll
                         for (int m = 0; m < kM; ++m) {
-                            const Frag v = Op::rows(vt, pitch_v, 16 * m, k0, lane);
+                            const Frag v = Op::rows(vt, kPitch, 16 * m, k0, lane);
                             dkey[m] = Op::mma(e_ahead[k], v, dkey[m]);
                             if constexpr (kLow) dkey[m] = Op::mma(dl, v, dkey[m]);
                         }
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             if (task + kWaves < tasks) fetch(task + kWaves, 0);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                const E *q = qt + (16 * m + col) * pitch_k + 16 * n + quad, *k = kt + (16 * m + col) * pitch_k + 16 * n + quad;
+                const E *q = qt + (16 * m + col) * kPitch + 16 * n + quad, *k = kt + (16 * m + col) * kPitch + 16 * n + quad;
                 dq[m] *= in[m];
                 dkey[m] *= out[m];
 #pragma unroll
@@ -273,7 +282,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             if (!bad) {
 #pragma unroll
                 for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-                    const Frag k = Op::cols(kt, pitch_k, 16 * n, k0, lane), q = Op::cols(qt, pitch_k, 16 * n, k0, lane);
+                    const Frag k = Op::cols(kt, kPitch, 16 * n, k0, lane), q = Op::cols(qt, kPitch, 16 * n, k0, lane);
 #pragma unroll
                     for (int m = 0; m < kM; ++m) {
                         if (16 * m >= k0) dq[m] = Op::mma(k, Op::cols(dt, kPitchP, 16 * m, k0, lane), dq[m]);
@@ -288,8 +297,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                     for (int r = 0; r < kC; ++r)
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
-                            if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * pitch_k + d0 + v]);
-                            if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * pitch_k + d0 + v]);
+                            if (r <= own) dq[m][v] += to_f32(dt[r * kPitchP + own]) * to_f32(kt[r * kPitch + d0 + v]);
+                            if (r >= own) dkey[m][v] += to_f32(dt[own * kPitchP + r]) * to_f32(qt[r * kPitch + d0 + v]);
                         }
                 }
             }
@@ -306,9 +315,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             for (int m = 0; m < kM; ++m) acc[m] = floatx4_t{0, 0, 0, 0};
             if (kTile && has_e) {
                 for (int k0 = 0; k0 < dk; k0 += Op::kStep) {
-                    const Frag a = Op::cols(et, pitch_e, 16 * n, k0, lane);
+                    const Frag a = Op::cols(et, kPitch, 16 * n, k0, lane);
 #pragma unroll
-                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::in_places(Op::rows(kt, pitch_k, 16 * m, k0, lane)), acc[m]);
+                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(a, Op::in_places(Op::rows(kt, kPitch, 16 * m, k0, lane)), acc[m]);
                 }
             }
             for (int g = 0; !kTile && g < dk && has_e; g += kAhead * Op::kStep) {
@@ -317,7 +326,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                 for (int k = 0; k < kAhead; ++k) {
                     if (g + k * Op::kStep >= dk) break;
 #pragma unroll
-                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(e_ahead[k], Op::rows(kt, pitch_k, 16 * m, g + k * Op::kStep, lane), acc[m]);
+                    for (int m = 0; m < kM; ++m) acc[m] = Op::mma(e_ahead[k], Op::rows(kt, kPitch, 16 * m, g + k * Op::kStep, lane), acc[m]);
                 }
             }
 #pragma unroll
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
             if (!bad) {
 #pragma unroll
                 for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
-                    const Frag o = Op::cols(ot, pitch_v, 16 * n, k0, lane);
+                    const Frag o = Op::cols(ot, kPitch, 16 * n, k0, lane);
 #pragma unroll
                     for (int m = 0; m < kM; ++m)
                         if (16 * m < k0 + Op::kStep) acc[m] = Op::mma(o, Op::rows(pt, kPitchP, 16 * m, k0, lane), acc[m]);
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 4 && sizeof(typename Op::
                 for (int m = 0; m < kM; ++m)
                     for (int r = 16 * m + c0; r < kC; ++r)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + Op::place(r)]) * to_f32(ot[r * pitch_v + d0 + v]);
+                        for (int v = 0; v < 4; ++v) acc[m][v] += to_f32(pt[(16 * m + c0) * kPitchP + Op::place(r)]) * to_f32(ot[r * kPitch + d0 + v]);
             }
 #pragma unroll
             for (int m = 0; m < kM; ++m)
@@ -435,9 +444,6 @@ struct LaBackward {
     void *dq, *dk, *dv;              // where the heads' sums go
 };
 
-// 16-bit E goes through LDS where a piece of it fits there beside the rows
-template <typename Op> static bool la_tiled(const LaArgs &p) { return sizeof(typename Op::E) == 2 && p.k.dim <= 128 && p.v.dim <= 128; }
-
 template <typename Op, typename T> static int la_backward(const LaBackward &b, float *dinitial, void *stream) {
     const LaArgs &p = b.a;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -457,7 +463,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (!one || p.dfinal || dinitial) {
         LaWalk &s = w[n];
         s.a = p.dout; s.b = p.q;
-        s.out = p.dstates; s.out_t = la_tiled<Op>(p) ? nullptr : p.dstates_t; s.low = p.low;
+        s.out = p.dstates; s.out_t = LaBwdShape<Op, 128>::kTile && p.k.dim <= 128 && p.v.dim <= 128 ? nullptr : p.dstates_t; s.low = p.low;
         s.from = p.dfinal; s.to = dinitial;
         s.reverse = 1;
         s.exact = dinitial != nullptr;
@@ -470,30 +476,20 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (n && (rc = la_walks<Op, T>(p, w, n, stream)) != SS2D_OK) return rc;
     const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
     if (total > 0) {
-        const int dk = la_up(p.k.dim, Op::kStep), dv = la_up(p.v.dim, Op::kStep), c = Op::kChunk, m = c / 16;
-        size_t tiles = sizeof(typename Op::E) * c * (2 * (dk + Op::kPad) + 2 * (dv + Op::kPad) + 2 * (c + Op::kPad));
-        // eight wavefronts where a workgroup has a CU to itself, four where two or more share it
-        const bool tiled = la_tiled<Op>(p);
-        if (tiled) tiles += sizeof(typename Op::E) * la_state_dim(p.k.dim) * (la_state_dim(p.v.dim) + Op::kPad);
-        const int waves = tiles > 72 * 1024 ? 8 : 4;
-        const size_t bytes = tiles + sizeof(float2) * c + sizeof(float) * (2 * m * c + 2 * waves * c + waves + 1);
-        auto go = [&](auto kernel) {
+        const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
+        auto go = [&](auto kernel, int waves, int bytes) {
             // (up to 157 KB of LDS: this runtime asks for no attribute above 64)
-            kernel<<<total, waves * kWave, bytes, st>>>(p, b.head_sums, total, make_fastdiv(dk / kVecOf<T>), make_fastdiv(dv / kVecOf<T>));
+            kernel<<<total, waves * kWave, bytes, st>>>(p, b.head_sums, total);
             return launch_status();
         };
-        const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
-        auto sized = [&](auto count) {
-            constexpr int kWaves = decltype(count)::value;
+        auto sized = [&](auto dim) {
+            constexpr int kDim = decltype(dim)::value, kWaves = LaBwdShape<Op, kDim>::kWaves, kBytes = LaBwdShape<Op, kDim>::kBytes;
             constexpr bool k16 = sizeof(typename Op::E) == 2;
-            if (k16 && tiled) {
-                if (b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, k16, k16, true>) : go(la_bwd_kernel<Op, T, kWaves, k16, k16, false>);
-                return fast ? go(la_bwd_kernel<Op, T, kWaves, k16, false, true>) : go(la_bwd_kernel<Op, T, kWaves, k16, false, false>);
-            }
-            if (k16 && b.low) return fast ? go(la_bwd_kernel<Op, T, kWaves, false, k16, true>) : go(la_bwd_kernel<Op, T, kWaves, false, k16, false>);
-            return fast ? go(la_bwd_kernel<Op, T, kWaves, false, false, true>) : go(la_bwd_kernel<Op, T, kWaves, false, false, false>);
+            if (k16 && b.low) return fast ? go(la_bwd_kernel<Op, T, kDim, k16, true>, kWaves, kBytes) : go(la_bwd_kernel<Op, T, kDim, k16, false>, kWaves, kBytes);
+            return fast ? go(la_bwd_kernel<Op, T, kDim, false, true>, kWaves, kBytes) : go(la_bwd_kernel<Op, T, kDim, false, false>, kWaves, kBytes);
         };
-        rc = waves == 8 ? sized(std::integral_constant<int, 8>{}) : sized(std::integral_constant<int, 4>{});
+        const int dim = p.k.dim > p.v.dim ? p.k.dim : p.v.dim;
+        rc = dim <= 64 ? sized(std::integral_constant<int, 64>{}) : dim <= 128 ? sized(std::integral_constant<int, 128>{}) : sized(std::integral_constant<int, 256>{});
         if (rc != SS2D_OK) return rc;
         auto sum = [&](const LaSide &side, void *out) {
             if (side.div <= 1) return;
