@@ -1,0 +1,236 @@
+"""What linear_attention_fn, linear_attention_step_fn and qk_norm_rotate_fn refuse: every case on the CPU first, where nothing can be launched (tensors that
+say they are the GPU's; a launch fails the test), then on the GPU through the native host calls; and the checks of the C entries, which
+are made before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+import vmamba_amd
+from vmamba_amd import _lib, linear_attention, qk_norm
+
+F32, F16, BF16, F64 = torch.float32, torch.float16, torch.bfloat16, torch.float64
+HERE = ctypes.c_void_p(256)          # an aligned address, never read: the calls with it are refused first
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is the GPU's."""
+    is_cuda = property(lambda self: True)
+
+
+def on_cpu(*shape, dtype=F32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+
+
+def on_gpu(*shape, dtype=F32):
+    return torch.zeros(*shape, dtype=dtype, device="cuda:0")
+
+
+def attention(make, *, B=2, T=5, Hq=4, Hk=2, Hv=4, dk=8, dv=6, **change):
+    a = dict(q=make(B, T, Hq, dk), k=make(B, T, Hk, dk), v=make(B, T, Hv, dv), log_decay=None, scale=None, initial_state=None, cu_seqlens=None)
+    return a | {n: c(make) if callable(c) else c for n, c in change.items()}
+
+
+ATTENTION = {
+    "no q": dict(q=None), "q a number": dict(q=3), "k none": dict(k=None), "v a list": dict(v=[1.0]),
+    "rank of q": dict(q=lambda m: m(5, 4, 8)), "rank of v": dict(v=lambda m: m(2, 5, 4, 6, 1)),
+    "64 bits": dict(q=lambda m: m(2, 5, 4, 8, dtype=F64), k=lambda m: m(2, 5, 2, 8, dtype=F64), v=lambda m: m(2, 5, 4, 6, dtype=F64)),
+    "whole numbers": dict(q=lambda m: m(2, 5, 4, 8, dtype=torch.int32)), "k's type": dict(k=lambda m: m(2, 5, 2, 8, dtype=BF16)),
+    "v's type": dict(v=lambda m: m(2, 5, 4, 6, dtype=F16)), "batch": dict(k=lambda m: m(1, 5, 2, 8)), "tokens": dict(v=lambda m: m(2, 6, 4, 6)),
+    "key dimension": dict(k=lambda m: m(2, 5, 2, 7)), "heads that do not divide": dict(Hk=3), "no heads": dict(Hk=0), "no values": dict(dv=0), "no keys": dict(dk=0),
+    "keys too wide": dict(dk=257), "values too wide": dict(dv=257), "q not dense": dict(q=lambda m: m(2, 5, 8, 4).transpose(2, 3)),
+    "decay's shape": dict(log_decay=lambda m: m(2, 5, 2)), "decay's tokens": dict(log_decay=lambda m: m(2, 1, 4)), "decay's heads": dict(log_decay=lambda m: m(3)),
+    "decay's type": dict(log_decay=lambda m: m(2, 5, 4, dtype=BF16)), "decay a number": dict(log_decay=-0.1),
+    "state's type": dict(initial_state=lambda m: m(2, 4, 8, 6, dtype=BF16)), "state's shape": dict(initial_state=lambda m: m(2, 4, 6, 8)),
+    "state's sequences": dict(initial_state=lambda m: m(1, 4, 8, 6)),
+    "places in a batch of two": dict(cu_seqlens=lambda m: m(3, dtype=torch.int32)), "places of 64 bits": dict(B=1, cu_seqlens=lambda m: m(3, dtype=torch.int64)),
+    "one place": dict(B=1, cu_seqlens=lambda m: m(1, dtype=torch.int32)), "places' rank": dict(B=1, cu_seqlens=lambda m: m(1, 3, dtype=torch.int32)),
+    "every other place": dict(B=1, cu_seqlens=lambda m: m(6, dtype=torch.int32)[::2]),
+    "state of packed sequences": dict(B=1, cu_seqlens=lambda m: m(3, dtype=torch.int32), initial_state=lambda m: m(1, 4, 8, 6)),
+}
+
+
+def step(make, *, B=2, Hq=4, Hk=2, Hv=4, dk=8, dv=6, **change):
+    a = dict(q=make(B, Hq, dk), k=make(B, Hk, dk), v=make(B, Hv, dv), log_decay=None, state=make(B, 4, dk, dv))
+    return a | {n: c(make) if callable(c) else c for n, c in change.items()}
+
+
+STEP = {
+    "with tokens": dict(q=lambda m: m(2, 1, 4, 8)), "k's type": dict(k=lambda m: m(2, 2, 8, dtype=F16)), "batch": dict(v=lambda m: m(3, 4, 6)), "no state": dict(state=None),
+    "state's type": dict(state=lambda m: m(2, 4, 8, 6, dtype=F16)), "state's shape": dict(state=lambda m: m(2, 4, 6, 8)), "states in one place": dict(state=lambda m: m(1, 4, 8, 6).expand(2, 4, 8, 6)),
+    "states that overlap": dict(state=lambda m: m(400).as_strided((2, 4, 8, 6), (191, 48, 6, 1))), "a state turned": dict(state=lambda m: m(2, 4, 6, 8).transpose(2, 3)),
+    "heads of one state": dict(state=lambda m: m(2, 1, 8, 6).expand(2, 4, 8, 6)), "decay's shape": dict(log_decay=lambda m: m(2, 1)), "decay's type": dict(log_decay=lambda m: m(2, 4, dtype=BF16)),
+    "gradients": dict(k=lambda m: m(2, 2, 8).requires_grad_()), "a state with a gradient": dict(state=lambda m: m(2, 4, 8, 6).requires_grad_()), "heads": dict(Hq=3), "too wide": dict(dk=300),
+}
+
+
+def norm(make, *, B=2, T=5, Hq=4, Hk=2, D=8, **change):
+    a = dict(q=make(B, T, Hq, D), k=make(B, T, Hk, D), q_weight=None, k_weight=None, positions=None, frequencies=None)
+    return a | {n: c(make) if callable(c) else c for n, c in change.items()}
+
+
+INT = torch.int64
+NORM = {
+    "no k": dict(k=None), "k's type": dict(k=lambda m: m(2, 5, 2, 8, dtype=BF16)), "64 bits": dict(q=lambda m: m(2, 5, 4, 8, dtype=F64)), "rank": dict(q=lambda m: m(2, 5, 8)),
+    "tokens": dict(k=lambda m: m(2, 4, 2, 8)), "dimension": dict(k=lambda m: m(2, 5, 2, 6)), "too wide": dict(D=513), "nothing": dict(D=0), "not dense": dict(k=lambda m: m(2, 5, 8, 2).transpose(2, 3)),
+    "weight's shape": dict(q_weight=lambda m: m(7)), "weight's type": dict(k_weight=lambda m: m(8, dtype=BF16)), "weights of two types": dict(
+        q=lambda m: m(2, 5, 4, 8, dtype=BF16), k=lambda m: m(2, 5, 2, 8, dtype=BF16), q_weight=lambda m: m(8), k_weight=lambda m: m(8, dtype=BF16)),
+    "positions alone": dict(positions=lambda m: m(2, 5, dtype=INT)), "frequencies alone": dict(frequencies=lambda m: m(4)),
+    "positions of floats": dict(positions=lambda m: m(2, 5), frequencies=lambda m: m(4)), "frequencies of halves": dict(positions=lambda m: m(2, 5, dtype=INT), frequencies=lambda m: m(4, dtype=F16)),
+    "positions' shape": dict(positions=lambda m: m(2, 4, dtype=INT), frequencies=lambda m: m(4)), "positions' batch": dict(positions=lambda m: m(1, 5, dtype=INT), frequencies=lambda m: m(4)),
+    "axes": dict(positions=lambda m: m(2, 5, 3, dtype=INT), frequencies=lambda m: m(2, 2)), "axes without frequencies": dict(positions=lambda m: m(2, 5, 1, dtype=INT), frequencies=lambda m: m(4)),
+    "too many pairs": dict(positions=lambda m: m(5, dtype=INT), frequencies=lambda m: m(5)), "frequencies' rank": dict(positions=lambda m: m(5, dtype=INT), frequencies=lambda m: m(1, 1, 4)),
+}
+CALLS = [(vmamba_amd.linear_attention_fn, attention, ATTENTION), (vmamba_amd.linear_attention_step_fn, step, STEP), (vmamba_amd.qk_norm_rotate_fn, norm, NORM)]
+CASES = [pytest.param(call, build, change, id=f"{build.__name__}: {name}") for call, build, changes in CALLS for name, change in changes.items()]
+
+
+@pytest.mark.parametrize("call,build,change", CASES)
+def test_refused_before_anything_runs(call, build, change, monkeypatch):
+    monkeypatch.setattr(_lib, "launch", lambda *a: pytest.fail("launched"))
+    alike = lambda like, /, **tensors: [linear_attention._check(t is None or isinstance(t, torch.Tensor), f"{n} must be a tensor") for n, t in tensors.items()]  # noqa: E731
+    monkeypatch.setattr(linear_attention, "check_plain", alike)
+    monkeypatch.setattr(qk_norm, "check_plain", alike)
+    with pytest.raises(RuntimeError) as error:
+        call(**build(on_cpu, **change))
+    assert "ss2d_" not in str(error.value), "said by the kernels' entry, not by the caller's checks"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call,build,change", CASES)
+def test_refused_on_the_gpu(call, build, change):
+    print("CASE refused", build.__name__, sorted(change), flush=True)
+    with pytest.raises(RuntimeError) as error:
+        call(**build(on_gpu, **change))
+    assert "ss2d_" not in str(error.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call,build,changes", CALLS, ids=["attention", "step", "norm"])
+def test_tensors_elsewhere_are_refused(call, build, changes):
+    """Each tensor in turn on the CPU, of a class of its own, or without memory."""
+    full = build(on_gpu)
+    full |= dict(log_decay=on_gpu(4)) if "log_decay" in full else dict(q_weight=on_gpu(8), k_weight=on_gpu(8), positions=on_gpu(5, dtype=INT), frequencies=on_gpu(4))
+    full |= dict(initial_state=on_gpu(2, 4, 8, 6)) if "initial_state" in full else {}
+    with torch.no_grad():
+        call(**full)
+        for name, t in full.items():
+            if not isinstance(t, torch.Tensor):
+                continue
+            for other in (t.cpu(), t.as_subclass(OnGpu), torch.empty(t.shape, dtype=t.dtype, device="meta")):
+                with pytest.raises(RuntimeError):
+                    call(**full | {name: other})
+
+
+@pytest.mark.parametrize("call,build,changes", CALLS, ids=["attention", "step", "norm"])
+def test_no_cpu_path(call, build, changes):
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        call(**build(torch.zeros))
+
+
+# ---- the C entries -------------------------------------------------------------------------------------------------------------------
+def test_struct_layouts_match_the_header():
+    assert ctypes.sizeof(_lib.LinearAttentionParams) == 12 * 4 + 8 * 8 + 12 * 8 and _lib.LinearAttentionParams.q.offset == 48
+    assert ctypes.sizeof(_lib.LinearAttentionBwdParams) == 208 + 7 * 8 + 3 * 8 + 8 and _lib.LinearAttentionBwdParams.decay_per_head.offset == 288
+    assert ctypes.sizeof(_lib.LinearAttentionStepParams) == 10 * 4 + 6 * 8 + 9 * 8 and _lib.LinearAttentionStepParams.state_batch_stride.offset == 152
+    assert ctypes.sizeof(_lib.QkNormRotateParams) == 14 * 4 + 8 * 8 + 9 * 8 and _lib.QkNormRotateParams.q_batch_stride.offset == 120
+    assert ctypes.sizeof(_lib.QkNormRotateBwdParams) == 192 + 6 * 8 + 6 * 8
+
+
+def fill(p, **values):
+    for name, value in values.items():
+        setattr(p, name, value)
+    return p
+
+
+def sequences(**change):
+    p = fill(_lib.LinearAttentionParams(), batch=2, seqlen=100, heads=4, q_heads=4, k_heads=2, v_heads=4, key_dim=64, value_dim=64, dtype=_lib.SS2D_BF16, decay_dtype=_lib.SS2D_F32, scale=1.0,
+             q=256, k=256, v=256, out=256, q_token_stride=256, k_token_stride=128, v_token_stride=256)
+    return fill(p, **change)
+
+
+INVALID = [dict(batch=-1), dict(seqlen=-1), dict(heads=-4), dict(key_dim=0), dict(value_dim=0), dict(dtype=7), dict(dtype=-1), dict(q_heads=0), dict(k_heads=3), dict(v_heads=-2),
+           dict(decay=256, decay_dtype=_lib.SS2D_F16), dict(cu_seqlens=256, n_seqs=3), dict(batch=1, cu_seqlens=256, n_seqs=0), dict(n_seqs=-1), dict(q=None), dict(k=None), dict(v=None)]
+
+
+@pytest.mark.parametrize("change", INVALID, ids=str)
+def test_sequences_of_bad_arguments(change):
+    L, p = _lib.lib(), sequences(**change)
+    g = fill(_lib.LinearAttentionBwdParams(), fwd=p, dout=256, dq=256, dk=256, dv=256)
+    assert L.ss2d_linear_attention_workspace_bytes(p) == _lib.SS2D_EINVAL and L.ss2d_linear_attention_fwd(p, HERE, 1 << 40, None) == _lib.SS2D_EINVAL
+    assert L.ss2d_linear_attention_bwd_workspace_bytes(g) == _lib.SS2D_EINVAL and L.ss2d_linear_attention_bwd(g, HERE, 1 << 40, None) == _lib.SS2D_EINVAL
+
+
+def test_sequences_of_too_much():
+    L = _lib.lib()
+    for change in (dict(key_dim=257), dict(value_dim=300), dict(batch=2 ** 31 - 1, seqlen=1), dict(seqlen=2 ** 31 - 1, batch=64), dict(batch=1, cu_seqlens=256, n_seqs=2 ** 31 - 1),
+                   dict(heads=2 ** 31 - 4, q_heads=1, k_heads=1, v_heads=1, seqlen=1)):
+        p = sequences(**change)
+        g = fill(_lib.LinearAttentionBwdParams(), fwd=p, dout=256, dq=256, dk=256, dv=256)
+        assert L.ss2d_linear_attention_workspace_bytes(p) == _lib.SS2D_ENOTSUP and L.ss2d_linear_attention_fwd(p, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP, change
+        assert L.ss2d_linear_attention_bwd_workspace_bytes(g) == _lib.SS2D_ENOTSUP and L.ss2d_linear_attention_bwd(g, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP, change
+
+
+def test_sequences_workspace_and_results():
+    L = _lib.lib()
+    assert L.ss2d_linear_attention_workspace_bytes(None) == _lib.SS2D_EINVAL and L.ss2d_linear_attention_bwd(None, HERE, 1, None) == _lib.SS2D_EINVAL
+    p = sequences()
+    g = fill(_lib.LinearAttentionBwdParams(), fwd=p, dout=256, dq=256, dk=256, dv=256)
+    need, need_bwd = L.ss2d_linear_attention_workspace_bytes(p), L.ss2d_linear_attention_bwd_workspace_bytes(g)
+    # tables: 2 x 2 chunks of 4 heads; the backward has 2 states of 64 x 64 in bf16 for each at least
+    assert need >= 4 * 4 * 64 * 8 and need_bwd >= 2 * 16 * 64 * 64 * 2
+    for call, params, bytes_ in ((L.ss2d_linear_attention_fwd, p, need), (L.ss2d_linear_attention_bwd, g, need_bwd)):
+        assert call(params, None, bytes_, None) == _lib.SS2D_EINVAL
+        assert call(params, ctypes.c_void_p(264), bytes_, None) == _lib.SS2D_EINVAL
+        assert call(params, HERE, bytes_ - 1, None) == _lib.SS2D_ENOMEM
+    assert L.ss2d_linear_attention_fwd(sequences(out=None), HERE, need, None) == _lib.SS2D_EINVAL
+    for missing in ("dout", "dq", "dk", "dv"):
+        assert L.ss2d_linear_attention_bwd(fill(_lib.LinearAttentionBwdParams(), **(dict(fwd=p, dout=256, dq=256, dk=256, dv=256) | {missing: None})), HERE, need_bwd, None) == _lib.SS2D_EINVAL
+    assert L.ss2d_linear_attention_bwd(fill(_lib.LinearAttentionBwdParams(), fwd=p, dout=256, dq=256, dk=256, dv=256, ddecay=256), HERE, need_bwd, None) == _lib.SS2D_EINVAL
+    low = fill(_lib.LinearAttentionBwdParams(), fwd=sequences(decay=256), dout=256, dq=256, dk=256, dv=256, ddecay=256)
+    assert L.ss2d_linear_attention_bwd_workspace_bytes(low) >= need_bwd + 2 * 16 * 64 * 64 * 2       # (and what the states' rounding left)
+    for empty in (dict(batch=0), dict(heads=0)):
+        p = sequences(**empty, q=None, k=None, v=None)
+        assert L.ss2d_linear_attention_workspace_bytes(p) == 0 and L.ss2d_linear_attention_fwd(p, None, 0, None) == _lib.SS2D_OK
+        assert L.ss2d_linear_attention_bwd(fill(_lib.LinearAttentionBwdParams(), fwd=p), None, 0, None) == _lib.SS2D_OK
+
+
+def test_step_of_bad_arguments():
+    L = _lib.lib()
+    make = lambda **change: fill(_lib.LinearAttentionStepParams(), **(dict(  # noqa: E731
+        batch=2, heads=4, q_heads=4, k_heads=2, v_heads=4, key_dim=64, value_dim=32, dtype=_lib.SS2D_F16, decay_dtype=_lib.SS2D_F32, scale=1.0, q=256, k=256, v=256, state=256, out=256,
+        state_batch_stride=4 * 64 * 32) | change))
+    assert L.ss2d_linear_attention_step(None, None) == _lib.SS2D_EINVAL
+    for change in (dict(batch=-1), dict(heads=-1), dict(key_dim=0), dict(value_dim=0), dict(k_heads=3), dict(q_heads=0), dict(dtype=9), dict(decay=256, decay_dtype=_lib.SS2D_BF16), dict(q=None),
+                   dict(k=None), dict(v=None), dict(state=None), dict(out=None), dict(state_batch_stride=4 * 64 * 32 - 1), dict(state_batch_stride=0)):
+        assert L.ss2d_linear_attention_step(make(**change), None) == _lib.SS2D_EINVAL, change
+    for change in (dict(key_dim=257), dict(value_dim=1000), dict(batch=2 ** 31 - 1)):
+        assert L.ss2d_linear_attention_step(make(**change), None) == _lib.SS2D_ENOTSUP, change
+    assert L.ss2d_linear_attention_step(make(batch=0, q=None), None) == _lib.SS2D_OK
+
+
+def test_norm_of_bad_arguments():
+    L = _lib.lib()
+    full = dict(batch=2, seqlen=10, q_heads=4, k_heads=2, dim=64, dtype=_lib.SS2D_BF16, weight_dtype=_lib.SS2D_F32, eps=1e-6, q=256, k=256, q_out=256, k_out=256)
+    make = lambda **change: fill(_lib.QkNormRotateParams(), **(full | change))  # noqa: E731
+    turned = dict(positions=256, frequencies=256, axes=2, per_axis=16)
+    assert L.ss2d_qk_norm_rotate(None, None) == _lib.SS2D_EINVAL
+    for change in (dict(batch=-1), dict(seqlen=-1), dict(q_heads=-1), dict(k_heads=-1), dict(dim=0), dict(dtype=5), dict(q_weight=256, weight_dtype=_lib.SS2D_F16), dict(q=None), dict(k=None),
+                   dict(q_out=None), dict(k_out=None), turned | dict(frequencies=None), turned | dict(axes=0), turned | dict(per_axis=17), turned | dict(axes=2 ** 30, per_axis=4),
+                   dict(k_heads=2 ** 30)):
+        assert L.ss2d_qk_norm_rotate(make(**change), None) == _lib.SS2D_EINVAL, change
+    assert L.ss2d_qk_norm_rotate(make(dim=513), None) == _lib.SS2D_ENOTSUP
+    for empty in (dict(batch=0), dict(seqlen=0), dict(q_heads=0, k_heads=0)):
+        assert L.ss2d_qk_norm_rotate(make(**empty, q=None, k=None, q_out=None, k_out=None), None) == _lib.SS2D_OK
+    need = L.ss2d_qk_norm_rotate_bwd_workspace_bytes(64)
+    assert need > 0 and L.ss2d_qk_norm_rotate_bwd_workspace_bytes(0) == _lib.SS2D_EINVAL and L.ss2d_qk_norm_rotate_bwd_workspace_bytes(513) == _lib.SS2D_EINVAL
+    grads = dict(dq_out=256, dk_out=256, dq=256, dk=256)
+    back = lambda fwd, **change: fill(_lib.QkNormRotateBwdParams(), **(grads | dict(fwd=fwd) | change))  # noqa: E731
+    assert L.ss2d_qk_norm_rotate_bwd(None, HERE, need, None) == _lib.SS2D_EINVAL
+    for missing in grads:
+        assert L.ss2d_qk_norm_rotate_bwd(back(make(), **{missing: None}), HERE, need, None) == _lib.SS2D_EINVAL
+    assert L.ss2d_qk_norm_rotate_bwd(back(make(), dq_weight=256), HERE, need, None) == _lib.SS2D_EINVAL          # of a weight that is not there
+    weighed = make(q_weight=256)
+    assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), None, need, None) == _lib.SS2D_EINVAL
+    assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), ctypes.c_void_p(260), need, None) == _lib.SS2D_EINVAL
+    assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), HERE, need - 1, None) == _lib.SS2D_ENOMEM

@@ -428,3 +428,125 @@ def test_two_streams_and_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(mine, state)
+
+
+@pytest.mark.parametrize("shape", [(1, 70, 2, 1, 2, 65, 64), (2, 70, 2, 2, 2, 64, 129), (1, 129, 1, 1, 1, 200, 33), (1, 65, 2, 2, 1, 128, 96), (1, 40, 1, 1, 3, 48, 80)], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_dimensions_between_the_kernels(shape, dtype):
+    """Both sides of the dimensions at which another kernel is taken, with all that the backward can be asked for."""
+    print("CASE dimensions", shape, dtype, flush=True)
+    B, T, Hq, Hk, Hv, dk, dv = shape
+    q, k, v, g, dout, normal = inputs(*shape, dtype, ("token", 1), 3)
+    state, dfinal = (normal(B, max(Hq, Hk, Hv), dk, dv).to(DEV) for _ in range(2))
+    got = run_all(q, k, v, g, state, dout, dfinal)
+    want, size = reference(q, k, v, g, state, dk ** -0.5, [(b, 0, T) for b in range(B)], dout, dfinal)
+    for name in got:
+        check(name, got[name], want[name], size[name], dtype, (dk, dv, 0), T)
+
+
+def test_far_apart_in_memory():
+    """Tokens 2^24 bytes apart, and batches more than 2^31 values apart: the same bits as side by side."""
+    q, k, v, g, dout, normal = inputs(2, 40, 2, 2, 2, 32, 16, BF16, ("token", 1), 5)
+    want = run_all(q, k, v, g, None, dout, None)
+    memory = torch.zeros(2 ** 31 + 2 ** 20, dtype=BF16, device=DEV)
+    far = memory.as_strided(k.shape, (2 ** 31 + 64, 80, 32, 1)).copy_(k)
+    again = run_all(q, far, v, g, None, dout, None)
+    assert far.stride(0) > 2 ** 31 and all(torch.equal(want[n], again[n]) for n in want)
+    far = memory.as_strided(v.shape, (40 * 2 ** 23 + 64, 2 ** 23, 16, 1)).copy_(v)
+    assert far.stride(1) * 2 == 2 ** 24
+    again = run_all(q, k, far, g, None, dout, None)
+    assert all(torch.equal(want[n], again[n]) for n in want)
+    again = run_all(q, k, v, g, None, memory.as_strided(dout.shape, (40 * 2 ** 23 + 64, 2 ** 23, 16, 1)).copy_(dout), None)
+    assert all(torch.equal(want[n], again[n]) for n in want)
+
+
+def test_a_long_sequence_behind_many_empty_ones():
+    """More pieces of states to join than a launch has workgroups; the same bits as of the long sequence alone."""
+    q, k, v, g, dout, normal = inputs(1, 5000, 4, 4, 4, 16, 16, BF16, ("token", 1), 9)
+    alone = torch.tensor([0, 5000], dtype=torch.int32, device=DEV)
+    many = torch.tensor([0] * 70000 + [5000], dtype=torch.int32, device=DEV)
+    dfinal = normal(1, 4, 16, 16).to(DEV)
+    want = run_all(q, k, v, g, None, dout, dfinal, cu=alone)
+    got = run_all(q, k, v, g, None, dout, torch.cat([torch.zeros(69999, 4, 16, 16, device=DEV), dfinal]), cu=many)
+    for name in want:
+        assert torch.equal(want[name], got[name][-1:] if name == "final" else got[name]), name
+    assert not got["final"][:-1].any()
+
+
+def test_broadcast_inputs_and_gradients():
+    """Inputs that repeat one row of memory, and gradients that do (sum().backward()): those of the same values laid out whole."""
+    q, k, v, g, dout, normal = inputs(3, 80, 4, 1, 4, 32, 24, BF16, ("head", 1), 11)
+    leaf = k[:1].detach().requires_grad_()
+    out = linear_attention_fn(q, leaf.expand(3, -1, 4, -1), v, g)
+    out.sum().backward()
+    whole = k[:1].repeat(3, 1, 4, 1).requires_grad_()
+    other = linear_attention_fn(q, whole, v, g)
+    assert torch.equal(out, other)
+    other.backward(torch.ones_like(other))
+    assert torch.equal(leaf.grad, whole.grad.sum((0, 2), keepdim=True))
+
+
+class Seen(torch.overrides.TorchFunctionMode):
+    """A mode that follows operators: the calls then go through Python."""
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+def test_through_python_as_through_the_extension():
+    from vmamba_amd.norm import native_stands
+    q, k, v, g, dout, normal = inputs(1, 90, 4, 2, 4, 40, 24, BF16, ("token", 1), 13)
+    state, dfinal = normal(2, 4, 40, 24).to(DEV), normal(2, 4, 40, 24).to(DEV)
+    cu = torch.tensor([3, 50, 85], dtype=torch.int32, device=DEV)
+    want = run_all(q, k, v, g, state, dout, dfinal, cu=cu)
+    with Seen():
+        assert not native_stands(q)
+        got = run_all(q, k, v, g, state, dout, dfinal, cu=cu)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+    token, mine, theirs = (q[0, 0, None], k[0, 0, None], v[0, 0, None], g[0, 0]), state[:1].clone(), state[:1].clone()
+    want = linear_attention_step_fn(*token, mine)
+    with Seen():
+        got = linear_attention_step_fn(*token, theirs)
+    assert torch.equal(want, got) and torch.equal(mine, theirs)
+
+
+@pytest.mark.parametrize("seen", [False, True])
+def test_gradients_that_are_refused(seen):
+    """Second derivatives, a batch of gradients at once, and saved tensors of which a hook made something else; what a hook brings back whole is taken."""
+    import contextlib
+    q, k, v, g, dout, normal = inputs(1, 50, 2, 2, 2, 16, 16, F32, ("token", 1), 17)
+    want = run_all(q, k, v, g, None, dout, None)
+    with Seen() if seen else contextlib.nullcontext():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, g)]
+        out = linear_attention_fn(*leaves)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(out, leaves, dout, create_graph=True)
+        out = linear_attention_fn(*leaves)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, leaves, torch.stack([dout, dout]), is_grads_batched=True)
+        with torch.autograd.graph.save_on_cpu():
+            out = linear_attention_fn(*leaves)
+        for d, name in zip(torch.autograd.grad(out, leaves, dout), ("dq", "dk", "dv", "dg")):
+            assert torch.equal(d, want[name])
+        for spoil in (lambda t: t.cpu(), lambda t: t[:, :7], lambda t: t.double(), lambda t: t.transpose(0, 1)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spoil):
+                out = linear_attention_fn(*leaves)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(out, leaves, dout)
+
+
+@pytest.mark.parametrize("seen", [False, True])
+def test_step_and_autograd(seen):
+    """The state's change is seen by what saved it; inference mode and its tensors are taken."""
+    import contextlib
+    token = [torch.randn(2, 2, 16, device=DEV) for _ in range(3)]
+    state, w = torch.randn(2, 2, 16, 16, device=DEV), torch.randn(2, 2, 16, 16, device=DEV, requires_grad=True)
+    with Seen() if seen else contextlib.nullcontext():
+        product = state * w
+        linear_attention_step_fn(*token, None, state)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+        with torch.inference_mode():
+            mine = state.clone()
+            out = linear_attention_step_fn(*token, None, mine)
+        want = linear_attention_step_fn(*token, None, state)
+    assert torch.equal(out, want) and torch.equal(mine, state)

@@ -236,3 +236,64 @@ def test_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+class Seen(torch.overrides.TorchFunctionMode):
+    """A mode that follows operators: the calls then go through Python."""
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("seen", [False, True])
+def test_through_python_and_what_is_refused(seen):
+    """The Python path gives the extension's bits; second derivatives, batches of gradients and saved tensors of which a hook made something else are refused."""
+    import contextlib
+    q, k, ws, at, f, normal = case(2, 33, 4, 2, 40, BF16, F32, 32, 2)
+    douts = [normal(*t.shape).to(DEV, BF16) for t in (q, k)]
+
+    def step(**more):
+        leaves = [t.detach().requires_grad_() for t in (q, k, *ws)]
+        outs = qk_norm_rotate_fn(*leaves, at, f)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, **{"grad_outputs": douts} | more))
+
+    want = step()
+    with Seen() if seen else contextlib.nullcontext():
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            step(create_graph=True)
+        with pytest.raises(RuntimeError):
+            step(grad_outputs=[torch.stack([t, t]) for t in douts], is_grads_batched=True)
+        with torch.autograd.graph.save_on_cpu():
+            assert all(torch.equal(a, b) for a, b in zip(step(), want))
+        for spoil in (lambda t: t.cpu(), lambda t: t[:, :7] if t.dim() > 2 else t, lambda t: t.double()):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spoil), pytest.raises(RuntimeError):
+                step()
+
+
+def test_one_gradient_alone():
+    """Of queries alone, of a weight alone, and of one output's gradient alone."""
+    q, k, ws, at, f, normal = case(2, 20, 4, 2, 32, F32, F32, 32, 1)
+    dq, dk = (normal(*t.shape).to(DEV) for t in (q, k))
+    leaves = [t.detach().requires_grad_() for t in (q, k, *ws)]
+    outs = qk_norm_rotate_fn(*leaves, at, f)
+    whole = torch.autograd.grad(outs, leaves, [dq, torch.zeros_like(dk)], retain_graph=True)
+    alone = torch.autograd.grad(outs[0], leaves, dq, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(whole, alone))
+    for i, leaf in enumerate(leaves):
+        args = [t.detach() for t in (q, k, *ws)]
+        args[i] = leaf
+        out = qk_norm_rotate_fn(*args, at, f)
+        assert torch.equal(torch.autograd.grad(out[0] if i in (0, 2) else out[1], leaf, dq if i in (0, 2) else dk)[0],
+                           torch.autograd.grad(outs, leaf, [dq, dk], retain_graph=True)[0])
+
+
+def test_more_rows_than_a_launch_has_workgroups():
+    """2^26 and some tokens, 16 to a workgroup's round: the last ones as they come alone."""
+    T = 2 ** 26 + 1000
+    q = torch.zeros(1, T, 1, 8, dtype=BF16, device=DEV)
+    q[:, -3000:] = torch.randn(1, 3000, 1, 8, device=DEV)
+    weight = torch.randn(8, device=DEV)
+    outs = qk_norm_rotate_fn(q, q, weight, weight)
+    alone = qk_norm_rotate_fn(q[:, -3000:], q[:, -3000:], weight, weight)
+    for out, want in zip(outs, alone):
+        assert torch.equal(out[:, -3000:], want) and not out[:, :-3000].any()

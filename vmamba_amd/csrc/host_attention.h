@@ -29,8 +29,8 @@ inline bool recorded(std::initializer_list<const at::Tensor *> tensors) {
 }
 template <typename P> void strides3(const at::Tensor &t, P &batch, P &token, P &head) { batch = t.stride(0); token = t.stride(1); head = t.stride(2); }
 // What comes into a backward: memory on the inputs' device, its last dimension dense
-inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, const char *name) {
-    TORCH_CHECK(on_gpu(g, x), name, " must be a plain tensor with memory of its own, on the device of q");
+inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, at::IntArrayRef shape, const char *name) {
+    TORCH_CHECK(on_gpu(g, x) && has_shape(g, shape), name, " must be a plain tensor with memory of its own, on the device of q and shaped as what it is the gradient of");
     return dense_last(g) ? g : g.contiguous();
 }
 
@@ -105,6 +105,16 @@ inline variable_list attend(const Sides &s, const at::Tensor &state, const at::T
     return made;
 }
 
+inline bool state_fits(const at::Tensor &state, const at::Tensor &q, at::IntArrayRef shape) {
+    return !state.defined() || (on_gpu(state, q) && state.scalar_type() == at::kFloat && has_shape(state, shape));
+}
+
+inline bool sequences_fit(const Sides &s, const at::Tensor &state, const at::Tensor &cu) {
+    if (cu.defined() && (!on_gpu(cu, s.q) || cu.scalar_type() != at::kInt || cu.dim() != 1 || cu.numel() < 2 || cu.numel() > INT32_MAX || !cu.is_contiguous() || s.q.size(0) != 1))
+        return false;
+    return state_fits(state, s.q, {cu.defined() ? cu.numel() - 1 : s.q.size(0), s.heads, s.q.size(3), s.v.size(3)}) && (!state.defined() || state.is_contiguous());
+}
+
 struct LinearAttention : torch::autograd::Function<LinearAttention> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const Maybe &decay_in, const Maybe &state_in,
                                  const Maybe &cu_in, double scale, bool want_final) {
@@ -121,14 +131,16 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_attention_fn is differentiable once: its gradients have none (create_graph)");
         const variable_list saved = ctx->get_saved_variables();
         Sides s = {saved[0], saved[1], saved[2], saved[3]};
-        s.read(4);
         const at::Tensor &state = saved[4], &cu = saved[5];
+        TORCH_CHECK(s.read(4) && sequences_fit(s, state, cu), "linear_attention_fn: what a hook made of its saved tensors is not what it saved");
         variable_list result(8);
         at::Tensor dout = grads[0], dfinal = grads.size() > 1 ? grads[1] : at::Tensor();
         if (!dout.defined() && !dfinal.defined()) return result;
-        if (!dout.defined()) dout = at::zeros({s.q.size(0), s.q.size(1), s.heads, s.v.size(3)}, s.q.options());
-        dout = gradient(dout, s.q, "dout");
-        if (dfinal.defined()) dfinal = gradient(dfinal, s.q, "dfinal").contiguous();
+        const int64_t n_seqs = cu.defined() ? cu.numel() - 1 : s.q.size(0), out_shape[4] = {s.q.size(0), s.q.size(1), s.heads, s.v.size(3)},
+                      state_shape[4] = {n_seqs, s.heads, s.q.size(3), s.v.size(3)};
+        if (!dout.defined()) dout = at::zeros(out_shape, s.q.options());
+        dout = gradient(dout, s.q, out_shape, "dout");
+        if (dfinal.defined()) dfinal = gradient(dfinal, s.q, state_shape, "dfinal").contiguous();
         ss2d_linear_attention_bwd_params p = {};
         p.fwd = describe(s, state, cu, ctx->saved_data["scale"].toDouble());
         for (int i = 0; i < 3; ++i) result[i] = at::empty(saved[i].sizes(), saved[i].options());
@@ -146,22 +158,13 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     }
 };
 
-inline bool state_fits(const at::Tensor &state, const at::Tensor &q, at::IntArrayRef shape) {
-    return !state.defined() || (on_gpu(state, q) && state.scalar_type() == at::kFloat && has_shape(state, shape));
-}
-
 // linear_attention.py:linear_attention_fn -- (out,) or (out, final state), or None
 static py::object linear_attention(const py::tuple &kinds, const py::object &q, const py::object &k, const py::object &v, const py::object &decay, const py::object &state_in,
                                    const py::object &cu_in, c10::optional<double> scale_in, bool want_final) {
     bool ok = true;
     Sides s = {exactly(q, kinds, ok), exactly(k, kinds, ok), exactly(v, kinds, ok), exactly(decay, kinds, ok)};
-    at::Tensor state = exactly(state_in, kinds, ok);
-    const at::Tensor cu = exactly(cu_in, kinds, ok);
-    if (!ok || !s.read(4)) return py::none();
-    if (cu.defined() && (!on_gpu(cu, s.q) || cu.scalar_type() != at::kInt || cu.dim() != 1 || cu.numel() < 2 || cu.numel() > INT32_MAX || !cu.is_contiguous() || s.q.size(0) != 1))
-        return py::none();
-    if (!state_fits(state, s.q, {cu.defined() ? cu.numel() - 1 : s.q.size(0), s.heads, s.q.size(3), s.v.size(3)})) return py::none();
-    if (state.defined() && !state.is_contiguous()) return py::none();
+    const at::Tensor state = exactly(state_in, kinds, ok), cu = exactly(cu_in, kinds, ok);
+    if (!ok || !s.read(4) || !sequences_fit(s, state, cu)) return py::none();
     const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt((double)s.q.size(3));
     const variable_list made = recorded({&s.q, &s.k, &s.v, &s.decay, &state}) ? LinearAttention::apply(s.q, s.k, s.v, maybe(s.decay), maybe(state), maybe(cu), scale, want_final)
                                                                            : attend(s, state, cu, scale, want_final);
@@ -202,7 +205,7 @@ struct NormArgs {
     double eps;
     bool interleaved;
 
-    bool read() {
+    bool read() const {
         if (!q.defined() || !q.is_cuda() || !plain(q) || !on_gpu(k, q) || dtype_code(q.scalar_type()) < 0 || k.scalar_type() != q.scalar_type()) return false;
         if (q.dim() != 4 || k.dim() != 4 || k.size(0) != q.size(0) || k.size(1) != q.size(1) || k.size(3) != q.size(3)) return false;
         if (q.size(3) < 1 || q.size(3) > kMaxNorm || !dense_last(q) || !dense_last(k)) return false;
@@ -270,7 +273,8 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rotate_fn is differentiable once: its gradients have none (create_graph)");
         const variable_list saved = ctx->get_saved_variables();
         const NormArgs a = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
-        const at::Tensor dq = gradient(grads[0], a.q, "dq_out"), dk = gradient(grads[1], a.q, "dk_out");
+        TORCH_CHECK(a.read(), "qk_norm_rotate_fn: what a hook made of its saved tensors is not what it saved");
+        const at::Tensor dq = gradient(grads[0], a.q, a.q.sizes(), "dq_out"), dk = gradient(grads[1], a.q, a.k.sizes(), "dk_out");
         variable_list result(8);
         result[0] = at::empty(a.q.sizes(), a.q.options());
         result[1] = at::empty(a.k.sizes(), a.k.options());

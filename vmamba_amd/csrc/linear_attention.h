@@ -19,6 +19,8 @@ namespace ss2d {
 
 constexpr int kLaMaxDim = 256;       // of a key or value
 constexpr int kLaTile = 64;          // sides of the piece of a state that a workgroup walks
+constexpr int kLaThreads = 512;      // of the largest workgroups
+constexpr int64_t kLaLaunch = 0xffffffff;                            // threads of a launch
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LaSide {                      // q, k, v, out or a gradient: (batch, token, head, dim), the last one dense
@@ -234,7 +236,8 @@ struct LaWalk {
     int32_t reverse;                 // from the last chunk to the first, weights scale exp(G_t) instead of exp(G_C - G_s)
     int32_t exact;                   // the states are kept in 32 bits: three parts to a weighted 16-bit operand instead of two
 };
-int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest);                        // sizes of the tables and segments, for `tiles` workgroups a head
+// Sizes of the tables and segments, for `tiles` workgroups a head; a launch takes `lanes` threads for each chunk and head.
+int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes);
 int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
 template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w, int n, void *stream);        // states before all chunks, one walk or two side by side
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }            // (what is below 2^-126 is 0)

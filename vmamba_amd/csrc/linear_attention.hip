@@ -308,13 +308,14 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 
 // What comes into each segment of a sequence, from the segments' own sums: in their place.  A workgroup takes 16 columns of a piece; the sums of
 // sixteen segments are on their way at once.
-__global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, int chunk, uint32_t total) {
+constexpr uint32_t kLaJoins = 1 << 20;
+__device__ __forceinline__ void la_join(const LaArgs &p, const LaWalk &w0, const LaWalk &w1, int chunk, uint32_t total, uint32_t at_block) {
     constexpr int kAhead = 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const bool second = blockIdx.x >= total;
+    const bool second = at_block >= total;
     const LaWalk w = second ? w1 : w0;
     const int tiles_a = (w.a.dim + kLaTile - 1) / kLaTile, tiles = tiles_a * ((w.b.dim + kLaTile - 1) / kLaTile);
-    const uint32_t block = second ? blockIdx.x - total : blockIdx.x, id = block / 4;
+    const uint32_t block = second ? at_block - total : at_block, id = block / 4;
     const int i = block % 4, tile = id % (uint32_t)tiles, h = id / (uint32_t)tiles % (uint32_t)p.heads, n = id / (uint32_t)tiles / (uint32_t)p.heads;
     const int4 s = la_sequence(p, n);
     const int n_chunks = (s.y - s.x + chunk - 1) / chunk, segs = (n_chunks + p.seg_chunks - 1) / p.seg_chunks;
@@ -345,6 +346,9 @@ __global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const L
             }
     }
 }
+__global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, int chunk, uint32_t total, uint32_t all) {
+    for (uint32_t block = blockIdx.x; block < all; block += gridDim.x) la_join(p, w0, w1, chunk, total, block);
+}
 
 static int64_t la_tiles(const LaArgs &p) { return (int64_t)((p.k.dim + kLaTile - 1) / kLaTile) * ((p.v.dim + kLaTile - 1) / kLaTile); }
 
@@ -366,8 +370,8 @@ template <typename Op, typename T, bool kLocal, bool kBoth> static void la_walk_
 template <typename Op, typename T> static int la_segments(const LaArgs &p, const LaWalk *w, int n, hipStream_t st) {
     if (p.max_segs <= p.n_seqs) return SS2D_OK;
     la_walk_launch<Op, T, true, false>(p, w, n, st);
-    const uint32_t total = (uint32_t)((int64_t)p.n_seqs * p.heads * la_tiles(p) * 4);
-    la_join_kernel<<<total * (uint32_t)n, kBlock, 0, st>>>(p, w[0], w[n - 1], Op::kChunk, total);
+    const uint32_t total = (uint32_t)((int64_t)p.n_seqs * p.heads * la_tiles(p) * 4), grid = total * (uint32_t)n;
+    la_join_kernel<<<grid < kLaJoins ? grid : kLaJoins, kBlock, 0, st>>>(p, w[0], w[n - 1], Op::kChunk, total, grid);
     return launch_status();
 }
 
@@ -392,7 +396,7 @@ template int la_walks<OperandBf16, bf16_t>(const LaArgs &, const LaWalk *, int, 
 // out transposed (lane: one token, four neighbouring values), so that what a token has to be multiplied with is one value of the lane.
 // The weights behind the diagonal are zeros; a product of zero with what is infinite or NaN would reach tokens in front of it, so a
 // chunk that holds such a value sums its pairs one by one.
-constexpr int kLaThreads = 512, kLaWaves = kLaThreads / kWave;
+constexpr int kLaWaves = kLaThreads / kWave;
 
 template <typename Op, typename T, int kTiles, int kParts, bool kFast>
 __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel(const LaArgs p, const LaWalk w, uint32_t total) {
@@ -617,7 +621,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void la_nobody_kernel
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 // Segments: where the sequences alone do not give the chip its workgroups (two to a CU, of `tiles` for a head), each is cut so that they do, into
 // `shortest` chunks at least: a segment is walked twice.
-int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
+int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
     const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= (tiles > (p.v.dim + kLaTile - 1) / kLaTile ? 384 : 192) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk;
     int64_t chunks, segs, seg_chunks;
@@ -634,7 +638,7 @@ int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest) {
         p.segs_per_seq = per_seq <= seg_chunks ? 1 : (int)((per_seq + seg_chunks - 1) / seg_chunks);
         segs = (int64_t)p.segs_per_seq * p.n_seqs;
     }
-    if (chunks * p.heads > 0x7fffffff / 4 || segs * p.heads * la_tiles(p) > 0x7fffffff / 16) return SS2D_EINVAL;
+    if (chunks > kLaLaunch / lanes / p.heads || segs > kLaLaunch / kLaThreads / p.heads / la_tiles(p)) return SS2D_ENOTSUP;
     p.per_seq = (int)per_seq;
     p.max_chunks = (int)chunks;
     p.seg_chunks = (int)seg_chunks;
@@ -694,7 +698,7 @@ LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int 
     s.batch = batch; s.token = token; s.head = head;
     s.div = own_heads > 0 ? heads / own_heads : 1;
     s.dim = dim;
-    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0 && token * size < (1 << 24);
+    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0 && token >= 0 && token * size < (1 << 24);
     return s;
 }
 
@@ -733,7 +737,7 @@ int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) 
 
 static int la_forward_plan(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) {
     const int rc = la_arguments(p, a, empty);
-    return rc != SS2D_OK || empty ? rc : la_plan(a, la_chunk(p->dtype), (a.v.dim + kLaTile - 1) / kLaTile, 2);
+    return rc != SS2D_OK || empty ? rc : la_plan(a, la_chunk(p->dtype), (a.v.dim + kLaTile - 1) / kLaTile, 2, la_chunk(p->dtype));
 }
 
 static int64_t la_round(int64_t n) { return (n + 255) / 256 * 256; }

@@ -517,7 +517,7 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
     const int rc = la_arguments(&f, b.a, empty);
     if (rc != SS2D_OK || empty) return rc;
     LaArgs &a = b.a;
-    const int planned = la_plan(a, la_chunk(f.dtype), (int64_t)((f.key_dim + kLaTile - 1) / kLaTile) * ((f.value_dim + kLaTile - 1) / kLaTile) * 2, 4);
+    const int planned = la_plan(a, la_chunk(f.dtype), (int64_t)((f.key_dim + kLaTile - 1) / kLaTile) * ((f.value_dim + kLaTile - 1) / kLaTile) * 2, 4, kLaThreads);
     if (planned != SS2D_OK) return planned;
     const int size = f.dtype == SS2D_F32 ? 4 : 2;
     if (params->ddecay && !f.decay) return SS2D_EINVAL;

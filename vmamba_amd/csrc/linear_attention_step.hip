@@ -80,7 +80,7 @@ template <typename T> static int la_step(const LaStepArgs &a, int batch, hipStre
     const bool vec = dv % 4 == 0 && (uintptr_t)a.state % 16 == 0 && a.state_batch % 4 == 0;
     auto go = [&](auto kernel, int cols) {
         const int64_t tiles = (dv + cols - 1) / cols, total = heads * tiles;
-        if (total > 0x7fffffff) return (int)SS2D_EINVAL;
+        if (total > kLaLaunch / kBlock) return (int)SS2D_ENOTSUP;
         kernel<<<(uint32_t)total, kBlock, 0, stream>>>(a, (int)tiles);
         return launch_status();
     };

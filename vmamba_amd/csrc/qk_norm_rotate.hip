@@ -405,6 +405,7 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
 }
 
 constexpr int64_t kQnShares = 1024;                                  // workgroups of the backward: four to a CU
+constexpr int64_t kQnGrid = 1 << 22;                                 // of the forward (a launch's threads fit 32 bits)
 
 template <typename T, bool kBack> static int qn_launch(const QnArgs &a, bool vec, uint32_t grid, hipStream_t st) {
     if (!vec) qk_norm_rotate_any_kernel<T, kBack><<<grid, kBlock, 0, st>>>(a);
@@ -426,12 +427,12 @@ extern "C" int ss2d_qk_norm_rotate(const ss2d_qk_norm_rotate_params *p, void *st
     const int rc = qn_arguments(p, a, vec, false, nullptr);
     if (rc != SS2D_OK || a.rounds == 0) return rc;
     if ((p->q_heads && (!p->q || !p->q_out)) || (p->k_heads && (!p->k || !p->k_out))) return SS2D_EINVAL;
-    if (a.rounds > 0x7fffffff) return SS2D_EINVAL;
+    const uint32_t grid = (uint32_t)(a.rounds < kQnGrid ? a.rounds : kQnGrid);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (p->dtype) {
-    case SS2D_F32: return qn_launch<float, false>(a, vec, (uint32_t)a.rounds, st);
-    case SS2D_BF16: return qn_launch<bf16_t, false>(a, vec, (uint32_t)a.rounds, st);
-    default: return qn_launch<f16_t, false>(a, vec, (uint32_t)a.rounds, st);
+    case SS2D_F32: return qn_launch<float, false>(a, vec, grid, st);
+    case SS2D_BF16: return qn_launch<bf16_t, false>(a, vec, grid, st);
+    default: return qn_launch<f16_t, false>(a, vec, grid, st);
     }
 }
 

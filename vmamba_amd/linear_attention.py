@@ -43,7 +43,7 @@ def _dense_last(t):
 def _check_sides(q, k, v, what, rank):
     check_plain(q, q=q, k=k, v=v)
     _check(q.dtype in _DTYPE_CODE, f"{what} not implemented for input type '{q.dtype}'")
-    _check(k.dtype == q.dtype and v.dtype == q.dtype, "k and v must have q's dtype")
+    _check(k is not None and v is not None and k.dtype == q.dtype and v.dtype == q.dtype, "k and v must have q's dtype")
     layout = "(batch, tokens, heads, dim)" if rank == 4 else "(batch, heads, dim)"
     _check(q.dim() == rank and k.dim() == rank and v.dim() == rank, f"q, k, v must be {layout}")
     _check(k.shape[:-2] == q.shape[:-2] and v.shape[:-2] == q.shape[:-2], f"q, k, v must agree in {'batch and tokens' if rank == 4 else 'batch'}")
@@ -70,6 +70,20 @@ def _check_state(state, q, shape, name):
         return
     check_plain(q, **{name: state})
     _check(state.dtype == torch.float32 and tuple(state.shape) == shape, f"{name} must be float32 of shape {shape}")
+
+
+def _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens):
+    heads = _check_sides(q, k, v, "linear_attention_fn", 4)
+    _check_decay(log_decay, q, heads, (q.shape[0], q.shape[1], heads))
+    n_seqs = q.shape[0]
+    if cu_seqlens is not None:
+        check_plain(q, cu_seqlens=cu_seqlens)
+        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must be int32 of shape (sequences + 1,)")
+        _check(cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous")
+        _check(q.shape[0] == 1, "packed sequences (cu_seqlens) must stand in a batch of one")
+        n_seqs = cu_seqlens.numel() - 1
+    _check_state(initial_state, q, (n_seqs, heads, q.shape[3], v.shape[3]), "initial_state")
+    return heads, n_seqs
 
 
 def _params(q, k, v, log_decay, scale, initial_state, cu_seqlens, heads, out, final_state):
@@ -139,16 +153,17 @@ class LinearAttentionHip(torch.autograd.Function):
     def backward(ctx, dout, dfinal):
         _check(not torch.is_grad_enabled(), "linear_attention_fn is differentiable once: its gradients have none (create_graph)")
         q, k, v, log_decay, initial_state, cu_seqlens = ctx.saved_tensors
-        heads = max(q.shape[2], k.shape[2], v.shape[2])
+        heads, n_seqs = _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens)          # (a hook may have made something else of them)
         if dout is None:
             if dfinal is None:
                 return (None,) * 8
             dout = q.new_zeros((*q.shape[:2], heads, v.shape[3]))
         check_plain(q, dout=dout, dfinal=dfinal)
+        _check(tuple(dout.shape) == (*q.shape[:2], heads, v.shape[3]), "dout must have out's shape")
+        _check(dfinal is None or tuple(dfinal.shape) == (n_seqs, heads, q.shape[3], v.shape[3]), "dfinal must have final_state's shape")
         if not _dense_last(dout):
             dout = dout.contiguous()
-        if dfinal is not None:
-            dfinal = dfinal.contiguous()
+        dfinal, initial_state = (t if t is None else t.contiguous() for t in (dfinal, initial_state))
         want = ctx.needs_input_grad
         dq, dk, dv, ddecay, dstate = linear_attention_bwd(q, k, v, log_decay, ctx.scale, initial_state, cu_seqlens, dout, dfinal,
                                                           log_decay is not None and want[3], initial_state is not None and want[4])
@@ -174,16 +189,7 @@ def linear_attention_fn(q, k, v, log_decay=None, scale=None, initial_state=None,
         native = _lib.host().linear_attention(TENSOR_KINDS, q, k, v, log_decay, initial_state, cu_seqlens, scale, bool(output_final_state))
         if native is not None:
             return native
-    heads = _check_sides(q, k, v, "linear_attention_fn", 4)
-    _check_decay(log_decay, q, heads, (q.shape[0], q.shape[1], heads))
-    n_seqs = q.shape[0]
-    if cu_seqlens is not None:
-        check_plain(q, cu_seqlens=cu_seqlens)
-        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must be int32 of shape (sequences + 1,)")
-        _check(cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous")
-        _check(q.shape[0] == 1, "packed sequences (cu_seqlens) must stand in a batch of one")
-        n_seqs = cu_seqlens.numel() - 1
-    _check_state(initial_state, q, (n_seqs, heads, q.shape[3], v.shape[3]), "initial_state")
+    _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens)
     if initial_state is not None:
         initial_state = initial_state.contiguous()
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)

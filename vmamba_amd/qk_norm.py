@@ -16,6 +16,29 @@ _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, tor
 MAX_DIM = 512
 
 
+def _check_all(q, k, q_weight, k_weight, positions, frequencies):
+    check_plain(q, q=q, k=k, q_weight=q_weight, k_weight=k_weight, positions=positions, frequencies=frequencies)
+    _check(q.dtype in _DTYPE_CODE, f"qk_norm_rotate_fn not implemented for input type '{q.dtype}'")
+    _check(k is not None and k.dtype == q.dtype, "k must have q's dtype")
+    _check(q.dim() == 4 and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3],
+           "q and k must be (batch, tokens, heads, dim) and agree in batch, tokens and dim")
+    _check(1 <= q.shape[3] <= MAX_DIM, f"heads must have 1 to {MAX_DIM} values")
+    for name, t in (("q", q), ("k", k)):
+        _check(_dense_last(t), f"{name} must be contiguous in its last dimension")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        _check(w.dtype in (torch.float32, q.dtype) and w.dtype == weights[0].dtype, "weights must be of one type, float32 or q's dtype")
+        _check(tuple(w.shape) == (q.shape[3],), f"weights must have shape ({q.shape[3]},)")
+    _check((positions is None) == (frequencies is None), "positions and frequencies go together")
+    if positions is not None:
+        _check(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
+        _check(frequencies.dtype in (torch.float32, torch.float64) and frequencies.dim() in (1, 2), "frequencies must be float32 or float64 of shape (pairs,) or (axes, pairs)")
+        axes = (frequencies.shape[0],) if frequencies.dim() == 2 else ()
+        _check(tuple(positions.shape) in ((*q.shape[:2], *axes), (q.shape[1], *axes)),
+               f"positions must have shape {(*q.shape[:2], *axes)} or {(q.shape[1], *axes)}")
+        _check(2 * frequencies.numel() <= q.shape[3], f"a head of {q.shape[3]} values has no {frequencies.numel()} pairs")
+
+
 def _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
     p = _lib.QkNormRotateParams()
     p.batch, p.seqlen, p.q_heads, p.dim = q.shape
@@ -50,7 +73,10 @@ class QkNormRotateHip(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         _check(not torch.is_grad_enabled(), "qk_norm_rotate_fn is differentiable once: its gradients have none (create_graph)")
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+        _check_all(q, k, q_weight, k_weight, positions, frequencies)               # (a hook may have made something else of them)
+        q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
         check_plain(q, dq_out=dq_out, dk_out=dk_out)
+        _check(dq_out.shape == q.shape and dk_out.shape == k.shape, "gradients must have the outputs' shapes")
         dq_out, dk_out = (t if _dense_last(t) else t.contiguous() for t in (dq_out, dk_out))
         g = _lib.QkNormRotateBwdParams()
         g.fwd = _params(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved)
@@ -82,26 +108,6 @@ def qk_norm_rotate_fn(q, k, q_weight=None, k_weight=None, positions=None, freque
         native = _lib.host().qk_norm_rotate(TENSOR_KINDS, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
         if native is not None:
             return native
-    check_plain(q, q=q, k=k, q_weight=q_weight, k_weight=k_weight, positions=positions, frequencies=frequencies)
-    _check(q.dtype in _DTYPE_CODE, f"qk_norm_rotate_fn not implemented for input type '{q.dtype}'")
-    _check(k is not None and k.dtype == q.dtype, "k must have q's dtype")
-    _check(q.dim() == 4 and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3],
-           "q and k must be (batch, tokens, heads, dim) and agree in batch, tokens and dim")
-    _check(1 <= q.shape[3] <= MAX_DIM, f"heads must have 1 to {MAX_DIM} values")
-    for name, t in (("q", q), ("k", k)):
-        _check(_dense_last(t), f"{name} must be contiguous in its last dimension")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        _check(w.dtype in (torch.float32, q.dtype) and w.dtype == weights[0].dtype, "weights must be of one type, float32 or q's dtype")
-        _check(tuple(w.shape) == (q.shape[3],), f"weights must have shape ({q.shape[3]},)")
-    q_weight, k_weight = (w.contiguous() if w is not None else None for w in (q_weight, k_weight))
-    _check((positions is None) == (frequencies is None), "positions and frequencies go together")
-    if positions is not None:
-        _check(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
-        _check(frequencies.dtype in (torch.float32, torch.float64) and frequencies.dim() in (1, 2), "frequencies must be float32 or float64 of shape (pairs,) or (axes, pairs)")
-        axes = (frequencies.shape[0],) if frequencies.dim() == 2 else ()
-        _check(tuple(positions.shape) in ((*q.shape[:2], *axes), (q.shape[1], *axes)),
-               f"positions must have shape {(*q.shape[:2], *axes)} or {(q.shape[1], *axes)}")
-        _check(2 * frequencies.numel() <= q.shape[3], f"a head of {q.shape[3]} values has no {frequencies.numel()} pairs")
-        frequencies = frequencies.contiguous()
+    _check_all(q, k, q_weight, k_weight, positions, frequencies)
+    q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
     return QkNormRotateHip.apply(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved))
