@@ -11,7 +11,7 @@ partial sum moves a result by at most u * size.  Half a step is 2^-8 in bf16, 2^
 import pytest
 import torch
 
-from vmamba_amd import linear_attention_fn, linear_attention_step_fn
+from vmamba_amd import linear_attention_fn, linear_attention_step_fn, qk_norm_rotate_fn
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -550,3 +550,34 @@ def test_step_and_autograd(seen):
             out = linear_attention_step_fn(*token, None, mine)
         want = linear_attention_step_fn(*token, None, state)
     assert torch.equal(out, want) and torch.equal(mine, state)
+
+
+def test_capture_beside_an_eager_graph():
+    """An eager graph of the same leaves on another stream: the captured call says so before anything of it is recorded; without it the capture goes through."""
+    q, k, v, g, dout, normal = inputs(1, 100, 2, 2, 2, 32, 32, BF16, ("token", 1), 19)
+    leaves = [t.requires_grad_() for t in (q, k, v, g)]
+    stream = torch.cuda.Stream()
+    eager = linear_attention_fn(*leaves)
+    want = [eager.detach(), *torch.autograd.grad(eager, leaves, dout, retain_graph=True)]
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            held = torch.zeros(8, device=DEV)
+            with pytest.raises(RuntimeError, match="still lives"):
+                linear_attention_fn(*leaves)
+            with pytest.raises(RuntimeError, match="still lives"):
+                qk_norm_rotate_fn(q, k)
+            linear_attention_fn(*[t.detach() for t in leaves])       # (without gradients nothing is in the way)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = linear_attention_fn(*leaves)
+        got = [out, *torch.autograd.grad(out, leaves, dout)]
+    for _ in range(2):
+        for t in got:
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del held

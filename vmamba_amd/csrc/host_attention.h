@@ -27,6 +27,19 @@ inline bool recorded(std::initializer_list<const at::Tensor *> tensors) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// A call with gradients that is captured: an eager graph of the same leaves that still lives holds their gradients' nodes on another stream, and the engine,
+// which would have the two streams wait for one another at the backward's end, cannot inside a capture and takes the process with it.
+inline void refuse_capture(std::initializer_list<const at::Tensor *> tensors, const char *what) {
+    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA((*tensors.begin())->device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+    for (const at::Tensor *t : tensors) {
+        if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        TORCH_CHECK(!node || !node->stream().has_value() || *node->stream() == stream.unwrap(), what,
+                    ": this capture's leaves belong to an autograd graph that was recorded on another stream and still lives; drop it first");
+    }
+}
 template <typename P> void strides3(const at::Tensor &t, P &batch, P &token, P &head) { batch = t.stride(0); token = t.stride(1); head = t.stride(2); }
 // What comes into a backward: memory on the inputs' device, its last dimension dense
 inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, at::IntArrayRef shape, const char *name) {
@@ -166,8 +179,10 @@ static py::object linear_attention(const py::tuple &kinds, const py::object &q, 
     const at::Tensor state = exactly(state_in, kinds, ok), cu = exactly(cu_in, kinds, ok);
     if (!ok || !s.read(4) || !sequences_fit(s, state, cu)) return py::none();
     const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt((double)s.q.size(3));
-    const variable_list made = recorded({&s.q, &s.k, &s.v, &s.decay, &state}) ? LinearAttention::apply(s.q, s.k, s.v, maybe(s.decay), maybe(state), maybe(cu), scale, want_final)
-                                                                           : attend(s, state, cu, scale, want_final);
+    const bool record = recorded({&s.q, &s.k, &s.v, &s.decay, &state});
+    if (record) refuse_capture({&s.q, &s.k, &s.v, &s.decay, &state}, "linear_attention_fn");
+    const variable_list made = record ? LinearAttention::apply(s.q, s.k, s.v, maybe(s.decay), maybe(state), maybe(cu), scale, want_final)
+                                      : attend(s, state, cu, scale, want_final);
     return want_final ? py::object(py::make_tuple(made[0], made[1])) : py::cast(made[0]);
 }
 
@@ -301,9 +316,9 @@ static py::object qk_norm_rotate(const py::tuple &kinds, const py::object &q, co
     NormArgs a = {exactly(q, kinds, ok),         exactly(k, kinds, ok),           exactly(q_weight, kinds, ok), exactly(k_weight, kinds, ok),
                   exactly(positions, kinds, ok), exactly(frequencies, kinds, ok), eps,                          interleaved};
     if (!ok || !a.read()) return py::none();
-    const variable_list made = recorded({&a.q, &a.k, &a.q_weight, &a.k_weight})
-                                   ? QkNormRotate::apply(a.q, a.k, maybe(a.q_weight), maybe(a.k_weight), maybe(a.positions), maybe(a.frequencies), eps, interleaved)
-                                   : norm_rotate(a);
+    const bool record = recorded({&a.q, &a.k, &a.q_weight, &a.k_weight});
+    if (record) refuse_capture({&a.q, &a.k, &a.q_weight, &a.k_weight}, "qk_norm_rotate_fn");
+    const variable_list made = record ? QkNormRotate::apply(a.q, a.k, maybe(a.q_weight), maybe(a.k_weight), maybe(a.positions), maybe(a.frequencies), eps, interleaved) : norm_rotate(a);
     return py::make_tuple(made[0], made[1]);
 }
 

@@ -183,7 +183,9 @@ def linear_attention_fn(q, k, v, log_decay=None, scale=None, initial_state=None,
     initial_state (sequences, heads, key_dim, value_dim) float32.
 
     Returns out (batch, tokens, heads, value_dim) in q's dtype, with ``output_final_state`` (out, final_state): the states behind the last tokens,
-    float32, which linear_attention_step_fn carries on."""
+    float32, which linear_attention_step_fn carries on.
+
+    Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
     if native_stands(q):
         native = _lib.host().linear_attention(TENSOR_KINDS, q, k, v, log_decay, initial_state, cu_seqlens, scale, bool(output_final_state))

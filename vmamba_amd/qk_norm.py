@@ -102,7 +102,9 @@ def qk_norm_rotate_fn(q, k, q_weight=None, k_weight=None, positions=None, freque
     positions int32 or int64 with frequencies float32 or float64: (batch, tokens) or (tokens,) with (pairs,), or several axes (batch, tokens, axes) or
     (tokens, axes) with (axes, pairs): pair a * pairs + i of a head turns by positions[.., a] * frequencies[a, i], a product in 64 bits.  Pair
     i is values (i, i + R / 2) of the first R = 2 * frequencies.numel() values of a head, with ``interleaved`` values (2 i, 2 i + 1); what is behind them is
-    not turned.  Without positions nothing is."""
+    not turned.  Without positions nothing is.
+
+    Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
     if native_stands(q):
         native = _lib.host().qk_norm_rotate(TENSOR_KINDS, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
