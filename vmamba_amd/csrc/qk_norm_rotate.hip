@@ -30,7 +30,7 @@ struct QnArgs {
     int32_t pos64, freq64, axes, per_axis, pairs;                    // pairs = axes * per_axis
     int32_t batch, tokens, dim, w_dtype, interleaved, round, has_w;  // round: tokens of a workgroup's round
     int64_t rounds;
-    FastDiv by_heads[2], by_pairs;
+    FastDiv by_heads[2], by_pairs, by_tokens;
     float eps;
     float *partial;                  // backward: [workgroup][side][dim]
 };
@@ -110,19 +110,30 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
     const int64_t all = (int64_t)p.batch * p.tokens;
     float w[2][8], dw[2][8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[k][i] = in ? qn_weight(p.side[k].w, i < 4 ? first + i : second + i - 4, p.w_dtype) : 0.0f;
+            w[k][i] = 1.0f;
             dw[k][i] = 0.0f;
         }
+        if (!p.side[k].w) continue;                                  // (T's own type otherwise; all four loads are on their way at once)
+        if (p.w_dtype == SS2D_F32) {
+            qn_load4(reinterpret_cast<const float *>(p.side[k].w) + first, w[k]);
+            qn_load4(reinterpret_cast<const float *>(p.side[k].w) + second, w[k] + 4);
+        } else {
+            qn_load4(reinterpret_cast<const T *>(p.side[k].w) + first, w[k]);
+            qn_load4(reinterpret_cast<const T *>(p.side[k].w) + second, w[k] + 4);
+        }
+    }
     for (int64_t round = blockIdx.x; round < p.rounds; round += gridDim.x) {
         const int64_t token0 = round * p.round;
         const int n_tokens = (int)(all - token0 < p.round ? all - token0 : p.round);
-        const int b0 = (int)(token0 / p.tokens), t0 = (int)(token0 - (int64_t)b0 * p.tokens);
+        uint32_t b0, t0;
+        if (all <= 0x7fffffff) divmod((uint32_t)token0, p.by_tokens, b0, t0);
+        else { b0 = (uint32_t)(token0 / p.tokens); t0 = (uint32_t)(token0 - (int64_t)b0 * p.tokens); }
         auto place = [&](int t, int &b, int &at) {                   // the round's t-th token
-            b = b0;
-            at = t0 + t;
+            b = (int)b0;
+            at = (int)t0 + t;
             while (at >= p.tokens) { at -= p.tokens; ++b; }
         };
         if (round != blockIdx.x) __syncthreads();
@@ -144,6 +155,7 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
         __syncthreads();
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
+            if (gridDim.y == 2 && side != (int)blockIdx.y) continue;
             const QnSide &s = p.side[side];
             const int rows = n_tokens * s.heads;
             const T *x = reinterpret_cast<const T *>(s.x), *dy = reinterpret_cast<const T *>(s.dy);
@@ -374,6 +386,7 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
     vec = p->dim % 8 == 0 && 2 * a.pairs % 8 == 0;
     const int64_t size = p->dtype == SS2D_F32 ? 4 : 2;
     for (const QnSide &s : a.side) {
+        if (s.w && (uintptr_t)s.w % (p->weight_dtype == SS2D_F32 ? 16 : 8) != 0) vec = false;
         if (s.heads == 0) continue;
         uintptr_t bits = (uintptr_t)s.x | (uintptr_t)s.y | (uintptr_t)(s.batch * size) | (uintptr_t)(s.token * size) | (uintptr_t)(s.head * size);
         if (back) bits |= (uintptr_t)s.dy | (uintptr_t)(s.dy_batch * size) | (uintptr_t)(s.dy_token * size) | (uintptr_t)(s.dy_head * size);
@@ -400,6 +413,7 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
     a.round = (int)round;
     for (int i = 0; i < 2; ++i) a.by_heads[i] = make_fastdiv((uint32_t)(a.side[i].heads > 0 ? a.side[i].heads : 1));
     a.by_pairs = make_fastdiv((uint32_t)(a.pairs > 0 ? a.pairs : 1));
+    a.by_tokens = make_fastdiv((uint32_t)(a.tokens > 0 ? a.tokens : 1));
     a.rounds = all > 0 && heads > 0 ? (all + round - 1) / round : 0;
     return SS2D_OK;
 }
@@ -407,7 +421,9 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
 constexpr int64_t kQnShares = 1024;                                  // workgroups of the backward: four to a CU
 constexpr int64_t kQnGrid = 1 << 22;                                 // of the forward (a launch's threads fit 32 bits)
 
-template <typename T, bool kBack> static int qn_launch(const QnArgs &a, bool vec, uint32_t grid, hipStream_t st) {
+template <typename T, bool kBack> static int qn_launch(const QnArgs &a, bool vec, uint32_t shares, hipStream_t st) {
+    // few rounds (a workgroup to a CU at most): queries and keys to workgroups of their own, one after the other they take longer
+    const dim3 grid(shares, !kBack && vec && shares <= 256 ? 2 : 1);
     if (!vec) qk_norm_rotate_any_kernel<T, kBack><<<grid, kBlock, 0, st>>>(a);
     else if (a.dim <= 32) qk_norm_rotate_kernel<T, 4, kBack><<<grid, kBlock, 0, st>>>(a);
     else if (a.dim <= 64) qk_norm_rotate_kernel<T, 8, kBack><<<grid, kBlock, 0, st>>>(a);
