@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 // sixteen segments are on their way at once.
 constexpr uint32_t kLaJoins = 1 << 20;
 __device__ __forceinline__ void la_join(const LaArgs &p, const LaWalk &w0, const LaWalk &w1, int chunk, uint32_t total, uint32_t at_block) {
-    constexpr int kAhead = 16;
+    constexpr int kAhead = 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool second = at_block >= total;
     const LaWalk w = second ? w1 : w0;
@@ -336,21 +336,33 @@ __device__ __forceinline__ void la_join(const LaArgs &p, const LaWalk &w0, const
             if (ia + v < w.a.dim && ib < w.b.dim) state[v] = w.from[la_state_at(p, w, n, h, ia + v, ib)];
     auto place = [&](int q) { return ((int64_t)s.w + (w.reverse ? segs - 1 - q : q)) * p.heads + h; };
     auto at = [&](int q) { return reinterpret_cast<floatx4_t *>(w.local + (place(q) * tiles + tile) * (kLaTile * kLaTile) + i * 4 * kBlock + 4 * tid); };
-    for (int q0 = 0; q0 < segs; q0 += kAhead) {
+    struct Part {
         floatx4_t own[kAhead];
         float decay[kAhead];
+    } ring[2];
+    auto fetch = [&](int q0, Part &part) {
+        if (q0 >= segs - 1) return;                                  // (the last one's sum is none)
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
-            const int safe = min(q0 + q, segs - 2);                  // (the last one's sum is none)
-            own[q] = *at(safe);
-            decay[q] = decays[place(safe)];
+            const int safe = min(q0 + q, segs - 2);
+            part.own[q] = *at(safe);
+            part.decay[q] = decays[place(safe)];
         }
+    };
+    auto step = [&](int q0, Part &part) {
 #pragma unroll
         for (int q = 0; q < kAhead; ++q)
             if (q0 + q < segs) {
                 *at(q0 + q) = state;
-                state = state * decay[q] + own[q];
+                state = state * part.decay[q] + part.own[q];
             }
+    };
+    fetch(0, ring[0]);
+    for (int q0 = 0; q0 < segs; q0 += 2 * kAhead) {
+        fetch(q0 + kAhead, ring[1]);
+        step(q0, ring[0]);
+        fetch(q0 + 2 * kAhead, ring[0]);
+        step(q0 + kAhead, ring[1]);
     }
 }
 __global__ __launch_bounds__(kBlock) void la_join_kernel(const LaArgs p, const LaWalk w0, const LaWalk w1, int chunk, uint32_t total, uint32_t all) {
