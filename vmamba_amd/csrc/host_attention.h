@@ -2,6 +2,7 @@
 // into the C ABI, and the nodes of their gradients.  A call whose arguments are not what the kernels take is left to the Python callers (None), which
 // say what is wrong with them.  One token of one request took 23 us of the host through ctypes, queries and keys of a token 28.
 #pragma once
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 namespace attention {
@@ -17,6 +18,10 @@ template <typename F> int launch(const at::Tensor &x, F fn) {
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     return fn((void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream());
 }
+
+// at::empty on x's device without the way through the dispatcher (a microsecond a tensor): nobody follows these calls' operators
+inline at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &x) { return at::detail::empty_cuda(sizes, type, x.device(), c10::nullopt); }
+inline at::Tensor fresh_like(const at::Tensor &t) { return fresh(t.sizes(), t.scalar_type(), t); }
 
 inline bool dense_last(const at::Tensor &t) { return t.stride(-1) == 1 || t.size(-1) <= 1; }
 inline bool on_gpu(const at::Tensor &t, const at::Tensor &x) { return t.defined() && on(t, x) && plain(t); }
@@ -101,16 +106,16 @@ inline ss2d_linear_attention_params describe(const Sides &s, const at::Tensor &s
 
 inline at::Tensor workspace(int64_t need, const at::Tensor &x, const char *what) {
     expect(need < 0 ? (int)need : SS2D_OK, what);
-    return at::empty({need}, x.options().dtype(at::kByte));
+    return fresh({need}, at::kByte, x);
 }
 
 inline variable_list attend(const Sides &s, const at::Tensor &state, const at::Tensor &cu, double scale, bool want_final) {
-    const at::Tensor out = at::empty({s.q.size(0), s.q.size(1), s.heads, s.v.size(3)}, s.q.options());
+    const at::Tensor out = fresh({s.q.size(0), s.q.size(1), s.heads, s.v.size(3)}, s.q.scalar_type(), s.q);
     variable_list made = {out};
     ss2d_linear_attention_params p = describe(s, state, cu, scale);
     p.out = out.data_ptr();
     if (want_final) {
-        made.push_back(at::empty({cu.defined() ? cu.numel() - 1 : s.q.size(0), s.heads, s.q.size(3), s.v.size(3)}, s.q.options().dtype(at::kFloat)));
+        made.push_back(fresh({cu.defined() ? cu.numel() - 1 : s.q.size(0), s.heads, s.q.size(3), s.v.size(3)}, at::kFloat, s.q));
         p.final_state = (float *)made[1].data_ptr();
     }
     const at::Tensor space = workspace(ss2d_linear_attention_workspace_bytes(&p), s.q, "ss2d_linear_attention_fwd");
@@ -156,10 +161,10 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         if (dfinal.defined()) dfinal = gradient(dfinal, s.q, state_shape, "dfinal").contiguous();
         ss2d_linear_attention_bwd_params p = {};
         p.fwd = describe(s, state, cu, ctx->saved_data["scale"].toDouble());
-        for (int i = 0; i < 3; ++i) result[i] = at::empty(saved[i].sizes(), saved[i].options());
+        for (int i = 0; i < 3; ++i) result[i] = fresh_like(saved[i]);
         int edge = 3;                                                // (of the tensors that there are)
         for (int i = 3; i < 5; ++i)
-            if (saved[i].defined() && ctx->needs_input_grad(edge++)) result[i] = at::empty(saved[i].sizes(), saved[i].options());
+            if (saved[i].defined() && ctx->needs_input_grad(edge++)) result[i] = fresh_like(saved[i]);
         p.dout = dout.data_ptr(); p.dfinal_state = (const float *)ptr_of(dfinal);
         p.dq = result[0].data_ptr(); p.dk = result[1].data_ptr(); p.dv = result[2].data_ptr();
         p.ddecay = const_cast<void *>(ptr_of(result[3])); p.dinitial_state = (float *)ptr_of(result[4]);
@@ -196,7 +201,7 @@ static py::object linear_attention_step(const py::tuple &kinds, const py::object
     const int64_t B = s.q.size(0), dk = s.q.size(2), dv = s.v.size(2), each = s.heads * dk * dv;
     if (B == 0 || !state_fits(state, s.q, {B, s.heads, dk, dv}) || recorded({&s.q, &s.k, &s.v, &s.decay, &state})) return py::none();
     if ((B > 1 && state.stride(0) < each) || !(state.is_contiguous() || state[0].is_contiguous())) return py::none();
-    const at::Tensor out = at::empty({B, s.heads, dv}, s.q.options());
+    const at::Tensor out = fresh({B, s.heads, dv}, s.q.scalar_type(), s.q);
     ss2d_linear_attention_step_params p = {};
     p.batch = (int)B; p.heads = (int)s.heads; p.q_heads = (int)s.q.size(1); p.k_heads = (int)s.k.size(1); p.v_heads = (int)s.v.size(1);
     p.key_dim = (int)dk; p.value_dim = (int)dv; p.dtype = s.code;
@@ -266,7 +271,7 @@ struct NormArgs {
 };
 
 inline variable_list norm_rotate(const NormArgs &a) {
-    const variable_list made = {at::empty(a.q.sizes(), a.q.options()), at::empty(a.k.sizes(), a.k.options())};
+    const variable_list made = {fresh_like(a.q), fresh_like(a.k)};
     ss2d_qk_norm_rotate_params p = a.describe();
     p.q_out = made[0].data_ptr(); p.k_out = made[1].data_ptr();
     expect(launch(a.q, [&](void *stream) { return ss2d_qk_norm_rotate(&p, stream); }), "ss2d_qk_norm_rotate");
@@ -291,11 +296,11 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
         TORCH_CHECK(a.read(), "qk_norm_rotate_fn: what a hook made of its saved tensors is not what it saved");
         const at::Tensor dq = gradient(grads[0], a.q, a.q.sizes(), "dq_out"), dk = gradient(grads[1], a.q, a.k.sizes(), "dk_out");
         variable_list result(8);
-        result[0] = at::empty(a.q.sizes(), a.q.options());
-        result[1] = at::empty(a.k.sizes(), a.k.options());
+        result[0] = fresh_like(a.q);
+        result[1] = fresh_like(a.k);
         int edge = 2;                                                // (of the tensors that there are)
         for (int i = 2; i < 4; ++i)
-            if (saved[i].defined() && ctx->needs_input_grad(edge++)) result[i] = at::empty(saved[i].sizes(), saved[i].options());
+            if (saved[i].defined() && ctx->needs_input_grad(edge++)) result[i] = fresh_like(saved[i]);
         ss2d_qk_norm_rotate_bwd_params g = {};
         g.fwd = a.describe();
         g.dq_out = dq.data_ptr(); g.dk_out = dk.data_ptr();
