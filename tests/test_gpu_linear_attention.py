@@ -4,7 +4,7 @@ Every result is a sum of products of the inputs, of decays and, for gradients, o
 their magnitudes (the same formula of |q|, |k|, |v|, ...: no term is negative then).  A relative rounding u of an operand or a
 partial sum moves a result by at most u * size.  Half a step is 2^-8 in bf16, 2^-11 in fp16, 2^-24 in fp32.
   bf16: an operand that is computed (a pair's weight, a state) is rounded once, and the result once: 2^-8 size + 2^-8 |result|.  What is kept in 32 bits (states,
-        decays' gradients in fp32) comes of operands split in two: 2^-16 size for each of at most three such splits.
+        decays' gradients in fp32) comes of operands split in two at least: 2^-16 size for each of at most three such splits; in three: 2^-24.
   fp16, fp32: fp32 throughout; fp16 results are rounded once.
   Sums in fp32: a result passes at most N = dk + dv + 4 C + 4 (chunks) + 64 additions and products; an exp of x is good to 2^-22 + |x| 2^-23, and
   x below -40 contributes nothing to speak of.  (N + 200) 2^-24 size in all."""
@@ -54,11 +54,11 @@ def reference(q, k, v, g, state, scale, pieces, dout=None, dfinal=None):
     return both
 
 
-def check(name, got, want, size, dtype, dims, tokens):
+def check(name, got, want, size, dtype, dims, tokens, split=2.0 ** -16):
     C = 64 if dtype == BF16 else 32
     terms = (sum(dims) + 4 * C + 4 * (tokens // C + 1) + 264) * 2.0 ** -24
     kept = got.dtype == F32 and dtype == BF16
-    operand = 3 * 2.0 ** -16 if kept else 2.0 ** -8 if dtype == BF16 else 0.0
+    operand = 3 * split if kept else 2.0 ** -8 if dtype == BF16 else 0.0
     bound = (operand + terms) * size + HALF[got.dtype] * want.abs() + 1e-30 + (2.0 ** -25 if got.dtype == F16 else 0.0)     # (fp16's smallest step)
     off = (got.double().cpu() - want).abs()
     assert got.shape == want.shape, name
@@ -581,3 +581,32 @@ def test_capture_beside_an_eager_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     del held
+
+
+@pytest.mark.parametrize("decay", [("head", 1), ("token", 1)], ids=["head", "own"])
+@pytest.mark.parametrize("shape", [(1, 31, 4, 2, 4, 32, 48), (4, 8, 3, 3, 3, 64, 36), (1, 200, 2, 2, 2, 128, 128), (1, 97, 2, 1, 2, 256, 256), (2, 300, 2, 1, 2, 64, 16)], ids=str)
+def test_what_16_bit_inputs_leave_in_32(shape, decay):
+    """States and the gradients of states and of single precision decays, of bf16 inputs: three parts of each operand, 24 bits."""
+    print("CASE kept", shape, decay, flush=True)
+    B, T, Hq, Hk, Hv, dk, dv = shape
+    q, k, v, g, dout, normal = inputs(*shape, BF16, decay, T + 1)
+    state, dfinal = (normal(B, max(Hq, Hk, Hv), dk, dv).to(DEV) for _ in range(2))
+    got = run_all(q, k, v, g, state, dout, dfinal)
+    want, size = reference(q, k, v, g, state, dk ** -0.5, [(b, 0, T) for b in range(B)], dout, dfinal)
+    for name in ("final", "dg", "dstate"):
+        check(name, got[name], want[name], size[name], BF16, (dk, dv, B * T if name == "dg" else 0), T, split=2.0 ** -24)
+
+
+def test_a_learnt_decay_over_many_chunks():
+    """One decay for all tokens of a head: what rounding does to it is the same in every chunk.  A sum of 32 maps' tokens in single precision, against 64 bits."""
+    gen = torch.Generator().manual_seed(21)
+    q, k, v, dout = (torch.randn(8, 784, h, d, generator=gen).to(DEV) for h, d in ((1, 64), (1, 64), (2, 32), (2, 32)))
+    g = torch.tensor([-0.004, -0.02], device=DEV)
+    got = run_all(q, k, v, g, None, dout, None)["dg"].double()
+    at = torch.arange(784, device=DEV, dtype=torch.float64)
+    apart = at[:, None] - at[None]
+    pairs = (q[:, :, 0].double() @ k[:, :, 0].double().transpose(1, 2).contiguous())[:, None] * (dout.double().transpose(1, 2) @ v.double().permute(0, 2, 3, 1).contiguous())
+    terms = pairs * (apart * (apart * g.double()[:, None, None]).clamp(max=0).exp()).tril() * 64 ** -0.5
+    want, size = terms.sum((0, 2, 3)), terms.abs().sum((0, 2, 3))
+    # of 32-term sums of products, added over 25 chunks and 8 maps; each step's half step at most
+    assert bool(((got - want).abs() <= (64 + 32 + 32 + 25 + 8) * 2.0 ** -24 * size).all())

@@ -49,7 +49,7 @@ struct LaArgs {
     int4 *seqs;                      // packed: {start, end, first chunk, first segment}, and {rows before, rows' end, chunks, segments} behind them
     float2 *cum;                     // [chunk][head][C]: G in log2 units, high and low part
     void *states, *dstates, *dstates_t;
-    int64_t low;                     // elements from a state's bf16 value to what the rounding left, 0: not kept
+    int64_t low;                     // elements from a state's bf16 value to what its rounding left, and on to what that one's left; 0: not kept
     float *local;                    // [segment][head][tile][4096] and behind it [segment][head] decays; for the backward twice
     int64_t local_floats;
 };
@@ -210,6 +210,33 @@ __device__ __forceinline__ int la_here(int x) {
     return x;
 }
 
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }            // (what is below 2^-126 is 0)
+
+// What a chunk leaves of the state that it finds.  It is multiplied in chunk after chunk, and where a head's decay is learnt all of them are alike and so is
+// what rounding does to them: in single precision it is a pair of floats.
+template <typename E> struct LaKeep {
+    float high, low;
+    __device__ __forceinline__ void set(float2 end) {
+        if constexpr (sizeof(E) == 4) {
+            const double keep = exp2((double)end.x + (double)end.y);
+            high = (float)keep;
+            low = (float)(keep - (double)high);
+        } else high = fast_exp2(end.x + end.y);
+    }
+    __device__ __forceinline__ float of(float v) const {
+        if constexpr (sizeof(E) == 4) return fmaf(v, high, v * low);
+        return v * high;
+    }
+    __device__ __forceinline__ void scale(floatx4_t &v) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = of(v[i]);
+    }
+    __device__ __forceinline__ void add(floatx4_t &v, floatx4_t more) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], high, fmaf(v[i], low, more[i]));
+    }
+};
+
 inline __host__ __device__ int la_up(int n, int m) { return (n + m - 1) / m * m; }
 // Rows of a state stand at a pitch that every operand's step divides, with zeros behind them
 inline __host__ __device__ int la_state_dim(int d) { return la_up(d, 32); }
@@ -240,6 +267,4 @@ struct LaWalk {
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes);
 int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
 template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w, int n, void *stream);        // states before all chunks, one walk or two side by side
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }            // (what is below 2^-126 is 0)
-
 }  // namespace ss2d

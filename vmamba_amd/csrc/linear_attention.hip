@@ -190,7 +190,8 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 
     struct Rows {
         u32x4_t a[kN], b[kN];
-        float weight, decay;
+        float weight;
+        LaKeep<E> keep;
     } ring[2];
     double sum = 0.0;
     auto fetch = [&](int i, Rows &r) {                               // the i-th chunk of the walk
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
             const float2 g = cum[tid];
             r.weight = w.reverse ? p.scale * fast_exp2(g.x + g.y) : fast_exp2((end.x - g.x) + (end.y - g.y));
         }
-        r.decay = fast_exp2(end.x + end.y);
+        r.keep.set(end);
     };
     auto stage = [&](int i) {                                        // the piece before chunk i, for the stores of that chunk's step
         if constexpr (kStaged) {
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
             put_piece<T, E>(bt + row * kPitch + c0, held_piece<kFast>(r.b[j], row < len && c0 < w.b.dim - b0));
         }
         if (tid < kC) weights[Op::place(tid)] = r.weight;
-        const float keep = r.decay;
+        const LaKeep<E> keep = r.keep;
         __syncthreads();
         if (i + 2 < here.count) fetch(i + 2, r);
         if constexpr (!kLocal) {                                     // the state as the chunk finds it, whole rows of the piece at a time
@@ -266,13 +267,21 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
                         floatx4_t rest;
 #pragma unroll
                         for (int v = 0; v < 4; ++v) rest[v] = acc[j][v] - to_f32(from_f32<bf16_t>(acc[j][v]));
-                        Op::put4(reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia + w.low, rest);
+                        E *to = reinterpret_cast<E *>(w.out) + base + (int64_t)(ib + 16 * j) * da + ia + w.low;
+                        Op::put4(to, rest);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) rest[v] -= to_f32(from_f32<bf16_t>(rest[v]));
+                        Op::put4(to + w.low, rest);
                     }
         }
+        // (in single precision a chunk's sum is made for itself: added product by product to the state, the sum of all chunks, each of them would be rounded to that)
+        constexpr bool kApart = sizeof(E) == 4;
+        floatx4_t mine[kApart ? 4 : 1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            acc[j] *= keep;
-            if constexpr (kBoth) turned[j] *= keep;
+            if constexpr (kApart) mine[j] = floatx4_t{0, 0, 0, 0};
+            else keep.scale(acc[j]);
+            if constexpr (kBoth) keep.scale(turned[j]);
         }
 #pragma unroll
         for (int k0 = 0; k0 < kC; k0 += Op::kStep) {
@@ -285,10 +294,14 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (!kBoth && j >= 2 && w.b.dim - b0 <= 32) break;       // (nothing there)
-                    acc[j] = Op::mma(fa[q], fb[j], acc[j]);
+                    floatx4_t &sum = kApart ? mine[kApart ? j : 0] : acc[j];
+                    sum = Op::mma(fa[q], fb[j], sum);
                     if constexpr (kBoth) turned[j] = Op::mma(fb[j], fa[q], turned[j]);
                 }
         }
+        if constexpr (kApart)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) keep.add(acc[j], mine[j]);
         stage(i + 1);
         __syncthreads();
     };
@@ -303,7 +316,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4_t *>(local + i * 4 * kBlock + 4 * tid) = acc[i];
         if (here.tile == 0 && tid == 0)
-            w.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)here.seg * p.heads + h] = exp2f((float)sum);
+            w.local[(int64_t)p.max_segs * p.heads * tiles * (kLaTile * kLaTile) + (int64_t)here.seg * p.heads + h] = (float)exp2(sum);
     } else if (w.to && last) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -432,6 +445,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
     float *weights = reinterpret_cast<float *>(pt + kC * kPitchP);   // of a token's value in the state behind the chunk
     float2 *cum = reinterpret_cast<float2 *>(weights + kC);
     int *bad = reinterpret_cast<int *>(cum + kC);
+    LaKeep<E> *kept = reinterpret_cast<LaKeep<E> *>(bad + 2);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
     const int mine = wave % 4, half = wave / 4;                      // columns 16 mine .., tokens and keys of this half
     const int tiles = (p.v.dim + kLaTile - 1) / kLaTile;
@@ -542,6 +556,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
                 re = make_float2(__shfl(rc.x, kC - 1, kC), __shfl(rc.y, kC - 1, kC));
             }
             cum[tid] = rc;
+            if (sizeof(E) == 4 && tid == 0) kept->set(re);
             weights[Op::place(tid)] = fast_exp2((re.x - rc.x) + (re.y - rc.y));
         }
         __syncthreads();
@@ -608,10 +623,11 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
                 if (t < len) store4(out + (int64_t)t * p.out.token, acc[m] * p.scale, p.v.dim - value + col - quad, p.out.aligned);
             }
             if (i + 1 < here.count || (last && w.to)) {              // somebody wants the state behind this chunk
-                const float2 end = cum[kC - 1];
-                const float keep = fast_exp2(end.x + end.y);
+                LaKeep<E> keep;
+                if constexpr (sizeof(E) == 4) keep = *kept;
+                else keep.set(cum[kC - 1]);
 #pragma unroll
-                for (int d = 0; d < kHalf; ++d) state[d] *= keep;
+                for (int d = 0; d < kHalf; ++d) keep.scale(state[d]);
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     Frag parts[kParts], keys[kHalf];
@@ -795,8 +811,8 @@ int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
     take(p.cum, sizeof(float2) * entries * chunk);
     p.low = low ? entries * state : 0;
     if (backward) {
-        take(p.states, (low ? 2 : 1) * size * entries * state);
-        take(p.dstates, (low ? 2 : 1) * size * entries * state);
+        take(p.states, (low ? 3 : 1) * size * entries * state);
+        take(p.dstates, (low ? 3 : 1) * size * entries * state);
         take(p.dstates_t, size * entries * state);
     }
     p.local_floats = p.max_segs > p.n_seqs ? (la_round(4 * (int64_t)p.max_segs * p.heads * (tiles * kLaTile * kLaTile + 1)) / 4) : 0;

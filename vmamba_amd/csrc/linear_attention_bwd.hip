@@ -27,6 +27,18 @@ __device__ __forceinline__ float dot_frags(u32x4_t a, u32x4_t b) {
     for (int i = 0; i < 4; ++i) sum = fmaf(unpack_lo<bf16_t>(a[i]), unpack_lo<bf16_t>(b[i]), fmaf(unpack_hi<bf16_t>(a[i]), unpack_hi<bf16_t>(b[i]), sum));
     return sum;
 }
+// Of states in three parts
+__device__ __forceinline__ float dot_parts(u32x4_t a, const u32x4_t (&al)[2], u32x4_t b, const u32x4_t (&bl)[2]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum = fmaf(unpack_lo<bf16_t>(a[i]) + (unpack_lo<bf16_t>(al[0][i]) + unpack_lo<bf16_t>(al[1][i])),
+                   unpack_lo<bf16_t>(b[i]) + (unpack_lo<bf16_t>(bl[0][i]) + unpack_lo<bf16_t>(bl[1][i])), sum);
+        sum = fmaf(unpack_hi<bf16_t>(a[i]) + (unpack_hi<bf16_t>(al[0][i]) + unpack_hi<bf16_t>(al[1][i])),
+                   unpack_hi<bf16_t>(b[i]) + (unpack_hi<bf16_t>(bl[0][i]) + unpack_hi<bf16_t>(bl[1][i])), sum);
+    }
+    return sum;
+}
 
 // Eight wavefronts where a workgroup has a CU's LDS to itself, four where two or more share it
 template <typename Op, int kDim> struct LaBwdShape {
@@ -41,7 +53,7 @@ template <typename Op, int kDim> struct LaBwdShape {
 // A workgroup owns a chunk of one head: weights of its pairs to LDS, then its wavefronts take 16 columns of dq and dk, or of dv, at a time, as the
 // outputs' kernel does (transposed products, states straight from memory; those of a wavefront's first columns are on their way from the start).
 // kTile: E comes through LDS, where dk reads its rows and dv its columns; otherwise memory holds it both ways.
-// kLow: dq's and dk's share of the states with what their rounding to bf16 left, for a decay's gradient in single precision.
+// kLow: dq's and dk's share of the states with what their rounding to bf16 left and what that one's left, for a decay's gradient in single precision.
 // kDim: what both dimensions fit; the rows' pitch in LDS hangs on it, so that operands are read at fixed distances.
 template <typename Op, typename T, int kDim, bool kLow, bool kFast>
 __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_bwd_kernel(const LaArgs p, float *head_sums, uint32_t total) {
@@ -242,28 +254,34 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
                     const int k0 = g + k * Op::kStep;
                     if (k0 >= dv) break;
                     if (kTile && has_e) e_ahead[k] = Op::rows(et, kPitch, 16 * n, k0, lane);
-                    Frag sl, dl;
-                    if constexpr (kLow) {
-                        if (has_s) sl = Op::rows(states + p.low, sv, 16 * n, k0, lane);
-                        if (has_e) dl = Op::rows(dstates + p.low, sv, 16 * n, k0, lane);
-                    }
+                    Frag sl[2], dl[2];
+                    if constexpr (kLow)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (has_s) sl[i] = Op::rows(states + (1 + i) * p.low, sv, 16 * n, k0, lane);
+                            if (has_e) dl[i] = Op::rows(dstates + (1 + i) * p.low, sv, 16 * n, k0, lane);
+                        }
                     if (has_s)
 #pragma unroll
                         for (int m = 0; m < kM; ++m) {
                             const Frag o = Op::rows(ot, kPitch, 16 * m, k0, lane);
                             dq[m] = Op::mma(s_ahead[k], o, dq[m]);
-                            if constexpr (kLow) dq[m] = Op::mma(sl, o, dq[m]);
+                            if constexpr (kLow)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) dq[m] = Op::mma(sl[i], o, dq[m]);
                         }
                     if (has_e)
 #pragma unroll
                         for (int m = 0; m < kM; ++m) {
                             const Frag v = Op::rows(vt, kPitch, 16 * m, k0, lane);
                             dkey[m] = Op::mma(e_ahead[k], v, dkey[m]);
-                            if constexpr (kLow) dkey[m] = Op::mma(dl, v, dkey[m]);
+                            if constexpr (kLow)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) dkey[m] = Op::mma(dl[i], v, dkey[m]);
                         }
                     if (has_s && has_e && p.ddecay) {
-                        se += dot_frags(s_ahead[k], e_ahead[k]);
-                        if constexpr (kLow) se += dot_frags(s_ahead[k], dl) + dot_frags(sl, e_ahead[k]);
+                        if constexpr (kLow) se += dot_parts(s_ahead[k], sl, e_ahead[k], dl);
+                        else se += dot_frags(s_ahead[k], e_ahead[k]);
                     }
                 }
             }
@@ -403,7 +421,9 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
         if (lane >= d) before += b;
     }
     const float until_t = __shfl_up(until, 1), before_t = __shfl_up(before, 1);      // (a token's key is not before it)
-    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + fast_exp2(end.x + end.y) * states_both;
+    LaKeep<E> keep;
+    keep.set(end);
+    float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + keep.of(states_both);
     if (head_sums) {
         dg = sum_groups(sum_columns(lane < e.z ? dg : 0.0f));
         if (lane == 0) head_sums[entry] = dg;
