@@ -48,6 +48,7 @@ struct LaArgs {
     int4 *chunks;                    // {batch, first token, tokens, sequence}; no tokens: unused; sequence -1: rows of no sequence
     int4 *seqs;                      // packed: {start, end, first chunk, first segment}, and {rows before, rows' end, chunks, segments} behind them
     float2 *cum;                     // [chunk][head][C]: G in log2 units, high and low part
+    float2 *kept;                    // [chunk][head]: exp of the whole chunk's sum, high and low part
     void *states, *dstates, *dstates_t;
     int64_t low;                     // elements from a state's bf16 value to what its rounding left, and on to what that one's left; 0: not kept
     float *local;                    // [segment][head][tile][4096] and behind it [segment][head] decays; for the backward twice
@@ -214,13 +215,18 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 
 // What a chunk leaves of the state that it finds.  It is multiplied in chunk after chunk, and where a head's decay is learnt all of them are alike and so is
 // what rounding does to them: in single precision it is a pair of floats.
+__device__ __forceinline__ float2 la_kept(float2 end) {
+    const double keep = exp2((double)end.x + (double)end.y);
+    const float high = (float)keep;
+    return make_float2(high, (float)(keep - (double)high));
+}
 template <typename E> struct LaKeep {
     float high, low;
-    __device__ __forceinline__ void set(float2 end) {
+    // of a chunk that ends with the sum `end` and whose pair stands at *kept
+    __device__ __forceinline__ void set(float2 end, const float2 *kept) {
         if constexpr (sizeof(E) == 4) {
-            const double keep = exp2((double)end.x + (double)end.y);
-            high = (float)keep;
-            low = (float)(keep - (double)high);
+            high = kept->x;
+            low = kept->y;
         } else high = fast_exp2(end.x + end.y);
     }
     __device__ __forceinline__ float of(float v) const {

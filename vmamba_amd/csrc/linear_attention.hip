@@ -102,7 +102,9 @@ __global__ __launch_bounds__(kBlock) void la_chunks_kernel(const LaArgs p, int64
     const int c = (int)(id / p.heads), h = (int)(id - (int64_t)c * p.heads);
     const int4 e = la_find_chunk(p, c, kChunk);
     if (h == 0 && t == 0) p.chunks[c] = e;
-    p.cum[id * kChunk + t] = la_sum_decays<kChunk>(p.decay && t < e.z && e.w >= 0 ? la_decay(p, e.x, e.y + t, h) : 0.0f, t);
+    const float2 sum = la_sum_decays<kChunk>(p.decay && t < e.z && e.w >= 0 ? la_decay(p, e.x, e.y + t, h) : 0.0f, t);
+    p.cum[id * kChunk + t] = sum;
+    if (t == kChunk - 1) p.kept[id] = la_kept(sum);
 }
 
 // ---- the walk over the states ------------------------------------------------------------------------------------------------------
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
             const float2 g = cum[tid];
             r.weight = w.reverse ? p.scale * fast_exp2(g.x + g.y) : fast_exp2((end.x - g.x) + (end.y - g.y));
         }
-        r.keep.set(end);
+        r.keep.set(end, p.kept + (int64_t)(s.z + c) * p.heads + h);
     };
     auto stage = [&](int i) {                                        // the piece before chunk i, for the stores of that chunk's step
         if constexpr (kStaged) {
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
     float *weights = reinterpret_cast<float *>(pt + kC * kPitchP);   // of a token's value in the state behind the chunk
     float2 *cum = reinterpret_cast<float2 *>(weights + kC);
     int *bad = reinterpret_cast<int *>(cum + kC);
-    LaKeep<E> *kept = reinterpret_cast<LaKeep<E> *>(bad + 2);
+    float2 *kept = reinterpret_cast<float2 *>(bad + 2);              // (kOwn: of this chunk)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = 4 * (lane >> 4);
     const int mine = wave % 4, half = wave / 4;                      // columns 16 mine .., tokens and keys of this half
     const int tiles = (p.v.dim + kLaTile - 1) / kLaTile;
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
                 re = make_float2(__shfl(rc.x, kC - 1, kC), __shfl(rc.y, kC - 1, kC));
             }
             cum[tid] = rc;
-            if (sizeof(E) == 4 && tid == 0) kept->set(re);
+            if (kOwn && sizeof(E) == 4 && tid == 0) *kept = la_kept(re);
             weights[Op::place(tid)] = fast_exp2((re.x - rc.x) + (re.y - rc.y));
         }
         __syncthreads();
@@ -624,8 +626,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
             }
             if (i + 1 < here.count || (last && w.to)) {              // somebody wants the state behind this chunk
                 LaKeep<E> keep;
-                if constexpr (sizeof(E) == 4) keep = *kept;
-                else keep.set(cum[kC - 1]);
+                keep.set(cum[kC - 1], kOwn ? kept : p.kept + (int64_t)(s.z + here.begin + i) * p.heads + h);
 #pragma unroll
                 for (int d = 0; d < kHalf; ++d) keep.scale(state[d]);
 #pragma unroll
@@ -809,6 +810,7 @@ int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
     take(p.chunks, sizeof(int4) * (int64_t)p.max_chunks);
     take(p.seqs, p.cu ? sizeof(int4) * ((int64_t)p.n_seqs + 1) : 0);
     take(p.cum, sizeof(float2) * entries * chunk);
+    take(p.kept, sizeof(float2) * entries);
     p.low = low ? entries * state : 0;
     if (backward) {
         take(p.states, (low ? 3 : 1) * size * entries * state);

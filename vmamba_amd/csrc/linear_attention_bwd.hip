@@ -422,7 +422,7 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
     }
     const float until_t = __shfl_up(until, 1), before_t = __shfl_up(before, 1);      // (a token's key is not before it)
     LaKeep<E> keep;
-    keep.set(end);
+    keep.set(end, p.kept + entry);
     float dg = between + from + (col > 0 ? until_t : 0.0f) + after + (lane > 0 ? before_t : 0.0f) + keep.of(states_both);
     if (head_sums) {
         dg = sum_groups(sum_columns(lane < e.z ? dg : 0.0f));
