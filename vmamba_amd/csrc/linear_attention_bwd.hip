@@ -431,14 +431,42 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
 }
 
 // Gradients of what several heads share: the heads' sum, of `per` neighbouring values in single precision, dim apart
-template <typename T> __global__ __launch_bounds__(kBlock) void la_sum_heads_kernel(const float *x, T *out, int64_t total, int dim, int per) {
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (i >= total) return;
-    const int64_t group = i / dim;
-    const float *at = x + group * per * dim + (i - group * dim);
-    float sum = 0.0f;
-    for (int k = 0; k < per; ++k) sum += at[(int64_t)k * dim];
-    out[i] = from_f32<T>(sum);
+// (dimensions that four divides: four neighbours to a thread).
+struct LaSum {
+    const float *x;
+    void *out;
+    int64_t total;                   // results, in units of kVec
+    int32_t dim, per;                // of a head, in units of kVec; heads to one
+};
+struct LaSums { LaSum side[3]; };
+template <typename T, int kVec> __global__ __launch_bounds__(kBlock) void la_sum_heads_kernel(const LaSums sums) {
+    int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    LaSum s = sums.side[0];
+#pragma unroll
+    for (int k = 1; k < 3; ++k)
+        if (i >= s.total) {
+            i -= s.total;
+            s = sums.side[k];
+        }
+    if (i >= s.total) return;
+    const int64_t group = i / s.dim, at = group * s.per * s.dim + (i - group * s.dim);
+    float sum[kVec];
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) sum[v] = 0.0f;
+    if constexpr (kVec == 4) {
+        const floatx4_t *x = reinterpret_cast<const floatx4_t *>(s.x) + at;
+#pragma unroll 4
+        for (int k = 0; k < s.per; ++k) {
+            const floatx4_t more = x[(int64_t)k * s.dim];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[v] += more[v];
+        }
+        store4(reinterpret_cast<T *>(s.out) + 4 * i, floatx4_t{sum[0], sum[1], sum[2], sum[3]}, 4, (uintptr_t)s.out % (4 * sizeof(T)) == 0);
+    } else {
+#pragma unroll 4
+        for (int k = 0; k < s.per; ++k) sum[0] += s.x[at + (int64_t)k * s.dim];
+        reinterpret_cast<T *>(s.out)[i] = from_f32<T>(sum[0]);
+    }
 }
 
 // A learnt decay's gradient: the chunks' sums of its head, a workgroup to a head
@@ -511,14 +539,25 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
         const int dim = p.k.dim > p.v.dim ? p.k.dim : p.v.dim;
         rc = dim <= 64 ? sized(std::integral_constant<int, 64>{}) : dim <= 128 ? sized(std::integral_constant<int, 128>{}) : sized(std::integral_constant<int, 256>{});
         if (rc != SS2D_OK) return rc;
+        LaSums sums = {};
+        int n_sums = 0;
+        int64_t values = 0;
+        bool fours = true;
         auto sum = [&](const LaSide &side, void *out) {
             if (side.div <= 1) return;
-            const int64_t n = (int64_t)p.batch * p.tokens * (p.heads / side.div) * side.dim;
-            la_sum_heads_kernel<T><<<(uint32_t)((n + kBlock - 1) / kBlock), kBlock, 0, st>>>(reinterpret_cast<const float *>(side.p), reinterpret_cast<T *>(out), n, side.dim, side.div);
+            const int64_t heads = (int64_t)p.batch * p.tokens * (p.heads / side.div);
+            sums.side[n_sums++] = LaSum{reinterpret_cast<const float *>(side.p), out, heads * side.dim, side.dim, side.div};
+            values += heads * side.dim;
+            fours = fours && side.dim % 4 == 0;
         };
         sum(p.dq, b.dq);
         sum(p.dk, b.dk);
         sum(p.dv, b.dv);
+        if (fours)
+            for (LaSum &s : sums.side) { s.total /= 4; s.dim /= 4; }
+        const int64_t each = fours ? kBlock * 4 : kBlock;
+        if (values > 0 && fours) la_sum_heads_kernel<T, 4><<<(uint32_t)((values + each - 1) / each), kBlock, 0, st>>>(sums);
+        else if (values > 0) la_sum_heads_kernel<T, 1><<<(uint32_t)((values + each - 1) / each), kBlock, 0, st>>>(sums);
     }
     if (b.head_sums) la_sum_decays_kernel<T><<<p.heads, kBlock, 0, st>>>(b.head_sums, p.ddecay, p.max_chunks, p.heads, p.ddecay_f32);
     return launch_status();
