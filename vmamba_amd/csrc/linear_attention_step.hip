@@ -2,7 +2,8 @@
 //     S = exp(g) S + k v^T,   o = scale q^T S.
 // The state is read and written once and everything else is small, so memory bounds it: 8 bytes per value of the state.  A
 // workgroup owns some columns (values) of one head's state for all keys; a row of them is kVec floats to a lane, all rows of a
-// round on their way at once, and the lanes' sums meet in LDS.
+// round on their way at once, and the lanes' sums meet in LDS.  256 sequences, 32 heads of 128 x 128: 182 us for 1.08 GB, 5.9 TB/s (a copy's rate is 5.3).  One
+// sequence, 8 heads of 64 x 64: 5.2 us, a launch and two trips to memory, in workgroups of 16 columns.
 #include "linear_attention.h"
 
 namespace ss2d {

@@ -6,6 +6,8 @@
 // pairs four first and four second values, so that no pair spans two lanes -- and the weights stay there too.  Angles are computed
 // once per token and pair for all its heads, in LDS: a product in 64 bits, its whole turns taken off there (a position of a million
 // times a frequency has no digits left for the fraction in 32), and then sine and cosine in single precision.
+// 4 x 4096 tokens of 32 + 8 heads of 128, bf16: 66 us for 335 MB, 5.1 TB/s, what a copy reaches; backward 116 for 503 MB, 4.3 TB/s (two rows of a lane in
+// flight instead of four, for its registers).  Rounds of one token took 153 us each: 40 rows leave most lanes of the last step idle.
 #include "ss2d_common.h"
 
 namespace ss2d {
