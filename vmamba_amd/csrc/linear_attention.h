@@ -272,6 +272,6 @@ struct LaWalk {
 };
 // Sizes of the tables and segments, for `tiles` workgroups a head; a launch takes `lanes` threads for each chunk and head.
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes);
-int la_tables(const LaArgs &p, int chunk, void *stream);                               // chunks, seqs and cum
+int la_tables(const LaArgs &p, int chunk, int out_bytes, void *stream);                // chunks, seqs, cum and kept; out_bytes: of a value of p.out, to clear its rows of no sequence, or 0
 template <typename Op, typename T> int la_walks(const LaArgs &p, const LaWalk *w, int n, void *stream);        // states before all chunks, one walk or two side by side
 }  // namespace ss2d

@@ -93,8 +93,9 @@ template <int kChunk> __device__ __forceinline__ float2 la_sum_decays(float deca
     return make_float2(high, (float)(sum - (double)high));
 }
 
-// The chunks' entries and decays: C lanes to a chunk and head.  A latency: 5 us for 8192 chunks and heads.
-template <int kChunk>
+// The chunks' entries and decays: C lanes to a chunk and head.  A latency: 5 us for 8192 chunks and heads.  kOut: bytes of an output's value, whose rows of no
+// sequence are cleared here; 0: they are not this call's.
+template <int kChunk, int kOut>
 __global__ __launch_bounds__(kBlock) void la_chunks_kernel(const LaArgs p, int64_t total) {
     const int t = threadIdx.x % kChunk;
     const int64_t id = (int64_t)blockIdx.x * (kBlock / kChunk) + threadIdx.x / kChunk;
@@ -105,6 +106,13 @@ __global__ __launch_bounds__(kBlock) void la_chunks_kernel(const LaArgs p, int64
     const float2 sum = la_sum_decays<kChunk>(p.decay && t < e.z && e.w >= 0 ? la_decay(p, e.x, e.y + t, h) : 0.0f, t);
     p.cum[id * kChunk + t] = sum;
     if (t == kChunk - 1) p.kept[id] = la_kept(sum);
+    if constexpr (kOut > 0) {
+        using Bits = std::conditional_t<kOut == 2, uint16_t, uint32_t>;
+        if (e.w >= 0) return;
+        Bits *out = reinterpret_cast<Bits *>(p.out.p) + (int64_t)e.y * p.out.token + (int64_t)h * p.out.head;
+        for (int r = 0; r < e.z; ++r, out += p.out.token)
+            for (int d = t; d < p.v.dim; d += kChunk) out[d] = 0;
+    }
 }
 
 // ---- the walk over the states ------------------------------------------------------------------------------------------------------
@@ -663,33 +671,28 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
             if (key0 + 16 * d + quad + v < p.k.dim && value < p.v.dim) w.to[la_state_at(p, w, n, h, key0 + 16 * d + quad + v, value)] = state[d][v];
 }
 
-// Rows of no sequence
-template <typename T> __global__ __launch_bounds__(kBlock) void la_nobody_kernel(const LaArgs p) {
-    const int4 all = p.seqs[p.n_seqs];
-    const int64_t rows = (int64_t)all.x + (p.tokens - all.y), row = (int64_t)p.heads * p.v.dim;
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < rows * row; i += (int64_t)gridDim.x * kBlock) {
-        const int64_t r = i / row;
-        reinterpret_cast<T *>(p.out.p)[(r < all.x ? r : all.y + (r - all.x)) * row + (i - r * row)] = from_f32<T>(0.0f);
-    }
-}
-
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 // Segments: where the sequences alone do not give the chip its workgroups (two to a CU, of `tiles` for a head), each is cut so that they do, into
 // `shortest` chunks at least: a segment is walked twice.
+constexpr int kLaWhole = 5;          // chunks of a sequence that is never cut
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
     const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= (tiles > (p.v.dim + kLaTile - 1) / kLaTile ? 384 : 192) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk;
     int64_t chunks, segs, seg_chunks;
     if (p.cu) {
         chunks = (int64_t)p.tokens / chunk + p.n_seqs + 2;
-        seg_chunks = (per_seq * p.heads * tiles + 767) / 768;        // whatever the longest of them is
-        seg_chunks = seg_chunks < shortest ? shortest : seg_chunks;
+        // Whatever the longest of them is.  As if all tokens were one sequence, three times the workgroups that are there at once, since most of the segments are
+        // shorter than that, and five chunks at least; against half of the workgroups and two chunks, prompts / training: 12 011 tokens in 16 sequences, 24 heads of
+        // 128 x 64, bf16, 148 -> 139 / 659 -> 628 us; 30 000 in 4, 16 heads of 128, 291 -> 283 / 1525 -> 1263; 8192 in 40, 32 heads of 64, 105 -> 107 / 369 -> 378.
+        seg_chunks = (per_seq * p.heads * tiles + 1535) / 1536;
+        seg_chunks = seg_chunks < kLaWhole ? kLaWhole : seg_chunks;
         segs = per_seq <= seg_chunks ? p.n_seqs : chunks / seg_chunks + p.n_seqs;
     } else {
         chunks = per_seq * p.n_seqs;
         const int64_t each = (want + p.n_seqs - 1) / p.n_seqs;
         seg_chunks = (per_seq + each - 1) / each;
-        seg_chunks = seg_chunks < shortest ? shortest : seg_chunks;
+        // (a few chunks take less than the two launches that cutting them takes: 300 tokens, 8 heads of 64, bf16, 20.0 -> 18.8 us, training 60 -> 53)
+        seg_chunks = per_seq <= kLaWhole ? kLaWhole : seg_chunks < shortest ? shortest : seg_chunks;
         p.segs_per_seq = per_seq <= seg_chunks ? 1 : (int)((per_seq + seg_chunks - 1) / seg_chunks);
         segs = (int64_t)p.segs_per_seq * p.n_seqs;
     }
@@ -701,14 +704,17 @@ int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
     return SS2D_OK;
 }
 
-int la_tables(const LaArgs &p, int chunk, void *stream) {
+int la_tables(const LaArgs &p, int chunk, int out_bytes, void *stream) {
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (p.cu) la_sequences_kernel<<<1, kBlock, 0, st>>>(p, chunk);
     const int64_t total = (int64_t)p.max_chunks * p.heads;
     if (total == 0) return launch_status();
     const int64_t per = kBlock / chunk, grid = (total + per - 1) / per;
-    if (chunk == 64) la_chunks_kernel<64><<<(uint32_t)grid, kBlock, 0, st>>>(p, total);
-    else la_chunks_kernel<32><<<(uint32_t)grid, kBlock, 0, st>>>(p, total);
+    auto go = [&](auto kernel) { kernel<<<(uint32_t)grid, kBlock, 0, st>>>(p, total); };
+    const bool clear = p.cu && out_bytes > 0;
+    if (chunk == 64) clear ? go(la_chunks_kernel<64, 2>) : go(la_chunks_kernel<64, 0>);          // (bf16)
+    else if (clear) out_bytes == 2 ? go(la_chunks_kernel<32, 2>) : go(la_chunks_kernel<32, 4>);
+    else go(la_chunks_kernel<32, 0>);
     return launch_status();
 }
 
@@ -716,7 +722,7 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     int rc = SS2D_OK;
     const bool own = !p.cu && p.per_seq <= kLaOwnChunks && p.k.dim <= kLaOwnKeys && p.max_segs <= p.n_seqs;
-    if (!own && (rc = la_tables(p, Op::kChunk, stream)) != SS2D_OK) return rc;
+    if (!own && (rc = la_tables(p, Op::kChunk, (int)sizeof(T), stream)) != SS2D_OK) return rc;
     LaWalk w = {};
     w.a = p.k; w.b = p.v;
     w.from = p.initial; w.to = p.final;
@@ -746,7 +752,6 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
     else if (p.k.dim <= 64) sized(std::integral_constant<int, 4>{});
     else if (p.k.dim <= 128) sized(std::integral_constant<int, 8>{});
     else sized(std::integral_constant<int, 16>{});
-    if (p.cu && p.tokens > 0) la_nobody_kernel<T><<<256, kBlock, 0, st>>>(p);
     return launch_status();
 }
 

@@ -498,7 +498,7 @@ struct LaBackward {
 template <typename Op, typename T> static int la_backward(const LaBackward &b, float *dinitial, void *stream) {
     const LaArgs &p = b.a;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    int rc = la_tables(p, Op::kChunk, stream);
+    int rc = la_tables(p, Op::kChunk, 0, stream);
     if (rc != SS2D_OK) return rc;
     // S by keys, dense along values; E the same way, and for dv by values, dense along keys
     LaWalk w[2] = {};
