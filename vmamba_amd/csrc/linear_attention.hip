@@ -672,12 +672,14 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
-// Segments: where the sequences alone do not give the chip its workgroups (two to a CU, of `tiles` for a head), each is cut so that they do, into
-// `shortest` chunks at least: a segment is walked twice.
+// Segments: where the sequences alone do not give the chip its workgroups (`tiles` for a head), each is cut so that there are two to a CU, into
+// `shortest` chunks at least: a segment is walked twice.  192 workgroups are enough, since the cut costs two launches and the second reading; 128 where
+// chains are short.  us cut / whole, forward: 96 workgroups of 25 chunks 48 / 75, 128 of 8 30 / 25, of 16 40 / 40; gradients: 192 of 25 124 / 119, 256 of 8 69 / 57,
+// of 16 112 / 99, of 32 144 / 133, 192 of 64 220 / 226.
 constexpr int kLaWhole = 5;          // chunks of a sequence that is never cut
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
-    const int64_t alone = (int64_t)p.n_seqs * p.heads * tiles, want = alone >= (tiles > (p.v.dim + kLaTile - 1) / kLaTile ? 384 : 192) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
-    const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk;
+    const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk, alone = (int64_t)p.n_seqs * p.heads * tiles;
+    const int64_t want = alone >= 192 || (alone >= 128 && per_seq <= 16) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     int64_t chunks, segs, seg_chunks;
     if (p.cu) {
         chunks = (int64_t)p.tokens / chunk + p.n_seqs + 2;
