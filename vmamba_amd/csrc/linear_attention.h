@@ -29,7 +29,7 @@ struct LaSide {                      // q, k, v, out or a gradient: (batch, toke
     int64_t batch, token, head;      // strides in elements
     int32_t div;                     // heads of the state to one of this
     int32_t dim;
-    int32_t aligned;                 // base and strides are multiples of 16 bytes (outputs: of four values), and rows of whole pieces, at strides below 2^24 bytes
+    int32_t pieces;                  // what is read: heads of a piece of 16 bytes at least, tokens at strides below 2^24 bytes
 };
 
 struct LaArgs {
@@ -142,13 +142,15 @@ struct OperandBf16 {
 // ---- tiles ------------------------------------------------------------------------------------------------------------------------
 template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 
-// 16 bytes' worth of row `row` of `rows` (one at least), from column c on.  kFast: the side is aligned, its dimension a multiple of a piece and a chunk's
-// offsets fit 32 bits; the load is then unconditional -- a row or column that is not there repeats another -- so that nothing waits for it before
-// it is used, and held_piece() makes zeros of it there.  Otherwise element by element, zeros for what is not there.
+// 16 bytes' worth of row `row` of `rows` (one at least), from column c on, c a multiple of a piece.  kFast: rows hold a piece at least and a chunk's offsets
+// fit 32 bits; the load is then unconditional, wherever it begins -- a row or column that is not there repeats another, the last piece is the one that ends
+// with its row -- so that nothing waits for it before it is used, and held_piece() puts it in its place and makes zeros of what is not there.  Otherwise
+// element by element.  (Rows off the 16-byte grid by elements, as they all were: 8 x 4096 tokens, 16 heads of 128 660 us, so 243.)
 template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(const T *base, int64_t stride, int row, int rows, int c, int cols) {
     if constexpr (kFast) {
-        const uint32_t at = (uint32_t)min(row, rows - 1) * (uint32_t)stride + (uint32_t)(c < cols ? c : 0);
-        return *reinterpret_cast<const u32x4_t *>(reinterpret_cast<const char *>(base) + at * (uint32_t)sizeof(T));
+        typedef uint32_t here __attribute__((ext_vector_type(4), aligned(2)));
+        const uint32_t at = (uint32_t)min(row, rows - 1) * (uint32_t)stride + (uint32_t)min(c, cols - kVecOf<T>);
+        return *reinterpret_cast<const here *>(reinterpret_cast<const char *>(base) + at * (uint32_t)sizeof(T));
     }
     union { T e[kVecOf<T>]; u32x4_t w; } u;
     u.w = u32x4_t{0, 0, 0, 0};
@@ -158,8 +160,17 @@ template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(
             if (c + i < cols) u.e[i] = base[row * stride + c + i];
     return u.w;
 }
-template <bool kFast> __device__ __forceinline__ u32x4_t held_piece(u32x4_t piece, bool in) {
+template <bool kFast, typename T> __device__ __forceinline__ u32x4_t held_piece(u32x4_t piece, bool in, int c, int cols) {
     if constexpr (kFast) {
+        if (cols % kVecOf<T> != 0) {                                 // the last piece: its first values are those that end the one before
+            const int bytes = max(c + kVecOf<T> - cols, 0) * (int)sizeof(T);
+            if (bytes & 8) piece = u32x4_t{piece[2], piece[3], 0, 0};
+            if (bytes & 4) piece = u32x4_t{piece[1], piece[2], piece[3], 0};
+            if (sizeof(T) == 2 && bytes & 2)
+                piece = u32x4_t{__builtin_amdgcn_alignbit(piece[1], piece[0], 16), __builtin_amdgcn_alignbit(piece[2], piece[1], 16), __builtin_amdgcn_alignbit(piece[3], piece[2], 16),
+                                piece[3] >> 16};
+        }
+        in = in && c < cols;
 #pragma unroll
         for (int i = 0; i < 4; ++i) piece[i] = in ? piece[i] : 0u;
     }
@@ -194,11 +205,13 @@ template <typename T, typename E> __device__ __forceinline__ void put_piece(E *l
     }
 }
 
-// Four neighbouring results of one token to memory, `left` of them inside the row
-template <typename T> __device__ __forceinline__ void store4(T *p, floatx4_t v, int left, bool aligned) {
-    if (aligned && left >= 4) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<floatx4_t *>(p) = v;
-        else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_from_f32<T>(v[0], v[1]), pack2_from_f32<T>(v[2], v[3]));
+// Four neighbouring results of one token to memory, wherever they begin, `left` of them inside the row
+template <typename T> __device__ __forceinline__ void store4(T *p, floatx4_t v, int left) {
+    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t two __attribute__((ext_vector_type(2), aligned(2)));
+    if (left >= 4) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<four *>(p) = four{v[0], v[1], v[2], v[3]};
+        else *reinterpret_cast<two *>(p) = two{pack2_from_f32<T>(v[0], v[1]), pack2_from_f32<T>(v[2], v[3])};
         return;
     }
 #pragma unroll

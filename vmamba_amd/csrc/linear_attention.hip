@@ -175,8 +175,8 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
     const bool last = w.reverse ? here.begin == 0 : here.begin + here.count >= here.chunks;
     if (kLocal && (lone || last)) return;                            // (nobody asks for the last one's sum)
     const int64_t b = p.cu ? 0 : n;
-    const T *pa = reinterpret_cast<const T *>(w.a.p) + b * w.a.batch + (int64_t)(h / w.a.div) * w.a.head + a0;
-    const T *pb = reinterpret_cast<const T *>(w.b.p) + b * w.b.batch + (int64_t)(h / w.b.div) * w.b.head + b0;
+    const T *pa = reinterpret_cast<const T *>(w.a.p) + b * w.a.batch + (int64_t)(h / w.a.div) * w.a.head;
+    const T *pb = reinterpret_cast<const T *>(w.b.p) + b * w.b.batch + (int64_t)(h / w.b.div) * w.b.head;
 
     floatx4_t acc[4], turned[kBoth ? 4 : 1];                         // element (16 wave + 4 (lane / 16) + v, 16 i + lane % 16); (16 wave + lane % 16, 16 i + 4 (lane / 16) + v)
     const int quad = 4 * (lane >> 4), col = lane & 15, ia = a0 + 16 * wave + quad, ib = b0 + col, ja = a0 + 16 * wave + col, jb = b0 + quad;
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
-            r.a[j] = load_piece<kFast>(pa + (int64_t)t0 * w.a.token, w.a.token, row, len, c0, w.a.dim - a0);
-            r.b[j] = load_piece<kFast>(pb + (int64_t)t0 * w.b.token, w.b.token, row, len, c0, w.b.dim - b0);
+            r.a[j] = load_piece<kFast>(pa + (int64_t)t0 * w.a.token, w.a.token, row, len, a0 + c0, w.a.dim);
+            r.b[j] = load_piece<kFast>(pb + (int64_t)t0 * w.b.token, w.b.token, row, len, b0 + c0, w.b.dim);
         }
         if (tid < kC) {
             const float2 g = cum[tid];
@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
-            put_piece<T, E>(at + row * kPitch + c0, held_piece<kFast>(r.a[j], row < len && c0 < w.a.dim - a0));
-            put_piece<T, E>(bt + row * kPitch + c0, held_piece<kFast>(r.b[j], row < len && c0 < w.b.dim - b0));
+            put_piece<T, E>(at + row * kPitch + c0, held_piece<kFast, T>(r.a[j], row < len, a0 + c0, w.a.dim));
+            put_piece<T, E>(bt + row * kPitch + c0, held_piece<kFast, T>(r.b[j], row < len, b0 + c0, w.b.dim));
         }
         if (tid < kC) weights[Op::place(tid)] = r.weight;
         const LaKeep<E> keep = r.keep;
@@ -401,7 +401,7 @@ static int64_t la_tiles(const LaArgs &p) { return (int64_t)((p.k.dim + kLaTile -
 template <typename Op, typename T, bool kLocal, bool kBoth> static void la_walk_launch(const LaArgs &p, const LaWalk *w, int n, hipStream_t st) {
     constexpr int kMost = Op::kMostParts, kLess = kMost < 2 ? kMost : 2;
     const LaWalk &w0 = w[0], &w1 = w[n - 1];
-    const bool fast = w0.a.aligned && w0.b.aligned && w1.a.aligned && w1.b.aligned;
+    const bool fast = w0.a.pieces && w0.b.pieces && w1.a.pieces && w1.b.pieces;
     const uint32_t total = (uint32_t)((int64_t)p.max_segs * p.heads * la_tiles(p)), grid = total * (uint32_t)n;
     if (w0.exact || w1.exact) {
         if (fast) la_walk_kernel<Op, T, kLocal, kMost, true, kBoth><<<grid, kBlock, 0, st>>>(p, w0, w1, total);
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
     const int64_t b = p.cu ? 0 : n;
     const T *pq = reinterpret_cast<const T *>(p.q.p) + b * p.q.batch + (int64_t)(h / p.q.div) * p.q.head;
     const T *pk = reinterpret_cast<const T *>(p.k.p) + b * p.k.batch + (int64_t)(h / p.k.div) * p.k.head;
-    const T *pv = reinterpret_cast<const T *>(p.v.p) + b * p.v.batch + (int64_t)(h / p.v.div) * p.v.head + v0;
+    const T *pv = reinterpret_cast<const T *>(p.v.p) + b * p.v.batch + (int64_t)(h / p.v.div) * p.v.head;
     T *out = reinterpret_cast<T *>(p.out.p) + b * p.out.batch + (s.x + (int64_t)here.begin * kC) * p.out.token + (int64_t)h * p.out.head + v0 + 16 * mine + quad;
     pq += (s.x + (int64_t)here.begin * kC) * p.q.token;              // (these walk along: of the next chunk to be fetched)
     pk += (s.x + (int64_t)here.begin * kC) * p.k.token;
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 #pragma unroll
         for (int j = 0; j < kNv; ++j) {
             const int at = tid + j * kLaThreads, row = at / kPerValue, d = at % kPerValue * kVec;
-            rv[j] = load_piece<kFast>(pv, p.v.token, row, len, d, p.v.dim - v0);
+            rv[j] = load_piece<kFast>(pv, p.v.token, row, len, v0 + d, p.v.dim);
         }
         if (tid < kC) {
             if constexpr (kOwn) decay = p.decay && tid < len ? la_decay(p, b, s.x + (int64_t)(here.begin + i) * kC + tid, h) : 0.0f;
@@ -543,13 +543,13 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 #pragma unroll
             for (int j = 0; j < kNk; ++j) {
                 const int at = tid + j * kLaThreads, row = at / kPerKey, d = at % kPerKey * kVec;
-                rq[j] = held_piece<kFast>(rq[j], row < len && d < p.k.dim);
-                rk[j] = held_piece<kFast>(rk[j], row < len && d < p.k.dim);
+                rq[j] = held_piece<kFast, T>(rq[j], row < len, d, p.k.dim);
+                rk[j] = held_piece<kFast, T>(rk[j], row < len, d, p.k.dim);
             }
 #pragma unroll
             for (int j = 0; j < kNv; ++j) {
                 const int at = tid + j * kLaThreads, row = at / kPerValue, d = at % kPerValue * kVec;
-                rv[j] = held_piece<kFast>(rv[j], row < len && d < p.v.dim - v0);
+                rv[j] = held_piece<kFast, T>(rv[j], row < len, v0 + d, p.v.dim);
             }
         }
 #pragma unroll
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 #pragma unroll
             for (int m = 0; m < kHalfM; ++m) {
                 const int t = 16 * ms[m] + col;
-                if (t < len) store4(out + (int64_t)t * p.out.token, acc[m] * p.scale, p.v.dim - value + col - quad, p.out.aligned);
+                if (t < len) store4(out + (int64_t)t * p.out.token, acc[m] * p.scale, p.v.dim - value + col - quad);
             }
             if (i + 1 < here.count || (last && w.to)) {              // somebody wants the state behind this chunk
                 LaKeep<E> keep;
@@ -738,7 +738,7 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
         const size_t bytes = sizeof(typename Op::E) * ((2 * c + kLaTile) * (keys + Op::kPad) + c * (kLaTile + Op::kPad + c + Op::kPad)) + c * (sizeof(float) + sizeof(float2)) + 16;
         kernel<<<total, kLaThreads, bytes, st>>>(p, w, total);       // (up to 146 KB of LDS: this runtime asks for no attribute above 64)
     };
-    const bool fast = p.q.aligned && p.k.aligned && p.v.aligned;
+    const bool fast = p.q.pieces && p.k.pieces && p.v.pieces;
     auto sized = [&](auto tiles) {
         constexpr int kTiles = decltype(tiles)::value, kMost = Op::kMostParts, kLess = kMost < 2 ? kMost : 2;
         auto parted = [&](auto own_sums) {
@@ -757,17 +757,13 @@ template <typename Op, typename T> static int la_forward(const LaArgs &p, void *
     return launch_status();
 }
 
-static bool la_aligned(const void *p, int64_t a, int64_t b, int64_t c, int64_t bytes, int64_t size) {
-    return ((uintptr_t)p | (uintptr_t)(a * size) | (uintptr_t)(b * size) | (uintptr_t)(c * size)) % bytes == 0;
-}
-
-LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size, int bytes) {
+LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size) {
     LaSide s = {};
     s.p = const_cast<void *>(ptr);
     s.batch = batch; s.token = token; s.head = head;
     s.div = own_heads > 0 ? heads / own_heads : 1;
     s.dim = dim;
-    s.aligned = la_aligned(ptr, batch, token, head, bytes, size) && dim * size % bytes == 0 && token >= 0 && token * size < (1 << 24);
+    s.pieces = dim * size >= 16 && token >= 0 && token * size < (1 << 24);
     return s;
 }
 
@@ -793,11 +789,11 @@ int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty) 
     a.cu = p->cu_seqlens;
     a.initial = p->initial_state; a.final = p->final_state;
     const int size = p->dtype == SS2D_F32 ? 4 : 2;
-    a.q = la_side(p->q, p->q_batch_stride, p->q_token_stride, p->q_head_stride, p->heads, p->q_heads, p->key_dim, size, 16);
-    a.k = la_side(p->k, p->k_batch_stride, p->k_token_stride, p->k_head_stride, p->heads, p->k_heads, p->key_dim, size, 16);
-    a.v = la_side(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->heads, p->v_heads, p->value_dim, size, 16);
+    a.q = la_side(p->q, p->q_batch_stride, p->q_token_stride, p->q_head_stride, p->heads, p->q_heads, p->key_dim, size);
+    a.k = la_side(p->k, p->k_batch_stride, p->k_token_stride, p->k_head_stride, p->heads, p->k_heads, p->key_dim, size);
+    a.v = la_side(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->heads, p->v_heads, p->value_dim, size);
     const int64_t row = (int64_t)p->heads * p->value_dim;
-    a.out = la_side(p->out, row * p->seqlen, row, p->value_dim, p->heads, p->heads, p->value_dim, size, 4 * size);
+    a.out = la_side(p->out, row * p->seqlen, row, p->value_dim, p->heads, p->heads, p->value_dim, size);
     if (a.heads == 0 || a.n_seqs == 0) { empty = true; return SS2D_OK; }
     const bool rows = a.tokens > 0;
     if (rows && (!p->q || !p->k || !p->v)) return SS2D_EINVAL;

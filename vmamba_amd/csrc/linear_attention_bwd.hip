@@ -87,8 +87,8 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
     const int64_t row0 = (int64_t)e.x * p.tokens + e.y;
     auto put = [&](const LaSide &side, int t, int d, floatx4_t v) {  // four values of a gradient, in single precision where heads are still to be summed
         const int64_t at = e.x * side.batch + (int64_t)(e.y + la_here(t)) * side.token + (int64_t)h * side.head + d;
-        if (side.div > 1) store4(reinterpret_cast<float *>(side.p) + at, v, side.dim - d, side.aligned);
-        else store4(reinterpret_cast<T *>(side.p) + at, v, side.dim - d, side.aligned);
+        if (side.div > 1) store4(reinterpret_cast<float *>(side.p) + at, v, side.dim - d);
+        else store4(reinterpret_cast<T *>(side.p) + at, v, side.dim - d);
     };
     auto put_decay = [&](int t, float v) {
         const int64_t at = (row0 + t) * p.heads + h;
@@ -167,7 +167,7 @@ __global__ __launch_bounds__((LaBwdShape<Op, kDim>::kWaves * kWave), 2) void la_
                 for (int j = 0; j < kN; ++j) {
                     const int at = i + tid + j * kThreads, r = at / kPerRow, d = at % kPerRow * kVec;
                     if (kPieces % (kN * kThreads) == 0 || r < kC) {
-                        const u32x4_t held = held_piece<kFast>(piece[side][j], r < e.z && d < sides[side]->dim);
+                        const u32x4_t held = held_piece<kFast, T>(piece[side][j], r < e.z, d, sides[side]->dim);
                         put_piece<T, E>(tiles[side] + r * kPitch + d, held);
                         if (side < 3) bad |= piece_bad<T>(held);
                     }
@@ -464,7 +464,7 @@ template <typename T, int kVec> __global__ __launch_bounds__(kBlock) void la_sum
 #pragma unroll
             for (int v = 0; v < 4; ++v) sum[v] += more[v];
         }
-        store4(reinterpret_cast<T *>(s.out) + 4 * i, floatx4_t{sum[0], sum[1], sum[2], sum[3]}, 4, (uintptr_t)s.out % (4 * sizeof(T)) == 0);
+        store4(reinterpret_cast<T *>(s.out) + 4 * i, floatx4_t{sum[0], sum[1], sum[2], sum[3]}, 4);
     } else {
 #pragma unroll 4
         for (int k = 0; k < s.per; ++k) sum[0] += s.x[at + (int64_t)k * s.dim];
@@ -527,7 +527,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (n && (rc = la_walks<Op, T>(p, w, n, stream)) != SS2D_OK) return rc;
     const uint32_t total = (uint32_t)p.max_chunks * (uint32_t)p.heads;
     if (total > 0) {
-        const bool fast = p.q.aligned && p.k.aligned && p.v.aligned && p.dout.aligned;
+        const bool fast = p.q.pieces && p.k.pieces && p.v.pieces && p.dout.pieces;
         auto go = [&](auto kernel, int waves, int bytes) {
             // (up to 157 KB of LDS: this runtime asks for no attribute above 64)
             kernel<<<total, waves * kWave, bytes, st>>>(p, b.head_sums, total);
@@ -566,7 +566,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     return launch_status();
 }
 
-LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size, int bytes);
+LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size);
 int la_arguments(const ss2d_linear_attention_params *p, LaArgs &a, bool &empty);
 int la_chunk(int dtype);
 int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low);
@@ -584,7 +584,7 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
     const int size = f.dtype == SS2D_F32 ? 4 : 2;
     if (params->ddecay && !f.decay) return SS2D_EINVAL;
     b.low = f.dtype == SS2D_BF16 && params->ddecay && f.decay_dtype == SS2D_F32;
-    a.dout = la_side(params->dout, params->dout_batch_stride, params->dout_token_stride, params->dout_head_stride, f.heads, f.heads, f.value_dim, size, 16);
+    a.dout = la_side(params->dout, params->dout_batch_stride, params->dout_token_stride, params->dout_head_stride, f.heads, f.heads, f.value_dim, size);
     a.dfinal = params->dfinal_state;
     a.ddecay = params->ddecay;
     a.ddecay_f32 = f.decay_dtype == SS2D_F32;
@@ -593,7 +593,7 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
         const bool shared = own != f.heads;
         to = ptr;
         const int64_t row = (int64_t)f.heads * dim;
-        side = la_side(shared ? base + at : ptr, row * f.seqlen, row, dim, f.heads, own, dim, shared ? 4 : size, shared ? 16 : 4 * size);
+        side = la_side(shared ? base + at : ptr, row * f.seqlen, row, dim, f.heads, own, dim, shared ? 4 : size);
         if (shared) at += (4 * row * f.seqlen * f.batch + 255) / 256 * 256;
     };
     gradient(a.dq, b.dq, params->dq, f.q_heads, f.key_dim);

@@ -90,7 +90,7 @@ template <typename T> static int la_step(const LaStepArgs &a, int batch, hipStre
     return heads * ((dv + 63) / 64) >= 512 ? go(la_step_kernel<T, 4, 64>, 64) : go(la_step_kernel<T, 4, 16>, 16);
 }
 
-LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size, int bytes);
+LaSide la_side(const void *ptr, int64_t batch, int64_t token, int64_t head, int heads, int own_heads, int dim, int size);
 
 }  // namespace ss2d
 
@@ -105,9 +105,9 @@ extern "C" int ss2d_linear_attention_step(const ss2d_linear_attention_step_param
     if (!p->q || !p->k || !p->v || !p->state || !p->out) return SS2D_EINVAL;
     if (p->batch > 1 && p->state_batch_stride < (int64_t)p->heads * p->key_dim * p->value_dim) return SS2D_EINVAL;
     LaStepArgs a = {};
-    a.q = la_side(p->q, p->q_batch_stride, 0, p->q_head_stride, p->heads, p->q_heads, p->key_dim, 1, 1);
-    a.k = la_side(p->k, p->k_batch_stride, 0, p->k_head_stride, p->heads, p->k_heads, p->key_dim, 1, 1);
-    a.v = la_side(p->v, p->v_batch_stride, 0, p->v_head_stride, p->heads, p->v_heads, p->value_dim, 1, 1);
+    a.q = la_side(p->q, p->q_batch_stride, 0, p->q_head_stride, p->heads, p->q_heads, p->key_dim, 1);
+    a.k = la_side(p->k, p->k_batch_stride, 0, p->k_head_stride, p->heads, p->k_heads, p->key_dim, 1);
+    a.v = la_side(p->v, p->v_batch_stride, 0, p->v_head_stride, p->heads, p->v_heads, p->value_dim, 1);
     a.decay = p->decay; a.decay_dtype = p->decay_dtype; a.decay_batch = p->decay_batch_stride; a.decay_head = p->decay_head_stride;
     a.heads = p->heads; a.state = p->state; a.state_batch = p->state_batch_stride; a.out = p->out; a.scale = p->scale;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
