@@ -430,7 +430,8 @@ def test_two_streams_and_graphs():
         assert torch.equal(out, want) and torch.equal(mine, state)
 
 
-@pytest.mark.parametrize("shape", [(1, 70, 2, 1, 2, 65, 64), (2, 70, 2, 2, 2, 64, 129), (1, 129, 1, 1, 1, 200, 33), (1, 65, 2, 2, 1, 128, 96), (1, 40, 1, 1, 3, 48, 80)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 70, 2, 1, 2, 65, 64), (2, 70, 2, 2, 2, 64, 129), (1, 129, 1, 1, 1, 200, 33), (1, 65, 2, 2, 1, 128, 96), (1, 40, 1, 1, 3, 48, 80), (1, 70, 2, 1, 2, 9, 11),
+                                   (2, 66, 1, 1, 1, 13, 8), (1, 90, 1, 2, 2, 66, 71), (1, 33, 1, 1, 1, 7, 4)], ids=str)
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
 def test_dimensions_between_the_kernels(shape, dtype):
     """Both sides of the dimensions at which another kernel is taken, with all that the backward can be asked for."""
@@ -610,3 +611,19 @@ def test_a_learnt_decay_over_many_chunks():
     want, size = terms.sum((0, 2, 3)), terms.abs().sum((0, 2, 3))
     # of 32-term sums of products, added over 25 chunks and 8 maps; each step's half step at most
     assert bool(((got - want).abs() <= (64 + 32 + 32 + 25 + 8) * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (32, 20), (37, 50)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_rows_off_the_grid(dtype, dk, dv):
+    """Views that begin one value behind a 16-byte boundary, their rows an odd number of values apart, with NaN all around: the same bits as of copies."""
+    q, k, v, g, dout, normal = inputs(2, 77, 2, 2, 2, dk, dv, dtype, ("token", 1), 23)
+    want = run_all(q, k, v, g, None, dout, None)
+
+    def off(t):
+        B, T, H, d = t.shape
+        memory = torch.full((B * T * (H * d + 3) + 9,), float("nan"), dtype=dtype, device=DEV)
+        return memory.as_strided(t.shape, (T * (H * d + 3), H * d + 3, d, 1), 1).copy_(t)
+
+    got = run_all(off(q), off(k), off(v), g, None, off(dout), None)
+    assert all(torch.equal(want[n], got[n]) for n in want)

@@ -145,7 +145,7 @@ template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 // 16 bytes' worth of row `row` of `rows` (one at least), from column c on, c a multiple of a piece.  kFast: rows hold a piece at least and a chunk's offsets
 // fit 32 bits; the load is then unconditional, wherever it begins -- a row or column that is not there repeats another, the last piece is the one that ends
 // with its row -- so that nothing waits for it before it is used, and held_piece() puts it in its place and makes zeros of what is not there.  Otherwise
-// element by element.  (Rows off the 16-byte grid by elements, as they all were: 8 x 4096 tokens, 16 heads of 128 660 us, so 243.)
+// element by element.  (8 x 4096 tokens, 16 heads of 127 in bf16: 264 us, element by element 728; of 128, one value off the 16-byte grid, 253 and 660, on it 203.)
 template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(const T *base, int64_t stride, int row, int rows, int c, int cols) {
     if constexpr (kFast) {
         typedef uint32_t here __attribute__((ext_vector_type(4), aligned(2)));

@@ -172,6 +172,7 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
     const int a0 = here.tile % tiles_a * kLaTile, b0 = here.tile / tiles_a * kLaTile, h = here.h, n = here.n;
     const int4 s = here.s;
     const bool lone = here.chunks <= p.seg_chunks;                   // the sequence has this one segment
+    const bool whole = w.a.dim - a0 >= kLaTile && w.b.dim - b0 >= kLaTile;           // the tiles' columns are all there
     const bool last = w.reverse ? here.begin == 0 : here.begin + here.count >= here.chunks;
     if (kLocal && (lone || last)) return;                            // (nobody asks for the last one's sum)
     const int64_t b = p.cu ? 0 : n;
@@ -237,11 +238,18 @@ __global__ __launch_bounds__(kBlock, 2) void la_walk_kernel(const LaArgs p, cons
     auto step = [&](int i, Rows &r) {
         const int c = here.begin + (w.reverse ? here.count - 1 - i : i), len = min(kC, s.y - s.x - c * kC);
         const int64_t at_chunk = (int64_t)(s.z + c) * p.heads + h;
+        if (len < kC || !whole)
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
+                r.a[j] = held_piece<kFast, T>(r.a[j], row < len, a0 + c0, w.a.dim);
+                r.b[j] = held_piece<kFast, T>(r.b[j], row < len, b0 + c0, w.b.dim);
+            }
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const int at_ = tid + j * kBlock, row = at_ / kPerRow, c0 = at_ % kPerRow * kVec;
-            put_piece<T, E>(at + row * kPitch + c0, held_piece<kFast, T>(r.a[j], row < len, a0 + c0, w.a.dim));
-            put_piece<T, E>(bt + row * kPitch + c0, held_piece<kFast, T>(r.b[j], row < len, b0 + c0, w.b.dim));
+            put_piece<T, E>(at + row * kPitch + c0, r.a[j]);
+            put_piece<T, E>(bt + row * kPitch + c0, r.b[j]);
         }
         if (tid < kC) weights[Op::place(tid)] = r.weight;
         const LaKeep<E> keep = r.keep;
