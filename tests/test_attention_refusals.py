@@ -234,3 +234,51 @@ def test_norm_of_bad_arguments():
     assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), None, need, None) == _lib.SS2D_EINVAL
     assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), ctypes.c_void_p(260), need, None) == _lib.SS2D_EINVAL
     assert L.ss2d_qk_norm_rotate_bwd(back(weighed, dq_weight=256), HERE, need - 1, None) == _lib.SS2D_ENOMEM
+
+
+# ---- traced calls ----------------------------------------------------------------------------------------------------------------------
+def behind_the_tracer(*like):
+    """Results as kernels make them, in memory that no operator of torch's writes: twice the inputs."""
+    made = [torch.empty(tuple(map(int, t.shape)), dtype=t.dtype) for t in like]
+    for out, t in zip(made, like):
+        out.numpy()[...] = 2 * t.detach().numpy()
+    return made
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_a_traced_call_is_run_again(monkeypatch):
+    """A traced module calls the operator with its own inputs, of other sizes too, instead of giving the example's results back; with tensors that do not
+    fit it refuses as the call itself does."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(qk_norm, "check_plain", lambda *a, **b: None)
+
+    class Native:
+        @staticmethod
+        def linear_attention(kinds, q, k, v, *rest):
+            return behind_the_tracer(v)[0]
+
+        @staticmethod
+        def qk_norm_rotate(kinds, q, k, *rest):
+            return tuple(behind_the_tracer(q, k))
+
+    monkeypatch.setattr(_lib, "host", lambda: Native)
+    monkeypatch.setattr(linear_attention, "linear_attention_fwd", lambda q, k, v, *rest: (behind_the_tracer(v)[0], None))
+    monkeypatch.setattr(qk_norm, "qk_norm_rotate_fwd", lambda q, k, *rest: tuple(behind_the_tracer(q, k)), raising=False)
+    make = lambda B, T: [torch.randn(B, T, 2, 8) for _ in range(3)]  # noqa: E731
+    with torch.no_grad():
+        attend = torch.jit.trace(lambda q, k, v: vmamba_amd.linear_attention_fn(q, k, v) + 1, make(2, 5))
+        rotate = torch.jit.trace(lambda q, k: sum(vmamba_amd.qk_norm_rotate_fn(q, k)), make(2, 5)[:2])
+        for sizes in ((2, 5), (1, 7)):
+            q, k, v = make(*sizes)
+            assert torch.equal(attend(q, k, v), 2 * v + 1) and torch.equal(rotate(q, k), 2 * q + 2 * k)
+        with pytest.raises(RuntimeError, match="agree"):
+            attend(q, k[:, :5], v)
+        with pytest.raises(RuntimeError, match="agree"):
+            rotate(q, k[:, :5])
+
+
+def test_a_traced_step_is_refused(monkeypatch):
+    monkeypatch.setattr(torch.jit, "is_tracing", lambda: True)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        vmamba_amd.linear_attention_step_fn(**step(on_cpu))

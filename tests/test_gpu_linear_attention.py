@@ -627,3 +627,24 @@ def test_rows_off_the_grid(dtype, dk, dv):
 
     got = run_all(off(q), off(k), off(v), g, None, off(dout), None)
     assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced():
+    """A traced call is the call, for inputs of other values and sizes too, whatever stands behind it; a token's state is not left to a trace."""
+    def layer(q, k, v, g):
+        q, k = qk_norm_rotate_fn(q, k)
+        out, final = linear_attention_fn(q, k, v, g, output_final_state=True)
+        return out + 1, final * 2
+
+    with torch.no_grad():
+        q, k, v, g, _, _ = inputs(2, 50, 4, 2, 4, 32, 24, BF16, ("token", 1), 29)
+        traced = torch.jit.trace(layer, (q, k, v, g))
+        for sizes in ((2, 50), (1, 131)):
+            q, k, v, g, _, _ = inputs(*sizes, 4, 2, 4, 32, 24, BF16, ("token", 1), 31)
+            assert all(torch.equal(a, b) for a, b in zip(traced(q, k, v, g), layer(q, k, v, g)))
+        with pytest.raises(RuntimeError, match="agree"):
+            traced(q, k, v[:, :100], g)
+        state = torch.zeros(1, 4, 32, 24, device=DEV)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(linear_attention_step_fn, (q[:, 0], k[:, 0], v[:, 0], g[:, 0], state))

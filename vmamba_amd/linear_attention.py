@@ -10,7 +10,7 @@ here.  Arguments are checked as csms6s.py does and fail with RuntimeError.
 import torch
 
 from . import _lib
-from .norm import TENSOR_KINDS, native_stands
+from .norm import TENSOR_KINDS, native_stands, untraced
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
 MAX_HEAD_DIM = 256
@@ -143,9 +143,12 @@ def linear_attention_bwd(q, k, v, log_decay, scale, initial_state, cu_seqlens, d
 class LinearAttentionHip(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, scale, cu_seqlens, want_final):
-        out, final = linear_attention_fwd(q, k, v, log_decay, scale, initial_state, cu_seqlens, want_final)
+        with untraced():                                             # (a trace holds this call, with whatever tensors it is given when it runs)
+            _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens)
+            ctx.scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+            dense = initial_state if initial_state is None else initial_state.contiguous()
+            out, final = linear_attention_fwd(q, k, v, log_decay, ctx.scale, dense, cu_seqlens, want_final)
         ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens)
-        ctx.scale = scale
         ctx.set_materialize_grads(False)
         return out, final
 
@@ -187,14 +190,10 @@ def linear_attention_fn(q, k, v, log_decay=None, scale=None, initial_state=None,
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
-    if native_stands(q):
+    if native_stands(q) and not torch.jit.is_tracing():              # (its memory is made where a tracer does not see it)
         native = _lib.host().linear_attention(TENSOR_KINDS, q, k, v, log_decay, initial_state, cu_seqlens, scale, bool(output_final_state))
         if native is not None:
             return native
-    _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens)
-    if initial_state is not None:
-        initial_state = initial_state.contiguous()
-    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     out, final = LinearAttentionHip.apply(q, k, v, log_decay, initial_state, scale, cu_seqlens, bool(output_final_state))
     return (out, final) if output_final_state else out
 
@@ -204,8 +203,9 @@ def linear_attention_step_fn(q, k, v, log_decay, state, scale=None):
 
     q (batch, q_heads, key_dim), k, v and log_decay ((batch, heads), (heads,) or None) as in linear_attention_fn, without the tokens.  The states have to
     be dense but for the batch's stride, which keeps them apart.  For inference: it refuses tensors that require a gradient while
-    gradients are recorded."""
+    gradients are recorded, and to be traced (torch.jit.trace), since a trace would not hold what becomes of the state."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
+    _check(not torch.jit.is_tracing(), "linear_attention_step_fn changes its state behind a tracer's back: it cannot be traced")
     if native_stands(q):
         native = _lib.host().linear_attention_step(TENSOR_KINDS, q, k, v, log_decay, state, scale)
         if native is not None:

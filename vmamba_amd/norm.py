@@ -250,6 +250,18 @@ def native_stands(x):
     return type(x) in TENSOR_KINDS and x.is_cuda and not torch.compiler.is_compiling() and not operators_seen()
 
 
+class untraced:
+    """Within it torch.jit.trace records nothing and sizes are plain numbers: for the inside of an autograd function, which is recorded as one call."""
+    def __enter__(self):
+        self.state = torch._C._get_tracing_state()
+        if self.state is not None:
+            torch._C._set_tracing_state(None)
+
+    def __exit__(self, *_):
+        if self.state is not None:
+            torch._C._set_tracing_state(self.state)
+
+
 def calls_unseen():
     """True when nothing but autograd follows the operators that are called: no mode or transform (operators_seen), no compiler or tracer."""
     return not (torch.compiler.is_compiling() or torch.jit.is_tracing() or operators_seen() or torch.is_autocast_enabled())

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .linear_attention import _check, _dense_last, _ptr, check_plain
-from .norm import TENSOR_KINDS, native_stands
+from .norm import TENSOR_KINDS, native_stands, untraced
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
 MAX_DIM = 512
@@ -58,13 +58,22 @@ def _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
     return p
 
 
+def qk_norm_rotate_fwd(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+    """(q, k) of arguments that qk_norm_rotate_fn has checked."""
+    q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
+    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    p = _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
+    p.q_out, p.k_out = (t.data_ptr() for t in outs)
+    _lib.check(_lib.launch(q, _lib.lib().ss2d_qk_norm_rotate, p), "ss2d_qk_norm_rotate")
+    return outs
+
+
 class QkNormRotateHip(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
-        outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        p = _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
-        p.q_out, p.k_out = (t.data_ptr() for t in outs)
-        _lib.check(_lib.launch(q, _lib.lib().ss2d_qk_norm_rotate, p), "ss2d_qk_norm_rotate")
+        with untraced():                                             # (a trace holds this call, with whatever tensors it is given when it runs)
+            _check_all(q, k, q_weight, k_weight, positions, frequencies)
+            outs = qk_norm_rotate_fwd(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
         ctx.eps, ctx.interleaved = eps, interleaved
         return outs
@@ -106,10 +115,8 @@ def qk_norm_rotate_fn(q, k, q_weight=None, k_weight=None, positions=None, freque
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
-    if native_stands(q):
+    if native_stands(q) and not torch.jit.is_tracing():              # (its memory is made where a tracer does not see it)
         native = _lib.host().qk_norm_rotate(TENSOR_KINDS, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
         if native is not None:
             return native
-    _check_all(q, k, q_weight, k_weight, positions, frequencies)
-    q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
     return QkNormRotateHip.apply(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved))
