@@ -282,3 +282,9 @@ def test_a_traced_step_is_refused(monkeypatch):
     monkeypatch.setattr(torch.jit, "is_tracing", lambda: True)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         vmamba_amd.linear_attention_step_fn(**step(on_cpu))
+
+
+def test_a_learnt_decay_of_no_sequences_is_not_left_out():
+    """A gradient that is asked for without the decays it is of is refused here too."""
+    p = fill(_lib.LinearAttentionBwdParams(), fwd=sequences(batch=0, q=None, k=None, v=None), ddecay=256, decay_per_head=1)
+    assert _lib.lib().ss2d_linear_attention_bwd(p, None, 0, None) == _lib.SS2D_EINVAL

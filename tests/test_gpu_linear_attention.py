@@ -648,3 +648,20 @@ def test_traced():
         state = torch.zeros(1, 4, 32, 24, device=DEV)
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(linear_attention_step_fn, (q[:, 0], k[:, 0], v[:, 0], g[:, 0], state))
+
+
+@pytest.mark.parametrize("seen", [False, True])
+@pytest.mark.parametrize("own", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+def test_a_learnt_decay_without_sequences(own, seen):
+    """The gradient of what all tokens of a head share is zero where there are none, not what its memory held before."""
+    import contextlib
+    for B, T in ((0, 5), (2, 0)):
+        q, k, v = (torch.zeros(B, T, 7, 16, device=DEV, dtype=own) for _ in range(3))
+        g = torch.full((7,), -0.5, device=DEV, dtype=own, requires_grad=True)
+        with Seen() if seen else contextlib.nullcontext():
+            out = linear_attention_fn(q, k, v, g)
+            dout = torch.zeros_like(out)
+            spoiled = [torch.full((7,), float("nan"), device=DEV, dtype=own) for _ in range(64)]    # (what a new tensor of that size is given next)
+            del spoiled
+            dg, = torch.autograd.grad(out, g, dout)
+        assert dg.shape == (7,) and not dg.any(), (B, T)

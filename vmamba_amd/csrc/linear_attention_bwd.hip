@@ -607,6 +607,16 @@ static int64_t la_backward_plan(const ss2d_linear_attention_bwd_params *params, 
     return at;
 }
 
+// No sequence at all: what all tokens of a head share has a gradient still, the sum of none
+static int la_no_decays(const ss2d_linear_attention_bwd_params &g, hipStream_t st) {
+    const ss2d_linear_attention_params &f = g.fwd;
+    if (!g.ddecay || !g.decay_per_head || f.heads == 0) return SS2D_OK;
+    if (!f.decay) return SS2D_EINVAL;
+    if (f.decay_dtype == SS2D_F16) la_sum_decays_kernel<f16_t><<<f.heads, kBlock, 0, st>>>(nullptr, g.ddecay, 0, f.heads, 0);
+    else la_sum_decays_kernel<bf16_t><<<f.heads, kBlock, 0, st>>>(nullptr, g.ddecay, 0, f.heads, f.decay_dtype == SS2D_F32);
+    return launch_status();
+}
+
 }  // namespace ss2d
 
 using namespace ss2d;
@@ -622,7 +632,7 @@ extern "C" int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params 
     bool empty;
     const int64_t need = la_backward_plan(params, b, empty, reinterpret_cast<char *>(workspace));
     if (need < 0) return (int)need;
-    if (empty) return SS2D_OK;
+    if (empty) return la_no_decays(*params, reinterpret_cast<hipStream_t>(stream));
     if (b.a.tokens > 0 && (!params->dout || !params->dq || !params->dk || !params->dv)) return SS2D_EINVAL;
     if (!workspace || (uintptr_t)workspace % 16 != 0) return SS2D_EINVAL;
     if (workspace_bytes < need) return SS2D_ENOMEM;
