@@ -288,3 +288,27 @@ def test_a_learnt_decay_of_no_sequences_is_not_left_out():
     """A gradient that is asked for without the decays it is of is refused here too."""
     p = fill(_lib.LinearAttentionBwdParams(), fwd=sequences(batch=0, q=None, k=None, v=None), ddecay=256, decay_per_head=1)
     assert _lib.lib().ss2d_linear_attention_bwd(p, None, 0, None) == _lib.SS2D_EINVAL
+
+
+class Kept:
+    """What a backward is given besides the gradients."""
+    scale, eps, interleaved, needs_input_grad = 1.0, 1e-6, False, (True,) * 8
+
+    def __init__(self, *saved):
+        self.saved_tensors = saved
+
+
+def test_gradients_of_another_type_are_refused(monkeypatch):
+    """Saved tensors that a hook brought back in single precision: the gradients, which are still bf16, are not read as that."""
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(qk_norm, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(linear_attention, "linear_attention_bwd", lambda *a: pytest.fail("called"))
+    monkeypatch.setattr(_lib, "launch", lambda *a: pytest.fail("launched"))
+    q, k, v = on_cpu(2, 5, 4, 8), on_cpu(2, 5, 2, 8), on_cpu(2, 5, 4, 6)
+    with torch.no_grad():
+        for dout, dfinal in ((on_cpu(2, 5, 4, 6, dtype=BF16), None), (None, on_cpu(2, 4, 8, 6, dtype=BF16)), (on_cpu(2, 5, 4, 6), on_cpu(2, 4, 8, 6, dtype=BF16))):
+            with pytest.raises(RuntimeError):
+                linear_attention.LinearAttentionHip.backward(Kept(q, k, v, None, None, None), dout, dfinal)
+        for dq, dk in ((BF16, F32), (F32, BF16), (BF16, BF16)):
+            with pytest.raises(RuntimeError):
+                qk_norm.QkNormRotateHip.backward(Kept(q, k, None, None, None, None), on_cpu(*q.shape, dtype=dq), on_cpu(*k.shape, dtype=dk))

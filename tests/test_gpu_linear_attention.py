@@ -665,3 +665,20 @@ def test_a_learnt_decay_without_sequences(own, seen):
             del spoiled
             dg, = torch.autograd.grad(out, g, dout)
         assert dg.shape == (7,) and not dg.any(), (B, T)
+
+
+@pytest.mark.parametrize("seen", [False, True])
+@pytest.mark.parametrize("other", [F32, F16], ids=["fp32", "fp16"])
+def test_saved_tensors_of_another_type(other, seen):
+    """A hook that brings bf16 back as another type: the gradients that come in are bf16 still, and are not read as what they are not."""
+    import contextlib
+    q, k, v, g, dout, normal = inputs(1, 50, 2, 2, 2, 16, 16, BF16, ("token", 0), 37)
+    with Seen() if seen else contextlib.nullcontext():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, g)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.to(other)):
+            out = linear_attention_fn(*leaves)
+            turned = qk_norm_rotate_fn(*leaves[:2])
+        with pytest.raises(RuntimeError, match="type"):
+            torch.autograd.grad(out, leaves, dout)
+        with pytest.raises(RuntimeError, match="type"):
+            torch.autograd.grad(turned, leaves[:2], [torch.ones_like(t) for t in turned])

@@ -46,9 +46,11 @@ inline void refuse_capture(std::initializer_list<const at::Tensor *> tensors, co
     }
 }
 template <typename P> void strides3(const at::Tensor &t, P &batch, P &token, P &head) { batch = t.stride(0); token = t.stride(1); head = t.stride(2); }
-// What comes into a backward: memory on the inputs' device, its last dimension dense
-inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, at::IntArrayRef shape, const char *name) {
-    TORCH_CHECK(on_gpu(g, x) && has_shape(g, shape), name, " must be a plain tensor with memory of its own, on the device of q and shaped as what it is the gradient of");
+// What comes into a backward: memory on the inputs' device, its last dimension dense, its type that of what it is the gradient of (the inputs' may have
+// changed since: a hook brought them back as something else)
+inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, at::IntArrayRef shape, at::ScalarType type, const char *name) {
+    TORCH_CHECK(on_gpu(g, x) && has_shape(g, shape) && g.scalar_type() == type, name,
+                " must be a plain tensor with memory of its own, on the device of q and of the shape and type of what it is the gradient of");
     return dense_last(g) ? g : g.contiguous();
 }
 
@@ -157,8 +159,8 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         const int64_t n_seqs = cu.defined() ? cu.numel() - 1 : s.q.size(0), out_shape[4] = {s.q.size(0), s.q.size(1), s.heads, s.v.size(3)},
                       state_shape[4] = {n_seqs, s.heads, s.q.size(3), s.v.size(3)};
         if (!dout.defined()) dout = at::zeros(out_shape, s.q.options());
-        dout = gradient(dout, s.q, out_shape, "dout");
-        if (dfinal.defined()) dfinal = gradient(dfinal, s.q, state_shape, "dfinal").contiguous();
+        dout = gradient(dout, s.q, out_shape, s.q.scalar_type(), "dout");
+        if (dfinal.defined()) dfinal = gradient(dfinal, s.q, state_shape, at::kFloat, "dfinal").contiguous();
         ss2d_linear_attention_bwd_params p = {};
         p.fwd = describe(s, state, cu, ctx->saved_data["scale"].toDouble());
         for (int i = 0; i < 3; ++i) result[i] = fresh_like(saved[i]);
@@ -294,7 +296,8 @@ struct QkNormRotate : torch::autograd::Function<QkNormRotate> {
         const variable_list saved = ctx->get_saved_variables();
         const NormArgs a = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
         TORCH_CHECK(a.read(), "qk_norm_rotate_fn: what a hook made of its saved tensors is not what it saved");
-        const at::Tensor dq = gradient(grads[0], a.q, a.q.sizes(), "dq_out"), dk = gradient(grads[1], a.q, a.k.sizes(), "dk_out");
+        const at::Tensor dq = gradient(grads[0], a.q, a.q.sizes(), a.q.scalar_type(), "dq_out"),
+                         dk = gradient(grads[1], a.q, a.k.sizes(), a.q.scalar_type(), "dk_out");
         variable_list result(8);
         result[0] = fresh_like(a.q);
         result[1] = fresh_like(a.k);

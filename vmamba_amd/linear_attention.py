@@ -162,8 +162,8 @@ class LinearAttentionHip(torch.autograd.Function):
                 return (None,) * 8
             dout = q.new_zeros((*q.shape[:2], heads, v.shape[3]))
         check_plain(q, dout=dout, dfinal=dfinal)
-        _check(tuple(dout.shape) == (*q.shape[:2], heads, v.shape[3]), "dout must have out's shape")
-        _check(dfinal is None or tuple(dfinal.shape) == (n_seqs, heads, q.shape[3], v.shape[3]), "dfinal must have final_state's shape")
+        _check(tuple(dout.shape) == (*q.shape[:2], heads, v.shape[3]) and dout.dtype == q.dtype, "dout must have out's shape and type")
+        _check_state(dfinal, q, (n_seqs, heads, q.shape[3], v.shape[3]), "dfinal")
         if not _dense_last(dout):
             dout = dout.contiguous()
         dfinal, initial_state = (t if t is None else t.contiguous() for t in (dfinal, initial_state))

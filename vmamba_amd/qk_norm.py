@@ -85,7 +85,7 @@ class QkNormRotateHip(torch.autograd.Function):
         _check_all(q, k, q_weight, k_weight, positions, frequencies)               # (a hook may have made something else of them)
         q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
         check_plain(q, dq_out=dq_out, dk_out=dk_out)
-        _check(dq_out.shape == q.shape and dk_out.shape == k.shape, "gradients must have the outputs' shapes")
+        _check(dq_out.shape == q.shape and dk_out.shape == k.shape and dq_out.dtype == dk_out.dtype == q.dtype, "gradients must have the outputs' shapes and type")
         dq_out, dk_out = (t if _dense_last(t) else t.contiguous() for t in (dq_out, dk_out))
         g = _lib.QkNormRotateBwdParams()
         g.fwd = _params(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved)
