@@ -312,3 +312,30 @@ def test_gradients_of_another_type_are_refused(monkeypatch):
         for dq, dk in ((BF16, F32), (F32, BF16), (BF16, BF16)):
             with pytest.raises(RuntimeError):
                 qk_norm.QkNormRotateHip.backward(Kept(q, k, None, None, None, None), on_cpu(*q.shape, dtype=dq), on_cpu(*k.shape, dtype=dk))
+
+
+MANY = 2 ** 32 + 64                  # 64, counted in 32 bits
+
+
+def stretched(*shape, dtype=F32):
+    """A tensor of this shape in the memory of one value a row, whatever the number of rows."""
+    return on_cpu(*(1 if n > 2 ** 20 else n for n in shape), dtype=dtype).expand(*shape)
+
+
+@pytest.mark.parametrize("build,sizes", [(attention, dict(T=MANY)), (attention, dict(B=MANY)), (attention, dict(Hv=MANY)), (attention, dict(Hq=MANY, Hk=MANY, Hv=MANY)),
+                                         (attention, dict(B=1, cu_seqlens=lambda m: torch.empty(MANY, dtype=torch.int32, device="meta"))),
+                                         (norm, dict(T=MANY)), (norm, dict(B=MANY)), (norm, dict(Hk=MANY))],
+                         ids=["tokens", "batch", "heads of v", "heads", "sequences", "norm tokens", "norm batch", "norm heads"])
+def test_sizes_over_32_bits_are_refused(build, sizes, monkeypatch):
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(qk_norm, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(linear_attention, "linear_attention_fwd", lambda *a: pytest.fail("called"))
+    monkeypatch.setattr(qk_norm, "qk_norm_rotate_fwd", lambda *a: pytest.fail("called"))
+    with pytest.raises(RuntimeError, match="no dimension of more|no more than"):
+        {attention: vmamba_amd.linear_attention_fn, norm: vmamba_amd.qk_norm_rotate_fn}[build](**build(stretched, **sizes))
+
+
+def test_a_step_of_more_sequences_than_32_bits_is_refused(monkeypatch):
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    with pytest.raises(RuntimeError, match="no dimension of more"):
+        vmamba_amd.linear_attention_step_fn(**step(stretched, B=MANY))

@@ -14,6 +14,7 @@ from .norm import TENSOR_KINDS, native_stands, untraced
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
 MAX_HEAD_DIM = 256
+MAX_SIZE = 2 ** 31 - 1               # of batch, tokens, heads and sequences, which the C entries count in 32 bits
 
 
 def _check(cond, msg):
@@ -50,6 +51,7 @@ def _check_sides(q, k, v, what, rank):
     _check(k.shape[-1] == q.shape[-1], "k must have q's head dimension")
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check(_dense_last(t), f"{name} must be contiguous in its last dimension")
+        _check(max(t.shape) <= MAX_SIZE, f"{name} must have no dimension of more than {MAX_SIZE}")
         _check(t.shape[-2] >= 1 and 1 <= t.shape[-1] <= MAX_HEAD_DIM, f"{name} must have heads of 1 to {MAX_HEAD_DIM} values")
     heads = max(q.shape[-2], k.shape[-2], v.shape[-2])
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -82,6 +84,7 @@ def _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens):
         _check(cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous")
         _check(q.shape[0] == 1, "packed sequences (cu_seqlens) must stand in a batch of one")
         n_seqs = cu_seqlens.numel() - 1
+        _check(n_seqs <= MAX_SIZE, f"cu_seqlens must have no more than {MAX_SIZE} sequences")
     _check_state(initial_state, q, (n_seqs, heads, q.shape[3], v.shape[3]), "initial_state")
     return heads, n_seqs
 

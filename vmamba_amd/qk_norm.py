@@ -9,7 +9,7 @@ GPU tensors only: there is no CPU path here.  Arguments are checked as csms6s.py
 import torch
 
 from . import _lib
-from .linear_attention import _check, _dense_last, _ptr, check_plain
+from .linear_attention import MAX_SIZE, _check, _dense_last, _ptr, check_plain
 from .norm import TENSOR_KINDS, native_stands, untraced
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
@@ -25,6 +25,7 @@ def _check_all(q, k, q_weight, k_weight, positions, frequencies):
     _check(1 <= q.shape[3] <= MAX_DIM, f"heads must have 1 to {MAX_DIM} values")
     for name, t in (("q", q), ("k", k)):
         _check(_dense_last(t), f"{name} must be contiguous in its last dimension")
+        _check(max(t.shape) <= MAX_SIZE, f"{name} must have no dimension of more than {MAX_SIZE}")
     weights = [w for w in (q_weight, k_weight) if w is not None]
     for w in weights:
         _check(w.dtype in (torch.float32, q.dtype) and w.dtype == weights[0].dtype, "weights must be of one type, float32 or q's dtype")
