@@ -670,8 +670,8 @@ int ss2d_product_f32(const float *a, const float *b, const float *bias, const fl
  *   outside 0 .. seqlen are moved into it, a descending one is taken as the one before it; rows of no sequence get zeros.
  *   initial_state, final_state (n_seqs or batch, heads, key_dim, value_dim) fp32, dense, either or both NULL; of a sequence without
  *   tokens the final state is the initial one.  out (batch, seqlen, heads, value_dim) dtype, dense.
- * Dimensions up to 256, and no more chunks and heads than a launch has threads for (SS2D_ENOTSUP beyond).  States and sums are
- * fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
+ * Dimensions up to 256, no more chunks and heads than a launch has threads for, and tokens that 32 bits count with three chunks of 64 behind them and, of
+ * packed sequences, one more for each (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
  */
 typedef struct ss2d_linear_attention_params {
     int32_t batch, seqlen, heads, q_heads, k_heads, v_heads, key_dim, value_dim;

@@ -339,3 +339,16 @@ def test_a_step_of_more_sequences_than_32_bits_is_refused(monkeypatch):
     monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
     with pytest.raises(RuntimeError, match="no dimension of more"):
         vmamba_amd.linear_attention_step_fn(**step(stretched, B=MANY))
+
+
+@pytest.mark.parametrize("dtype,chunk", [(_lib.SS2D_BF16, 64), (_lib.SS2D_F16, 32), (_lib.SS2D_F32, 32)], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("sequences_", [0, 1, 100_000])
+def test_tokens_at_the_end_of_32_bits(sequences_, dtype, chunk):
+    """Places of tokens, rounded up to chunks and with a chunk for each packed sequence behind them, stay 32-bit numbers, or the call is refused."""
+    L = _lib.lib()
+    one = dict(batch=1, heads=1, q_heads=1, k_heads=1, v_heads=1, key_dim=8, value_dim=8, dtype=dtype) | (dict(cu_seqlens=256, n_seqs=sequences_) if sequences_ else {})
+    most = 2 ** 31 - 1 - (sequences_ + 3) * chunk
+    assert L.ss2d_linear_attention_workspace_bytes(sequences(seqlen=most, **one)) > 8 * most
+    for tokens in (most + 1, 2 ** 31 - chunk, 2 ** 31 - 2, 2 ** 31 - 1):
+        p = sequences(seqlen=tokens, **one)
+        assert L.ss2d_linear_attention_workspace_bytes(p) == _lib.SS2D_ENOTSUP and L.ss2d_linear_attention_fwd(p, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP, tokens

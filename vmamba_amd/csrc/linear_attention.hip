@@ -686,6 +686,9 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 // of 16 112 / 99, of 32 144 / 133, 192 of 64 220 / 226.
 constexpr int kLaWhole = 5;          // chunks of a sequence that is never cut
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
+    // Places of tokens are 32-bit numbers on the GPU, those of whole chunks too; the table of packed sequences' chunks runs on behind the last token by a chunk
+    // for each sequence and two (la_find_chunk).
+    if (p.tokens + ((p.cu ? (int64_t)p.n_seqs : 0) + 3) * chunk > 0x7fffffff) return SS2D_ENOTSUP;
     const int64_t per_seq = ((int64_t)p.tokens + chunk - 1) / chunk, alone = (int64_t)p.n_seqs * p.heads * tiles;
     const int64_t want = alone >= 192 || (alone >= 128 && per_seq <= 16) ? 1 : (512 + p.heads * tiles - 1) / (p.heads * tiles);
     int64_t chunks, segs, seg_chunks;
