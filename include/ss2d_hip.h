@@ -736,7 +736,7 @@ int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *params, 
  * q (batch, seqlen, q_heads, dim), k (.., k_heads, dim): dtype, the last dimension dense, either with 0 heads; q_out, k_out dense; weights (dim) of
  * weight_dtype (SS2D_F32 or dtype) or NULL (1); positions int32 or int64 (batch, seqlen, axes) by strides, or NULL (no rotation); frequencies
  * (axes, per_axis) float or double, dense.  Angles are 64-bit products.  The LayerNorm of a row without centring
- * (classification/models/vmamba.py:52-57 is the framework's norm of a map's channels).  dim up to 512 (SS2D_ENOTSUP beyond).
+ * (classification/models/vmamba.py:52-57 is the framework's norm of a map's channels).  dim up to 512, seqlen up to 2^31 - 17 (SS2D_ENOTSUP beyond).
  */
 typedef struct ss2d_qk_norm_rotate_params {
     int32_t batch, seqlen, q_heads, k_heads, dim;

@@ -352,3 +352,14 @@ def test_tokens_at_the_end_of_32_bits(sequences_, dtype, chunk):
     for tokens in (most + 1, 2 ** 31 - chunk, 2 ** 31 - 2, 2 ** 31 - 1):
         p = sequences(seqlen=tokens, **one)
         assert L.ss2d_linear_attention_workspace_bytes(p) == _lib.SS2D_ENOTSUP and L.ss2d_linear_attention_fwd(p, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP, tokens
+
+
+def test_norm_of_tokens_at_the_end_of_32_bits():
+    """A round of 16 tokens that begins in front of a batch's last one counts past it before it goes on in the next batch."""
+    L = _lib.lib()
+    for tokens in (2 ** 31 - 16, 2 ** 31 - 1):
+        p = fill(_lib.QkNormRotateParams(), batch=2, seqlen=tokens, q_heads=1, k_heads=1, dim=8, dtype=_lib.SS2D_BF16, eps=1e-6)
+        assert L.ss2d_qk_norm_rotate(p, None) == _lib.SS2D_ENOTSUP
+        assert L.ss2d_qk_norm_rotate_bwd(fill(_lib.QkNormRotateBwdParams(), fwd=p), HERE, 1 << 40, None) == _lib.SS2D_ENOTSUP
+    p.seqlen = 2 ** 31 - 17
+    assert L.ss2d_qk_norm_rotate(p, None) == _lib.SS2D_EINVAL        # (no queries: refused for that)

@@ -368,7 +368,7 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
     if (!p) return SS2D_EINVAL;
     if (p->batch < 0 || p->seqlen < 0 || p->q_heads < 0 || p->k_heads < 0 || p->dim < 1 || p->dtype < SS2D_F32 || p->dtype > SS2D_F16) return SS2D_EINVAL;
     if ((p->q_weight || p->k_weight) && p->weight_dtype != SS2D_F32 && p->weight_dtype != p->dtype) return SS2D_EINVAL;
-    if (p->dim > kQnMaxDim) return SS2D_ENOTSUP;
+    if (p->dim > kQnMaxDim || p->seqlen > 0x7fffffff - kQnTokens) return SS2D_ENOTSUP;       // (a round's tokens are counted on from its first one's place)
     a = {};
     if (p->positions) {
         if (!p->frequencies || p->axes < 1 || p->per_axis < 1 || p->per_axis > p->dim || p->axes > p->dim || 2 * p->axes * p->per_axis > p->dim) return SS2D_EINVAL;
