@@ -363,3 +363,31 @@ def test_norm_of_tokens_at_the_end_of_32_bits():
         assert L.ss2d_qk_norm_rotate_bwd(fill(_lib.QkNormRotateBwdParams(), fwd=p), HERE, 1 << 40, None) == _lib.SS2D_ENOTSUP
     p.seqlen = 2 ** 31 - 17
     assert L.ss2d_qk_norm_rotate(p, None) == _lib.SS2D_EINVAL        # (no queries: refused for that)
+
+
+def test_captures_are_looked_at_through_python(monkeypatch):
+    """A call with gradients asks whether it may be captured before anything is launched, with its own leaves and not with copies of them; one without does not."""
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(qk_norm, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(linear_attention, "linear_attention_fwd", lambda *a: pytest.fail("called"))
+    monkeypatch.setattr(qk_norm, "qk_norm_rotate_fwd", lambda *a: pytest.fail("called"))
+    asked = []
+
+    class Native:
+        @staticmethod
+        def refuse_capture(tensors, what):
+            asked.append((tensors, what))
+            raise RuntimeError("still lives")
+
+    monkeypatch.setattr(_lib, "host", lambda: Native)
+    leaf = on_cpu(2, 4, 6, 8).transpose(2, 3).requires_grad_()       # (not dense: this one is what brings the call through Python)
+    weight = on_cpu(16)[::2].requires_grad_()
+    with pytest.raises(RuntimeError, match="still lives"):
+        vmamba_amd.linear_attention_fn(**attention(on_cpu, initial_state=leaf))
+    with pytest.raises(RuntimeError, match="still lives"):
+        vmamba_amd.qk_norm_rotate_fn(**norm(on_cpu, q_weight=weight))
+    assert [what for _, what in asked] == ["linear_attention_fn", "qk_norm_rotate_fn"] and asked[0][0][4] is leaf and asked[1][0][2] is weight
+    monkeypatch.setattr(linear_attention, "linear_attention_fwd", lambda q, k, v, *a: (torch.zeros_like(v), None))
+    with torch.no_grad():
+        vmamba_amd.linear_attention_fn(**attention(on_cpu, initial_state=leaf))
+    assert len(asked) == 2

@@ -682,3 +682,41 @@ def test_saved_tensors_of_another_type(other, seen):
             torch.autograd.grad(out, leaves, dout)
         with pytest.raises(RuntimeError, match="type"):
             torch.autograd.grad(turned, leaves[:2], [torch.ones_like(t) for t in turned])
+
+
+def test_capture_beside_an_eager_graph_through_python():
+    """As through the extension: of a mode that follows operators, and of leaves that are not dense, whose copies are no leaves.  Nothing of such a call is launched, so no
+    backward comes to it."""
+    import contextlib
+    import gc
+    q, k, v, g, dout, normal = inputs(1, 100, 2, 2, 2, 32, 32, BF16, ("token", 1), 41)
+    state, weight = normal(1, 2, 32, 32).to(DEV).transpose(2, 3).requires_grad_(), normal(64).to(DEV)[::2].requires_grad_()
+    qg = q.detach().requires_grad_()
+    with Seen():
+        eager = [linear_attention_fn(qg, k, v, g), linear_attention_fn(q, k, v, g, initial_state=state), *qk_norm_rotate_fn(q, k, weight)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+        held = torch.zeros(8, device=DEV)
+        for mode, call in ((Seen, lambda: linear_attention_fn(qg, k, v, g)), (Seen, lambda: qk_norm_rotate_fn(qg, k)),
+                           (contextlib.nullcontext, lambda: linear_attention_fn(q, k, v, g, initial_state=state)), (contextlib.nullcontext, lambda: qk_norm_rotate_fn(q, k, weight))):
+            with mode(), pytest.raises(RuntimeError, match="still lives"):
+                call()
+            with mode(), torch.no_grad():
+                call()                                               # (without gradients nothing is in the way)
+    del eager
+    gc.collect()                                                     # (the refusals' tracebacks hold the refused calls)
+    # their graph gone, the same leaves are captured, and replayed
+    want = linear_attention_fn(q, k, v, g, initial_state=state)
+    want = [want.detach(), *torch.autograd.grad(want, state, dout)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = linear_attention_fn(q, k, v, g, initial_state=state)
+        got = [out, *torch.autograd.grad(out, state, dout)]
+    for _ in range(2):
+        for t in got:
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del held

@@ -34,8 +34,8 @@ inline bool recorded(std::initializer_list<const at::Tensor *> tensors) {
 }
 // A call with gradients that is captured: an eager graph of the same leaves that still lives holds their gradients' nodes on another stream, and the engine,
 // which would have the two streams wait for one another at the backward's end, cannot inside a capture and takes the process with it.
-inline void refuse_capture(std::initializer_list<const at::Tensor *> tensors, const char *what) {
-    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA((*tensors.begin())->device().index());
+inline void refuse_capture(at::ArrayRef<const at::Tensor *> tensors, const char *what) {
+    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(tensors.front()->device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
     for (const at::Tensor *t : tensors) {
@@ -44,6 +44,13 @@ inline void refuse_capture(std::initializer_list<const at::Tensor *> tensors, co
         TORCH_CHECK(!node || !node->stream().has_value() || *node->stream() == stream.unwrap(), what,
                     ": this capture's leaves belong to an autograd graph that was recorded on another stream and still lives; drop it first");
     }
+}
+// The same for a call that goes through Python: tensors or None, the first one on the call's device
+static void refuse_capture_of(const std::vector<Maybe> &tensors, const std::string &what) {
+    std::vector<const at::Tensor *> leaves;
+    for (const Maybe &t : tensors)
+        if (t.has_value()) leaves.push_back(&*t);
+    refuse_capture(leaves, what.c_str());
 }
 template <typename P> void strides3(const at::Tensor &t, P &batch, P &token, P &head) { batch = t.stride(0); token = t.stride(1); head = t.stride(2); }
 // What comes into a backward: memory on the inputs' device, its last dimension dense, its type that of what it is the gradient of (the inputs' may have

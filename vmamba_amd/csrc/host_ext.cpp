@@ -287,6 +287,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("scan_bwd", &scan_bwd);
     m.def("cross_scan", &cross_scan);
     m.def("cross_merge", &cross_merge);
+    m.def("refuse_capture", &attention::refuse_capture_of);
     m.def("linear_attention", &attention::linear_attention);
     m.def("linear_attention_step", &attention::linear_attention_step);
     m.def("qk_norm_rotate", &attention::qk_norm_rotate);

@@ -148,6 +148,8 @@ class LinearAttentionHip(torch.autograd.Function):
     def forward(ctx, q, k, v, log_decay, initial_state, scale, cu_seqlens, want_final):
         with untraced():                                             # (a trace holds this call, with whatever tensors it is given when it runs)
             _check_sequences(q, k, v, log_decay, initial_state, cu_seqlens)
+            if ctx.next_functions:                                   # (gradients are recorded)
+                _lib.host().refuse_capture([q, k, v, log_decay, initial_state], "linear_attention_fn")
             ctx.scale = q.shape[3] ** -0.5 if scale is None else float(scale)
             dense = initial_state if initial_state is None else initial_state.contiguous()
             out, final = linear_attention_fwd(q, k, v, log_decay, ctx.scale, dense, cu_seqlens, want_final)

@@ -74,6 +74,8 @@ class QkNormRotateHip(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
         with untraced():                                             # (a trace holds this call, with whatever tensors it is given when it runs)
             _check_all(q, k, q_weight, k_weight, positions, frequencies)
+            if ctx.next_functions:                                   # (gradients are recorded)
+                _lib.host().refuse_capture([q, k, q_weight, k_weight], "qk_norm_rotate_fn")
             outs = qk_norm_rotate_fwd(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
         ctx.eps, ctx.interleaved = eps, interleaved
