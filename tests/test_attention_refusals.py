@@ -391,3 +391,21 @@ def test_captures_are_looked_at_through_python(monkeypatch):
     with torch.no_grad():
         vmamba_amd.linear_attention_fn(**attention(on_cpu, initial_state=leaf))
     assert len(asked) == 2
+
+
+def test_forward_derivatives_are_refused(monkeypatch):
+    """A token's step has no derivative of either kind: a tangent that comes in is not dropped."""
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    monkeypatch.setattr(linear_attention, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(qk_norm, "check_plain", lambda *a, **b: None)
+    monkeypatch.setattr(linear_attention, "linear_attention_fwd", lambda q, k, v, *a: (torch.zeros_like(v), None))
+    monkeypatch.setattr(qk_norm, "qk_norm_rotate_fwd", lambda q, k, *a: (torch.zeros_like(q), torch.zeros_like(k)))
+    monkeypatch.setattr(_lib, "launch", lambda *a: pytest.fail("launched"))
+    with forward_ad.dual_level():
+        for call, build, _ in CALLS:
+            args = build(torch.zeros)
+            for name in ("q", "k", "v", "state"):
+                if name in args:
+                    with pytest.raises(RuntimeError):
+                        call(**args | {name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})

@@ -8,6 +8,7 @@ its state updated in place.  Both run on the HIP kernels of libss2d_hip.so (ss2d
 here.  Arguments are checked as csms6s.py does and fail with RuntimeError.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .norm import TENSOR_KINDS, native_stands, untraced
@@ -225,6 +226,8 @@ def linear_attention_step_fn(q, k, v, log_decay, state, scale=None):
     _check(state.shape[0] <= 1 or state.stride(0) >= per_sequence, "the states of a batch must not overlap")
     _check(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state))),
            "linear_attention_step_fn has no gradient: call it under torch.no_grad(), or linear_attention_fn")
+    _check(forward_ad._current_level < 0 or all(t is None or forward_ad.unpack_dual(t).tangent is None for t in (q, k, v, log_decay, state)),
+           "linear_attention_step_fn has no derivative forward either")
     p = _lib.LinearAttentionStepParams()
     out = torch.empty((shape[0], heads, shape[3]), dtype=q.dtype, device=q.device)
     p.batch, p.heads, p.q_heads, p.k_heads, p.v_heads, p.key_dim, p.value_dim = q.shape[0], heads, q.shape[1], k.shape[1], v.shape[1], shape[2], shape[3]
