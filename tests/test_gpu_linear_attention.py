@@ -720,3 +720,44 @@ def test_capture_beside_an_eager_graph_through_python():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     del held
+
+
+def quadratic(q, k, v, g, state, scale, pieces):
+    """(out, final states) of a batch of one in 64 bits, as sums over the pairs of tokens of each piece and head."""
+    H = v.shape[2]
+    outs, finals = [], []
+    for n, (lo, hi) in enumerate(pieces):
+        for h in range(H):
+            qh, kh, vh = q[0, lo:hi, h * q.shape[2] // H], k[0, lo:hi, h * k.shape[2] // H], v[0, lo:hi, h]
+            G = g[0, lo:hi, h].cumsum(0)
+            apart = (G[:, None] - G[None]).masked_fill(~torch.ones(hi - lo, hi - lo, dtype=torch.bool, device=q.device).tril(), -float("inf"))
+            end = G[-1] if hi > lo else G.sum()
+            outs.append((((qh @ kh.t()) * apart.exp()) @ vh + (qh * G.exp()[:, None]) @ state[n, h]) * scale)
+            finals.append((kh * (end - G).exp()[:, None]).t() @ vh + end.exp() * state[n, h])
+    rows = [torch.stack(outs[n * H:(n + 1) * H], 1) for n in range(len(pieces))]
+    return torch.cat(rows)[None], torch.stack(finals).view(len(pieces), H, q.shape[3], v.shape[3])
+
+
+@pytest.mark.parametrize("packed", [False, True], ids=["one", "packed"])
+@pytest.mark.parametrize("Hk,H,dk,dv", [(1, 1, 64, 64), (2, 2, 128, 128), (1, 2, 192, 256), (1, 1, 130, 96), (1, 3, 80, 144), (2, 2, 33, 200)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_segments_of_states_in_several_pieces(Hk, H, dk, dv, dtype, packed):
+    """Sequences that are cut, of heads whose states take more than one workgroup: what comes into a segment is read back by pieces, in either order.  Decays of which
+    a segment leaves something; all that is kept in 32 bits comes of operands in three parts."""
+    print("CASE pieces", Hk, H, dk, dv, dtype, packed, flush=True)
+    lengths = [0, 700, 37, 411, 0, 64, 330] if packed else [1301]
+    starts = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    T, pieces = starts[-1], list(zip(starts, starts[1:]))
+    q, k, v, g, dout, normal = inputs(1, T, Hk, Hk, H, dk, dv, dtype, ("token", 1), 43)
+    g = g * 0.05
+    state, dfinal = (normal(len(lengths), H, dk, dv).to(DEV) for _ in range(2))
+    got = run_all(q, k, v, g, state, dout, dfinal, torch.tensor(starts, dtype=torch.int32, device=DEV) if packed else None)
+    both = []
+    for size in (False, True):
+        of = lambda t: t.double().abs() if size else t.double()  # noqa: E731
+        leaves = [t.detach().requires_grad_() for t in (of(q), of(k), of(v), g.double(), of(state))]
+        out, final = quadratic(*leaves, dk ** -0.5, pieces)
+        grads = torch.autograd.grad((out * of(dout)).sum() + (final * of(dfinal)).sum(), leaves)
+        both.append({n: t.detach().cpu() for n, t in zip(("out", "final", "dq", "dk", "dv", "dg", "dstate"), (out, final, *grads))})
+    for name in got:
+        check(name, got[name], both[0][name], both[1][name], dtype, (dk, dv), max(lengths), split=2.0 ** -24)
