@@ -409,3 +409,17 @@ def test_forward_derivatives_are_refused(monkeypatch):
                 if name in args:
                     with pytest.raises(RuntimeError):
                         call(**args | {name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
+
+
+@pytest.mark.parametrize("dtype,decay,parts", [(_lib.SS2D_BF16, None, 2), (_lib.SS2D_BF16, 256, 6), (_lib.SS2D_F32, 256, 3)], ids=["bf16", "bf16, decays' gradients", "fp32"])
+def test_a_backward_asks_for_the_states_that_it_keeps(dtype, decay, parts):
+    """Both states of each chunk, in bf16 with what their rounding left where decays' gradients are in single precision; what is behind a chunk in both
+    orders only where it is read so.  Besides them the tables: a few values a token and head."""
+    L, T, H, D = _lib.lib(), 6400, 16, 128
+    p = sequences(batch=1, seqlen=T, heads=H, q_heads=H, k_heads=H, v_heads=H, key_dim=D, value_dim=D, dtype=dtype, decay=decay)
+    g = fill(_lib.LinearAttentionBwdParams(), fwd=p, dout=256, dq=256, dk=256, dv=256, ddecay=decay)
+    chunk, size = (64, 2) if dtype == _lib.SS2D_BF16 else (32, 4)
+    states = parts * (T // chunk) * H * D * D * size
+    segments = 2 * 4 * (D * D + 1) * H * (512 // (H * 2 * 4) + 1)    # their own sums: two workgroups to a CU, of both walks
+    tables = T * H * 8 + (T // chunk) * (H * 8 + 16)
+    assert states <= L.ss2d_linear_attention_bwd_workspace_bytes(g) <= states + segments + tables + 16 * 256

@@ -266,6 +266,10 @@ __device__ __forceinline__ float load_decay(const void *p, int64_t at, int dtype
                                                                                           : to_f32(reinterpret_cast<const f16_t *>(p)[at]);
 }
 
+// Whether the gradients read the states behind the chunks (E) in both orders from memory: of bf16 heads up to 128 they turn them in LDS
+constexpr int kLaTurnDim = 128;
+inline bool la_turned(const LaArgs &p, int dtype) { return dtype != SS2D_BF16 || p.k.dim > kLaTurnDim || p.v.dim > kLaTurnDim; }
+
 // A sequence's {start, end, first chunk, first segment}, whichever way the sequences stand
 __device__ __forceinline__ int4 la_sequence(const LaArgs &p, int n) {
     return p.cu ? p.seqs[n] : make_int4(0, p.tokens, n * p.per_seq, n * p.segs_per_seq);

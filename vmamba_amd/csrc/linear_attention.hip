@@ -836,7 +836,7 @@ int64_t la_carve(LaArgs &p, int dtype, char *base, bool backward, bool low) {
     if (backward) {
         take(p.states, (low ? 3 : 1) * size * entries * state);
         take(p.dstates, (low ? 3 : 1) * size * entries * state);
-        take(p.dstates_t, size * entries * state);
+        take(p.dstates_t, la_turned(p, dtype) ? size * entries * state : 0);
     }
     p.local_floats = p.max_segs > p.n_seqs ? (la_round(4 * (int64_t)p.max_segs * p.heads * (tiles * kLaTile * kLaTile + 1)) / 4) : 0;
     take(p.local, 4 * p.local_floats * (backward ? 2 : 1));

@@ -42,7 +42,7 @@ __device__ __forceinline__ float dot_parts(u32x4_t a, const u32x4_t (&al)[2], u3
 
 // Eight wavefronts where a workgroup has a CU's LDS to itself, four where two or more share it
 template <typename Op, int kDim> struct LaBwdShape {
-    static constexpr bool kTile = sizeof(typename Op::E) == 2 && kDim <= 128;
+    static constexpr bool kTile = sizeof(typename Op::E) == 2 && kDim <= kLaTurnDim;
     static constexpr int kC = Op::kChunk, kPitch = kDim + Op::kPad, kM = kC / 16;
     static constexpr int kTiles = (int)sizeof(typename Op::E) * (4 * kC * kPitch + 2 * kC * (kC + Op::kPad) + (kTile ? kDim * kPitch : 0));
     static constexpr int kWaves = kTiles > 78 * 1024 ? 8 : 4;
@@ -514,7 +514,7 @@ template <typename Op, typename T> static int la_backward(const LaBackward &b, f
     if (!one || p.dfinal || dinitial) {
         LaWalk &s = w[n];
         s.a = p.dout; s.b = p.q;
-        s.out = p.dstates; s.out_t = LaBwdShape<Op, 128>::kTile && p.k.dim <= 128 && p.v.dim <= 128 ? nullptr : p.dstates_t; s.low = p.low;
+        s.out = p.dstates; s.out_t = la_turned(p, sizeof(typename Op::E) == 2 ? SS2D_BF16 : SS2D_F32) ? p.dstates_t : nullptr; s.low = p.low;
         s.from = p.dfinal; s.to = dinitial;
         s.reverse = 1;
         s.exact = dinitial != nullptr;
