@@ -669,7 +669,8 @@ int ss2d_product_f32(const float *a, const float *b, const float *bias, const fl
  *   cu_seqlens NULL, or n_seqs + 1 ascending places (device memory): sequence i is tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of batch 1.  Places
  *   outside 0 .. seqlen are moved into it, a descending one is taken as the one before it; rows of no sequence get zeros.
  *   initial_state, final_state (n_seqs or batch, heads, key_dim, value_dim) fp32, dense, either or both NULL; of a sequence without
- *   tokens the final state is the initial one.  out (batch, seqlen, heads, value_dim) dtype, dense.
+ *   tokens the final state is the initial one.  out (batch, seqlen, heads, value_dim) dtype, dense; of SS2D_BF16 it may differ by a rounding where final_state is
+ *   not NULL, since the states are then summed to 24 bits in place of 16.
  * Dimensions up to 256, no more chunks and heads than a launch has threads for, and tokens that 32 bits count with three chunks of 64 behind them and, of
  * packed sequences, one more for each (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
  */

@@ -4,8 +4,8 @@
 // is cut into chunks of C tokens.  With G_t the sum of the chunk's g up to and with t, and S the state before the chunk,
 //     o_t = scale sum_(s <= t) exp(G_t - G_s) (q_t . k_s) v_s + scale exp(G_t) q_t^T S,
 //     S after = exp(G_C) S + sum_s exp(G_C - G_s) k_s v_s^T,
-// so only the states are walked from chunk to chunk (linear_attention.hip); outputs (same file) and gradients (linear_attention_bwd.hip) of all
-// chunks are independent of one another.  Everything that is a sum of g stands as a pair of floats from a sum in 64 bits and
+// so what goes from chunk to chunk is the state alone.  Outputs and states are one walk over a sequence's chunks (linear_attention.hip); for the gradients two
+// walks store the states before and behind every chunk, and the chunks are then independent of one another (linear_attention_bwd.hip).  Everything that is a sum of g stands as a pair of floats from a sum in 64 bits and
 // goes through exp as a difference first: a decay of -inf (a reset) or a long sum loses nothing.
 //
 // Operands.  bf16 goes to the 16-bit matrix cores as it is; what is computed on the way (weights of pairs, states) is rounded to bf16
@@ -145,7 +145,8 @@ template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 // 16 bytes' worth of row `row` of `rows` (one at least), from column c on, c a multiple of a piece.  kFast: rows hold a piece at least and a chunk's offsets
 // fit 32 bits; the load is then unconditional, wherever it begins -- a row or column that is not there repeats another, the last piece is the one that ends
 // with its row -- so that nothing waits for it before it is used, and held_piece() puts it in its place and makes zeros of what is not there.  Otherwise
-// element by element.  (8 x 4096 tokens, 16 heads of 127 in bf16: 264 us, element by element 728; of 128, one value off the 16-byte grid, 253 and 660, on it 203.)
+// element by element.  (8 x 4096 tokens, 16 heads of 127 in bf16, the outputs alone: 248 us, element by element 634; of 128, one value off the 16-byte grid, 221 and 641,
+// on it 208.  With the final state 264 and 253.)
 template <bool kFast, typename T> __device__ __forceinline__ u32x4_t load_piece(const T *base, int64_t stride, int row, int rows, int c, int cols) {
     if constexpr (kFast) {
         typedef uint32_t here __attribute__((ext_vector_type(4), aligned(2)));

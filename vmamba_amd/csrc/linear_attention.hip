@@ -451,11 +451,13 @@ template int la_walks<OperandBf16, bf16_t>(const LaArgs &, const LaWalk *, int, 
 // The weights behind the diagonal are zeros; a product of zero with what is infinite or NaN would reach tokens in front of it, so a
 // chunk that holds such a value sums its pairs one by one.
 // 8 x 4096 tokens, 16 heads of 128 x 128, bf16: 198-220 us for 555 MB, 2.7 TB/s.  Neither memory nor the matrix cores bound it (busy 12 %) but a chunk's chain -- rows to
-// LDS, pairs, outputs, state, three barriers between them -- of which two workgroups share a CU: 357 vector instructions of a wavefront and 2900 cycles of
-// LDS reads a chunk.  The call took 320 us with four wavefronts of all keys in place of eight of half of them, 474 with the states of all chunks through memory.
+// LDS, pairs, outputs, state, three barriers between them, 357 vector instructions of a wavefront and 2900 cycles of LDS reads -- which nothing else hides: these are
+// 256 workgroups, one to a CU.  Two would fit, and 16 x 2048 tokens, which are two, take 158 us for the same work.  The call took 320 us
+// with four wavefronts of all keys in place of eight of half of them, 474 with the states of all chunks through memory.
 constexpr int kLaWaves = kLaThreads / kWave;
 // kOwn, of sequences of a few chunks and up to 64 keys: it sums their decays itself, which takes a chunk less than another launch takes for all of them
-// (37 tokens, 8 heads of 64: 10.4 -> 7.8 us a call).
+// (37 tokens, 8 heads of 64, bf16: 10.9 -> 8.6 us a call; 120 tokens 12.2 -> 9.9, 256, four chunks, 16.6 -> 15.4).  Keys of 128 and 256 would gain as much at one or two
+// chunks (11.0 -> 8.5 and 13.6 -> 10.1 at 37 tokens); the kernels of these sizes are not there twice.
 constexpr int kLaOwnChunks = 4, kLaOwnKeys = 64;
 
 template <typename Op, typename T, int kTiles, int kParts, bool kFast, bool kOwn>
@@ -682,8 +684,9 @@ __global__ __launch_bounds__(kLaThreads, kTiles <= 8 ? 4 : 2) void la_out_kernel
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 // Segments: where the sequences alone do not give the chip its workgroups (`tiles` for a head), each is cut so that there are two to a CU, into
 // `shortest` chunks at least: a segment is walked twice.  192 workgroups are enough, since the cut costs two launches and the second reading; 128 where
-// chains are short.  us cut / whole, forward: 96 workgroups of 25 chunks 48 / 75, 128 of 8 30 / 25, of 16 40 / 40; gradients: 192 of 25 124 / 119, 256 of 8 69 / 57,
-// of 16 112 / 99, of 32 144 / 133, 192 of 64 220 / 226.
+// chains are short.  us cut / whole, heads of 64, bf16, forward: 128 workgroups of 8 chunks 32 / 27, of 16 42 / 44, of 25 55 / 63, of 64 101 / 140; 192 of 8 42 / 27, of 25 78 / 62,
+// of 64 168 / 148.  A training step whose walks for the gradients are cut or whole: 192 of 16 139 / 130, of 25 177 / 173, of 32 220 / 218, of 64 416 / 423; 256 of 64
+// 522 / 502; in single precision 192 of 25 200 / 191, of 32 263 / 262, of 64 479 / 486.  So the border is right up to 32 chunks and 2 % off at 64.
 constexpr int kLaWhole = 5;          // chunks of a sequence that is never cut
 int la_plan(LaArgs &p, int chunk, int64_t tiles, int shortest, int lanes) {
     // Places of tokens are 32-bit numbers on the GPU, those of whole chunks too; the table of packed sequences' chunks runs on behind the last token by a chunk

@@ -21,7 +21,7 @@ struct QnSide {
     void *y;                         // dense; forward: the result, backward: dx
     const void *w;                   // (dim) or NULL
     int64_t batch, token, head, dy_batch, dy_token, dy_head;
-    int32_t heads, aligned;
+    int32_t heads;
 };
 
 struct QnArgs {
@@ -234,7 +234,8 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotate_kernel(const QnArgs p) 
     }
 }
 
-// Any dimension, alignment and number of pairs: a wavefront to a row, a pair or two single values to a lane at a time.
+// Any dimension, alignment and number of pairs: a wavefront to a row, a pair or two single values to a lane at a time, the weights again for each row.
+// 4 x 4096 tokens of 32 + 8 heads, bf16: of 128, one value off the grid of 8 bytes, 344 us (72 on it), with the gradients 875 (191); of 100 291 and 812.
 template <typename T, bool kBack>
 __global__ __launch_bounds__(kBlock) void qk_norm_rotate_any_kernel(const QnArgs p) {
     constexpr int kSlots = kBlock / kWave, kMost = kQnMaxDim / 2 / kWave;
@@ -377,8 +378,8 @@ static int qn_arguments(const ss2d_qk_norm_rotate_params *p, QnArgs &a, bool &ve
         a.pos_batch = p->position_batch_stride; a.pos_token = p->position_token_stride; a.pos_axis = p->position_axis_stride;
     }
     a.batch = p->batch; a.tokens = p->seqlen; a.dim = p->dim; a.w_dtype = p->weight_dtype; a.interleaved = p->interleaved != 0; a.eps = p->eps;
-    a.side[0] = {p->q, nullptr, p->q_out, p->q_weight, p->q_batch_stride, p->q_token_stride, p->q_head_stride, 0, 0, 0, p->q_heads, 0};
-    a.side[1] = {p->k, nullptr, p->k_out, p->k_weight, p->k_batch_stride, p->k_token_stride, p->k_head_stride, 0, 0, 0, p->k_heads, 0};
+    a.side[0] = {p->q, nullptr, p->q_out, p->q_weight, p->q_batch_stride, p->q_token_stride, p->q_head_stride, 0, 0, 0, p->q_heads};
+    a.side[1] = {p->k, nullptr, p->k_out, p->k_weight, p->k_batch_stride, p->k_token_stride, p->k_head_stride, 0, 0, 0, p->k_heads};
     if (back) {
         a.side[0].dy = g->dq_out; a.side[0].y = g->dq;
         a.side[0].dy_batch = g->dq_batch_stride; a.side[0].dy_token = g->dq_token_stride; a.side[0].dy_head = g->dq_head_stride;

@@ -192,7 +192,7 @@ def linear_attention_fn(q, k, v, log_decay=None, scale=None, initial_state=None,
     initial_state (sequences, heads, key_dim, value_dim) float32.
 
     Returns out (batch, tokens, heads, value_dim) in q's dtype, with ``output_final_state`` (out, final_state): the states behind the last tokens,
-    float32, which linear_attention_step_fn carries on.
+    float32, which linear_attention_step_fn carries on.  In bfloat16 the states are then summed to 24 bits in place of 16, and out may be another by a rounding.
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a GPU tensor: vmamba_amd has no CPU path")
