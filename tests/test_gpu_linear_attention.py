@@ -761,3 +761,20 @@ def test_segments_of_states_in_several_pieces(Hk, H, dk, dv, dtype, packed):
         both.append({n: t.detach().cpu() for n, t in zip(("out", "final", "dq", "dk", "dv", "dg", "dstate"), (out, final, *grads))})
     for name in got:
         check(name, got[name], both[0][name], both[1][name], dtype, (dk, dv), max(lengths), split=2.0 ** -24)
+
+
+def test_what_is_not_dense_may_change_behind_the_forward():
+    """Of a state, weights and frequencies that are not dense it is a copy that is kept for the gradients: writing into them later, as a token's step does, changes none."""
+    q, k, v, g, dout, normal = inputs(1, 60, 2, 2, 2, 16, 16, F32, ("token", 1), 47)
+    state, weight, f = normal(1, 2, 16, 16).to(DEV).transpose(2, 3), normal(32).to(DEV)[::2], torch.rand(16, device=DEV)[::2]
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+
+    def both(spoil):
+        turned = qk_norm_rotate_fn(*leaves[:2], weight, None, torch.arange(60, device=DEV), f)
+        out = linear_attention_fn(*turned, leaves[2], g, initial_state=state)
+        if spoil:
+            for t in (state, weight, f):
+                t.fill_(7.0)
+        return torch.autograd.grad(out, leaves, dout)
+
+    assert all(torch.equal(a, b) for a, b in zip(both(False), both(True)))

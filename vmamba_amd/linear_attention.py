@@ -152,8 +152,8 @@ class LinearAttentionHip(torch.autograd.Function):
             if ctx.next_functions:                                   # (gradients are recorded)
                 _lib.host().refuse_capture([q, k, v, log_decay, initial_state], "linear_attention_fn")
             ctx.scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-            dense = initial_state if initial_state is None else initial_state.contiguous()
-            out, final = linear_attention_fwd(q, k, v, log_decay, ctx.scale, dense, cu_seqlens, want_final)
+            initial_state = initial_state if initial_state is None else initial_state.contiguous()
+            out, final = linear_attention_fwd(q, k, v, log_decay, ctx.scale, initial_state, cu_seqlens, want_final)
         ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens)
         ctx.set_materialize_grads(False)
         return out, final

@@ -61,7 +61,6 @@ def _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
 
 def qk_norm_rotate_fwd(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
     """(q, k) of arguments that qk_norm_rotate_fn has checked."""
-    q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
     outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     p = _params(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
     p.q_out, p.k_out = (t.data_ptr() for t in outs)
@@ -76,6 +75,7 @@ class QkNormRotateHip(torch.autograd.Function):
             _check_all(q, k, q_weight, k_weight, positions, frequencies)
             if ctx.next_functions:                                   # (gradients are recorded)
                 _lib.host().refuse_capture([q, k, q_weight, k_weight], "qk_norm_rotate_fn")
+            q_weight, k_weight, frequencies = (t if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
             outs = qk_norm_rotate_fwd(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
         ctx.eps, ctx.interleaved = eps, interleaved
