@@ -766,6 +766,70 @@ typedef struct ss2d_qk_norm_rotate_bwd_params {
 int64_t ss2d_qk_norm_rotate_bwd_workspace_bytes(int dim);
 int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * The selective scan of token sequences: tokens are rows, channels neighbours; with N = dstate values of a state h per channel,
+ *   step = softplus(delta + delta_bias) (without delta_softplus the sum itself),  h_t = exp(step_t A) h_(t-1) + step_t u_t B_t,
+ *   out_t = (C_t . h_t + D u_t) silu(z_t),  h_0 = initial_state or 0.
+ * The recurrence of ss2d_selective_scan_fwd (classification/models/csms6s.py:29-68) for a language model's layout, with states that come in and go out.
+ *   u, delta, z (batch, seqlen, dim): dtype, channels dense, other strides in elements; z NULL: no gate.
+ *   B, C (batch, seqlen, n_groups, dstate): dtype, states dense; channel d belongs to group d / (dim / n_groups).
+ *   A (dim, dstate), D (dim) or NULL (0), delta_bias (dim) or NULL (0): fp32, dense.
+ *   cu_seqlens NULL, or n_seqs + 1 ascending places (device memory): sequence i is tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of batch 1.  Places
+ *   outside 0 .. seqlen are moved into it; what descending ones leave in the results is not defined (nothing outside the tensors is touched).  Rows of no
+ *   sequence get zeros.
+ *   initial_state, final_state (n_seqs or batch, dim, dstate) fp32, dense, either or both NULL; of a sequence without tokens the final state is the initial one.
+ *   kept_states NULL or ss2d_token_scan_kept_states(params) floats: the states before every 64th token, which the gradients start from.
+ *   out (batch, seqlen, dim) dtype, dense.
+ * dstate up to 64 (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
+ */
+typedef struct ss2d_token_scan_params {
+    int32_t batch, seqlen, dim, dstate, n_groups, n_seqs, dtype, delta_softplus;
+    const void *u, *delta, *B, *C, *z;
+    const float *A, *D, *delta_bias, *initial_state;
+    const int32_t *cu_seqlens;
+    void *out;
+    float *final_state, *kept_states;
+    int64_t u_batch_stride, u_token_stride, delta_batch_stride, delta_token_stride, z_batch_stride, z_token_stride;
+    int64_t B_batch_stride, B_token_stride, B_group_stride, C_batch_stride, C_token_stride, C_group_stride;
+} ss2d_token_scan_params;
+
+int64_t ss2d_token_scan_workspace_bytes(const ss2d_token_scan_params *params);
+int64_t ss2d_token_scan_kept_states(const ss2d_token_scan_params *params);
+int ss2d_token_scan_fwd(const ss2d_token_scan_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Gradients of ss2d_token_scan_fwd, from the inputs again and the states that the forward kept (fwd.kept_states, read only; fwd.out and fwd.final_state are not looked
+ * at): dout (batch, seqlen, dim) dtype by its strides, dfinal_state as final_state or NULL.  du, ddelta, dz (not NULL where z is not), dB, dC: dtype, dense, in
+ * the shapes of what they are the gradients of; dA (dim, dstate), dD (dim), ddelta_bias (dim), dinitial_state: fp32, any of them NULL.
+ * No atomics: the same bits every time.  Rows of no sequence get zeros.
+ */
+typedef struct ss2d_token_scan_bwd_params {
+    ss2d_token_scan_params fwd;
+    const void *dout;
+    const float *dfinal_state;
+    void *du, *ddelta, *dB, *dC, *dz;
+    float *dA, *dD, *ddelta_bias, *dinitial_state;
+    int64_t dout_batch_stride, dout_token_stride;
+} ss2d_token_scan_bwd_params;
+
+int64_t ss2d_token_scan_bwd_workspace_bytes(const ss2d_token_scan_bwd_params *params);
+int ss2d_token_scan_bwd(const ss2d_token_scan_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * One token for each of `batch` sequences: the recurrence of ss2d_token_scan_fwd once, state (batch, dim, dstate) fp32 in place, dense but for the batch's
+ * stride, which keeps the states apart.  u, delta, z (or NULL), B, C as there without the tokens; out (batch, dim) dtype, dense.
+ */
+typedef struct ss2d_token_scan_step_params {
+    int32_t batch, dim, dstate, n_groups, dtype, delta_softplus;
+    const void *u, *delta, *B, *C, *z;
+    const float *A, *D, *delta_bias;
+    float *state;
+    void *out;
+    int64_t u_batch_stride, delta_batch_stride, z_batch_stride, B_batch_stride, B_group_stride, C_batch_stride, C_group_stride, state_batch_stride;
+} ss2d_token_scan_step_params;
+
+int ss2d_token_scan_step(const ss2d_token_scan_step_params *params, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

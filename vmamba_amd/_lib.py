@@ -29,7 +29,9 @@ EXPORTS = ("ss2d_abi_version", "ss2d_strerror", "ss2d_cross_scan", "ss2d_cross_m
            "ss2d_x_proj", "ss2d_x_proj_applies", "ss2d_x_proj_f32", "ss2d_dt_proj", "ss2d_dt_proj_f32", "ss2d_dt_proj_masked", "ss2d_cross_scan_flex", "ss2d_cross_scan_flex_ws", "ss2d_cross_scan_flex_static", "ss2d_cross_merge_flex",
            "ss2d_selective_scan_bwd", "ss2d_selective_scan_bwd_kernel", "ss2d_clear", "ss2d_round_pair", "ss2d_transpose_bcl", "ss2d_mlp_fused", "ss2d_linear_cl", "ss2d_linear_rows", "ss2d_linear_tiles", "ss2d_conv3x3s2_cl", "ss2d_linear_dw_f32", "ss2d_layer_norm_bwd_f32", "ss2d_layer_norm_bwd_f32_workspace_bytes", "ss2d_column_sums_f32", "ss2d_column_sums_f32_workspace_bytes", "ss2d_product_f32", "ss2d_product_f32_workspace_bytes", "ss2d_linear_dw_f32_workspace_bytes", "ss2d_linear_cf_ln", "ss2d_stem_conv_ln_gelu", "ss2d_stem_conv2_ln", "ss2d_mean_pool_cl",
            "ss2d_linear_attention_workspace_bytes", "ss2d_linear_attention_fwd", "ss2d_linear_attention_bwd_workspace_bytes", "ss2d_linear_attention_bwd",
-           "ss2d_linear_attention_step", "ss2d_qk_norm_rotate", "ss2d_qk_norm_rotate_bwd_workspace_bytes", "ss2d_qk_norm_rotate_bwd")
+           "ss2d_linear_attention_step", "ss2d_qk_norm_rotate", "ss2d_qk_norm_rotate_bwd_workspace_bytes", "ss2d_qk_norm_rotate_bwd",
+           "ss2d_token_scan_workspace_bytes", "ss2d_token_scan_kept_states", "ss2d_token_scan_fwd", "ss2d_token_scan_bwd_workspace_bytes", "ss2d_token_scan_bwd",
+           "ss2d_token_scan_step")
 
 
 class ScanParams(ctypes.Structure):
@@ -138,6 +140,35 @@ class QkNormRotateBwdParams(ctypes.Structure):
     _fields_ = (
         [("fwd", QkNormRotateParams)] + [(n, ctypes.c_void_p) for n in ("dq_out", "dk_out", "dq", "dk", "dq_weight", "dk_weight")]
         + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("dq", "dk") for axis in ("batch", "token", "head")]
+    )
+
+
+class TokenScanParams(ctypes.Structure):
+    """struct ss2d_token_scan_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "seqlen", "dim", "dstate", "n_groups", "n_seqs", "dtype", "delta_softplus")]
+        + [(n, ctypes.c_void_p) for n in ("u", "delta", "B", "C", "z", "A", "D", "delta_bias", "initial_state", "cu_seqlens", "out", "final_state", "kept_states")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("u", "delta", "z") for axis in ("batch", "token")]
+        + [(f"{n}_{axis}_stride", ctypes.c_int64) for n in ("B", "C") for axis in ("batch", "token", "group")]
+    )
+
+
+class TokenScanBwdParams(ctypes.Structure):
+    """struct ss2d_token_scan_bwd_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [("fwd", TokenScanParams)]
+        + [(n, ctypes.c_void_p) for n in ("dout", "dfinal_state", "du", "ddelta", "dB", "dC", "dz", "dA", "dD", "ddelta_bias", "dinitial_state")]
+        + [(f"dout_{axis}_stride", ctypes.c_int64) for axis in ("batch", "token")]
+    )
+
+
+class TokenScanStepParams(ctypes.Structure):
+    """struct ss2d_token_scan_step_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "dim", "dstate", "n_groups", "dtype", "delta_softplus")]
+        + [(n, ctypes.c_void_p) for n in ("u", "delta", "B", "C", "z", "A", "D", "delta_bias", "state", "out")]
+        + [(n, ctypes.c_int64) for n in ("u_batch_stride", "delta_batch_stride", "z_batch_stride", "B_batch_stride", "B_group_stride", "C_batch_stride",
+                                         "C_group_stride", "state_batch_stride")]
     )
 
 
@@ -311,6 +342,13 @@ def lib():
             getattr(L, name).restype, getattr(L, name).argtypes = ctypes.c_int, [ctypes.POINTER(params), ctypes.c_void_p]
         L.ss2d_qk_norm_rotate_bwd_workspace_bytes.restype = ctypes.c_int64
         L.ss2d_qk_norm_rotate_bwd_workspace_bytes.argtypes = [ctypes.c_int]
+        for name, params in (("ss2d_token_scan_workspace_bytes", TokenScanParams), ("ss2d_token_scan_kept_states", TokenScanParams),
+                             ("ss2d_token_scan_bwd_workspace_bytes", TokenScanBwdParams)):
+            getattr(L, name).restype, getattr(L, name).argtypes = ctypes.c_int64, [ctypes.POINTER(params)]
+        for name, params in (("ss2d_token_scan_fwd", TokenScanParams), ("ss2d_token_scan_bwd", TokenScanBwdParams)):
+            getattr(L, name).restype = ctypes.c_int
+            getattr(L, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+        L.ss2d_token_scan_step.restype, L.ss2d_token_scan_step.argtypes = ctypes.c_int, [ctypes.POINTER(TokenScanStepParams), ctypes.c_void_p]
         if L.ss2d_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.ss2d_abi_version()} != expected {ABI_VERSION}; rebuild")
         _lib = L

@@ -1,0 +1,388 @@
+// Forward of the selective scan of token sequences (token_scan.h).
+//
+// A tile of 16 tokens: the lanes take four channels of a token each, find step, step u and the skip term, and lay step and step u down in LDS; B and C
+// come as fp32 rows beside them.  Then every lane walks the 16 tokens of its channel's states; the sums C . h of the sets meet in DPP additions, go through LDS back to
+// the lanes of the first kind, which add the skip term, apply the gate and store.  The next tile's loads are on their way meanwhile.  A wavefront meets no
+// other: no workgroup barrier.
+#include "token_scan.h"
+
+namespace ss2d {
+
+template <typename T, int kSets, int kM, bool kLocal>
+__global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArgs p) {
+    using L = TsLane<kSets, kM>;
+    __shared__ __align__(16) float s_all[kWavesPerWg][kTsTile * (L::kPairPitch + 2 * L::kStates)];
+    const L l(threadIdx.x & (kWave - 1));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    float *s_step = s_all[wave], *s_B = s_step + kTsTile * L::kPairPitch, *s_C = s_B + kTsTile * L::kStates, *s_y = s_step;
+    uint32_t id = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    const int wg = (int)(id % (uint32_t)p.wgs); id /= (uint32_t)p.wgs;
+    const int g = (int)(id % (uint32_t)p.groups); id /= (uint32_t)p.groups;
+    const int segs = kLocal ? p.n_segs - 1 : p.n_segs, seg = (int)(id % (uint32_t)segs), b = (int)(id / (uint32_t)segs);
+    const int first = (wg * kWavesPerWg + wave) * L::kCh, n_chan = min(L::kCh, p.per_group - first);
+    if (n_chan <= 0) return;
+    const int c0 = g * p.per_group + first, s0 = seg * p.seg_len, s1 = min(s0 + p.seg_len, p.tokens);
+    const bool whole = n_chan == L::kCh;
+    const int mine = min(max(n_chan - l.at, 0), 4);                  // channels of a lane that stages
+    const int at = mine > 0 ? l.at : 0;
+    const bool there = l.chan < n_chan;
+    const int d = c0 + min(l.chan, n_chan - 1);
+
+    int t = s0;
+    TsSpan sp = {b, 0, p.tokens};
+    int64_t state_at = 0;
+    if constexpr (kLocal) {
+        sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, s1 - 1);
+        const int carry = sp.seq < 0 || sp.hi <= s1 ? kTsNothing : sp.lo >= s0 ? kTsStarts : kTsThrough;
+        if (wg == 0 && g == 0 && threadIdx.x == 0) p.flags[(int64_t)b * segs + seg] = carry;
+        if (carry == kTsNothing) return;
+        t = max(s0, sp.lo);
+        state_at = (((int64_t)b * segs + seg) * p.dim + d) * p.N;
+    } else {
+        sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, t);
+    }
+
+    const T *u = (const T *)p.u + (int64_t)b * p.u_b + c0 + at, *dl = (const T *)p.delta + (int64_t)b * p.dl_b + c0 + at;
+    const T *z = p.z ? (const T *)p.z + (int64_t)b * p.z_b + c0 + at : nullptr;
+    const T *Bp = (const T *)p.B + (int64_t)b * p.B_b + (int64_t)g * p.B_g, *Cp = (const T *)p.C + (int64_t)b * p.C_b + (int64_t)g * p.C_g;
+    T *out = (T *)p.out + (int64_t)b * p.tokens * p.dim + c0 + at;
+    const int bc_n = min(max(p.N - 4 * l.piece, 0), 4), bc_at = bc_n > 0 ? 4 * l.piece : 0;
+    const bool bc_whole = p.N == L::kStates;
+    float bias[4], skip[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = p.bias && i < mine ? p.bias[c0 + at + i] : 0.0f;
+        skip[i] = p.D && i < mine ? p.D[c0 + at + i] : 0.0f;
+    }
+    floatx4_t A2[kM], h[kM];
+    ts_read_state<kSets, kM>(p.A + (int64_t)d * p.N, p.N, l, true, A2);
+#pragma unroll
+    for (int m = 0; m < kM; ++m) A2[m] *= kLog2e;
+    auto start = [&](const TsSpan &s) { ts_read_state<kSets, kM>(p.initial ? p.initial + ((int64_t)s.seq * p.dim + d) * p.N : nullptr, p.N, l, there, h); };
+    auto nothing = [&](int from, int to) {                           // tokens of no sequence
+        if constexpr (!kLocal) {
+            const float zeros[4] = {0, 0, 0, 0};
+            for (int k = from + l.row; k < to; k += L::kRows) ts_store4<T>(out + (int64_t)k * p.dim, mine, whole, zeros);
+        }
+    };
+    if constexpr (!kLocal) {
+        if (p.cu && p.final)                                         // sequences without tokens, dealt out over the segments
+            for (int i = seg; i < p.n_seqs; i += p.n_segs) {
+                const int lo = min(max(p.cu[i], 0), p.tokens), hi = min(max(p.cu[i + 1], 0), p.tokens);
+                if (hi > lo) continue;
+                start({i, lo, lo});
+                ts_write_state<kSets, kM>(p.final + ((int64_t)i * p.dim + d) * p.N, p.N, l, there, h);
+            }
+        while (sp.seq < 0) {
+            nothing(t, min(sp.hi, s1));
+            t = sp.hi;
+            if (t >= s1) return;
+            sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, t);
+        }
+    }
+    if (t == sp.lo) start(sp);
+    else if constexpr (kLocal) {
+#pragma unroll
+        for (int m = 0; m < kM; ++m) h[m] = floatx4_t{0, 0, 0, 0};
+    } else {
+        ts_read_state<kSets, kM>(p.enter + (((int64_t)b * (p.n_segs - 1) + seg - 1) * p.dim + d) * p.N, p.N, l, there, h);
+    }
+
+    Raw4<T> ru[L::kRounds], rd[L::kRounds], rz[L::kRounds], rB[L::kBcRounds], rC[L::kBcRounds];
+    auto request = [&](int from, int to) {                           // tokens from .. to - 1 of one tile
+#pragma unroll
+        for (int r = 0; r < L::kRounds; ++r) {
+            const int64_t k = min(from + r * L::kRows + l.row, to - 1);
+            ru[r] = ts_load4<T>(u + k * p.u_t, mine, whole);
+            rd[r] = ts_load4<T>(dl + k * p.dl_t, mine, whole);
+            if constexpr (!kLocal) if (z) rz[r] = ts_load4<T>(z + k * p.z_t, mine, whole);
+        }
+#pragma unroll
+        for (int r = 0; r < L::kBcRounds; ++r) {
+            const int64_t k = min(from + r * L::kBcRows + l.bc_row, to - 1);
+            rB[r] = ts_load4<T>(Bp + k * p.B_t + bc_at, bc_n, bc_whole);
+            if constexpr (!kLocal) rC[r] = ts_load4<T>(Cp + k * p.C_t + bc_at, bc_n, bc_whole);
+        }
+    };
+    auto tile_end = [&](int from, const TsSpan &s) { return min(min(s.hi, s1), (from | (kTsTile - 1)) + 1); };
+    float sum[4] = {0, 0, 0, 0};                                     // kLocal: the steps of a lane's tokens and channels
+    int end = tile_end(t, sp);
+    request(t, end);
+    for (;;) {
+        const int n = end - t;
+        // ---- stage -----------------------------------------------------------------------------------------------------------
+        float extra[L::kRounds][4], gate[L::kRounds][4];
+#pragma unroll
+        for (int r = 0; r < L::kRounds; ++r) {
+            const int k = r * L::kRows + l.row;
+            float uv[4], dv[4], step[4];
+            ts_widen<T>(ru[r], uv);
+            ts_widen<T>(rd[r], dv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                step[i] = p.softplus ? softplus_log2(fmaf(dv[i], kLog2e, bias[i] * kLog2e)) : dv[i] + bias[i];
+                const bool in = k < n && (whole || i < mine);
+                step[i] = in ? step[i] : 0.0f;
+                uv[i] = in ? uv[i] : 0.0f;
+                extra[r][i] = skip[i] * uv[i];
+                if constexpr (kLocal) sum[i] += step[i];
+            }
+            float *to = s_step + k * L::kPairPitch + 2 * l.at;
+            *reinterpret_cast<float4 *>(to) = make_float4(step[0], step[0] * uv[0], step[1], step[1] * uv[1]);
+            *reinterpret_cast<float4 *>(to + 4) = make_float4(step[2], step[2] * uv[2], step[3], step[3] * uv[3]);
+            if constexpr (!kLocal) {
+                if (z) {
+                    float zv[4];
+                    ts_widen<T>(rz[r], zv);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) gate[r][i] = zv[i] * ts_sigmoid(zv[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) gate[r][i] = 1.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < L::kBcRounds; ++r) {
+            const int k = r * L::kBcRows + l.bc_row;
+            if (L::kBcRows > kTsTile && k >= kTsTile) continue;
+            float v[4];
+            ts_widen<T>(rB[r], v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = k < n ? v[i] : 0.0f;
+            *reinterpret_cast<float4 *>(s_B + k * L::kStates + 4 * l.piece) = bc_n > 0 ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(0, 0, 0, 0);
+            if constexpr (!kLocal) {
+                ts_widen<T>(rC[r], v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = k < n ? v[i] : 0.0f;
+                *reinterpret_cast<float4 *>(s_C + k * L::kStates + 4 * l.piece) = bc_n > 0 ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(0, 0, 0, 0);
+            }
+        }
+        // ---- the next tile, and what it starts with -----------------------------------------------------------------------------
+        const int next = end;
+        const bool ends = next == sp.hi;                             // (of the sequence)
+        const TsSpan was = sp;
+        int next_end = next, zeros_to = 0;
+        if (next < s1) {
+            if (ends) sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, next);
+            if (sp.seq < 0) zeros_to = min(sp.hi, s1);               // (behind the last sequence)
+            else next_end = tile_end(next, sp);
+        }
+        if (next_end > next) request(next, next_end);
+        __builtin_amdgcn_sched_barrier(0);
+        wave_lds_sync();
+        // ---- compute ---------------------------------------------------------------------------------------------------------
+        if constexpr (!kLocal) {
+            if (p.kept && t % kTsGrid == 0 && t > 0)
+                ts_write_state<kSets, kM>(p.kept + (((int64_t)b * p.n_grid + t / kTsGrid) * p.dim + d) * p.N, p.N, l, there, h);
+        }
+        float y[kTsTile];
+#pragma unroll
+        for (int k = 0; k < kTsTile; ++k) {
+            const float2 pair = *reinterpret_cast<const float2 *>(s_step + k * L::kPairPitch + 2 * l.chan);
+            y[k] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                floatx4_t kept;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) kept[v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]) * h[m][v];
+                h[m] = ts_outer(s_B[k * L::kStates + l.state(m) + l.col], pair.y, kept);
+                if constexpr (!kLocal) {
+                    const float4 c = *reinterpret_cast<const float4 *>(s_C + k * L::kStates + l.state(m));
+                    y[k] = fmaf(c.w, h[m][3], fmaf(c.z, h[m][2], fmaf(c.y, h[m][1], fmaf(c.x, h[m][0], y[k]))));
+                }
+            }
+        }
+        wave_lds_sync();
+        if constexpr (!kLocal) {
+            ts_sum_sets<kSets>(y);
+            constexpr int kLeft = kTsTile / kSets;
+#pragma unroll
+            for (int i = 0; i < kLeft; ++i) s_y[(kLeft * l.set + i) * L::kPitch + l.chan] = y[i];
+            wave_lds_sync();
+#pragma unroll
+            for (int r = 0; r < L::kRounds; ++r) {
+                const int k = r * L::kRows + l.row;
+                const float4 part = *reinterpret_cast<const float4 *>(s_y + k * L::kPitch + l.at);
+                const float o[4] = {(part.x + extra[r][0]) * gate[r][0], (part.y + extra[r][1]) * gate[r][1], (part.z + extra[r][2]) * gate[r][2],
+                                    (part.w + extra[r][3]) * gate[r][3]};
+                if (k < n) ts_store4<T>(out + (int64_t)(t + k) * p.dim, mine, whole, o);
+            }
+            wave_lds_sync();
+            if (ends && p.final) ts_write_state<kSets, kM>(p.final + ((int64_t)was.seq * p.dim + d) * p.N, p.N, l, there, h);
+        }
+        if (next_end == next) {
+            nothing(next, zeros_to);
+            break;
+        }
+        if (ends) start(sp);
+        t = next;
+        end = next_end;
+    }
+    if constexpr (kLocal) {
+        ts_write_state<kSets, kM>(p.end + state_at, p.N, l, there, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int over = L::kCols; over < kWave; over *= 2) sum[i] += __shfl_xor(sum[i], over, kWave);
+            if (l.row == 0 && i < mine) p.sums[((int64_t)b * segs + seg) * p.dim + c0 + at + i] = sum[i];
+        }
+    }
+}
+
+// What enters every segment but the first: a thread per (row, channel, state).  The product of a segment's decays is taken in two halves, so that neither
+// leaves the range of fp32 before the state would.
+__global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_t per_row) {
+    const uint32_t item = blockIdx.x * kBlock + threadIdx.x;
+    const int b = (int)blockIdx.y, segs = p.n_segs - 1;
+    if (item >= per_row) return;
+    const uint32_t d = item / (uint32_t)p.N;
+    const float A2 = 0.5f * kLog2e * p.A[item];
+    const float *end = p.end + (int64_t)b * segs * per_row + item, *sums = p.sums + (int64_t)b * segs * p.dim + d;
+    const int32_t *flags = p.flags + (int64_t)b * segs;
+    float *enter = p.enter + (int64_t)b * segs * per_row + item;
+    constexpr int kFly = 8;
+    float carry = 0.0f;
+    for (int s0 = 0; s0 < segs; s0 += kFly) {
+        float left[kFly], sum[kFly];
+        int flag[kFly];
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+            const int s = min(s0 + i, segs - 1);
+            left[i] = end[(int64_t)s * per_row];
+            sum[i] = sums[(int64_t)s * p.dim];
+            flag[i] = flags[s];
+        }
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+            if (s0 + i >= segs) break;
+            if (flag[i] == kTsThrough && carry != 0.0f) {
+                const float half = __builtin_amdgcn_exp2f(A2 * sum[i]);
+                carry = fabsf(carry) == __builtin_inff() ? carry + left[i] : fmaf(carry * half, half, left[i]);
+            } else {
+                carry = flag[i] == kTsNothing ? 0.0f : left[i];      // (of nothing, the segment's memory holds nothing)
+            }
+            enter[(int64_t)(s0 + i) * per_row] = carry;
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+static int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
+
+// Segments of the token axis.  A cut sequence is walked twice for what goes into the later segments.
+static void ts_cut(TsArgs &a) {
+    const int ch = kWave / ts_sets(a.N);
+    a.wgs = (int)(((int64_t)a.per_group + ch * kWavesPerWg - 1) / (ch * kWavesPerWg));
+    const int64_t waves = (int64_t)a.batch * a.groups * ((a.per_group + ch - 1) / ch);
+    constexpr int64_t kEnough = 768, kTarget = 2048;
+    int64_t n = waves >= kEnough ? 1 : (kTarget + waves - 1) / waves;
+    const int64_t most = (a.tokens + 2 * kTsGrid - 1) / (2 * kTsGrid);
+    n = n < most ? n : most;
+    n = n < 1 ? 1 : n;
+    const int64_t len = ((a.tokens + n - 1) / n + kTsGrid - 1) / kTsGrid * kTsGrid;
+    a.seg_len = (int)(len < kTsGrid ? kTsGrid : len);
+    a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
+    if (a.n_segs < 1) a.n_segs = 1;
+    a.n_grid = (int)((a.tokens + (int64_t)kTsGrid - 1) / kTsGrid);
+}
+
+static int64_t ts_carve(TsArgs &a, uint8_t *base) {
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { uint8_t *p = base ? base + at : nullptr; at += (bytes + 255) / 256 * 256; return p; };
+    const int64_t cuts = (int64_t)a.batch * (a.n_segs - 1);
+    a.end = (float *)take(cuts * a.dim * a.N * 4);
+    a.enter = (float *)take(cuts * a.dim * a.N * 4);
+    a.sums = (float *)take(cuts * a.dim * 4);
+    a.flags = (int32_t *)take(cuts * 4);
+    return at;
+}
+
+int ts_read(const ss2d_token_scan_params *p, TsArgs &a) {
+    a = {};
+    if (!p || p->batch < 0 || p->seqlen < 0 || p->dim < 0 || p->dstate < 1 || p->n_groups < 1 || p->n_seqs < 0) return SS2D_EINVAL;
+    if (p->dtype < SS2D_F32 || p->dtype > SS2D_F16 || p->dim % p->n_groups) return SS2D_EINVAL;
+    if (p->cu_seqlens && (p->batch != 1 || p->n_seqs < 1)) return SS2D_EINVAL;
+    if (p->dstate > kTsMaxState || p->seqlen > INT32_MAX - 2 * kTsGrid) return SS2D_ENOTSUP;
+    a.u = p->u; a.delta = p->delta; a.B = p->B; a.C = p->C; a.z = p->z; a.A = p->A; a.D = p->D; a.bias = p->delta_bias; a.initial = p->initial_state;
+    a.cu = p->cu_seqlens; a.out = p->out; a.final = p->final_state; a.kept = p->kept_states;
+    a.u_b = p->u_batch_stride; a.u_t = p->u_token_stride; a.dl_b = p->delta_batch_stride; a.dl_t = p->delta_token_stride; a.z_b = p->z_batch_stride; a.z_t = p->z_token_stride;
+    a.B_b = p->B_batch_stride; a.B_t = p->B_token_stride; a.B_g = p->B_group_stride; a.C_b = p->C_batch_stride; a.C_t = p->C_token_stride; a.C_g = p->C_group_stride;
+    a.batch = p->batch; a.tokens = p->seqlen; a.dim = p->dim; a.N = p->dstate; a.groups = p->n_groups; a.per_group = p->dim / p->n_groups;
+    a.n_seqs = p->cu_seqlens ? p->n_seqs : p->batch; a.softplus = p->delta_softplus != 0;
+    if (a.dim) {
+        if ((int64_t)a.dim * a.N > INT32_MAX - kBlock) return SS2D_ENOTSUP;
+        ts_cut(a);
+        const int64_t wgs = (int64_t)a.batch * a.n_segs * a.groups * a.wgs;
+        if (wgs > kTsLaunch / kBlock || (int64_t)a.batch * a.n_segs > INT32_MAX || a.batch > 65535 * (a.n_segs > 1 ? 1 : 32768)) return SS2D_ENOTSUP;
+    }
+    return SS2D_OK;
+}
+
+// fn(T, sets, m) of the kernel that takes a state of N
+template <typename T, typename F> static int ts_with(int N, F fn) {
+    using std::integral_constant;
+    if (N <= 4) return fn(T{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (N <= 8) return fn(T{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    if (N <= 16) return fn(T{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    if (N <= 32) return fn(T{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    return fn(T{}, integral_constant<int, 4>{}, integral_constant<int, 4>{});
+}
+
+// A state's tensors of sequences without tokens: the initial states, or zeros
+__global__ __launch_bounds__(kBlock) void ts_copy_kernel(const float *from, float *to, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i < n) to[i] = from ? from[i] : 0.0f;
+}
+int ts_copy(const float *from, float *to, int64_t n, hipStream_t st) {
+    if (!to || n == 0) return SS2D_OK;
+    if ((n + kBlock - 1) / kBlock > kTsLaunch / kBlock) return SS2D_ENOTSUP;
+    ts_copy_kernel<<<(uint32_t)((n + kBlock - 1) / kBlock), kBlock, 0, st>>>(from, to, n);
+    return launch_status();
+}
+
+}  // namespace ss2d
+
+using namespace ss2d;
+
+extern "C" int64_t ss2d_token_scan_workspace_bytes(const ss2d_token_scan_params *params) {
+    TsArgs a;
+    const int rc = ts_read(params, a);
+    if (rc != SS2D_OK) return rc;
+    return a.dim && a.batch ? ts_carve(a, nullptr) : 0;
+}
+
+extern "C" int64_t ss2d_token_scan_kept_states(const ss2d_token_scan_params *params) {
+    TsArgs a;
+    const int rc = ts_read(params, a);
+    return rc != SS2D_OK ? rc : (int64_t)a.batch * a.n_grid * a.dim * a.N;
+}
+
+extern "C" int ss2d_token_scan_fwd(const ss2d_token_scan_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
+    TsArgs a;
+    int rc = ts_read(params, a);
+    if (rc != SS2D_OK || a.dim == 0 || a.batch == 0) return rc;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (!a.A) return SS2D_EINVAL;
+    if (a.tokens == 0) return ts_copy(a.initial, a.final, (int64_t)a.n_seqs * a.dim * a.N, st);
+    if (!a.u || !a.delta || !a.B || !a.C || !a.out) return SS2D_EINVAL;
+    const int64_t need = ts_carve(a, (uint8_t *)workspace);
+    if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)) return SS2D_EINVAL;
+    if (workspace_bytes < need) return SS2D_ENOMEM;
+    auto run = [&](auto t, auto sets, auto m) {
+        using T = decltype(t);
+        const uint32_t wgs = (uint32_t)a.batch * a.groups * a.wgs;
+        if (a.n_segs > 1) {
+            ts_kernel<T, decltype(sets)::value, decltype(m)::value, true><<<wgs * (a.n_segs - 1), kBlock, 0, st>>>(a);
+            const uint32_t per_row = (uint32_t)a.dim * a.N;
+            ts_join_kernel<<<dim3((per_row + kBlock - 1) / kBlock, a.batch), kBlock, 0, st>>>(a, per_row);
+        }
+        ts_kernel<T, decltype(sets)::value, decltype(m)::value, false><<<wgs * a.n_segs, kBlock, 0, st>>>(a);
+        return launch_status();
+    };
+    switch (params->dtype) {
+    case SS2D_F32: return ts_with<float>(a.N, run);
+    case SS2D_F16: return ts_with<f16_t>(a.N, run);
+    default: return ts_with<bf16_t>(a.N, run);
+    }
+}
