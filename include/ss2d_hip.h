@@ -830,6 +830,86 @@ typedef struct ss2d_token_scan_step_params {
 
 int ss2d_token_scan_step(const ss2d_token_scan_step_params *params, void *stream);
 
+/*
+ * The short causal convolution that goes before such a scan, each channel for itself, width W = 2, 3 or 4 (SS2D_ENOTSUP otherwise):
+ *   out_t = act(bias + sum_j weight_j x_(t - W + 1 + j)),  act: SiLU where `silu` is not 0;  before a sequence's first token stand the W - 1 rows of its state.
+ * The depthwise convolution + SiLU of a block (classification/models/vmamba.py:654-658) along tokens.
+ *   x (batch, seqlen, dim): dtype, channels dense, other strides in elements; weight (dim, W), bias (dim) or NULL: weight_dtype (SS2D_F32 or dtype), dense.
+ *   cu_seqlens as in ss2d_token_scan_params; rows of no sequence get zeros.
+ *   initial_state (NULL: zeros), final_state (NULL: not wanted) (n_seqs or batch, W - 1, dim) dtype, dense, the oldest row first.  out (batch, seqlen, dim) dtype, dense.
+ */
+typedef struct ss2d_causal_conv_params {
+    int32_t batch, seqlen, dim, width, dtype, weight_dtype, silu, n_seqs;
+    const void *x, *weight, *bias, *initial_state;
+    const int32_t *cu_seqlens;
+    void *out, *final_state;
+    int64_t x_batch_stride, x_token_stride;
+} ss2d_causal_conv_params;
+
+int ss2d_causal_conv_fwd(const ss2d_causal_conv_params *params, void *stream);
+
+/*
+ * Its gradients, from the inputs again (fwd.out and fwd.final_state are not looked at): dout (batch, seqlen, dim) dtype by its strides, dfinal_state as final_state or
+ * NULL -> dx (batch, seqlen, dim) dtype, dense; dweight, dbias (weight_dtype) and dinitial_state (dtype), any of them NULL.  Sums are fp32.  No atomics: the same bits every time.
+ * workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
+ */
+typedef struct ss2d_causal_conv_bwd_params {
+    ss2d_causal_conv_params fwd;
+    const void *dout, *dfinal_state;
+    void *dx, *dweight, *dbias, *dinitial_state;
+    int64_t dout_batch_stride, dout_token_stride;
+} ss2d_causal_conv_bwd_params;
+
+int64_t ss2d_causal_conv_bwd_workspace_bytes(const ss2d_causal_conv_bwd_params *params);
+int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * One token for each of `batch` sequences: out as above, and state (batch, W - 1, dim) dtype moves up by a row in place, x its last; dense but for the
+ * batch's stride, which keeps the states apart.  x (batch, dim) by its stride; out (batch, dim) dense.
+ */
+typedef struct ss2d_causal_conv_step_params {
+    int32_t batch, dim, width, dtype, weight_dtype, silu;
+    const void *x, *weight, *bias;
+    void *state, *out;
+    int64_t x_batch_stride, state_batch_stride;
+} ss2d_causal_conv_step_params;
+
+int ss2d_causal_conv_step(const ss2d_causal_conv_step_params *params, void *stream);
+
+/*
+ * Group norm of channel-last activations with an activation behind it: x (batch, positions, channels) dense, dtype; a group is channels / groups neighbouring
+ * channels; over the positions and channels of one sample's group
+ *   out = act((x - mean) / sqrt(var + eps) * weight + bias),  act: SiLU where `silu` is not 0.  One position: tokens, each normalised by itself.
+ * The LayerNorm of a map's channels (classification/models/vmamba.py:52-57) is the one with one group and one position.
+ *   weight, bias (channels): weight_dtype (SS2D_F32 or dtype), either or both NULL (1, 0); out as x.
+ *   stats (batch, groups, 2) fp32 or NULL: mean and 1 / sqrt(var + eps), which the gradients start from.
+ * Sums are fp32, squares those of centred values.  workspace: ..._workspace_bytes(params) bytes (0 for short ones; or a negative status), 16-byte aligned.
+ */
+typedef struct ss2d_group_norm_params {
+    int64_t batch, positions;
+    int32_t channels, groups, dtype, weight_dtype, silu;
+    float eps;
+    const void *x, *weight, *bias;
+    void *out;
+    float *stats;
+} ss2d_group_norm_params;
+
+int64_t ss2d_group_norm_workspace_bytes(const ss2d_group_norm_params *params);
+int ss2d_group_norm_fwd(const ss2d_group_norm_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its gradients, from x and the statistics (fwd.stats, read only; fwd.out is not looked at): dout dense as x -> dx; dweight, dbias (weight_dtype), either or both
+ * NULL.  No atomics: the same bits every time.  workspace: ..._workspace_bytes(params) bytes, 16-byte aligned.
+ */
+typedef struct ss2d_group_norm_bwd_params {
+    ss2d_group_norm_params fwd;
+    const void *dout;
+    void *dx, *dweight, *dbias;
+} ss2d_group_norm_bwd_params;
+
+int64_t ss2d_group_norm_bwd_workspace_bytes(const ss2d_group_norm_bwd_params *params);
+int ss2d_group_norm_bwd(const ss2d_group_norm_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

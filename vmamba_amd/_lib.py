@@ -31,7 +31,8 @@ EXPORTS = ("ss2d_abi_version", "ss2d_strerror", "ss2d_cross_scan", "ss2d_cross_m
            "ss2d_linear_attention_workspace_bytes", "ss2d_linear_attention_fwd", "ss2d_linear_attention_bwd_workspace_bytes", "ss2d_linear_attention_bwd",
            "ss2d_linear_attention_step", "ss2d_qk_norm_rotate", "ss2d_qk_norm_rotate_bwd_workspace_bytes", "ss2d_qk_norm_rotate_bwd",
            "ss2d_token_scan_workspace_bytes", "ss2d_token_scan_kept_states", "ss2d_token_scan_fwd", "ss2d_token_scan_bwd_workspace_bytes", "ss2d_token_scan_bwd",
-           "ss2d_token_scan_step")
+           "ss2d_token_scan_step", "ss2d_causal_conv_fwd", "ss2d_causal_conv_bwd_workspace_bytes", "ss2d_causal_conv_bwd", "ss2d_causal_conv_step",
+           "ss2d_group_norm_workspace_bytes", "ss2d_group_norm_fwd", "ss2d_group_norm_bwd_workspace_bytes", "ss2d_group_norm_bwd")
 
 
 class ScanParams(ctypes.Structure):
@@ -170,6 +171,45 @@ class TokenScanStepParams(ctypes.Structure):
         + [(n, ctypes.c_int64) for n in ("u_batch_stride", "delta_batch_stride", "z_batch_stride", "B_batch_stride", "B_group_stride", "C_batch_stride",
                                          "C_group_stride", "state_batch_stride")]
     )
+
+
+class CausalConvParams(ctypes.Structure):
+    """struct ss2d_causal_conv_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "seqlen", "dim", "width", "dtype", "weight_dtype", "silu", "n_seqs")]
+        + [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "initial_state", "cu_seqlens", "out", "final_state")]
+        + [(f"x_{axis}_stride", ctypes.c_int64) for axis in ("batch", "token")]
+    )
+
+
+class CausalConvBwdParams(ctypes.Structure):
+    """struct ss2d_causal_conv_bwd_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [("fwd", CausalConvParams)] + [(n, ctypes.c_void_p) for n in ("dout", "dfinal_state", "dx", "dweight", "dbias", "dinitial_state")]
+        + [(f"dout_{axis}_stride", ctypes.c_int64) for axis in ("batch", "token")]
+    )
+
+
+class CausalConvStepParams(ctypes.Structure):
+    """struct ss2d_causal_conv_step_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("batch", "dim", "width", "dtype", "weight_dtype", "silu")]
+        + [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "state", "out")]
+        + [(n, ctypes.c_int64) for n in ("x_batch_stride", "state_batch_stride")]
+    )
+
+
+class GroupNormParams(ctypes.Structure):
+    """struct ss2d_group_norm_params (include/ss2d_hip.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int64) for n in ("batch", "positions")] + [(n, ctypes.c_int32) for n in ("channels", "groups", "dtype", "weight_dtype", "silu")]
+        + [("eps", ctypes.c_float)] + [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "out", "stats")]
+    )
+
+
+class GroupNormBwdParams(ctypes.Structure):
+    """struct ss2d_group_norm_bwd_params (include/ss2d_hip.h)."""
+    _fields_ = [("fwd", GroupNormParams)] + [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweight", "dbias")]
 
 
 class Ss2dError(RuntimeError):
@@ -343,12 +383,15 @@ def lib():
         L.ss2d_qk_norm_rotate_bwd_workspace_bytes.restype = ctypes.c_int64
         L.ss2d_qk_norm_rotate_bwd_workspace_bytes.argtypes = [ctypes.c_int]
         for name, params in (("ss2d_token_scan_workspace_bytes", TokenScanParams), ("ss2d_token_scan_kept_states", TokenScanParams),
-                             ("ss2d_token_scan_bwd_workspace_bytes", TokenScanBwdParams)):
+                             ("ss2d_token_scan_bwd_workspace_bytes", TokenScanBwdParams), ("ss2d_causal_conv_bwd_workspace_bytes", CausalConvBwdParams),
+                             ("ss2d_group_norm_workspace_bytes", GroupNormParams), ("ss2d_group_norm_bwd_workspace_bytes", GroupNormBwdParams)):
             getattr(L, name).restype, getattr(L, name).argtypes = ctypes.c_int64, [ctypes.POINTER(params)]
-        for name, params in (("ss2d_token_scan_fwd", TokenScanParams), ("ss2d_token_scan_bwd", TokenScanBwdParams)):
+        for name, params in (("ss2d_token_scan_fwd", TokenScanParams), ("ss2d_token_scan_bwd", TokenScanBwdParams), ("ss2d_causal_conv_bwd", CausalConvBwdParams),
+                             ("ss2d_group_norm_fwd", GroupNormParams), ("ss2d_group_norm_bwd", GroupNormBwdParams)):
             getattr(L, name).restype = ctypes.c_int
             getattr(L, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
-        L.ss2d_token_scan_step.restype, L.ss2d_token_scan_step.argtypes = ctypes.c_int, [ctypes.POINTER(TokenScanStepParams), ctypes.c_void_p]
+        for name, params in (("ss2d_token_scan_step", TokenScanStepParams), ("ss2d_causal_conv_fwd", CausalConvParams), ("ss2d_causal_conv_step", CausalConvStepParams)):
+            getattr(L, name).restype, getattr(L, name).argtypes = ctypes.c_int, [ctypes.POINTER(params), ctypes.c_void_p]
         if L.ss2d_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.ss2d_abi_version()} != expected {ABI_VERSION}; rebuild")
         _lib = L
