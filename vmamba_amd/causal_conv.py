@@ -9,7 +9,7 @@ the last width - 1 inputs, which ``causal_conv_step_fn`` carries on token by tok
 import torch
 
 from . import _lib
-from .norm import untraced
+from .norm import TENSOR_KINDS, native_stands, untraced
 from .token_scan import MAX_SIZE, _check, _ptr, check_places, check_plain, check_unseen, dense_last, workspace_of
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
@@ -114,6 +114,10 @@ def causal_conv_fn(x, weight, bias=None, activation=None, initial_state=None, ou
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a GPU tensor: vmamba_amd has no CPU path")
+    if native_stands(x) and not torch.jit.is_tracing():              # (its memory is made where a tracer does not see it)
+        native = _lib.host().causal_conv(TENSOR_KINDS, x, weight, bias, activation, initial_state, bool(output_final_state), cu_seqlens)
+        if native is not None:
+            return native
     out, final = CausalConvHip.apply(x, weight, bias, initial_state, activation, cu_seqlens, bool(output_final_state))
     return (out, final) if output_final_state else out
 
@@ -126,6 +130,10 @@ def causal_conv_step_fn(x, state, weight, bias=None, activation=None):
     (torch.jit.trace), since a trace would not hold what becomes of the state."""
     _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a GPU tensor: vmamba_amd has no CPU path")
     _check(not torch.jit.is_tracing(), "causal_conv_step_fn changes its state behind a tracer's back: it cannot be traced")
+    if native_stands(x):
+        native = _lib.host().causal_conv_step(TENSOR_KINDS, x, state, weight, bias, activation)
+        if native is not None:
+            return _lib.result(native, "ss2d_causal_conv_step")
     _check_sides(x, weight, bias, activation, "causal_conv_step_fn", 2)
     shape = (x.shape[0], weight.shape[1] - 1, x.shape[1])
     _check(state is not None, "state must be a tensor")

@@ -57,7 +57,7 @@ template <typename P> void strides3(const at::Tensor &t, P &batch, P &token, P &
 // changed since: a hook brought them back as something else)
 inline at::Tensor gradient(const at::Tensor &g, const at::Tensor &x, at::IntArrayRef shape, at::ScalarType type, const char *name) {
     TORCH_CHECK(on_gpu(g, x) && has_shape(g, shape) && g.scalar_type() == type, name,
-                " must be a plain tensor with memory of its own, on the device of q and of the shape and type of what it is the gradient of");
+                " must be a plain tensor with memory of its own, on the device of the inputs and of the shape and type of what it is the gradient of");
     return dense_last(g) ? g : g.contiguous();
 }
 

@@ -279,6 +279,7 @@ static py::object cross_merge(const py::tuple &kinds, const py::object &y_in) {
 }
 
 #include "host_attention.h"
+#include "host_tokens.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("forward_core", &forward_core);
@@ -291,4 +292,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_attention", &attention::linear_attention);
     m.def("linear_attention_step", &attention::linear_attention_step);
     m.def("qk_norm_rotate", &attention::qk_norm_rotate);
+    m.def("token_scan", &tokens::token_scan);
+    m.def("token_scan_step", &tokens::token_scan_step);
+    m.def("causal_conv", &tokens::causal_conv);
+    m.def("causal_conv_step", &tokens::causal_conv_step);
+    m.def("group_norm", &tokens::group_norm);
 }

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .causal_conv import ACTIVATIONS
-from .norm import untraced
+from .norm import TENSOR_KINDS, native_stands, untraced
 from .token_scan import MAX_SIZE, _check, _ptr, check_plain, workspace_of
 
 _DTYPE_CODE = {torch.float32: _lib.SS2D_F32, torch.bfloat16: _lib.SS2D_BF16, torch.float16: _lib.SS2D_F16}
@@ -92,4 +92,8 @@ def group_norm_fn(x, num_groups, weight=None, bias=None, eps=1e-5, activation=No
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a GPU tensor: vmamba_amd has no CPU path")
+    if type(num_groups) is int and native_stands(x) and not torch.jit.is_tracing():             # (its memory is made where a tracer does not see it)
+        native = _lib.host().group_norm(TENSOR_KINDS, x, num_groups, weight, bias, eps, activation)
+        if native is not None:
+            return native
     return GroupNormHip.apply(x, weight, bias, num_groups, float(eps), activation)

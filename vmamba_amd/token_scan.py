@@ -204,6 +204,10 @@ def selective_scan_tokens_fn(u, delta, A, B, C, D=None, z=None, delta_bias=None,
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(u, torch.Tensor) and u.is_cuda, "u must be a GPU tensor: vmamba_amd has no CPU path")
+    if native_stands(u) and not torch.jit.is_tracing():              # (its memory is made where a tracer does not see it)
+        native = _lib.host().token_scan(TENSOR_KINDS, u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus), initial_state, bool(output_final_state), cu_seqlens)
+        if native is not None:
+            return native
     out, final = SelectiveScanTokensHip.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus), cu_seqlens, bool(output_final_state))
     return (out, final) if output_final_state else out
 
@@ -216,6 +220,10 @@ def selective_scan_step_fn(u, delta, A, B, C, state, D=None, z=None, delta_bias=
     are recorded, and to be traced (torch.jit.trace), since a trace would not hold what becomes of the state."""
     _check(isinstance(u, torch.Tensor) and u.is_cuda, "u must be a GPU tensor: vmamba_amd has no CPU path")
     _check(not torch.jit.is_tracing(), "selective_scan_step_fn changes its state behind a tracer's back: it cannot be traced")
+    if native_stands(u):
+        native = _lib.host().token_scan_step(TENSOR_KINDS, u, delta, A, B, C, state, D, z, delta_bias, bool(delta_softplus))
+        if native is not None:
+            return _lib.result(native, "ss2d_token_scan_step")
     dstate = _check_sides(u, delta, A, B, C, D, z, delta_bias, "selective_scan_step_fn", 2)
     shape = (*u.shape, dstate)
     _check(state is not None, "state must be a tensor")
