@@ -19,7 +19,7 @@ HIP_SOURCES = ["cross_scan.hip", "cross_merge.hip", "selective_scan.hip", "scan_
                "ss2d_core.hip", "ss2d_core_small.hip", "ss2d_core_tiled.hip", "core_pads.hip", "core_few.hip", "forward_core.hip", "vss_block.hip", "x_proj.hip", "dt_proj.hip", "proj_f32.hip", "cross_flex.hip",
                "selective_scan_bwd.hip", "scan_bwd_chan.hip", "scan_bwd_io.hip", "mlp_fused.hip", "linear_cl.hip", "linear_rows.hip", "linear_tiles.hip", "linear_dw.hip", "product_f32.hip", "stem_conv.hip", "stem_conv2.hip", "mean_pool.hip",
                "linear_attention.hip", "linear_attention_bwd.hip", "linear_attention_step.hip", "qk_norm_rotate.hip",
-               "token_scan.hip", "token_scan_bwd.hip", "token_scan_step.hip", "causal_conv.hip", "group_norm.hip"]
+               "token_scan.hip", "token_scan_bwd.hip", "token_scan_bwd_f32.hip", "token_scan_bwd_f16.hip", "token_scan_bwd_bf16.hip", "token_scan_step.hip", "causal_conv.hip", "group_norm.hip"]
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 

@@ -15,7 +15,7 @@
 namespace ss2d {
 
 constexpr int kTsTile = 16;          // tokens of a tile
-constexpr int kTsGrid = 64;          // tokens between the states that the forward keeps for the gradients, and what segments are multiples of
+constexpr int kTsGrid = 64;          // what segments are multiples of
 constexpr int kTsMaxState = 64;
 constexpr int64_t kTsLaunch = 0xffffffff;                            // threads of a launch
 
@@ -24,18 +24,29 @@ struct TsArgs {
     const float *A, *D, *bias, *initial;
     const int32_t *cu;
     void *out;
-    float *final, *kept;             // kept: [batch][token / kTsGrid][channel][state], the state before every kTsGrid-th token
+    float *final, *kept;             // kept: [batch][token / keep][channel][state], the state before every keep-th token
     int64_t u_b, u_t, dl_b, dl_t, z_b, z_t, B_b, B_t, B_g, C_b, C_t, C_g;
     int32_t batch, tokens, dim, N, groups, per_group, n_seqs, softplus;
+    int32_t near;                    // offsets inside a tile fit 32 bits
     int32_t wgs;                     // workgroups (of four wavefronts' channels) to a group
-    int32_t seg_len, n_segs, n_grid; // n_grid: kept states of a row
+    int32_t seg_len, n_segs, keep, n_kept;                           // n_kept: kept states of a row
     // workspace: of every segment but the last [batch][segment][channel](..)
     float *end, *sums;               // state behind it (N), from zeros or its last sequence's start; its steps' sum
     float *enter;                    // state before segment + 1 (N)
     int32_t *flags;                  // [batch][segment]: TsCarry
 };
 
+// Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th
+// token takes a quarter of the memory, and the gradients a second walk over every piece: 310 us in place of 262 of their kernel, 4 x 2048 tokens of 2048 channels.)
+inline int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
+// Whole wavefronts of channels, states that fill their lanes, offsets inside a tile that fit 32 bits: the kernels without masks
+inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / ts_sets(a.N)) == 0 && (a.N == 4 || a.N == 8 || a.N == 16 || a.N == 32 || a.N == 64); }
+inline int ts_keep(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+
 enum TsCarry { kTsNothing, kTsStarts, kTsThrough };                  // what a segment hands on: nothing, its last sequence began in it, it lies inside one
+
+// Wavefronts of a workgroup of the gradients' kernel: their states in LDS are 4 kM^2 KB each
+template <int kM> constexpr int kTsBwdWaves = kM == 4 ? 2 : 4;
 
 // The gradients' further arguments
 struct TsBwdArgs {
@@ -91,6 +102,10 @@ template <typename T> __device__ __forceinline__ Raw4<T> ts_load4(const T *p, in
         else r.w[i / 2] |= (uint32_t)p[i].bits << (i & 1) * 16;
     }
     return r;
+}
+// ... at a uniform place and 32 bits' worth of bytes on
+template <typename T> __device__ __forceinline__ Raw4<T> ts_load4_at(const T *base, uint32_t bytes) {
+    return ts_load4<T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + bytes), 4, true);
 }
 template <typename T> __device__ __forceinline__ void ts_widen(const Raw4<T> &r, float (&v)[4]) {
 #pragma unroll

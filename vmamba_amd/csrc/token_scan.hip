@@ -8,7 +8,8 @@
 
 namespace ss2d {
 
-template <typename T, int kSets, int kM, bool kLocal>
+// kLocal: what a segment leaves, instead of its outputs.  kQuick: see ts_quick.
+template <typename T, int kSets, int kM, bool kLocal, bool kQuick>
 __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArgs p) {
     using L = TsLane<kSets, kM>;
     __shared__ __align__(16) float s_all[kWavesPerWg][kTsTile * (L::kPairPitch + 2 * L::kStates)];
@@ -22,11 +23,12 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
     const int first = (wg * kWavesPerWg + wave) * L::kCh, n_chan = min(L::kCh, p.per_group - first);
     if (n_chan <= 0) return;
     const int c0 = g * p.per_group + first, s0 = seg * p.seg_len, s1 = min(s0 + p.seg_len, p.tokens);
-    const bool whole = n_chan == L::kCh;
-    const int mine = min(max(n_chan - l.at, 0), 4);                  // channels of a lane that stages
+    const bool whole = kQuick || n_chan == L::kCh;
+    const int mine = kQuick ? 4 : min(max(n_chan - l.at, 0), 4);                  // channels of a lane that stages
     const int at = mine > 0 ? l.at : 0;
-    const bool there = l.chan < n_chan;
-    const int d = c0 + min(l.chan, n_chan - 1);
+    const bool there = kQuick || l.chan < n_chan;
+    const int d = c0 + (kQuick ? l.chan : min(l.chan, n_chan - 1));
+    const int N = kQuick ? L::kStates : p.N;
 
     int t = s0;
     TsSpan sp = {b, 0, p.tokens};
@@ -37,28 +39,27 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
         if (wg == 0 && g == 0 && threadIdx.x == 0) p.flags[(int64_t)b * segs + seg] = carry;
         if (carry == kTsNothing) return;
         t = max(s0, sp.lo);
-        state_at = (((int64_t)b * segs + seg) * p.dim + d) * p.N;
+        state_at = (((int64_t)b * segs + seg) * p.dim + d) * N;
     } else {
         sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, t);
     }
 
-    const T *u = (const T *)p.u + (int64_t)b * p.u_b + c0 + at, *dl = (const T *)p.delta + (int64_t)b * p.dl_b + c0 + at;
-    const T *z = p.z ? (const T *)p.z + (int64_t)b * p.z_b + c0 + at : nullptr;
     const T *Bp = (const T *)p.B + (int64_t)b * p.B_b + (int64_t)g * p.B_g, *Cp = (const T *)p.C + (int64_t)b * p.C_b + (int64_t)g * p.C_g;
     T *out = (T *)p.out + (int64_t)b * p.tokens * p.dim + c0 + at;
-    const int bc_n = min(max(p.N - 4 * l.piece, 0), 4), bc_at = bc_n > 0 ? 4 * l.piece : 0;
-    const bool bc_whole = p.N == L::kStates;
-    float bias[4], skip[4];
+    const int bc_n = kQuick ? 4 : min(max(N - 4 * l.piece, 0), 4), bc_at = bc_n > 0 ? 4 * l.piece : 0;
+    const bool bc_whole = kQuick || N == L::kStates;
+    float bias[4], bias2[4], skip[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         bias[i] = p.bias && i < mine ? p.bias[c0 + at + i] : 0.0f;
+        bias2[i] = bias[i] * kLog2e;
         skip[i] = p.D && i < mine ? p.D[c0 + at + i] : 0.0f;
     }
     floatx4_t A2[kM], h[kM];
-    ts_read_state<kSets, kM>(p.A + (int64_t)d * p.N, p.N, l, true, A2);
+    ts_read_state<kSets, kM>(p.A + (int64_t)d * N, N, l, true, A2);
 #pragma unroll
     for (int m = 0; m < kM; ++m) A2[m] *= kLog2e;
-    auto start = [&](const TsSpan &s) { ts_read_state<kSets, kM>(p.initial ? p.initial + ((int64_t)s.seq * p.dim + d) * p.N : nullptr, p.N, l, there, h); };
+    auto start = [&](const TsSpan &s) { ts_read_state<kSets, kM>(p.initial ? p.initial + ((int64_t)s.seq * p.dim + d) * N : nullptr, N, l, there, h); };
     auto nothing = [&](int from, int to) {                           // tokens of no sequence
         if constexpr (!kLocal) {
             const float zeros[4] = {0, 0, 0, 0};
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                 const int lo = min(max(p.cu[i], 0), p.tokens), hi = min(max(p.cu[i + 1], 0), p.tokens);
                 if (hi > lo) continue;
                 start({i, lo, lo});
-                ts_write_state<kSets, kM>(p.final + ((int64_t)i * p.dim + d) * p.N, p.N, l, there, h);
+                ts_write_state<kSets, kM>(p.final + ((int64_t)i * p.dim + d) * N, N, l, there, h);
             }
         while (sp.seq < 0) {
             nothing(t, min(sp.hi, s1));
@@ -85,17 +86,37 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
 #pragma unroll
         for (int m = 0; m < kM; ++m) h[m] = floatx4_t{0, 0, 0, 0};
     } else {
-        ts_read_state<kSets, kM>(p.enter + (((int64_t)b * (p.n_segs - 1) + seg - 1) * p.dim + d) * p.N, p.N, l, there, h);
+        ts_read_state<kSets, kM>(p.enter + (((int64_t)b * (p.n_segs - 1) + seg - 1) * p.dim + d) * N, N, l, there, h);
     }
 
     Raw4<T> ru[L::kRounds], rd[L::kRounds], rz[L::kRounds], rB[L::kBcRounds], rC[L::kBcRounds];
-    auto request = [&](int from, int to) {                           // tokens from .. to - 1 of one tile
+    // tokens from .. to - 1 of one tile
+    const T *u0 = (const T *)p.u + (int64_t)b * p.u_b + c0, *dl0 = (const T *)p.delta + (int64_t)b * p.dl_b + c0, *z0 = p.z ? (const T *)p.z + (int64_t)b * p.z_b + c0 : nullptr;
+    T *out0 = (T *)p.out + (int64_t)b * p.tokens * p.dim + c0;
+    auto request = [&](int from, int to) {
+        if constexpr (kQuick) {                                      // (a uniform base, and 32 bits from there on)
+            auto row_of = [&](int k) { return (uint32_t)min(k, to - 1 - from); };
+#pragma unroll
+            for (int r = 0; r < L::kRounds; ++r) {
+                const uint32_t k = row_of(r * L::kRows + l.row);
+                ru[r] = ts_load4_at<T>(u0 + from * p.u_t, (k * (uint32_t)p.u_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                rd[r] = ts_load4_at<T>(dl0 + from * p.dl_t, (k * (uint32_t)p.dl_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                if constexpr (!kLocal) if (z0) rz[r] = ts_load4_at<T>(z0 + from * p.z_t, (k * (uint32_t)p.z_t + (uint32_t)at) * (uint32_t)sizeof(T));
+            }
+#pragma unroll
+            for (int r = 0; r < L::kBcRounds; ++r) {
+                const uint32_t k = row_of(r * L::kBcRows + l.bc_row);
+                rB[r] = ts_load4_at<T>(Bp + from * p.B_t, (k * (uint32_t)p.B_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
+                if constexpr (!kLocal) rC[r] = ts_load4_at<T>(Cp + from * p.C_t, (k * (uint32_t)p.C_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < L::kRounds; ++r) {
             const int64_t k = min(from + r * L::kRows + l.row, to - 1);
-            ru[r] = ts_load4<T>(u + k * p.u_t, mine, whole);
-            rd[r] = ts_load4<T>(dl + k * p.dl_t, mine, whole);
-            if constexpr (!kLocal) if (z) rz[r] = ts_load4<T>(z + k * p.z_t, mine, whole);
+            ru[r] = ts_load4<T>(u0 + at + k * p.u_t, mine, whole);
+            rd[r] = ts_load4<T>(dl0 + at + k * p.dl_t, mine, whole);
+            if constexpr (!kLocal) if (z0) rz[r] = ts_load4<T>(z0 + at + k * p.z_t, mine, whole);
         }
 #pragma unroll
         for (int r = 0; r < L::kBcRounds; ++r) {
@@ -112,52 +133,58 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
         const int n = end - t;
         // ---- stage -----------------------------------------------------------------------------------------------------------
         float extra[L::kRounds][4], gate[L::kRounds][4];
+        auto stage = [&](auto all) {                                 // all: 16 tokens, every lane's channels and states there
+            constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-        for (int r = 0; r < L::kRounds; ++r) {
-            const int k = r * L::kRows + l.row;
-            float uv[4], dv[4], step[4];
-            ts_widen<T>(ru[r], uv);
-            ts_widen<T>(rd[r], dv);
+            for (int r = 0; r < L::kRounds; ++r) {
+                const int k = r * L::kRows + l.row;
+                float uv[4], dv[4], step[4];
+                ts_widen<T>(ru[r], uv);
+                ts_widen<T>(rd[r], dv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                step[i] = p.softplus ? softplus_log2(fmaf(dv[i], kLog2e, bias[i] * kLog2e)) : dv[i] + bias[i];
-                const bool in = k < n && (whole || i < mine);
-                step[i] = in ? step[i] : 0.0f;
-                uv[i] = in ? uv[i] : 0.0f;
-                extra[r][i] = skip[i] * uv[i];
-                if constexpr (kLocal) sum[i] += step[i];
-            }
-            float *to = s_step + k * L::kPairPitch + 2 * l.at;
-            *reinterpret_cast<float4 *>(to) = make_float4(step[0], step[0] * uv[0], step[1], step[1] * uv[1]);
-            *reinterpret_cast<float4 *>(to + 4) = make_float4(step[2], step[2] * uv[2], step[3], step[3] * uv[3]);
-            if constexpr (!kLocal) {
-                if (z) {
-                    float zv[4];
-                    ts_widen<T>(rz[r], zv);
+                for (int i = 0; i < 4; ++i) {
+                    step[i] = p.softplus ? softplus_log2(fmaf(dv[i], kLog2e, bias2[i])) : dv[i] + bias[i];
+                    if constexpr (!kAll) {
+                        const bool in = k < n && (whole || i < mine);
+                        step[i] = in ? step[i] : 0.0f;
+                        uv[i] = in ? uv[i] : 0.0f;
+                    }
+                    extra[r][i] = skip[i] * uv[i];
+                    if constexpr (kLocal) sum[i] += step[i];
+                }
+                float *to = s_step + k * L::kPairPitch + 2 * l.at;
+                *reinterpret_cast<float4 *>(to) = make_float4(step[0], step[0] * uv[0], step[1], step[1] * uv[1]);
+                *reinterpret_cast<float4 *>(to + 4) = make_float4(step[2], step[2] * uv[2], step[3], step[3] * uv[3]);
+                if constexpr (!kLocal) {
+                    if (z0) {
+                        float zv[4];
+                        ts_widen<T>(rz[r], zv);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) gate[r][i] = zv[i] * ts_sigmoid(zv[i]);
-                } else {
+                        for (int i = 0; i < 4; ++i) gate[r][i] = zv[i] * ts_sigmoid(zv[i]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) gate[r][i] = 1.0f;
+                        for (int i = 0; i < 4; ++i) gate[r][i] = 1.0f;
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int r = 0; r < L::kBcRounds; ++r) {
-            const int k = r * L::kBcRows + l.bc_row;
-            if (L::kBcRows > kTsTile && k >= kTsTile) continue;
-            float v[4];
-            ts_widen<T>(rB[r], v);
+            for (int r = 0; r < L::kBcRounds; ++r) {
+                const int k = r * L::kBcRows + l.bc_row;
+                if (L::kBcRows > kTsTile && k >= kTsTile) continue;
+                auto put = [&](float *to, const Raw4<T> &raw) {
+                    float v[4];
+                    ts_widen<T>(raw, v);
+                    if constexpr (!kAll)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = k < n ? v[i] : 0.0f;
-            *reinterpret_cast<float4 *>(s_B + k * L::kStates + 4 * l.piece) = bc_n > 0 ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(0, 0, 0, 0);
-            if constexpr (!kLocal) {
-                ts_widen<T>(rC[r], v);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = k < n ? v[i] : 0.0f;
-                *reinterpret_cast<float4 *>(s_C + k * L::kStates + 4 * l.piece) = bc_n > 0 ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(0, 0, 0, 0);
+                        for (int i = 0; i < 4; ++i) v[i] = k < n && bc_n > 0 ? v[i] : 0.0f;
+                    *reinterpret_cast<float4 *>(to + k * L::kStates + 4 * l.piece) = make_float4(v[0], v[1], v[2], v[3]);
+                };
+                put(s_B, rB[r]);
+                if constexpr (!kLocal) put(s_C, rC[r]);
             }
-        }
+        };
+        if (kQuick && n == kTsTile) stage(std::true_type{});
+        else stage(std::false_type{});
         // ---- the next tile, and what it starts with -----------------------------------------------------------------------------
         const int next = end;
         const bool ends = next == sp.hi;                             // (of the sequence)
@@ -173,8 +200,8 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
         wave_lds_sync();
         // ---- compute ---------------------------------------------------------------------------------------------------------
         if constexpr (!kLocal) {
-            if (p.kept && t % kTsGrid == 0 && t > 0)
-                ts_write_state<kSets, kM>(p.kept + (((int64_t)b * p.n_grid + t / kTsGrid) * p.dim + d) * p.N, p.N, l, there, h);
+            if (p.kept && (t & (p.keep - 1)) == 0 && t > 0)
+                ts_write_state<kSets, kM>(p.kept + (((int64_t)b * p.n_kept + t / p.keep) * p.dim + d) * N, N, l, there, h);
         }
         float y[kTsTile];
 #pragma unroll
@@ -206,10 +233,12 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                 const float4 part = *reinterpret_cast<const float4 *>(s_y + k * L::kPitch + l.at);
                 const float o[4] = {(part.x + extra[r][0]) * gate[r][0], (part.y + extra[r][1]) * gate[r][1], (part.z + extra[r][2]) * gate[r][2],
                                     (part.w + extra[r][3]) * gate[r][3]};
-                if (k < n) ts_store4<T>(out + (int64_t)(t + k) * p.dim, mine, whole, o);
+                if (k >= n) continue;
+                if constexpr (kQuick) ts_store4<T>(reinterpret_cast<T *>(reinterpret_cast<char *>(out0 + (int64_t)t * p.dim) + ((uint32_t)k * (uint32_t)p.dim + (uint32_t)at) * (uint32_t)sizeof(T)), 4, true, o);
+                else ts_store4<T>(out + (int64_t)(t + k) * p.dim, mine, whole, o);
             }
             wave_lds_sync();
-            if (ends && p.final) ts_write_state<kSets, kM>(p.final + ((int64_t)was.seq * p.dim + d) * p.N, p.N, l, there, h);
+            if (ends && p.final) ts_write_state<kSets, kM>(p.final + ((int64_t)was.seq * p.dim + d) * N, N, l, there, h);
         }
         if (next_end == next) {
             nothing(next, zeros_to);
@@ -220,7 +249,7 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
         end = next_end;
     }
     if constexpr (kLocal) {
-        ts_write_state<kSets, kM>(p.end + state_at, p.N, l, there, h);
+        ts_write_state<kSets, kM>(p.end + state_at, N, l, there, h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -268,14 +297,12 @@ __global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
-static int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
-
 // Segments of the token axis.  A cut sequence is walked twice for what goes into the later segments.
 static void ts_cut(TsArgs &a) {
     const int ch = kWave / ts_sets(a.N);
     a.wgs = (int)(((int64_t)a.per_group + ch * kWavesPerWg - 1) / (ch * kWavesPerWg));
     const int64_t waves = (int64_t)a.batch * a.groups * ((a.per_group + ch - 1) / ch);
-    constexpr int64_t kEnough = 768, kTarget = 2048;
+    constexpr int64_t kEnough = 1536, kTarget = 4096;
     int64_t n = waves >= kEnough ? 1 : (kTarget + waves - 1) / waves;
     const int64_t most = (a.tokens + 2 * kTsGrid - 1) / (2 * kTsGrid);
     n = n < most ? n : most;
@@ -284,7 +311,6 @@ static void ts_cut(TsArgs &a) {
     a.seg_len = (int)(len < kTsGrid ? kTsGrid : len);
     a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
     if (a.n_segs < 1) a.n_segs = 1;
-    a.n_grid = (int)((a.tokens + (int64_t)kTsGrid - 1) / kTsGrid);
 }
 
 static int64_t ts_carve(TsArgs &a, uint8_t *base) {
@@ -310,6 +336,10 @@ int ts_read(const ss2d_token_scan_params *p, TsArgs &a) {
     a.B_b = p->B_batch_stride; a.B_t = p->B_token_stride; a.B_g = p->B_group_stride; a.C_b = p->C_batch_stride; a.C_t = p->C_token_stride; a.C_g = p->C_group_stride;
     a.batch = p->batch; a.tokens = p->seqlen; a.dim = p->dim; a.N = p->dstate; a.groups = p->n_groups; a.per_group = p->dim / p->n_groups;
     a.n_seqs = p->cu_seqlens ? p->n_seqs : p->batch; a.softplus = p->delta_softplus != 0;
+    a.near = a.dim < 1 << 24;
+    for (const int64_t stride : {a.u_t, a.dl_t, a.z_t, a.B_t, a.C_t}) a.near = a.near && stride >= 0 && stride < 1 << 24;
+    a.keep = ts_keep(a.N);
+    a.n_kept = (int)((a.tokens + (int64_t)a.keep - 1) / a.keep);
     if (a.dim) {
         if ((int64_t)a.dim * a.N > INT32_MAX - kBlock) return SS2D_ENOTSUP;
         ts_cut(a);
@@ -355,7 +385,7 @@ extern "C" int64_t ss2d_token_scan_workspace_bytes(const ss2d_token_scan_params 
 extern "C" int64_t ss2d_token_scan_kept_states(const ss2d_token_scan_params *params) {
     TsArgs a;
     const int rc = ts_read(params, a);
-    return rc != SS2D_OK ? rc : (int64_t)a.batch * a.n_grid * a.dim * a.N;
+    return rc != SS2D_OK ? rc : (int64_t)a.batch * a.n_kept * a.dim * a.N;
 }
 
 extern "C" int ss2d_token_scan_fwd(const ss2d_token_scan_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -369,17 +399,19 @@ extern "C" int ss2d_token_scan_fwd(const ss2d_token_scan_params *params, void *w
     const int64_t need = ts_carve(a, (uint8_t *)workspace);
     if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)) return SS2D_EINVAL;
     if (workspace_bytes < need) return SS2D_ENOMEM;
-    auto run = [&](auto t, auto sets, auto m) {
+    auto run_as = [&](auto t, auto sets, auto m, auto quick) {
         using T = decltype(t);
+        constexpr bool kQuick = decltype(quick)::value;
         const uint32_t wgs = (uint32_t)a.batch * a.groups * a.wgs;
         if (a.n_segs > 1) {
-            ts_kernel<T, decltype(sets)::value, decltype(m)::value, true><<<wgs * (a.n_segs - 1), kBlock, 0, st>>>(a);
+            ts_kernel<T, decltype(sets)::value, decltype(m)::value, true, kQuick><<<wgs * (a.n_segs - 1), kBlock, 0, st>>>(a);
             const uint32_t per_row = (uint32_t)a.dim * a.N;
             ts_join_kernel<<<dim3((per_row + kBlock - 1) / kBlock, a.batch), kBlock, 0, st>>>(a, per_row);
         }
-        ts_kernel<T, decltype(sets)::value, decltype(m)::value, false><<<wgs * a.n_segs, kBlock, 0, st>>>(a);
+        ts_kernel<T, decltype(sets)::value, decltype(m)::value, false, kQuick><<<wgs * a.n_segs, kBlock, 0, st>>>(a);
         return launch_status();
     };
+    auto run = [&](auto t, auto sets, auto m) { return ts_quick(a) ? run_as(t, sets, m, std::true_type{}) : run_as(t, sets, m, std::false_type{}); };
     switch (params->dtype) {
     case SS2D_F32: return ts_with<float>(a.N, run);
     case SS2D_F16: return ts_with<f16_t>(a.N, run);

@@ -1,0 +1,6 @@
+// The gradients' kernels of single precision (token_scan_bwd.h), in a source of their own: they take a minute to compile.
+#include "token_scan_bwd.h"
+
+namespace ss2d {
+template int ts_bwd_run<float>(const ss2d_token_scan_bwd_params *p, const TsBwdArgs &q, hipStream_t st);
+}  // namespace ss2d
