@@ -2,7 +2,7 @@
 //     y_t = act(bias + sum_j w_j x_(t - W + 1 + j)),   act = SiLU or none; what is before a sequence's first token is its state, the last W - 1 inputs.
 // With g_t = dout_t act'(..):   dx_t = sum_j w_j g_(t + W - 1 - j),   dw_j = sum over t of g_t x_(t - W + 1 + j),   dbias = sum g.
 //
-// Memory bounds it.  A thread takes the channels of one 16-byte piece (gradients: 8 or 16) and walks a strip of tokens with the window in registers; rows are
+// Memory bounds it.  A thread takes the channels of one 16-byte piece and walks a strip of tokens with the window in registers; rows are
 // loaded a chunk at a time, all on their way at once.  Threads side by side have neighbouring pieces, strips below each other.  The last
 // piece of a row ends with it, so that it may repeat channels of the one before: both write the same values.
 #include "row_piece.h"
@@ -16,6 +16,7 @@ struct CvArgs {
     void *out, *final;
     int64_t x_b, x_t;
     int32_t batch, tokens, dim, n_seqs, silu, weight_f32;
+    int32_t near;                    // every tensor's bytes are counted by 32 bits: a row is a uniform place and a lane's offset
     int32_t pieces, cols, piece_blocks, strip, strips;               // cols: pieces side by side in a workgroup; strips of a row
     // gradients
     const void *dout, *dfinal;
@@ -86,7 +87,24 @@ template <typename T, int kV> __device__ __forceinline__ void cv_copy_row(const 
 
 constexpr int kCvRows = 8;           // rows of a chunk
 
-template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock) void cv_kernel(const CvArgs p) {
+// Rows of a tensor from a lane's first one on.  at(): a row that is as far on in every lane (kNear: a uniform address, and the lane's offset, which costs no vector
+// instruction); any(): one that is not.
+template <typename T, bool kNear> struct CvRow {
+    const T *base;
+    int64_t stride;
+    uint32_t off;
+    __device__ __forceinline__ CvRow(const void *p, int64_t stride_, int64_t first) : base((const T *)p), stride(stride_), off(0) {
+        if constexpr (kNear) off = (uint32_t)first * (uint32_t)sizeof(T);
+        else base += first;
+    }
+    __device__ __forceinline__ const T *at(int k) const { return reinterpret_cast<const T *>(reinterpret_cast<const char *>(base + k * stride) + off); }
+    __device__ __forceinline__ const T *any(int k) const {
+        if constexpr (kNear) return reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + (off + (uint32_t)k * (uint32_t)(stride * (int64_t)sizeof(T))));
+        return base + k * stride;
+    }
+};
+
+template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(kBlock) void cv_kernel(const CvArgs p) {
     uint32_t group;
     const CvPlace c = cv_place<kV>(p, group);
     if (!c.there) return;
@@ -114,10 +132,13 @@ template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock) void 
 #pragma unroll
             for (int i = 0; i < kV; ++i) window[r][i] = v.get(i);
         }
-        for (int t = a; t < e; t += kCvRows) {
+        const CvRow<T, kNear> x_row(p.x, p.x_t, c.b * p.x_b + a * p.x_t + c.d), out_row(p.out, p.dim, ((int64_t)c.b * p.tokens + a) * p.dim + c.d);
+        for (int i0 = 0; a + i0 < e; i0 += kCvRows) {                // (as many tokens on in every lane)
+            const int t = a + i0;
+            const bool whole = t + kCvRows <= e;
             RowPiece<T, kV> rows[kCvRows];
 #pragma unroll
-            for (int k = 0; k < kCvRows; ++k) rows[k] = load_row_piece<T, kV>(x + (int64_t)min(t + k, e - 1) * p.x_t);
+            for (int k = 0; k < kCvRows; ++k) rows[k] = load_row_piece<T, kV>(whole ? x_row.at(i0 + k) : x_row.any(min(i0 + k, e - 1 - a)));
 #pragma unroll
             for (int k = 0; k < kCvRows; ++k) {
                 float y[kV];
@@ -132,7 +153,7 @@ template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock) void 
                     window[kW - 2][i] = now;
                     if (p.silu) y[i] *= ts_sigmoid(y[i]);
                 }
-                if (t + k < e) store_row_piece<T, kV>(out + (int64_t)(t + k) * p.dim, y);
+                if (whole || t + k < e) store_row_piece<T, kV>(const_cast<T *>(out_row.at(i0 + k)), y);
             }
         }
         if (e == sp.hi && p.final)
@@ -145,11 +166,13 @@ template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock) void 
     }
 }
 
-template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock, 2) void cv_grad_kernel(const CvArgs p) {
+constexpr int kCvGradRows = 4;
+
+template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(kBlock, 2) void cv_grad_kernel(const CvArgs p) {
     __shared__ float s_sum[kBlock * kV];
     uint32_t group;
     const CvPlace c = cv_place<kV>(p, group);
-    const T *x = (const T *)p.x + (int64_t)c.b * p.x_b + c.d, *dout = (const T *)p.dout + (int64_t)c.b * p.do_b + c.d;
+    const T *x = (const T *)p.x + (int64_t)c.b * p.x_b + c.d;
     T *dx = (T *)p.dx + (int64_t)c.b * p.tokens * p.dim + c.d;
     const int64_t state = (int64_t)(kW - 1) * p.dim;
     float w[kW][kV], bias[kV], dw[kW + 1][kV];
@@ -182,54 +205,74 @@ template <typename T, int kW, int kV> __global__ __launch_bounds__(kBlock, 2) vo
             }
         }
         const int stop = e + kW - 1;                                 // the strip's last dx needs the W - 1 tokens behind it
-        for (int t = a; t < stop; t += kCvRows) {
-            RowPiece<T, kV> rows[kCvRows], ups[kCvRows];
+        constexpr int kRows = kCvGradRows;
+        const CvRow<T, kNear> x_row(p.x, p.x_t, c.b * p.x_b + a * p.x_t + c.d), d_row(p.dout, p.do_t, c.b * p.do_b + a * p.do_t + c.d),
+            dx_row(p.dx, p.dim, ((int64_t)c.b * p.tokens + a) * p.dim + c.d);
+        for (int i0 = 0; a + i0 < stop; i0 += kRows) {               // (as many tokens on in every lane)
+            const int t = a + i0, last_row = min(sp.hi, stop) - 1 - a;
+            RowPiece<T, kV> rows[kRows], ups[kRows];
+            if (t + kRows <= e) {
 #pragma unroll
-            for (int k = 0; k < kCvRows; ++k) {
-                const int64_t at = min(min(t + k, sp.hi - 1), stop - 1);
-                rows[k] = load_row_piece<T, kV>(x + at * p.x_t);
-                ups[k] = load_row_piece<T, kV>(dout + at * p.do_t);
-            }
-#pragma unroll
-            for (int k = 0; k < kCvRows; ++k) {
-                const int now = t + k, to = now - kW + 1;            // the token that dx is found of
-                float d[kV];
-#pragma unroll
-                for (int i = 0; i < kV; ++i) {
-                    const float in = rows[k].get(i);
-                    float y = fmaf(w[kW - 1][i], in, bias[i]), gt = now < sp.hi ? ups[k].get(i) : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kW - 1; ++j) y = fmaf(w[j][i], window[j][i], y);
-                    if (p.silu) {
-                        const float sig = ts_sigmoid(y);
-                        gt *= sig * fmaf(y, 1.0f - sig, 1.0f);
-                        gt = now < sp.hi ? gt : 0.0f;
-                    }
-                    d[i] = w[0][i] * gt;
-#pragma unroll
-                    for (int j = 1; j < kW; ++j) d[i] = fmaf(w[j][i], g[kW - 1 - j][i], d[i]);
-                    const float own = now < e ? gt : 0.0f, seen = now < e ? in : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kW - 1; ++j) dw[j][i] = now < e ? fmaf(own, window[j][i], dw[j][i]) : dw[j][i];
-                    dw[kW - 1][i] = fmaf(own, seen, dw[kW - 1][i]);
-                    dw[kW][i] += own;
-#pragma unroll
-                    for (int j = 0; j < kW - 2; ++j) {
-                        window[j][i] = window[j + 1][i];
-                        g[j][i] = g[j + 1][i];
-                    }
-                    window[kW - 2][i] = in;
-                    g[kW - 2][i] = gt;
+                for (int k = 0; k < kRows; ++k) {
+                    rows[k] = load_row_piece<T, kV>(x_row.at(i0 + k));
+                    ups[k] = load_row_piece<T, kV>(d_row.at(i0 + k));
                 }
-                if (now >= stop || (to < a && (a != sp.lo || !p.dinitial))) continue;
-                const int last = to - (sp.hi - kW + 1);              // its row of the final state, if it is there
-                if (p.dfinal && last >= 0) {
-                    const RowPiece<T, kV> f = load_row_piece<T, kV>((const T *)p.dfinal + sp.seq * state + last * (int64_t)p.dim + c.d);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < kV; ++i) d[i] += f.get(i);
+                for (int k = 0; k < kRows; ++k) {
+                    rows[k] = load_row_piece<T, kV>(x_row.any(min(i0 + k, last_row)));
+                    ups[k] = load_row_piece<T, kV>(d_row.any(min(i0 + k, last_row)));
                 }
-                store_row_piece<T, kV>(to >= sp.lo ? dx + (int64_t)to * p.dim : (T *)p.dinitial + sp.seq * state + (to - sp.lo + kW - 1) * (int64_t)p.dim + c.d, d);
             }
+            auto chunk = [&](auto all) {                             // all: its tokens are the strip's
+                constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    const int now = t + k, to = now - kW + 1;        // the token that dx is found of
+                    const bool own = kAll || now < e;
+                    float d[kV];
+#pragma unroll
+                    for (int i = 0; i < kV; ++i) {
+                        const float in = rows[k].get(i);
+                        float y = fmaf(w[kW - 1][i], in, bias[i]), gt = ups[k].get(i);
+#pragma unroll
+                        for (int j = 0; j < kW - 1; ++j) y = fmaf(w[j][i], window[j][i], y);
+                        if (p.silu) {
+                            const float sig = ts_sigmoid(y);
+                            gt *= sig * fmaf(y, 1.0f - sig, 1.0f);
+                        }
+                        if (!kAll) gt = now < sp.hi ? gt : 0.0f;
+                        d[i] = w[0][i] * gt;
+#pragma unroll
+                        for (int j = 1; j < kW; ++j) d[i] = fmaf(w[j][i], g[kW - 1 - j][i], d[i]);
+#pragma unroll
+                        for (int j = 0; j < kW - 1; ++j) dw[j][i] = own ? fmaf(gt, window[j][i], dw[j][i]) : dw[j][i];
+                        dw[kW - 1][i] = own ? fmaf(gt, in, dw[kW - 1][i]) : dw[kW - 1][i];
+                        dw[kW][i] = own ? dw[kW][i] + gt : dw[kW][i];
+#pragma unroll
+                        for (int j = 0; j < kW - 2; ++j) {
+                            window[j][i] = window[j + 1][i];
+                            g[j][i] = g[j + 1][i];
+                        }
+                        window[kW - 2][i] = in;
+                        g[kW - 2][i] = gt;
+                    }
+                    if (kAll && to >= a) {                           // (before the tokens that a final state holds)
+                        store_row_piece<T, kV>(const_cast<T *>(dx_row.at(i0 + k - kW + 1)), d);
+                        continue;
+                    }
+                    if (now >= stop || (to < a && (a != sp.lo || !p.dinitial))) continue;
+                    const int last = to - (sp.hi - kW + 1);          // its row of the final state, if it is there
+                    if (p.dfinal && last >= 0) {
+                        const RowPiece<T, kV> f = load_row_piece<T, kV>((const T *)p.dfinal + sp.seq * state + last * (int64_t)p.dim + c.d);
+#pragma unroll
+                        for (int i = 0; i < kV; ++i) d[i] += f.get(i);
+                    }
+                    store_row_piece<T, kV>(to >= sp.lo ? dx + (int64_t)to * p.dim : (T *)p.dinitial + sp.seq * state + (to - sp.lo + kW - 1) * (int64_t)p.dim + c.d, d);
+                }
+            };
+            if (t + kRows <= e) chunk(std::true_type{});
+            else chunk(std::false_type{});
         }
         a = e;
     }
@@ -355,7 +398,15 @@ static int64_t cv_grid(CvArgs &a, int v, int longest, int least, int64_t enough)
     const int64_t wgs = ((int64_t)a.batch * a.strips + rows - 1) / rows * a.piece_blocks;
     return wgs > kTsLaunch / kBlock ? -1 : wgs;
 }
-static int64_t cv_grad_grid(CvArgs &a, int size) { return cv_grid(a, a.dim < 4 ? 1 : 4, 64, 8, 262144); }
+static int64_t cv_grad_grid(CvArgs &a, int size) { return cv_grid(a, a.dim < 16 / size ? 1 : 16 / size, 64, 8, 65536); }
+
+// Offsets of a tensor of these strides, and of a dense one, are below 4 GB from the first row's (a row before it and chunks behind the last among them)
+static bool cv_near(const CvArgs &a, int64_t size, int64_t batch, int64_t token) {
+    constexpr int64_t kMost = 0xffffffff;
+    if (batch < 0 || token < 0 || token > kMost / size || (a.batch > 1 && batch > kMost / size)) return false;
+    const __int128 far = (__int128)(a.batch - 1) * batch + (__int128)(a.tokens + 64) * token + a.dim, dense = ((__int128)a.batch * a.tokens + 64) * a.dim;
+    return far * size <= kMost && dense * size <= kMost;
+}
 
 // fn(T, width)
 template <typename F> static int cv_with(int dtype, int width, F fn) {
@@ -384,8 +435,10 @@ extern "C" int ss2d_causal_conv_fwd(const ss2d_causal_conv_params *params, void 
         if (!a.x || !a.weight || !a.out) return (int)SS2D_EINVAL;
         const int64_t wgs = cv_grid(a, a.dim < kV ? 1 : kV, 32, 4, 262144);
         if (wgs < 0) return (int)SS2D_ENOTSUP;
-        if (a.dim < kV) cv_kernel<T, kW, 1><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else cv_kernel<T, kW, kV><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        a.near = cv_near(a, sizeof(T), a.x_b, a.x_t);
+        if (a.dim < kV) cv_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (a.near) cv_kernel<T, kW, kV, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else cv_kernel<T, kW, kV, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
         return launch_status();
     });
 }
@@ -395,7 +448,7 @@ extern "C" int64_t ss2d_causal_conv_bwd_workspace_bytes(const ss2d_causal_conv_b
     const int rc = cv_read(params ? &params->fwd : nullptr, a);
     if (rc != SS2D_OK) return rc;
     if (a.dim == 0 || a.batch == 0 || a.tokens == 0) return 0;
-    const int64_t wgs = cv_grad_grid(a, 0);
+    const int64_t wgs = cv_grad_grid(a, params->fwd.dtype == SS2D_F32 ? 4 : 2);
     return wgs < 0 ? (int64_t)SS2D_ENOTSUP : wgs / a.piece_blocks * (params->fwd.width + 1) * a.dim * 4;
 }
 
@@ -409,7 +462,7 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
     const int width = params->fwd.width;
     return cv_with(params->fwd.dtype, width, [&](auto t, auto w) {
         using T = decltype(t);
-        constexpr int kW = decltype(w)::value;
+        constexpr int kW = decltype(w)::value, kV = 16 / (int)sizeof(T);
         const bool wide = params->fwd.weight_dtype == SS2D_F32;
         if (a.batch == 0 || a.tokens == 0) {                         // no tokens: the weights' gradients are zeros, the state's what came in
             int status = wide ? cv_copy<float>(nullptr, params->dweight, (int64_t)a.dim * kW, st) : cv_copy<T>(nullptr, params->dweight, (int64_t)a.dim * kW, st);
@@ -417,14 +470,16 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
             return status != SS2D_OK ? status : cv_copy<T>(a.dfinal, a.dinitial, (int64_t)a.n_seqs * (kW - 1) * a.dim, st);
         }
         if (!a.x || !a.weight || !a.dout || !a.dx) return (int)SS2D_EINVAL;
-        const int64_t wgs = cv_grad_grid(a, 0);
+        const int64_t wgs = cv_grad_grid(a, sizeof(T));
         if (wgs < 0) return (int)SS2D_ENOTSUP;
         const int64_t parts = wgs / a.piece_blocks;
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return (int)SS2D_EINVAL;
         if (workspace_bytes < parts * (kW + 1) * a.dim * 4) return (int)SS2D_ENOMEM;
         a.sums = (float *)workspace;
-        if (a.dim < 4) cv_grad_kernel<T, kW, 1><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else cv_grad_kernel<T, kW, 4><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        a.near = cv_near(a, sizeof(T), a.x_b, a.x_t) && cv_near(a, sizeof(T), a.do_b, a.do_t);
+        if (a.dim < kV) cv_grad_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (a.near) cv_grad_kernel<T, kW, kV, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else cv_grad_kernel<T, kW, kV, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
         if (params->dweight || params->dbias) {
             const dim3 grid((a.dim + kWave - 1) / kWave, kW + 1);
             if (wide) cv_sum_kernel<float><<<grid, kBlock, 0, st>>>(a.sums, (float *)params->dweight, (float *)params->dbias, a.dim, kW, parts);

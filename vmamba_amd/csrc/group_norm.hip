@@ -30,10 +30,11 @@ struct GnArgs {
     int32_t silu, weight_f32;
     // units
     int32_t per_row;                 // pieces of a position's row of a group
-    int32_t samples;                 // gradients: teams of a group, each with every samples-th sample
+    int32_t samples;                 // teams of a group, each with every samples-th sample
     // slices
     int32_t width, bundle_groups, bundles, group_parts;              // channels of a bundle; groups in it; bundles of a sample; parts of a group (1 where bundles hold whole ones)
     int32_t cols, slices, slice;     // pieces side by side; slices of a sample, positions of one
+    int32_t part_slices, part_slice; // those of the statistics
 };
 
 __device__ __forceinline__ float gn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kGnLog2e * x)); }
@@ -58,10 +59,23 @@ template <typename T, int kV> __device__ __forceinline__ void gn_weights(const G
     else read(T{});
 }
 
-// v summed over a team of kLanes lanes (up to 64: neighbours in a wavefront; 256: the workgroup)
+// v summed over a team of kLanes lanes (up to 64: neighbours in a wavefront; 256: the workgroup), left with all of them.  Inside a row of 16 lanes by
+// additions that take their operand from another lane: neighbours, pairs, then mirrored halves and rows (whose quads and halves are of one value by then).
+__device__ __forceinline__ float gn_swapped16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(f32_to_bits(v), f32_to_bits(v), false, false);
+    return bits_to_f32(r[0]) + bits_to_f32(r[1]);
+}
+__device__ __forceinline__ float gn_swapped32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f32_to_bits(v), f32_to_bits(v), false, false);
+    return bits_to_f32(r[0]) + bits_to_f32(r[1]);
+}
 template <int kLanes> __device__ __forceinline__ float gn_team_sum(float v, float *s_team) {
-#pragma unroll
-    for (int over = 1; over < (kLanes < kWave ? kLanes : kWave); over *= 2) v += __shfl_xor(v, over, kWave);
+    if constexpr (kLanes >= 2) v += dpp_move<0xB1>(0.0f, v);
+    if constexpr (kLanes >= 4) v += dpp_move<0x4E>(0.0f, v);
+    if constexpr (kLanes >= 8) v += dpp_move<0x141>(0.0f, v);
+    if constexpr (kLanes >= 16) v += dpp_move<0x140>(0.0f, v);
+    if constexpr (kLanes >= 32) v = gn_swapped16(v);
+    if constexpr (kLanes >= 64) v = gn_swapped32(v);
     if constexpr (kLanes > kWave) {
         __syncthreads();
         if (threadIdx.x % kWave == 0) s_team[threadIdx.x / kWave] = v;
@@ -72,53 +86,78 @@ template <int kLanes> __device__ __forceinline__ float gn_team_sum(float v, floa
 }
 
 // ---- units ------------------------------------------------------------------------------------------------------------------------
-template <typename T, int kV, int kLanes, int kK> __global__ __launch_bounds__(kBlock) void gn_unit_kernel(const GnArgs p) {
+// A team has a group, and every samples-th sample's, kUnits of them on their way at once.
+template <typename T, int kV, int kLanes, int kK, int kUnits> __global__ __launch_bounds__(kBlock) void gn_unit_kernel(const GnArgs p) {
     __shared__ float s_team[4];
     constexpr int kTeams = kBlock / kLanes;
-    const int64_t units = p.batch * p.groups, unit0 = (int64_t)blockIdx.x * kTeams + (int)threadIdx.x / kLanes, unit = unit0 < units ? unit0 : units - 1;
-    const int lane = (int)threadIdx.x % kLanes, g = (int)(unit % p.groups), c0 = g * p.cg, pieces = p.per_row * p.positions;
-    const int64_t row0 = unit / p.groups * p.positions;
-    const T *x = (const T *)p.x + row0 * p.channels + c0;
-    T *out = (T *)p.out + row0 * p.channels + c0;
-    RowPiece<T, kV> rows[kK];
+    const uint32_t teams = (uint32_t)p.samples * (uint32_t)p.groups, team0 = blockIdx.x * (uint32_t)kTeams + threadIdx.x / kLanes, team = min(team0, teams - 1);
+    const int lane = (int)threadIdx.x % kLanes, g = (int)(team % (uint32_t)p.groups), first = (int)(team / (uint32_t)p.groups), c0 = g * p.cg, pieces = p.per_row * p.positions;
+    const int64_t pitch = (int64_t)p.positions * p.channels;
+    RowPiece<T, kV> rows[kUnits][kK];
     int64_t at[kK];
     int col[kK], skip[kK];                                           // of a row's last piece, which ends with it, the values that the one before has
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-        const int q = min(lane + k * kLanes, pieces - 1), row = q / p.per_row, c = q % p.per_row * kV;
+        const int q = min(lane + k * kLanes, pieces - 1), row = p.positions == 1 ? 0 : q / p.per_row, c = (q - row * p.per_row) * kV;
         col[k] = min(c, p.cg - kV);
         skip[k] = lane + k * kLanes < pieces ? c - col[k] : kV;
-        at[k] = (int64_t)row * p.channels + col[k];
-        rows[k] = load_row_piece<T, kV>(x + at[k]);
+        at[k] = (int64_t)row * p.channels + c0 + col[k];
     }
-    float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kK; ++k)
+    for (int u = 0; u < kUnits; ++u) {
+        const T *from = (const T *)p.x + min((int64_t)first + (int64_t)u * p.samples, p.batch - 1) * pitch;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) sum += i >= skip[k] ? rows[k].get(i) : 0.0f;
-    const float count = (float)p.positions * (float)p.cg, mean = gn_team_sum<kLanes>(sum, s_team) / count;
-    sum = 0.0f;
+        for (int k = 0; k < kK; ++k) rows[u][k] = load_row_piece<T, kV>(from + at[k]);
+    }
+    float w[kK][kV], b[kK][kV];
 #pragma unroll
-    for (int k = 0; k < kK; ++k)
+    for (int k = 0; k < kK; ++k) gn_weights<T, kV>(p, c0 + col[k], w[k], b[k]);
+    const float share = 1.0f / ((float)p.positions * (float)p.cg);
+    const bool ragged = p.cg % kV != 0;                              // (uniform)
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            const float v = rows[k].get(i) - mean;
-            sum = i >= skip[k] ? fmaf(v, v, sum) : sum;
+    for (int u = 0; u < kUnits; ++u) {
+        const int64_t n = (int64_t)first + (int64_t)u * p.samples;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
+            float part = 0.0f;
+            if (ragged) {
+#pragma unroll
+                for (int i = 0; i < kV; ++i) part += i >= skip[k] ? rows[u][k].get(i) : 0.0f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kV; ++i) part += rows[u][k].get(i);
+                part = skip[k] ? 0.0f : part;
+            }
+            sum += part;
         }
-    const float rstd = 1.0f / sqrtf(gn_team_sum<kLanes>(sum, s_team) / count + p.eps);
-    if (unit0 >= units) return;
-    if (p.stats && lane == 0) p.stats[unit] = make_float2(mean, rstd);
+        const float mean = gn_team_sum<kLanes>(sum, s_team) * share;
+        sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kK; ++k) {
-        if (lane + k * kLanes >= pieces) break;
-        float w[kV], b[kV], y[kV];
-        gn_weights<T, kV>(p, c0 + col[k], w, b);
+        for (int k = 0; k < kK; ++k) {
+            float part = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            y[i] = fmaf((rows[k].get(i) - mean) * rstd, w[i], b[i]);
-            if (p.silu) y[i] *= gn_sigmoid(y[i]);
+            for (int i = 0; i < kV; ++i) {
+                const float v = rows[u][k].get(i) - mean;
+                part = !ragged || i >= skip[k] ? fmaf(v, v, part) : part;
+            }
+            sum += skip[k] < kV ? part : 0.0f;
         }
-        store_row_piece<T, kV>(out + at[k], y);
+        const float rstd = __builtin_amdgcn_rsqf(fmaf(gn_team_sum<kLanes>(sum, s_team), share, p.eps));
+        if (n >= p.batch || team0 >= teams) continue;
+        if (p.stats && lane == 0) p.stats[n * p.groups + g] = make_float2(mean, rstd);
+        T *to = (T *)p.out + n * pitch;
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
+            if (lane + k * kLanes >= pieces) break;
+            float y[kV];
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                y[i] = fmaf((rows[u][k].get(i) - mean) * rstd, w[k][i], b[k][i]);
+                if (p.silu) y[i] *= gn_sigmoid(y[i]);
+            }
+            store_row_piece<T, kV>(to + at[k], y);
+        }
     }
 }
 
@@ -129,72 +168,83 @@ __device__ __forceinline__ float gn_through(float dout, float n, float w, float 
     return dout * (sig * fmaf(y, 1.0f - sig, 1.0f));
 }
 
-template <typename T, int kV, int kLanes, int kK> __global__ __launch_bounds__(kBlock) void gn_unit_grad_kernel(const GnArgs p) {
+template <typename T, int kV, int kLanes, int kK, int kUnits> __global__ __launch_bounds__(kBlock) void gn_unit_grad_kernel(const GnArgs p) {
     __shared__ float s_team[4];
     constexpr int kTeams = kBlock / kLanes;
-    const int64_t team0 = (int64_t)blockIdx.x * kTeams + (int)threadIdx.x / kLanes, teams = (int64_t)p.samples * p.groups, team = team0 < teams ? team0 : teams - 1;
-    const int lane = (int)threadIdx.x % kLanes, g = (int)(team % p.groups), c0 = g * p.cg, first = (int)(team / p.groups);
+    const uint32_t teams = (uint32_t)p.samples * (uint32_t)p.groups, team0 = blockIdx.x * (uint32_t)kTeams + threadIdx.x / kLanes, team = min(team0, teams - 1);
+    const int lane = (int)threadIdx.x % kLanes, g = (int)(team % (uint32_t)p.groups), first = (int)(team / (uint32_t)p.groups), c0 = g * p.cg;
     float w[kK][kV], b[kK][kV], dw[kK][kV], db[kK][kV];
     int col[kK], skip[kK];
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
         const int c = min(lane + k * kLanes, p.per_row - 1) * kV;
-        col[k] = min(c, p.cg - kV);
-        skip[k] = lane + k * kLanes < p.per_row ? c - col[k] : kV;
-        gn_weights<T, kV>(p, c0 + col[k], w[k], b[k]);
+        col[k] = c0 + min(c, p.cg - kV);
+        skip[k] = lane + k * kLanes < p.per_row ? c0 + c - col[k] : kV;
+        gn_weights<T, kV>(p, col[k], w[k], b[k]);
 #pragma unroll
         for (int i = 0; i < kV; ++i) dw[k][i] = db[k][i] = 0.0f;
     }
     const float share = 1.0f / (float)p.cg;
-    RowPiece<T, kV> xs[kK], ds[kK];
-    float2 stat;
-    auto request = [&](int64_t n) {
-        n = n < p.batch ? n : p.batch - 1;
+    RowPiece<T, kV> xs[kUnits][kK], ds[kUnits][kK];
+    float2 stat[kUnits];
+    auto sample = [&](int64_t r, int u) { return (int64_t)first + (r * kUnits + u) * p.samples; };
+    auto request = [&](int64_t r) {
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
-            xs[k] = load_row_piece<T, kV>((const T *)p.x + n * p.channels + c0 + col[k]);
-            ds[k] = load_row_piece<T, kV>((const T *)p.dout + n * p.channels + c0 + col[k]);
-        }
-        stat = p.read_stats[n * p.groups + g];
-    };
-    request(first);
-    // (every team of a workgroup makes as many rounds, so that a workgroup's sums meet)
-    const int64_t rounds = (p.batch + p.samples - 1) / p.samples;
-    for (int64_t r = 0; r < rounds; ++r) {
-        const int64_t n = first + r * p.samples;
-        const bool in = n < p.batch && team0 < teams;
-        float v[kK][kV], d[kK][kV], m1 = 0.0f, m2 = 0.0f;
-        const float rstd = stat.y;
+        for (int u = 0; u < kUnits; ++u) {
+            const int64_t n = min(sample(r, u), p.batch - 1);
 #pragma unroll
-        for (int k = 0; k < kK; ++k)
-#pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                v[k][i] = (xs[k].get(i) - stat.x) * rstd;
-                d[k][i] = gn_through(ds[k].get(i), v[k][i], w[k][i], b[k][i], p.silu);
-                const bool own = i >= skip[k];
-                m1 = own ? fmaf(d[k][i], w[k][i], m1) : m1;
-                m2 = own ? fmaf(d[k][i] * w[k][i], v[k][i], m2) : m2;
-                dw[k][i] = in ? fmaf(d[k][i], v[k][i], dw[k][i]) : dw[k][i];
-                db[k][i] = in ? db[k][i] + d[k][i] : db[k][i];
+            for (int k = 0; k < kK; ++k) {
+                xs[u][k] = load_row_piece<T, kV>((const T *)p.x + n * p.channels + col[k]);
+                ds[u][k] = load_row_piece<T, kV>((const T *)p.dout + n * p.channels + col[k]);
             }
-        if (r + 1 < rounds) request(n + p.samples);
-        m1 = gn_team_sum<kLanes>(m1, s_team) * share;
-        m2 = gn_team_sum<kLanes>(m2, s_team) * share;
-        if (!in) continue;
+            stat[u] = p.read_stats[n * p.groups + g];
+        }
+    };
+    request(0);
+    // (every team of a workgroup makes as many rounds, so that a workgroup's sums meet)
+    const int64_t rounds = (p.batch + (int64_t)p.samples * kUnits - 1) / ((int64_t)p.samples * kUnits);
+    for (int64_t r = 0; r < rounds; ++r) {
+        float v[kUnits][kK][kV], d[kUnits][kK][kV], m1[kUnits], m2[kUnits], rstd[kUnits];
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
-            if (lane + k * kLanes >= p.per_row) break;
-            float o[kV];
+        for (int u = 0; u < kUnits; ++u) {
+            const bool in = sample(r, u) < p.batch;
+            m1[u] = m2[u] = 0.0f;
+            rstd[u] = stat[u].y;
 #pragma unroll
-            for (int i = 0; i < kV; ++i) o[i] = rstd * (fmaf(d[k][i], w[k][i], -m1) - v[k][i] * m2);
-            store_row_piece<T, kV>((T *)p.dx + n * p.channels + c0 + col[k], o);
+            for (int k = 0; k < kK; ++k)
+#pragma unroll
+                for (int i = 0; i < kV; ++i) {
+                    v[u][k][i] = (xs[u][k].get(i) - stat[u].x) * rstd[u];
+                    d[u][k][i] = in ? gn_through(ds[u][k].get(i), v[u][k][i], w[k][i], b[k][i], p.silu) : 0.0f;
+                    const float dn = d[u][k][i] * w[k][i];
+                    const bool own = i >= skip[k];
+                    m1[u] += own ? dn : 0.0f;
+                    m2[u] = own ? fmaf(dn, v[u][k][i], m2[u]) : m2[u];
+                    dw[k][i] = in ? fmaf(d[u][k][i], v[u][k][i], dw[k][i]) : dw[k][i];
+                    db[k][i] += d[u][k][i];
+                }
+        }
+        if (r + 1 < rounds) request(r + 1);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            m1[u] = gn_team_sum<kLanes>(m1[u], s_team) * share;
+            m2[u] = gn_team_sum<kLanes>(m2[u], s_team) * share;
+            if (sample(r, u) >= p.batch || team0 >= teams) continue;
+#pragma unroll
+            for (int k = 0; k < kK; ++k) {
+                if (lane + k * kLanes >= p.per_row) break;
+                float o[kV];
+#pragma unroll
+                for (int i = 0; i < kV; ++i) o[i] = rstd[u] * (fmaf(d[u][k][i], w[k][i], -m1[u]) - v[u][k][i] * m2[u]);
+                store_row_piece<T, kV>((T *)p.dx + sample(r, u) * p.channels + col[k], o);
+            }
         }
     }
     if (team0 >= teams || !p.sums) return;
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
         if (lane + k * kLanes >= p.per_row) break;
-        float *to = p.sums + (int64_t)first * 2 * p.channels + c0 + col[k];
+        float *to = p.sums + (int64_t)first * 2 * p.channels + col[k];
         store_row_piece<float, kV>(to, db[k]);
         store_row_piece<float, kV>(to + p.channels, dw[k]);
     }
@@ -220,16 +270,27 @@ template <int kV> __device__ __forceinline__ GnPlace gn_place(const GnArgs &p) {
     }
     q.begin = q.slice * p.slice; q.end = min(q.begin + p.slice, p.positions);
     q.piece = (int)threadIdx.x % p.cols; q.row = (int)threadIdx.x / p.cols; q.rows = kBlock / p.cols;
-    q.there = q.piece * kV < q.width;
+    q.there = q.piece * kV < q.width && q.row < q.rows;
     q.c = max(min(q.piece * kV, q.width - kV), 0);                   // inside the bundle
     return q;
+}
+
+// fn(i, group of the bundle) for the channels of a lane's piece
+template <int kV, typename F> __device__ __forceinline__ void gn_by_group(const GnArgs &p, const GnPlace &q, F fn) {
+    int g = p.group_parts > 1 ? 0 : q.c / p.cg, left = p.group_parts > 1 ? kV : (g + 1) * p.cg - q.c;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+        if (left == 0) { ++g; left = p.cg; }
+        fn(i, g);
+        --left;
+    }
 }
 
 constexpr int kGnRows = 8;           // rows of a chunk
 
 // fn(team of lanes) for every group of the bundle: s_out[group] from entries by rows and channels
 template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_stats_kernel(const GnArgs p) {
-    __shared__ float s_mean[kBlock * kV], s_square[kBlock * kV];
+    __shared__ float s_mean[kBlock * kV + 2], s_square[kBlock * kV + 2];
     const GnPlace q = gn_place<kV>(p);
     const int pitch = p.cols * kV;
     if (q.there) {
@@ -259,22 +320,45 @@ template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_stats
         }
     }
     __syncthreads();
-    // a team of lanes to a group of the bundle: the entries of its rows and channels
+    // each channel over the rows of threads
+    const int len = q.end - q.begin, wide = p.group_parts > 1 ? q.width : p.cg, least = len / q.rows, longer = len % q.rows;
+    const float len_share = 1.0f / (float)len;
+    float c_mean[2], c_square[2];                                    // (a bundle has 512 channels at most)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int c = (int)threadIdx.x + e * kBlock;
+        c_mean[e] = c_square[e] = 0.0f;
+        if (c >= q.width) break;
+        for (int r = 0; r < q.rows; ++r) c_mean[e] = fmaf((float)(least + (r < longer)), s_mean[r * pitch + c], c_mean[e]);
+        c_mean[e] *= len_share;
+        for (int r = 0; r < q.rows; ++r) {
+            const float held = (float)(least + (r < longer)), off = s_mean[r * pitch + c] - c_mean[e];
+            c_square[e] += fmaf(held * off, off, held > 0.0f ? s_square[r * pitch + c] : 0.0f);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int c = (int)threadIdx.x + e * kBlock;
+        if (c >= q.width) break;
+        s_mean[c] = c_mean[e];
+        s_square[c] = c_square[e];
+    }
+    __syncthreads();
+    // a team of lanes to a group of the bundle: its channels
     int lanes = kWave;
     while (lanes > 1 && lanes * q.k > kBlock) lanes /= 2;
-    const int team = (int)threadIdx.x / lanes, lane = (int)threadIdx.x % lanes, len = q.end - q.begin, wide = p.group_parts > 1 ? q.width : p.cg;
-    auto held = [&](int row) { return (float)((len - row + q.rows - 1) / q.rows); };       // positions of a row of threads (0: none)
+    const int team = (int)threadIdx.x / lanes, lane = (int)threadIdx.x % lanes;
     for (int j0 = 0; j0 < q.k; j0 += kBlock / lanes) {               // (as often for every lane)
-        const int j = min(j0 + team, q.k - 1), entries = min(q.rows, len) * wide;
+        const int j = min(j0 + team, q.k - 1);
         float sum = 0.0f;
-        for (int e = lane; e < entries; e += lanes) sum = fmaf(held(e / wide), s_mean[e / wide * pitch + j * wide + e % wide], sum);
+        for (int c = lane; c < wide; c += lanes) sum += s_mean[j * wide + c];
         for (int over = 1; over < lanes; over *= 2) sum += __shfl_xor(sum, over, kWave);
-        const float mean = sum / ((float)len * (float)wide);
+        const float mean = sum / (float)wide;
         sum = 0.0f;
-        for (int e = lane; e < entries; e += lanes) {
-            const int from = e / wide * pitch + j * wide + e % wide;
-            const float off = s_mean[from] - mean;
-            sum += fmaf(held(e / wide) * off, off, s_square[from]);
+        for (int c = lane; c < wide; c += lanes) {
+            const float off = s_mean[j * wide + c] - mean;
+            sum += fmaf((float)len * off, off, s_square[j * wide + c]);
         }
         for (int over = 1; over < lanes; over *= 2) sum += __shfl_xor(sum, over, kWave);
         if (lane == 0 && j0 + team < q.k) {
@@ -286,11 +370,16 @@ template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_stats
 
 // A sample's group from its parts, by a team of lanes
 __device__ __forceinline__ float2 gn_join(const GnArgs &p, int64_t unit, int lane, int lanes) {
-    const int n = p.group_parts * p.slices;
+    const int n = p.group_parts * p.part_slices;
     const float2 *from = p.parts + unit * n;
     auto held = [&](int e) {
-        const int part = e / p.slices, s = e % p.slices, width = p.group_parts > 1 ? min(p.width, p.cg - part * p.width) : p.cg;
-        return (float)min(p.slice, p.positions - s * p.slice) * (float)width;
+        int width = p.cg;
+        if (p.group_parts > 1) {
+            const int part = e / p.part_slices;
+            e -= part * p.part_slices;
+            width = min(p.width, p.cg - part * p.width);
+        }
+        return (float)min(p.part_slice, p.positions - e * p.part_slice) * (float)width;
     };
     const float count = (float)p.positions * (float)p.cg;
     float sum = 0.0f;
@@ -303,7 +392,7 @@ __device__ __forceinline__ float2 gn_join(const GnArgs &p, int64_t unit, int lan
         sum += fmaf(held(e) * off, off, from[e].y);
     }
     for (int over = 1; over < lanes; over *= 2) sum += __shfl_xor(sum, over, kWave);
-    return make_float2(mean, 1.0f / sqrtf(sum / count + p.eps));
+    return make_float2(mean, __builtin_amdgcn_rsqf(sum / count + p.eps));
 }
 
 constexpr int kGnMaxGroups = 512;    // of a bundle
@@ -311,6 +400,15 @@ constexpr int kGnMaxGroups = 512;    // of a bundle
 template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const GnArgs p) {
     __shared__ float2 s_stats[kGnMaxGroups];
     const GnPlace q = gn_place<kV>(p);
+    const int64_t at = q.n * p.positions * p.channels + q.c0 + q.c;
+    const T *x = (const T *)p.x + at;
+    T *out = (T *)p.out + at;
+    RowPiece<T, kV> rows[kGnRows];
+    auto request = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < kGnRows; ++k) rows[k] = load_row_piece<T, kV>(x + (int64_t)min(t + k * q.rows, q.end - 1) * p.channels);
+    };
+    if (q.there) request(q.begin + q.row);                           // on their way while the statistics are joined
     int lanes = kWave;
     while (lanes > 1 && lanes * q.k > kBlock) lanes /= 2;
     const int team = (int)threadIdx.x / lanes, lane = (int)threadIdx.x % lanes;
@@ -322,23 +420,16 @@ template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_apply
             if (p.stats && q.slice == 0) p.stats[q.n * p.groups + q.g0 + j] = s;
         }
     }
+    float w[kV], b[kV], mean[kV];
+    if (q.there) gn_weights<T, kV>(p, q.c0 + q.c, w, b);
     __syncthreads();
     if (!q.there) return;
-    const int64_t at = q.n * p.positions * p.channels + q.c0 + q.c;
-    const T *x = (const T *)p.x + at;
-    T *out = (T *)p.out + at;
-    float w[kV], b[kV], mean[kV];
-    gn_weights<T, kV>(p, q.c0 + q.c, w, b);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) {
-        const float2 s = s_stats[(q.c + i) / p.cg % q.k];            // (of a part of a group, its one)
-        mean[i] = s.x;
-        w[i] *= s.y;
-    }
+    gn_by_group<kV>(p, q, [&](int i, int g) {
+        mean[i] = s_stats[g].x;
+        w[i] *= s_stats[g].y;
+    });
     for (int t = q.begin + q.row; t < q.end; t += kGnRows * q.rows) {
-        RowPiece<T, kV> rows[kGnRows];
-#pragma unroll
-        for (int k = 0; k < kGnRows; ++k) rows[k] = load_row_piece<T, kV>(x + (int64_t)min(t + k * q.rows, q.end - 1) * p.channels);
+        if (t != q.begin + q.row) request(t);
 #pragma unroll
         for (int k = 0; k < kGnRows; ++k) {
             if (t + k * q.rows >= q.end) break;
@@ -364,18 +455,16 @@ template <typename T, int kV, bool kSums> __global__ __launch_bounds__(kBlock, 2
         T *dx = (T *)p.dx + at;
         float w[kV], b[kV], mean[kV], rstd[kV], m1[kV], m2[kV], d_sum[kV] = {}, dn_sum[kV] = {};
         gn_weights<T, kV>(p, q.c0 + q.c, w, b);
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            const int64_t unit = q.n * p.groups + q.g0 + (q.c + i) / p.cg % q.k;
-            const float2 s = p.read_stats[unit];
-            mean[i] = s.x;
-            rstd[i] = s.y;
+        gn_by_group<kV>(p, q, [&](int i, int g) {
+            const int64_t unit = q.n * p.groups + q.g0 + g;
+            mean[i] = p.read_stats[unit].x;
+            rstd[i] = p.read_stats[unit].y;
             m1[i] = m2[i] = 0.0f;
             if constexpr (!kSums) {
                 m1[i] = p.means[unit].x;
                 m2[i] = p.means[unit].y;
             }
-        }
+        });
         constexpr int kRows = kGnRows / 2;
         for (int t = q.begin + q.row; t < q.end; t += kRows * q.rows) {
             RowPiece<T, kV> xs[kRows], ds[kRows];
@@ -534,17 +623,25 @@ static bool gn_slices(GnArgs &a, int size) {
             a.bundles = (a.groups + a.bundle_groups - 1) / a.bundle_groups;
         }
     }
-    const int pieces = (a.width + v - 1) / v;
-    a.cols = 1;
-    while (a.cols < pieces) a.cols *= 2;
-    const int rows = kBlock / a.cols;
-    const int64_t others = a.batch * a.bundles, enough = 2048, most_slices = (a.positions + (int64_t)rows * 4 - 1) / (rows * 4);
-    int64_t n = (enough + others - 1) / (others > 0 ? others : 1);
-    n = n < most_slices ? n : most_slices;
-    n = n < 1 ? 1 : n;
-    a.slice = (int)((a.positions + n - 1) / n);
+    a.cols = (a.width + v - 1) / v;
+    return true;
+}
+
+// Slices of whole chunks of a workgroup's rows, as long as there are `enough` workgroups; false: too many
+static bool gn_cut(GnArgs &a, int64_t enough) {
+    const int64_t chunk = (int64_t)(kBlock / a.cols) * kGnRows, others = a.batch * a.bundles, chunks = (a.positions + chunk - 1) / chunk;
+    int64_t each = chunks * others / enough;
+    each = each < 1 ? 1 : each < chunks ? each : chunks;
+    a.slice = (int)(each * chunk < a.positions ? each * chunk : a.positions);
     a.slices = (int)((a.positions + (int64_t)a.slice - 1) / a.slice);
     return others * a.slices <= kGnLaunch / kBlock;
+}
+// The statistics', and then the values' slices, whose workgroups all join the statistics' parts
+static bool gn_cut_stats(GnArgs &a) {
+    if (!gn_cut(a, 768)) return false;
+    a.part_slices = a.slices;
+    a.part_slice = a.slice;
+    return true;
 }
 
 // fn(T, pieces' values, lanes, each) of a team
@@ -605,8 +702,8 @@ extern "C" int64_t ss2d_group_norm_workspace_bytes(const ss2d_group_norm_params 
     if (rc != SS2D_OK) return rc;
     int lanes, each;
     if (a.batch == 0 || a.positions == 0 || gn_unit(a, gn_vec(a.cg, gn_size(params->dtype)), lanes, each)) return 0;
-    if (!gn_slices(a, gn_size(params->dtype))) return SS2D_ENOTSUP;
-    return a.batch * a.groups * a.group_parts * a.slices * 8;
+    if (!gn_slices(a, gn_size(params->dtype)) || !gn_cut_stats(a)) return SS2D_ENOTSUP;
+    return a.batch * a.groups * a.group_parts * a.part_slices * 8;
 }
 
 extern "C" int ss2d_group_norm_fwd(const ss2d_group_norm_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -620,19 +717,27 @@ extern "C" int ss2d_group_norm_fwd(const ss2d_group_norm_params *params, void *w
     if (gn_unit(a, v, lanes, each))
         return gn_team(params->dtype, v, lanes, each, [&](auto t, auto vec, auto l, auto k) {
             constexpr int kLanes = decltype(l)::value, kTeams = kBlock / kLanes;
-            const int64_t wgs = (a.batch * a.groups + kTeams - 1) / kTeams;
-            if (wgs > kGnLaunch / kBlock) return (int)SS2D_ENOTSUP;
-            gn_unit_kernel<decltype(t), decltype(vec)::value, kLanes, decltype(k)::value><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-            return launch_status();
+            constexpr int kK = decltype(k)::value;
+            auto go = [&](auto units) {
+                constexpr int kUnits = decltype(units)::value;
+                a.samples = (int)((a.batch + kUnits - 1) / kUnits);
+                const int64_t wgs = ((int64_t)a.samples * a.groups + kTeams - 1) / kTeams;
+                if (wgs > kGnLaunch / kBlock) return (int)SS2D_ENOTSUP;
+                gn_unit_kernel<decltype(t), decltype(vec)::value, kLanes, kK, kUnits><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+                return launch_status();
+            };
+            if constexpr (kK == 1 && kLanes <= kWave)
+                if (a.batch * a.groups / kTeams >= 4096) return go(std::integral_constant<int, 4>{});
+            return go(std::integral_constant<int, 1>{});
         });
-    if (!gn_slices(a, size)) return SS2D_ENOTSUP;
+    if (!gn_slices(a, size) || !gn_cut_stats(a)) return SS2D_ENOTSUP;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return SS2D_EINVAL;
-    if (workspace_bytes < a.batch * a.groups * a.group_parts * a.slices * 8) return SS2D_ENOMEM;
+    if (workspace_bytes < a.batch * a.groups * a.group_parts * a.part_slices * 8) return SS2D_ENOMEM;
     a.parts = (float2 *)workspace;
     return gn_sliced(params->dtype, a.channels, [&](auto t, auto vec) {
-        const uint32_t wgs = (uint32_t)(a.batch * a.bundles * a.slices);
-        gn_stats_kernel<decltype(t), decltype(vec)::value><<<wgs, kBlock, 0, st>>>(a);
-        gn_apply_kernel<decltype(t), decltype(vec)::value><<<wgs, kBlock, 0, st>>>(a);
+        gn_stats_kernel<decltype(t), decltype(vec)::value><<<(uint32_t)(a.batch * a.bundles * a.slices), kBlock, 0, st>>>(a);
+        if (!gn_cut(a, 2048)) return (int)SS2D_ENOTSUP;
+        gn_apply_kernel<decltype(t), decltype(vec)::value><<<(uint32_t)(a.batch * a.bundles * a.slices), kBlock, 0, st>>>(a);
         return launch_status();
     });
 }
@@ -644,7 +749,7 @@ static int64_t gn_bwd_plan(const ss2d_group_norm_params *p, GnArgs &a, int &lane
         return (int64_t)a.samples * 2 * a.channels * 4;
     }
     lanes = 0;
-    if (!gn_slices(a, gn_size(p->dtype))) return SS2D_ENOTSUP;
+    if (!gn_slices(a, gn_size(p->dtype)) || !gn_cut(a, 1024)) return SS2D_ENOTSUP;
     return (a.batch * a.slices * 2 * a.channels * 4 + 15) / 16 * 16 + a.batch * a.groups * 8;
 }
 
@@ -692,7 +797,8 @@ extern "C" int ss2d_group_norm_bwd(const ss2d_group_norm_bwd_params *params, voi
             constexpr int kLanes = decltype(l)::value, kTeams = kBlock / kLanes;
             const int64_t wgs = ((int64_t)a.samples * a.groups + kTeams - 1) / kTeams;
             if (wgs > kGnLaunch / kBlock) return (int)SS2D_ENOTSUP;
-            gn_unit_grad_kernel<decltype(t), decltype(vec)::value, kLanes, decltype(k)::value><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+            constexpr int kK = decltype(k)::value, kUnits = kK == 1 ? 2 : 1;
+            gn_unit_grad_kernel<decltype(t), decltype(vec)::value, kLanes, kK, kUnits><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
             return launch_status();
         });
     } else {
@@ -701,10 +807,10 @@ extern "C" int ss2d_group_norm_bwd(const ss2d_group_norm_bwd_params *params, voi
         const int64_t teams = (a.batch * a.groups + kBlock / kWave - 1) / (kBlock / kWave);
         if (teams > kGnLaunch / kBlock) return SS2D_ENOTSUP;
         status = gn_sliced(dtype, a.channels, [&](auto t, auto vec) {
-            const uint32_t wgs = (uint32_t)(a.batch * a.bundles * a.slices);
-            gn_slice_grad_kernel<decltype(t), decltype(vec)::value, true><<<wgs, kBlock, 0, st>>>(a);
+            gn_slice_grad_kernel<decltype(t), decltype(vec)::value, true><<<(uint32_t)(a.batch * a.bundles * a.slices), kBlock, 0, st>>>(a);
             gn_means_kernel<decltype(t)><<<(uint32_t)teams, kBlock, 0, st>>>(a);
-            gn_slice_grad_kernel<decltype(t), decltype(vec)::value, false><<<wgs, kBlock, 0, st>>>(a);
+            if (!gn_cut(a, 2048)) return (int)SS2D_ENOTSUP;
+            gn_slice_grad_kernel<decltype(t), decltype(vec)::value, false><<<(uint32_t)(a.batch * a.bundles * a.slices), kBlock, 0, st>>>(a);
             return launch_status();
         });
     }
