@@ -15,7 +15,7 @@
 namespace ss2d {
 
 constexpr int kTsTile = 16;          // tokens of a tile
-constexpr int kTsGrid = 64;          // what segments are multiples of
+constexpr int kTsGrid = 64;          // tokens of a segment at least
 constexpr int kTsMaxState = 64;
 constexpr int64_t kTsLaunch = 0xffffffff;                            // threads of a launch
 
@@ -38,6 +38,13 @@ struct TsArgs {
 
 // Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th
 // token takes a quarter of the memory, and the gradients a second walk over every piece: 310 us in place of 262 of their kernel, 4 x 2048 tokens of 2048 channels.)
+// Tokens of n segments, a multiple of `keep`: a segment begins with a kept state
+inline int ts_seg_len(int64_t tokens, int64_t n, int keep) {
+    n = n < 1 ? 1 : n;
+    int64_t len = ((tokens + n - 1) / n + keep - 1) / keep * keep;
+    len = len < kTsGrid ? kTsGrid : len;
+    return (int)len;
+}
 inline int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
 // Whole wavefronts of channels, states that fill their lanes, offsets inside a tile that fit 32 bits: the kernels without masks
 inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / ts_sets(a.N)) == 0 && (a.N == 4 || a.N == 8 || a.N == 16 || a.N == 32 || a.N == 64); }

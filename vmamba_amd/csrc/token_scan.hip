@@ -297,18 +297,17 @@ __global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
-// Segments of the token axis.  A cut sequence is walked twice for what goes into the later segments.
+// Segments of the token axis.  A cut sequence is walked twice for what goes into the later segments, so it is cut only where its wavefronts are fewer than one and a half to
+// a SIMD, and then into as many as come to four workgroups on every CU: what is between two whole numbers of them waits for the last.
 static void ts_cut(TsArgs &a) {
     const int ch = kWave / ts_sets(a.N);
     a.wgs = (int)(((int64_t)a.per_group + ch * kWavesPerWg - 1) / (ch * kWavesPerWg));
-    const int64_t waves = (int64_t)a.batch * a.groups * ((a.per_group + ch - 1) / ch);
-    constexpr int64_t kEnough = 1536, kTarget = 4096;
-    int64_t n = waves >= kEnough ? 1 : (kTarget + waves - 1) / waves;
+    const int64_t waves = (int64_t)a.batch * a.groups * ((a.per_group + ch - 1) / ch), wgs = (int64_t)a.batch * a.groups * a.wgs;
+    constexpr int64_t kEnough = 1536, kTarget = 1024;
+    int64_t n = waves >= kEnough ? 1 : kTarget / (wgs > 0 ? wgs : 1);
     const int64_t most = (a.tokens + 2 * kTsGrid - 1) / (2 * kTsGrid);
     n = n < most ? n : most;
-    n = n < 1 ? 1 : n;
-    const int64_t len = ((a.tokens + n - 1) / n + kTsGrid - 1) / kTsGrid * kTsGrid;
-    a.seg_len = (int)(len < kTsGrid ? kTsGrid : len);
+    a.seg_len = ts_seg_len(a.tokens, n, a.keep);
     a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
     if (a.n_segs < 1) a.n_segs = 1;
 }

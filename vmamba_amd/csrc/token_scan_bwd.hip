@@ -19,13 +19,16 @@ static int ts_bwd_read(const ss2d_token_scan_bwd_params *p, TsBwdArgs &q) {
     if (a.dim == 0 || a.tokens == 0) return SS2D_OK;
     const int ch = kWave / (a.N <= 4 ? 1 : a.N <= 8 ? 2 : 4) * (a.N <= 32 ? kTsBwdWaves<1> : kTsBwdWaves<4>);
     a.wgs = (a.per_group + ch - 1) / ch;
-    // segments: two wavefronts to a SIMD fill the chip, and what is handed from one to the next costs a sixth of the gradients
-    const int64_t wgs = (int64_t)a.batch * a.groups * a.wgs;
-    constexpr int64_t kTarget = 1024;
-    int64_t n = (kTarget + wgs - 1) / wgs;
-    const int64_t most = (a.tokens + (int64_t)kTsGrid - 1) / kTsGrid;
-    n = n < most ? n : most;
-    a.seg_len = (int)(((a.tokens + n - 1) / n + kTsGrid - 1) / kTsGrid * kTsGrid);
+    // Segments: two workgroups to a CU are what the gradients' registers leave room for, so that their rounds are of 512, and what is handed from one segment to the next
+    // costs a fifth of what goes into it.  (4 x 2048 tokens of 2048 channels, 4 segments 482 us with the forward, 6 502, 8 480; 8 x 784 of 768, 8 states: 169, 7 segments; 13: 173.)
+    const int64_t wgs = (int64_t)a.batch * a.groups * a.wgs, most = (a.tokens + (int64_t)kTsGrid - 1) / kTsGrid;
+    int64_t n = 1;
+    double least = 0;
+    for (int64_t k = 1; k <= most && k <= 512 && (k == 1 || wgs * (k - 1) < 4096); ++k) {
+        const double cost = (double)((wgs * k + 511) / 512) / (double)k * (1.0 + 0.2 * (double)(k - 1) / (double)k);
+        if (k == 1 || cost < 0.99 * least) { least = cost; n = k; }
+    }
+    a.seg_len = ts_seg_len(a.tokens, n, a.keep);
     a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
     if (wgs * a.n_segs > kTsLaunch / kBlock || (a.n_segs > 1 && a.batch > 65535)) return SS2D_ENOTSUP;
     return SS2D_OK;
