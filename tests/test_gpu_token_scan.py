@@ -230,3 +230,34 @@ def test_prompt_then_tokens():
     check("final", state, want["final"], size["final"], args, [(0, 0, 90)])
     check("final", final, want["final"], size["final"], args, [(0, 0, 90)])
     check("out", whole, want["out"], size["out"], args, [(0, 0, 90)])
+
+
+@pytest.mark.parametrize("shape", [(1, 2000, 64, 16, 1), (2, 700, 128, 16, 2), (1, 3000, 16, 16, 1), (1, 600, 32, 64, 1), (2, 500, 64, 32, 2), (1, 900, 256, 4, 1), (1, 1100, 1, 1, 1), (9, 333, 640, 16, 1)],
+                         ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_long_sequences(shape, dtype):
+    """Many segments, of channels and states that fill their lanes and of those that do not."""
+    print("CASE token_scan long", shape, dtype, flush=True)
+    args, dout, dfinal, _ = inputs(*shape, dtype, shape[1])
+    got = run_all(args, dout, dfinal)
+    pieces = [(b, 0, shape[1]) for b in range(shape[0])]
+    want, size = reference(args, pieces, dout, dfinal)
+    for name in got:
+        check(name, got[name], want[name], size[name], args, pieces)
+
+
+@pytest.mark.parametrize("N", [16, 32, 64, 4])
+def test_packed_where_lanes_are_full(N):
+    """As test_packed, with segments' ends inside and at the ends of sequences, and a lone row before them."""
+    lengths = [255, 0, 1, 256, 16, 17, 700, 0, 64, 31]
+    starts = [1 + sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    T = starts[-1] + 40
+    cu = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    args, dout, dfinal, _ = inputs(1, T, 128, N, 2, BF16, 6, n_seqs=len(lengths))
+    got = run_all(args, dout, dfinal, cu)
+    pieces = [(0, lo, lo + n) for lo, n in zip(starts, lengths)]
+    want, size = reference(args, pieces, dout, dfinal)
+    for name in got:
+        check(name, got[name], want[name], size[name], args, pieces)
+    for name in ("out", "du", "ddelta", "dz", "dB", "dC"):
+        assert not got[name][0, :1].any() and not got[name][0, starts[-1]:].any(), name
