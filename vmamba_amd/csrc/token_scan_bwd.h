@@ -356,9 +356,9 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
             const float zeros[4] = {0, 0, 0, 0};
             if (works)
                 for (int k = a + l.row; k < e; k += L::kRows) {
-                    ts_store4<T>(du + (int64_t)k * p.dim + at, mine, whole, zeros);
-                    ts_store4<T>(dd + (int64_t)k * p.dim + at, mine, whole, zeros);
-                    if (z) ts_store4<T>(dz + (int64_t)k * p.dim + at, mine, whole, zeros);
+                    ts_store4<T, true>(du + (int64_t)k * p.dim + at, mine, whole, zeros);
+                    ts_store4<T, true>(dd + (int64_t)k * p.dim + at, mine, whole, zeros);
+                    if (z) ts_store4<T, true>(dz + (int64_t)k * p.dim + at, mine, whole, zeros);
                 }
             for (int i = threadIdx.x; i < (e - a) * N * 2; i += kThreads) pBC[i / (N * 2) * bc_row + i % (N * 2)] = 0.0f;
             if (!more) break;
@@ -550,14 +550,14 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                         sum_bias[i] += d_out[i];
                         sum_D[i] = fmaf(tok.z, tok.w, sum_D[i]);
                     }
-                    ts_store4<T>(row_of(du), mine, whole, u_out);
-                    ts_store4<T>(row_of(dd), mine, whole, d_out);
+                    ts_store4<T, true>(row_of(du), mine, whole, u_out);
+                    ts_store4<T, true>(row_of(dd), mine, whole, d_out);
                     if (z) {
                         const float4 y4 = *reinterpret_cast<const float4 *>(s_y + k * L::kPitch + l.at);
                         const float yv[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) u_out[i] = through[r][i] * fmaf(skip[i], uv[i], yv[i]);
-                        ts_store4<T>(row_of(dz), mine, whole, u_out);
+                        ts_store4<T, true>(row_of(dz), mine, whole, u_out);
                     }
                 }
                 wave_lds_sync();
