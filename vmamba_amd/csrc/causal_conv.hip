@@ -86,6 +86,10 @@ template <typename T, int kV> __device__ __forceinline__ void cv_copy_row(const 
 }
 
 constexpr int kCvRows = 8;           // rows of a chunk
+// Values of a forward below which a thread takes two channels and four rows: its instructions are a quarter, and where every wavefront runs once, fetching them is what
+// it waits for.  37 tokens of 1024 channels 5.4 -> 3.3 us, 8 x 512 of 2048 (2^23) 11.5 -> 11.1; twice as many 14.2, and 19.1 by that form.
+constexpr int64_t kCvFew = 1 << 23;
+constexpr int kCvFewRows = 4;
 
 // Rows of a tensor from a lane's first one on.  at(): a row that is as far on in every lane (kNear: a uniform address, and the lane's offset, which costs no vector
 // instruction); any(): one that is not.
@@ -104,7 +108,7 @@ template <typename T, bool kNear> struct CvRow {
     }
 };
 
-template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(kBlock) void cv_kernel(const CvArgs p) {
+template <typename T, int kW, int kV, bool kNear, int kRows> __global__ __launch_bounds__(kBlock) void cv_kernel(const CvArgs p) {
     uint32_t group;
     const CvPlace c = cv_place<kV>(p, group);
     if (!c.there) return;
@@ -112,7 +116,7 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
     T *out = (T *)p.out + (int64_t)c.b * p.tokens * p.dim + c.d, *final = (T *)p.final + c.d;
     const int64_t state = (int64_t)(kW - 1) * p.dim;
     float w[kW][kV], bias[kV];
-    cv_weights<T, kW, kV>(p, c.d, w, bias);
+    bool read = false;
     if (p.cu && p.final)                                             // sequences without tokens, dealt out over the strips
         for (int i = c.strip; i < p.n_seqs; i += p.strips)
             if (min(max(p.cu[i + 1], 0), p.tokens) <= min(max(p.cu[i], 0), p.tokens))
@@ -125,22 +129,28 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
             a = e;
             continue;
         }
+        RowPiece<T, kV> before[kW - 1], rows[kRows];
+#pragma unroll
+        for (int r = 0; r < kW - 1; ++r) before[r] = cv_line<T, kW, kV>(p, x, sp, c.d, a - kW + 1 + r);
+        const CvRow<T, kNear> x_row(p.x, p.x_t, c.b * p.x_b + a * p.x_t + c.d), out_row(p.out, p.dim, ((int64_t)c.b * p.tokens + a) * p.dim + c.d);
+        auto request = [&](int i0) {                                 // (as many tokens on in every lane)
+            const bool whole = a + i0 + kRows <= e;
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) rows[k] = load_row_piece<T, kV>(whole ? x_row.at(i0 + k) : x_row.any(min(i0 + k, e - 1 - a)));
+        };
+        request(0);
+        if (!read) cv_weights<T, kW, kV>(p, c.d, w, bias);           // (on their way with the first rows: 37 tokens are one latency)
+        read = true;
         float window[kW - 1][kV];
 #pragma unroll
-        for (int r = 0; r < kW - 1; ++r) {
-            const RowPiece<T, kV> v = cv_line<T, kW, kV>(p, x, sp, c.d, a - kW + 1 + r);
+        for (int r = 0; r < kW - 1; ++r)
 #pragma unroll
-            for (int i = 0; i < kV; ++i) window[r][i] = v.get(i);
-        }
-        const CvRow<T, kNear> x_row(p.x, p.x_t, c.b * p.x_b + a * p.x_t + c.d), out_row(p.out, p.dim, ((int64_t)c.b * p.tokens + a) * p.dim + c.d);
-        for (int i0 = 0; a + i0 < e; i0 += kCvRows) {                // (as many tokens on in every lane)
+            for (int i = 0; i < kV; ++i) window[r][i] = before[r].get(i);
+        for (int i0 = 0;;) {
             const int t = a + i0;
-            const bool whole = t + kCvRows <= e;
-            RowPiece<T, kV> rows[kCvRows];
+            const bool whole = t + kRows <= e;
 #pragma unroll
-            for (int k = 0; k < kCvRows; ++k) rows[k] = load_row_piece<T, kV>(whole ? x_row.at(i0 + k) : x_row.any(min(i0 + k, e - 1 - a)));
-#pragma unroll
-            for (int k = 0; k < kCvRows; ++k) {
+            for (int k = 0; k < kRows; ++k) {
                 float y[kV];
 #pragma unroll
                 for (int i = 0; i < kV; ++i) {
@@ -155,13 +165,21 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
                 }
                 if (whole || t + k < e) store_row_piece<T, kV>(const_cast<T *>(out_row.at(i0 + k)), y);
             }
+            i0 += kRows;
+            if (a + i0 >= e) break;
+            request(i0);
         }
-        if (e == sp.hi && p.final)
+        if (e == sp.hi && p.final) {
+#pragma unroll
+            for (int r = 0; r < kW - 1; ++r) before[r] = cv_line<T, kW, kV>(p, x, sp, c.d, e - kW + 1 + r);
+#pragma unroll
             for (int r = 0; r < kW - 1; ++r) {
-                const int t = e - kW + 1 + r;
-                const T *from = t >= sp.lo ? x + (int64_t)t * p.x_t : p.initial ? (const T *)p.initial + sp.seq * state + (t - sp.lo + kW - 1) * (int64_t)p.dim + c.d : nullptr;
-                cv_copy_row<T, kV>(from, final + sp.seq * state + r * (int64_t)p.dim);
+                float v[kV];
+#pragma unroll
+                for (int i = 0; i < kV; ++i) v[i] = before[r].get(i);
+                store_row_piece<T, kV>(final + sp.seq * state + r * (int64_t)p.dim, v);
             }
+        }
         a = e;
     }
 }
@@ -398,7 +416,10 @@ static int64_t cv_grid(CvArgs &a, int v, int longest, int least, int64_t enough)
     const int64_t wgs = ((int64_t)a.batch * a.strips + rows - 1) / rows * a.piece_blocks;
     return wgs > kTsLaunch / kBlock ? -1 : wgs;
 }
-static int64_t cv_grad_grid(CvArgs &a, int size) { return cv_grid(a, a.dim < 16 / size ? 1 : 16 / size, 64, 8, 65536); }
+// The gradients: two channels to a thread at any size.  (16-byte pieces, which the forward takes, need a quarter of the threads, but four times the registers and instructions:
+// 37 tokens of 1024 channels, forward and gradients, 12.9 us, 18.3 by those; 8 x 2048 of 2048 71, 84; 8 x 4096 136, 134.)
+constexpr int kCvGradPiece = 2;
+static int64_t cv_grad_grid(CvArgs &a) { return cv_grid(a, a.dim < kCvGradPiece ? 1 : kCvGradPiece, 64, 8, 131072); }
 
 // Offsets of a tensor of these strides, and of a dense one, are below 4 GB from the first row's (a row before it and chunks behind the last among them)
 static bool cv_near(const CvArgs &a, int64_t size, int64_t batch, int64_t token) {
@@ -433,12 +454,16 @@ extern "C" int ss2d_causal_conv_fwd(const ss2d_causal_conv_params *params, void 
         constexpr int kW = decltype(width)::value, kV = 16 / (int)sizeof(T);
         if (a.tokens == 0) return cv_copy<T>(a.initial, a.final, (int64_t)a.n_seqs * (kW - 1) * a.dim, st);
         if (!a.x || !a.weight || !a.out) return (int)SS2D_EINVAL;
-        const int64_t wgs = cv_grid(a, a.dim < kV ? 1 : kV, 32, 4, 262144);
+        const bool few = (int64_t)a.batch * a.tokens * a.dim <= kCvFew;
+        const int v = a.dim < kV ? 1 : few ? 2 : kV;
+        const int64_t wgs = cv_grid(a, v, few ? kCvFewRows : 32, 4, 262144);
         if (wgs < 0) return (int)SS2D_ENOTSUP;
         a.near = cv_near(a, sizeof(T), a.x_b, a.x_t);
-        if (a.dim < kV) cv_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else if (a.near) cv_kernel<T, kW, kV, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else cv_kernel<T, kW, kV, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        if (v == 1) cv_kernel<T, kW, 1, false, kCvRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (a.near && few) cv_kernel<T, kW, 2, true, kCvFewRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (a.near) cv_kernel<T, kW, kV, true, kCvRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (few) cv_kernel<T, kW, 2, false, kCvFewRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else cv_kernel<T, kW, kV, false, kCvRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
         return launch_status();
     });
 }
@@ -448,7 +473,7 @@ extern "C" int64_t ss2d_causal_conv_bwd_workspace_bytes(const ss2d_causal_conv_b
     const int rc = cv_read(params ? &params->fwd : nullptr, a);
     if (rc != SS2D_OK) return rc;
     if (a.dim == 0 || a.batch == 0 || a.tokens == 0) return 0;
-    const int64_t wgs = cv_grad_grid(a, params->fwd.dtype == SS2D_F32 ? 4 : 2);
+    const int64_t wgs = cv_grad_grid(a);
     return wgs < 0 ? (int64_t)SS2D_ENOTSUP : wgs / a.piece_blocks * (params->fwd.width + 1) * a.dim * 4;
 }
 
@@ -462,7 +487,7 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
     const int width = params->fwd.width;
     return cv_with(params->fwd.dtype, width, [&](auto t, auto w) {
         using T = decltype(t);
-        constexpr int kW = decltype(w)::value, kV = 16 / (int)sizeof(T);
+        constexpr int kW = decltype(w)::value;
         const bool wide = params->fwd.weight_dtype == SS2D_F32;
         if (a.batch == 0 || a.tokens == 0) {                         // no tokens: the weights' gradients are zeros, the state's what came in
             int status = wide ? cv_copy<float>(nullptr, params->dweight, (int64_t)a.dim * kW, st) : cv_copy<T>(nullptr, params->dweight, (int64_t)a.dim * kW, st);
@@ -470,16 +495,16 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
             return status != SS2D_OK ? status : cv_copy<T>(a.dfinal, a.dinitial, (int64_t)a.n_seqs * (kW - 1) * a.dim, st);
         }
         if (!a.x || !a.weight || !a.dout || !a.dx) return (int)SS2D_EINVAL;
-        const int64_t wgs = cv_grad_grid(a, sizeof(T));
+        const int64_t wgs = cv_grad_grid(a);
         if (wgs < 0) return (int)SS2D_ENOTSUP;
         const int64_t parts = wgs / a.piece_blocks;
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return (int)SS2D_EINVAL;
         if (workspace_bytes < parts * (kW + 1) * a.dim * 4) return (int)SS2D_ENOMEM;
         a.sums = (float *)workspace;
         a.near = cv_near(a, sizeof(T), a.x_b, a.x_t) && cv_near(a, sizeof(T), a.do_b, a.do_t);
-        if (a.dim < kV) cv_grad_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else if (a.near) cv_grad_kernel<T, kW, kV, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else cv_grad_kernel<T, kW, kV, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        if (a.dim < kCvGradPiece) cv_grad_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (a.near) cv_grad_kernel<T, kW, kCvGradPiece, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else cv_grad_kernel<T, kW, kCvGradPiece, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
         if (params->dweight || params->dbias) {
             const dim3 grid((a.dim + kWave - 1) / kWave, kW + 1);
             if (wide) cv_sum_kernel<float><<<grid, kBlock, 0, st>>>(a.sums, (float *)params->dweight, (float *)params->dbias, a.dim, kW, parts);
