@@ -778,7 +778,7 @@ int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *params, void *
  *   outside 0 .. seqlen are moved into it; what descending ones leave in the results is not defined (nothing outside the tensors is touched).  Rows of no
  *   sequence get zeros.
  *   initial_state, final_state (n_seqs or batch, dim, dstate) fp32, dense, either or both NULL; of a sequence without tokens the final state is the initial one.
- *   kept_states NULL or ss2d_token_scan_kept_states(params) floats: the states before every 64th token, which the gradients start from.
+ *   kept_states NULL or ss2d_token_scan_kept_states(params) floats: the states before every 16th token (dstate to 16; to 32: every 32nd; more: every 64th), which the gradients start from.
  *   out (batch, seqlen, dim) dtype, dense.
  * dstate up to 64 (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
  */

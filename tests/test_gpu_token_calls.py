@@ -573,3 +573,17 @@ def test_a_mixers_prompt_and_tokens(dtype):
             torch.cuda.synchronize()
             for i, n in enumerate(lengths):
                 assert bool(((got[i] - whole[i][n + t]).float().abs() <= bound * whole[i].float().abs().max()).all()), (t, i)
+
+
+@pytest.mark.parametrize("name", ["scan", "conv"])
+def test_more_places_than_half_of_what_32_bits_count(name):
+    """Over 2^30 sequences of which the last two have tokens: as those two alone."""
+    op = Op(name, 1, 90, F32, state=False, cu=[0, 40, 90])
+    many = torch.zeros(2 ** 30 + 101, dtype=torch.int32, device=DEV)
+    many[-2], many[-1] = 40, 90
+    found = []
+    for cu in (op.cu, many):
+        leaves = {n: t for n, t in op.leaves().items() if t is not None}
+        out = selective_scan_tokens_fn(**leaves, cu_seqlens=cu) if name == "scan" else causal_conv_fn(**leaves, activation="silu", cu_seqlens=cu)
+        found.append({"out": out.detach(), **dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), op.douts[0])))})
+    same(*found)

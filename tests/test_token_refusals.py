@@ -253,7 +253,7 @@ def test_convolutions_of_bad_arguments():
         assert L.ss2d_causal_conv_bwd_workspace_bytes(back(make(**change))) == _lib.SS2D_EINVAL
     for change in (dict(x=None), dict(weight=None), dict(out=None)):
         assert L.ss2d_causal_conv_fwd(make(**change), None) == _lib.SS2D_EINVAL, change
-    for change in (dict(width=1), dict(width=5), dict(seqlen=2 ** 31 - 1), dict(batch=2 ** 31 - 1, dim=2 ** 20)):
+    for change in (dict(width=1), dict(width=5), dict(seqlen=2 ** 31 - 1), dict(batch=2 ** 31 - 1, dim=2 ** 20), dict(dim=2 ** 30 + 1)):
         assert L.ss2d_causal_conv_fwd(make(**change), None) == L.ss2d_causal_conv_bwd(back(make(**change)), HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP, change
     need = L.ss2d_causal_conv_bwd_workspace_bytes(back(make()))
     assert need >= 5 * 64 * 4
@@ -267,7 +267,8 @@ def test_convolutions_of_bad_arguments():
                                                                       state_batch_stride=192) | change))
     for change in (dict(batch=-1), dict(dim=-1), dict(dtype=5), dict(weight_dtype=_lib.SS2D_BF16), dict(x=None), dict(weight=None), dict(state=None), dict(out=None), dict(state_batch_stride=191)):
         assert L.ss2d_causal_conv_step(step(**change), None) == _lib.SS2D_EINVAL, change
-    assert L.ss2d_causal_conv_step(step(width=5), None) == _lib.SS2D_ENOTSUP and L.ss2d_causal_conv_step(step(batch=0, x=None), None) == _lib.SS2D_OK
+    assert L.ss2d_causal_conv_step(step(width=5), None) == L.ss2d_causal_conv_step(step(dim=2 ** 30 + 1, state_batch_stride=1 << 40), None) == _lib.SS2D_ENOTSUP
+    assert L.ss2d_causal_conv_step(step(batch=0, x=None), None) == _lib.SS2D_OK
 
 
 def test_norms_of_bad_arguments():

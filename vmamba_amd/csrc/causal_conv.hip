@@ -2,7 +2,9 @@
 //     y_t = act(bias + sum_j w_j x_(t - W + 1 + j)),   act = SiLU or none; what is before a sequence's first token is its state, the last W - 1 inputs.
 // With g_t = dout_t act'(..):   dx_t = sum_j w_j g_(t + W - 1 - j),   dw_j = sum over t of g_t x_(t - W + 1 + j),   dbias = sum g.
 //
-// Memory bounds it.  A thread takes the channels of one 16-byte piece and walks a strip of tokens with the window in registers; rows are
+// Memory bounds it: 8 x 4096 tokens of 2048 channels in bf16 61 us (4.4 TB/s; a strip of 32 tokens 65, of 128 67), their gradients 90 (4.5 TB/s) and 6 for the sums over strips;
+// from the caches, which hold half of it, 46 and 83.
+// A thread takes the channels of one 16-byte piece (of few tokens: two channels) and walks a strip of tokens with the window in registers; rows are
 // loaded a chunk at a time, all on their way at once.  Threads side by side have neighbouring pieces, strips below each other.  The last
 // piece of a row ends with it, so that it may repeat channels of the one before: both write the same values.
 #include "row_piece.h"
@@ -87,7 +89,7 @@ template <typename T, int kV> __device__ __forceinline__ void cv_copy_row(const 
 
 constexpr int kCvRows = 8;           // rows of a chunk
 // Values of a forward below which a thread takes two channels and four rows: its instructions are a quarter, and where every wavefront runs once, fetching them is what
-// it waits for.  37 tokens of 1024 channels 5.4 -> 3.3 us, 8 x 512 of 2048 (2^23) 11.5 -> 11.1; twice as many 14.2, and 19.1 by that form.
+// it waits for.  37 tokens of 1024 channels 5.1 -> 3.0 us, 8 x 512 of 2048 (2^23) 14.5 -> 12.7; twice as many 18.4, and 23.2 by that form.
 constexpr int64_t kCvFew = 1 << 23;
 constexpr int kCvFewRows = 4;
 
@@ -118,9 +120,9 @@ template <typename T, int kW, int kV, bool kNear, int kRows> __global__ __launch
     float w[kW][kV], bias[kV];
     bool read = false;
     if (p.cu && p.final)                                             // sequences without tokens, dealt out over the strips
-        for (int i = c.strip; i < p.n_seqs; i += p.strips)
+        for (uint32_t i = c.strip; i < (uint32_t)p.n_seqs; i += p.strips)
             if (min(max(p.cu[i + 1], 0), p.tokens) <= min(max(p.cu[i], 0), p.tokens))
-                for (int r = 0; r < kW - 1; ++r) cv_copy_row<T, kV>(p.initial ? (const T *)p.initial + i * state + r * p.dim + c.d : nullptr, final + i * state + r * p.dim);
+                for (int r = 0; r < kW - 1; ++r) cv_copy_row<T, kV>(p.initial ? (const T *)p.initial + i * state + r * (int64_t)p.dim + c.d : nullptr, final + i * state + r * (int64_t)p.dim);
     for (int a = c.t0; a < c.t1;) {
         const TsSpan sp = ts_span_at(p.cu, p.n_seqs, p.tokens, c.b, a);
         const int e = min(sp.hi, c.t1);
@@ -200,10 +202,10 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
 #pragma unroll
         for (int i = 0; i < kV; ++i) dw[j][i] = 0.0f;
     if (c.there && p.cu && p.dinitial)
-        for (int i = c.strip; i < p.n_seqs; i += p.strips)
+        for (uint32_t i = c.strip; i < (uint32_t)p.n_seqs; i += p.strips)
             if (min(max(p.cu[i + 1], 0), p.tokens) <= min(max(p.cu[i], 0), p.tokens))
                 for (int r = 0; r < kW - 1; ++r)
-                    cv_copy_row<T, kV>(p.dfinal ? (const T *)p.dfinal + i * state + r * p.dim + c.d : nullptr, (T *)p.dinitial + i * state + r * p.dim + c.d);
+                    cv_copy_row<T, kV>(p.dfinal ? (const T *)p.dfinal + i * state + r * (int64_t)p.dim + c.d : nullptr, (T *)p.dinitial + i * state + r * (int64_t)p.dim + c.d);
     for (int a = c.t0; c.there && a < c.t1;) {
         const TsSpan sp = ts_span_at(p.cu, p.n_seqs, p.tokens, c.b, a);
         const int e = min(sp.hi, c.t1);
@@ -394,7 +396,7 @@ static int cv_read(const ss2d_causal_conv_params *p, CvArgs &a) {
     if (!p || p->batch < 0 || p->seqlen < 0 || p->dim < 0 || p->n_seqs < 0) return SS2D_EINVAL;
     if (p->dtype < SS2D_F32 || p->dtype > SS2D_F16 || (p->weight_dtype != SS2D_F32 && p->weight_dtype != p->dtype)) return SS2D_EINVAL;
     if (p->cu_seqlens && (p->batch != 1 || p->n_seqs < 1)) return SS2D_EINVAL;
-    if (p->width < 2 || p->width > 4 || p->seqlen > INT32_MAX - 256) return SS2D_ENOTSUP;
+    if (p->width < 2 || p->width > 4 || p->seqlen > INT32_MAX - 256 || p->dim > 1 << 30) return SS2D_ENOTSUP;
     a.x = p->x; a.weight = p->weight; a.bias = p->bias; a.initial = p->initial_state; a.cu = p->cu_seqlens; a.out = p->out; a.final = p->final_state;
     a.x_b = p->x_batch_stride; a.x_t = p->x_token_stride;
     a.batch = p->batch; a.tokens = p->seqlen; a.dim = p->dim; a.n_seqs = p->cu_seqlens ? p->n_seqs : p->batch; a.silu = p->silu != 0;
@@ -416,10 +418,11 @@ static int64_t cv_grid(CvArgs &a, int v, int longest, int least, int64_t enough)
     const int64_t wgs = ((int64_t)a.batch * a.strips + rows - 1) / rows * a.piece_blocks;
     return wgs > kTsLaunch / kBlock ? -1 : wgs;
 }
-// The gradients: two channels to a thread at any size.  (16-byte pieces, which the forward takes, need a quarter of the threads, but four times the registers and instructions:
-// 37 tokens of 1024 channels, forward and gradients, 12.9 us, 18.3 by those; 8 x 2048 of 2048 71, 84; 8 x 4096 136, 134.)
-constexpr int kCvGradPiece = 2;
-static int64_t cv_grad_grid(CvArgs &a) { return cv_grid(a, a.dim < kCvGradPiece ? 1 : kCvGradPiece, 64, 8, 131072); }
+// The gradients' likewise: 37 tokens of 1024 channels, forward and gradients, 17.3 -> 11.9 us, 2 x 1024 of 2048 (2^22) 27.5 -> 25.0, 8 x 512 (2^23) 38.2 and 38.0,
+// 8 x 4096 157 and 170 by two channels.  Strips: twice the threads take 8 x 2048 from 102 to 91 us, strips of 8 tokens, whose ends are read twice, 4 x 4096 of 1001 channels from 69 to 84.
+static bool cv_few(const CvArgs &a) { return (int64_t)a.batch * a.tokens * a.dim <= kCvFew; }
+static int cv_grad_vec(const CvArgs &a, int size) { return a.dim < 16 / size ? 1 : cv_few(a) ? 2 : 16 / size; }
+static int64_t cv_grad_grid(CvArgs &a, int size) { return cv_grid(a, cv_grad_vec(a, size), 64, cv_few(a) ? 8 : 16, 131072); }
 
 // Offsets of a tensor of these strides, and of a dense one, are below 4 GB from the first row's (a row before it and chunks behind the last among them)
 static bool cv_near(const CvArgs &a, int64_t size, int64_t batch, int64_t token) {
@@ -454,9 +457,9 @@ extern "C" int ss2d_causal_conv_fwd(const ss2d_causal_conv_params *params, void 
         constexpr int kW = decltype(width)::value, kV = 16 / (int)sizeof(T);
         if (a.tokens == 0) return cv_copy<T>(a.initial, a.final, (int64_t)a.n_seqs * (kW - 1) * a.dim, st);
         if (!a.x || !a.weight || !a.out) return (int)SS2D_EINVAL;
-        const bool few = (int64_t)a.batch * a.tokens * a.dim <= kCvFew;
+        const bool few = cv_few(a);
         const int v = a.dim < kV ? 1 : few ? 2 : kV;
-        const int64_t wgs = cv_grid(a, v, few ? kCvFewRows : 32, 4, 262144);
+        const int64_t wgs = cv_grid(a, v, few ? kCvFewRows : 64, 4, few ? 262144 : 131072);
         if (wgs < 0) return (int)SS2D_ENOTSUP;
         a.near = cv_near(a, sizeof(T), a.x_b, a.x_t);
         if (v == 1) cv_kernel<T, kW, 1, false, kCvRows><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
@@ -473,7 +476,7 @@ extern "C" int64_t ss2d_causal_conv_bwd_workspace_bytes(const ss2d_causal_conv_b
     const int rc = cv_read(params ? &params->fwd : nullptr, a);
     if (rc != SS2D_OK) return rc;
     if (a.dim == 0 || a.batch == 0 || a.tokens == 0) return 0;
-    const int64_t wgs = cv_grad_grid(a);
+    const int64_t wgs = cv_grad_grid(a, params->fwd.dtype == SS2D_F32 ? 4 : 2);
     return wgs < 0 ? (int64_t)SS2D_ENOTSUP : wgs / a.piece_blocks * (params->fwd.width + 1) * a.dim * 4;
 }
 
@@ -487,7 +490,7 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
     const int width = params->fwd.width;
     return cv_with(params->fwd.dtype, width, [&](auto t, auto w) {
         using T = decltype(t);
-        constexpr int kW = decltype(w)::value;
+        constexpr int kW = decltype(w)::value, kV = 16 / (int)sizeof(T);
         const bool wide = params->fwd.weight_dtype == SS2D_F32;
         if (a.batch == 0 || a.tokens == 0) {                         // no tokens: the weights' gradients are zeros, the state's what came in
             int status = wide ? cv_copy<float>(nullptr, params->dweight, (int64_t)a.dim * kW, st) : cv_copy<T>(nullptr, params->dweight, (int64_t)a.dim * kW, st);
@@ -495,16 +498,17 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
             return status != SS2D_OK ? status : cv_copy<T>(a.dfinal, a.dinitial, (int64_t)a.n_seqs * (kW - 1) * a.dim, st);
         }
         if (!a.x || !a.weight || !a.dout || !a.dx) return (int)SS2D_EINVAL;
-        const int64_t wgs = cv_grad_grid(a);
+        const int64_t wgs = cv_grad_grid(a, sizeof(T));
         if (wgs < 0) return (int)SS2D_ENOTSUP;
         const int64_t parts = wgs / a.piece_blocks;
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return (int)SS2D_EINVAL;
         if (workspace_bytes < parts * (kW + 1) * a.dim * 4) return (int)SS2D_ENOMEM;
         a.sums = (float *)workspace;
         a.near = cv_near(a, sizeof(T), a.x_b, a.x_t) && cv_near(a, sizeof(T), a.do_b, a.do_t);
-        if (a.dim < kCvGradPiece) cv_grad_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else if (a.near) cv_grad_kernel<T, kW, kCvGradPiece, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
-        else cv_grad_kernel<T, kW, kCvGradPiece, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        const int v = cv_grad_vec(a, sizeof(T));
+        if (v == 1) cv_grad_kernel<T, kW, 1, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else if (v == 2) a.near ? cv_grad_kernel<T, kW, 2, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a) : cv_grad_kernel<T, kW, 2, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
+        else a.near ? cv_grad_kernel<T, kW, kV, true><<<(uint32_t)wgs, kBlock, 0, st>>>(a) : cv_grad_kernel<T, kW, kV, false><<<(uint32_t)wgs, kBlock, 0, st>>>(a);
         if (params->dweight || params->dbias) {
             const dim3 grid((a.dim + kWave - 1) / kWave, kW + 1);
             if (wide) cv_sum_kernel<float><<<grid, kBlock, 0, st>>>(a.sums, (float *)params->dweight, (float *)params->dbias, a.dim, kW, parts);
@@ -517,7 +521,7 @@ extern "C" int ss2d_causal_conv_bwd(const ss2d_causal_conv_bwd_params *params, v
 extern "C" int ss2d_causal_conv_step(const ss2d_causal_conv_step_params *p, void *stream) {
     if (!p || p->batch < 0 || p->dim < 0) return SS2D_EINVAL;
     if (p->dtype < SS2D_F32 || p->dtype > SS2D_F16 || (p->weight_dtype != SS2D_F32 && p->weight_dtype != p->dtype)) return SS2D_EINVAL;
-    if (p->width < 2 || p->width > 4) return SS2D_ENOTSUP;
+    if (p->width < 2 || p->width > 4 || p->dim > 1 << 30) return SS2D_ENOTSUP;
     if (p->batch == 0 || p->dim == 0) return SS2D_OK;
     if (!p->x || !p->weight || !p->state || !p->out) return SS2D_EINVAL;
     if (p->batch > 1 && p->state_batch_stride < (int64_t)(p->width - 1) * p->dim) return SS2D_EINVAL;

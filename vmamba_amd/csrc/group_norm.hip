@@ -8,6 +8,8 @@
 //   slices  larger ones: a workgroup takes a slice of the positions for a bundle of whole groups (or a part of a wide one), channels side by side, so that rows are
 //           read whole however narrow the groups; statistics first (each channel's running mean and squares about it, joined by rows, channels and slices:
 //           no squares of what is not centred), then the values, which the caches still hold.
+// 8192 rows of 2048 channels, 16 groups, bf16: 16 us, gradients 20 (5 TB/s) and 6 for the weights' sums.  32 maps of 56 x 56 x 192, 32 groups, fp16: statistics 10.5 and
+// values 15.5 us, of one chunk of rows to each of 1280 workgroups: a launch, one latency and the copy's time each (7 and 10).
 #include "row_piece.h"
 
 namespace ss2d {
@@ -275,7 +277,7 @@ template <int kV> __device__ __forceinline__ GnPlace gn_place(const GnArgs &p) {
         q.g0 = q.bundle * p.bundle_groups; q.k = min(p.bundle_groups, p.groups - q.g0);
         q.c0 = q.g0 * p.cg; q.width = q.k * p.cg;
     }
-    q.begin = q.slice * p.slice; q.end = min(q.begin + p.slice, p.positions);
+    q.begin = q.slice * p.slice; q.end = q.begin + min(p.slice, p.positions - q.begin);
     q.piece = (int)threadIdx.x % p.cols; q.row = (int)threadIdx.x / p.cols; q.rows = kBlock / p.cols;
     q.there = q.piece * kV < q.width && q.row < q.rows;
     q.c = max(min(q.piece * kV, q.width - kV), 0);                   // inside the bundle

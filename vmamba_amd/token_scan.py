@@ -200,7 +200,8 @@ def selective_scan_tokens_fn(u, delta, A, B, C, D=None, z=None, delta_bias=None,
     initial_state (sequences, dim, dstate) float32.
 
     Returns out (batch, tokens, dim) in u's dtype, with ``output_final_state`` (out, final_state): the states behind the last tokens, float32, which
-    selective_scan_step_fn carries on.  States and sums are float32; recorded for gradients the call keeps the state before every 64th token.
+    selective_scan_step_fn carries on.  States and sums are float32; recorded for gradients the call keeps the states before
+    every 16th token (dstate up to 16; 32nd up to 32, else 64th): 4 bytes for each token and channel.
 
     Differentiable once.  Captured into a graph with gradients, its leaves may belong to no autograd graph that was recorded on another stream and still lives."""
     _check(isinstance(u, torch.Tensor) and u.is_cuda, "u must be a GPU tensor: vmamba_amd has no CPU path")
