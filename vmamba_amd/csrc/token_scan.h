@@ -199,6 +199,15 @@ template <int kSets> __device__ __forceinline__ void ts_sum_sets(float (&v)[16])
     }
 }
 
+// Wavefronts of a SIMD that walk as far keep together: the oldest would run ahead and leave the last ones a SIMD that they cannot fill.  The nearer the end,
+// the lower the priority: in the first half, to three quarters, seven eighths, behind.
+__device__ __forceinline__ void ts_keep_together(int left, int of) {
+    if (2 * left > of) __builtin_amdgcn_s_setprio(3);
+    else if (4 * left > of) __builtin_amdgcn_s_setprio(2);
+    else if (8 * left > of) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+}
+
 __device__ __forceinline__ float ts_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
 
 }  // namespace ss2d

@@ -135,6 +135,7 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
     request(t, end);
     for (;;) {
         const int n = end - t;
+        ts_keep_together(s1 - t, s1 - s0);
         // ---- stage -----------------------------------------------------------------------------------------------------------
         float extra[L::kRounds][4], gate[L::kRounds][4];
         auto stage = [&](auto all) {                                 // all: 16 tokens, every lane's channels and states there

@@ -106,6 +106,7 @@ __global__ __launch_bounds__(kBlock, 3) void ts_left_kernel(const TsBwdArgs q) {
     request(t, e);
     for (;;) {
         const int n = e - t;
+        ts_keep_together(e - s0, s1 - s0);
 #pragma unroll
         for (int r = 0; r < L::kRounds; ++r) {
             const int k = r * L::kRows + l.row;
@@ -350,6 +351,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
     for (int turn = 0;; turn ^= kTurns - 1) {
         const int a = now.a, e = now.e;
         const TsSpan sp = now.sp;
+        ts_keep_together(e - s0, s1 - s0);
         const bool more = a > s0;
         TsPiece next = now;
         if (more) next = piece_before(a);
