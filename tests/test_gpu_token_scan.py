@@ -261,3 +261,19 @@ def test_packed_where_lanes_are_full(N):
         check(name, got[name], want[name], size[name], args, pieces)
     for name in ("out", "du", "ddelta", "dz", "dB", "dC"):
         assert not got[name][0, :1].any() and not got[name][0, starts[-1]:].any(), name
+
+
+@pytest.mark.parametrize("shape,lengths", [((4, 512, 2048, 16, 1), None), ((4, 601, 1024, 8, 2), None), ((1, 2400, 2048, 16, 1), [700, 1, 0, 95, 160, 900, 444]), ((2, 700, 1100, 16, 1), None),
+                                           ((1, 1500, 2048, 32, 1), [640, 860])], ids=str)
+def test_what_segments_hand_back_from_shorter_ones(shape, lengths):
+    """Sizes at which what is handed from behind is found from shorter segments than the gradients' own."""
+    print("CASE token_scan handed back", shape, lengths, flush=True)
+    B, T = shape[:2]
+    starts = None if lengths is None else [50 + sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    pieces = [(b, 0, T) for b in range(B)] if starts is None else [(0, lo, lo + n) for lo, n in zip(starts, lengths)]
+    args, dout, dfinal, _ = inputs(*shape, BF16, T, n_seqs=len(pieces))
+    args["A"] = 0.02 * args["A"]                                     # (decays slow enough that a segment hands on what came in)
+    got = run_all(args, dout, dfinal, None if starts is None else torch.tensor(starts, dtype=torch.int32, device=DEV))
+    want, size = reference(args, pieces, dout, dfinal)
+    for name in got:
+        check(name, got[name], want[name], size[name], args, pieces)

@@ -63,8 +63,11 @@ struct TsBwdArgs {
     void *du, *ddelta, *dz;
     float *dinitial;
     int64_t do_b, do_t;
-    float *left, *gsums, *behind;    // as end, sums and enter, the other way: of every segment but the first
+    // what is handed from behind is found from shorter segments, `each` of them to one of the gradients': of the `slots` of them behind the first `each`, as end, sums, enter
+    // and flags, the other way
+    float *left, *gsums, *behind;
     int32_t *gflags;
+    int32_t each, slots, left_wgs;   // left_wgs: their workgroups to a group
     float *pBC;                      // [workgroup of a group][batch][token][group][state][B, C]: sums over a workgroup's channels
     float *pA;                       // [batch][segment][channel][state]
     float *pD;                       // [batch][segment][D, bias][channel]

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kBlock, 3) void ts_left_kernel(const TsBwdArgs q) {
     uint32_t id = xcd_contiguous_id(blockIdx.x, gridDim.x);
     const int wg = (int)(id % (uint32_t)p.wgs); id /= (uint32_t)p.wgs;
     const int g = (int)(id % (uint32_t)p.groups); id /= (uint32_t)p.groups;
-    const int segs = p.n_segs - 1, seg = (int)(id % (uint32_t)segs) + 1, b = (int)(id / (uint32_t)segs);
+    const int segs = q.slots, seg = (int)(id % (uint32_t)segs) + q.each, b = (int)(id / (uint32_t)segs);
     const int first = (wg * kWavesPerWg + wave) * L::kCh, n_chan = min(L::kCh, p.per_group - first);
     if (n_chan <= 0) return;
     const int c0 = g * p.per_group + first, s0 = seg * p.seg_len, s1 = s0 + min(p.seg_len, p.tokens - s0);
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kBlock, 3) void ts_left_kernel(const TsBwdArgs q) {
     const int mine = kQuick ? 4 : min(max(n_chan - l.at, 0), 4), at = mine > 0 ? l.at : 0, d = c0 + (kQuick ? l.chan : min(l.chan, n_chan - 1));
     const TsSpan sp = ts_span_at(p.cu, p.n_seqs, p.tokens, b, s0);
     const int carry = sp.seq < 0 || sp.lo >= s0 ? kTsNothing : sp.hi <= s1 ? kTsStarts : kTsThrough;
-    const int64_t slot = (int64_t)b * segs + seg - 1;
+    const int64_t slot = (int64_t)b * segs + seg - q.each;
     if (wg == 0 && g == 0 && threadIdx.x == 0) q.gflags[slot] = carry;
     if (carry == kTsNothing) return;
 
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kBlock, 3) void ts_left_kernel(const TsBwdArgs q) {
 static __global__ __launch_bounds__(kBlock) void ts_join_left_kernel(const TsBwdArgs q, uint32_t per_row) {
     const TsArgs &p = q.f;
     const uint32_t item = blockIdx.x * kBlock + threadIdx.x;
-    const int b = (int)blockIdx.y, segs = p.n_segs - 1;
+    const int b = (int)blockIdx.y, segs = q.slots;
     if (item >= per_row) return;
     const uint32_t d = item / (uint32_t)p.N;
     const float A2 = 0.5f * kLog2e * p.A[item];
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
         }
         if (works) {
             if (e == sp.hi) ts_read_state<kSets, kM>(of_seq(q.dfinal, sp.seq), N, l, there, ga);
-            else if (e == s1) ts_read_state<kSets, kM>(q.behind + (((int64_t)b * (p.n_segs - 1) + seg) * p.dim + d) * N, N, l, there, ga);
+            else if (e == s1) ts_read_state<kSets, kM>(q.behind + (((int64_t)b * q.slots + seg * q.each) * p.dim + d) * N, N, l, there, ga);
             const int low = tile_of(a), high = tile_of(e - 1);
             floatx4_t h[kM];
 #pragma unroll
@@ -641,9 +641,10 @@ template <typename T> int ts_bwd_run(const ss2d_token_scan_bwd_params *p, const 
         constexpr int kSets = decltype(sets)::value, kM = decltype(m)::value;
         constexpr bool kQuick = decltype(quick)::value, kPacked = decltype(packed)::value;
         if (a.n_segs > 1) {
-            TsBwdArgs left = q;                                      // (its workgroups are of four wavefronts always)
-            left.f.wgs = (a.per_group + kWave / kSets * kWavesPerWg - 1) / (kWave / kSets * kWavesPerWg);
-            ts_left_kernel<T, kSets, kM, kQuick><<<(uint32_t)(a.batch * a.groups * left.f.wgs * (a.n_segs - 1)), kBlock, 0, st>>>(left);
+            TsBwdArgs left = q;
+            left.f.wgs = q.left_wgs;
+            left.f.seg_len = a.seg_len / q.each;
+            ts_left_kernel<T, kSets, kM, kQuick><<<(uint32_t)(a.batch * a.groups * q.left_wgs * q.slots), kBlock, 0, st>>>(left);
             const uint32_t per_row = (uint32_t)a.dim * a.N;
             ts_join_left_kernel<<<dim3((per_row + kBlock - 1) / kBlock, a.batch), kBlock, 0, st>>>(q, per_row);
         }

@@ -31,6 +31,13 @@ static int ts_bwd_read(const ss2d_token_scan_bwd_params *p, TsBwdArgs &q) {
     a.seg_len = ts_seg_len(a.tokens, n, a.keep);
     a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
     if (wgs * a.n_segs > kTsLaunch / kBlock || (a.n_segs > 1 && a.batch > 65535)) return SS2D_ENOTSUP;
+    // What is handed from behind keeps fewer registers: as many workgroups, of four wavefronts always, as come to four on a CU
+    const int left_ch = kWave / ts_sets(a.N) * kWavesPerWg;
+    q.left_wgs = (a.per_group + left_ch - 1) / left_ch;
+    const auto slots = [&](int each) { return (int)((a.tokens + (int64_t)a.seg_len / each - 1) / (a.seg_len / each)) - each; };
+    q.each = 1;
+    while (a.n_segs > 1 && a.seg_len % (2 * q.each * kTsTile) == 0 && a.seg_len / (2 * q.each) >= kTsGrid && (int64_t)a.batch * a.groups * q.left_wgs * slots(2 * q.each) <= 1024) q.each *= 2;
+    q.slots = a.n_segs > 1 ? slots(q.each) : 0;
     return SS2D_OK;
 }
 
@@ -38,7 +45,7 @@ static int64_t ts_bwd_carve(TsBwdArgs &q, uint8_t *base) {
     const TsArgs &a = q.f;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { uint8_t *p = base ? base + at : nullptr; at += (bytes + 255) / 256 * 256; return p; };
-    const int64_t cuts = (int64_t)a.batch * (a.n_segs - 1), parts = (int64_t)a.batch * a.n_segs, states = (int64_t)a.dim * a.N;
+    const int64_t cuts = (int64_t)a.batch * q.slots, parts = (int64_t)a.batch * a.n_segs, states = (int64_t)a.dim * a.N;
     q.left = (float *)take(cuts * states * 4);
     q.behind = (float *)take(cuts * states * 4);
     q.gsums = (float *)take(cuts * a.dim * 4);
