@@ -47,7 +47,7 @@ inline int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
 // Whole wavefronts of channels, states that fill their lanes, offsets inside a tile that fit 32 bits: the kernels without masks
 inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / ts_sets(a.N)) == 0 && (a.N == 4 || a.N == 8 || a.N == 16 || a.N == 32 || a.N == 64); }
 // Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th token
-// takes a quarter of the memory and the gradients a second walk over every piece: 310 us of their kernel, 4 x 2048 tokens of 2048 channels, where it is 278 now.)
+// takes a quarter of the memory and the gradients a second walk over every piece: 310 us of their kernel, 4 x 2048 tokens of 2048 channels, where it was 278.)
 inline int ts_keep(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 enum TsCarry { kTsNothing, kTsStarts, kTsThrough };                  // what a segment hands on: nothing, its last sequence began in it, it lies inside one
@@ -203,7 +203,8 @@ template <int kSets> __device__ __forceinline__ void ts_sum_sets(float (&v)[16])
 }
 
 // Wavefronts of a SIMD that walk as far keep together: the oldest would run ahead and leave the last ones a SIMD that they cannot fill.  The nearer the end,
-// the lower the priority: in the first half, to three quarters, seven eighths, behind.
+// the lower the priority: in the first half, to three quarters, seven eighths, behind.  32768 tokens 480 -> 430 us, 4 x 2048 with their gradients 480 -> 452; bounds nearer the end
+// (15/16, 31/32, 63/64) 467, quarters 447, a turn of four priorities every four tiles 437.
 __device__ __forceinline__ void ts_keep_together(int left, int of) {
     if (2 * left > of) __builtin_amdgcn_s_setprio(3);
     else if (4 * left > of) __builtin_amdgcn_s_setprio(2);

@@ -5,9 +5,9 @@
 // the lanes of the first kind, which add the skip term, apply the gate and store.  The next tile's loads are on their way meanwhile.  A wavefront meets no
 // other: no workgroup barrier.
 //
-// Vector instructions bound it: 416 for a tile of 4096 values of states, 64 of them exponentials at half rate, a SIMD issues one in 97 %
-// of the slots.  32768 tokens of 2048 channels, 16 states, bf16: 285 us, and 215 for what 31 of 32 segments leave (without the sums, gates and outputs, 284 a
-// tile); one pass over the states of the same length, without segments, would keep an eighth of the SIMDs busy.
+// Vector instructions bound it: 416 for a tile of 4096 values of states, 80 of them exponentials and the like of twice the time, 91 % of a SIMD's cycles.  32768 tokens of 2048
+// channels, 16 states, bf16: 257 us, and 190 for what 31 of 32 segments leave (without the sums, gates and outputs, 284 a tile); one pass over the states of the same
+// length, without segments, would keep an eighth of the SIMDs busy.  Where wavefronts run as they come the last ones end alone: 290 and 215 us (ts_keep_together).
 #include "token_scan.h"
 
 namespace ss2d {
