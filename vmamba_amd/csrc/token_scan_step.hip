@@ -97,7 +97,7 @@ using namespace ss2d;
 extern "C" int ss2d_token_scan_step(const ss2d_token_scan_step_params *p, void *stream) {
     if (!p || p->batch < 0 || p->dim < 0 || p->dstate < 1 || p->n_groups < 1 || p->dim % p->n_groups) return SS2D_EINVAL;
     if (p->dtype < SS2D_F32 || p->dtype > SS2D_F16) return SS2D_EINVAL;
-    if (p->dstate > kTsMaxState) return SS2D_ENOTSUP;
+    if (p->dstate > kTsMaxState || p->dim > INT32_MAX - kBlock) return SS2D_ENOTSUP;    // (a workgroup's last channels are counted in 32 bits)
     if (p->batch == 0 || p->dim == 0) return SS2D_OK;
     if (!p->u || !p->delta || !p->A || !p->B || !p->C || !p->state || !p->out) return SS2D_EINVAL;
     if (p->batch > 1 && p->state_batch_stride < (int64_t)p->dim * p->dstate) return SS2D_EINVAL;
