@@ -22,3 +22,14 @@ def test_a_step_of_more_channels_than_a_workgroup_rounds_up_to(dim, dtype, dstat
     """A workgroup takes up to 256 channels: within as many of 2^31 its last channel's index does not fit 32 bits."""
     p = fill(_lib.TokenScanStepParams(), batch=1, dim=dim, dstate=dstate, n_groups=1, dtype=dtype, u=256, delta=256, A=256, B=256, C=256, state=256, out=256)
     assert _lib.lib().ss2d_token_scan_step(p, None) == _lib.SS2D_ENOTSUP
+
+
+@pytest.mark.parametrize("sizes", [dict(batch=4, seqlen=16384, n_groups=4096, dim=4096, dstate=16), dict(batch=1, seqlen=2 ** 26, n_groups=1, dim=1, dstate=64), dict(batch=1, seqlen=1, n_groups=1, dim=1500000000, dstate=1)],
+                         ids=["2^32 values of B", "one channel", "values of A, D and the bias"])
+def test_gradients_whose_sums_are_more_than_a_launch_counts(sizes):
+    """The forward is taken; with states kept for gradients it says at once that there are none."""
+    L = _lib.lib()
+    p = fill(_lib.TokenScanParams(), **sizes, dtype=_lib.SS2D_BF16, delta_softplus=1, u=256, delta=256, A=256, B=256, C=256, out=256)
+    g = fill(_lib.TokenScanBwdParams(), fwd=fill(p, kept_states=256), dout=256, du=256, ddelta=256, dB=256, dC=256)
+    assert L.ss2d_token_scan_workspace_bytes(p) >= 0
+    assert L.ss2d_token_scan_kept_states(p) == L.ss2d_token_scan_bwd_workspace_bytes(g) == L.ss2d_token_scan_bwd(g, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP

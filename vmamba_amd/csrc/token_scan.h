@@ -50,6 +50,13 @@ inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / 
 // takes a quarter of the memory and the gradients a second walk over every piece: 310 us of their kernel, 4 x 2048 tokens of 2048 channels, where it was 278.)
 inline int ts_keep(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
+// The gradients' sums have a thread to a value of B, and one to a value of A, D and the bias: launches count them in 32 bits
+inline bool ts_sums_fit(const TsArgs &a) {
+    constexpr int64_t kMost = kTsLaunch / kBlock * kBlock;
+    const __int128 values = (__int128)a.batch * a.tokens * a.groups * a.N;
+    return values <= kMost && (int64_t)a.dim * (a.N + 2) <= kMost;
+}
+
 enum TsCarry { kTsNothing, kTsStarts, kTsThrough };                  // what a segment hands on: nothing, its last sequence began in it, it lies inside one
 
 // Wavefronts of a workgroup of the gradients' kernel: their states in LDS are 4 kM^2 KB each

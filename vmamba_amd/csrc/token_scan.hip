@@ -389,6 +389,7 @@ extern "C" int64_t ss2d_token_scan_workspace_bytes(const ss2d_token_scan_params 
 extern "C" int64_t ss2d_token_scan_kept_states(const ss2d_token_scan_params *params) {
     TsArgs a;
     const int rc = ts_read(params, a);
+    if (rc == SS2D_OK && !ts_sums_fit(a)) return SS2D_ENOTSUP;       // (said by the forward that keeps states, not by the gradients at last)
     return rc != SS2D_OK ? rc : (int64_t)a.batch * a.n_kept * a.dim * a.N;
 }
 

@@ -30,7 +30,7 @@ static int ts_bwd_read(const ss2d_token_scan_bwd_params *p, TsBwdArgs &q) {
     }
     a.seg_len = ts_seg_len(a.tokens, n, a.keep);
     a.n_segs = (int)((a.tokens + (int64_t)a.seg_len - 1) / a.seg_len);
-    if (wgs * a.n_segs > kTsLaunch / kBlock || (a.n_segs > 1 && a.batch > 65535)) return SS2D_ENOTSUP;
+    if (wgs * a.n_segs > kTsLaunch / kBlock || (a.n_segs > 1 && a.batch > 65535) || !ts_sums_fit(a)) return SS2D_ENOTSUP;
     // What is handed from behind keeps fewer registers: as many workgroups, of four wavefronts always, as come to four on a CU (4 x 2048 tokens of 2048 channels: 768 in place
     // of 384, 59 -> 42 us)
     const int left_ch = kWave / ts_sets(a.N) * kWavesPerWg;
