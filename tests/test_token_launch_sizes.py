@@ -33,3 +33,12 @@ def test_gradients_whose_sums_are_more_than_a_launch_counts(sizes):
     g = fill(_lib.TokenScanBwdParams(), fwd=fill(p, kept_states=256), dout=256, du=256, ddelta=256, dB=256, dC=256)
     assert L.ss2d_token_scan_workspace_bytes(p) >= 0
     assert L.ss2d_token_scan_kept_states(p) == L.ss2d_token_scan_bwd_workspace_bytes(g) == L.ss2d_token_scan_bwd(g, HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP
+
+
+def test_a_convolutions_gradients_of_more_channels_than_their_sums_launch_counts():
+    L = _lib.lib()
+    make = lambda dim: fill(_lib.CausalConvBwdParams(), fwd=fill(_lib.CausalConvParams(), batch=1, seqlen=1, dim=dim, width=2, dtype=_lib.SS2D_BF16, weight_dtype=_lib.SS2D_BF16, x=256,  # noqa: E731
+                                                                weight=256, out=256), dout=256, dx=256)
+    for dim in (2 ** 30, 2 ** 30 - 63):
+        assert L.ss2d_causal_conv_bwd_workspace_bytes(make(dim)) == L.ss2d_causal_conv_bwd(make(dim), HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP
+    assert L.ss2d_causal_conv_bwd_workspace_bytes(make(2 ** 30 - 64)) == 3 * (2 ** 30 - 64) * 4

@@ -422,7 +422,8 @@ static int64_t cv_grid(CvArgs &a, int v, int longest, int least, int64_t enough)
 // 8 x 4096 157 and 170 by two channels.  Strips: twice the threads take 8 x 2048 from 102 to 91 us, strips of 8 tokens, whose ends are read twice, 4 x 4096 of 1001 channels from 69 to 84.
 static bool cv_few(const CvArgs &a) { return (int64_t)a.batch * a.tokens * a.dim <= kCvFew; }
 static int cv_grad_vec(const CvArgs &a, int size) { return a.dim < 16 / size ? 1 : cv_few(a) ? 2 : 16 / size; }
-static int64_t cv_grad_grid(CvArgs &a, int size) { return cv_grid(a, cv_grad_vec(a, size), 64, cv_few(a) ? 8 : 16, 131072); }
+// (the weights' sums take four threads a channel, which a launch counts in 32 bits)
+static int64_t cv_grad_grid(CvArgs &a, int size) { return a.dim > kTsLaunch / kBlock * kWave ? -1 : cv_grid(a, cv_grad_vec(a, size), 64, cv_few(a) ? 8 : 16, 131072); }
 
 // Offsets of a tensor of these strides, and of a dense one, are below 4 GB from the first row's (a row before it and chunks behind the last among them)
 static bool cv_near(const CvArgs &a, int64_t size, int64_t batch, int64_t token) {
