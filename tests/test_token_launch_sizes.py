@@ -42,3 +42,14 @@ def test_a_convolutions_gradients_of_more_channels_than_their_sums_launch_counts
     for dim in (2 ** 30, 2 ** 30 - 63):
         assert L.ss2d_causal_conv_bwd_workspace_bytes(make(dim)) == L.ss2d_causal_conv_bwd(make(dim), HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP
     assert L.ss2d_causal_conv_bwd_workspace_bytes(make(2 ** 30 - 64)) == 3 * (2 ** 30 - 64) * 4
+
+
+@pytest.mark.parametrize("weights", [dict(dweight=256), dict(dbias=256), dict(dweight=256, dbias=256)], ids=lambda v: " and ".join(v))
+def test_a_norms_gradients_of_more_channels_than_their_sums_launch_counts(weights):
+    """Without its weights' gradients it is taken as before."""
+    L = _lib.lib()
+    make = lambda channels, **grads: fill(_lib.GroupNormBwdParams(), fwd=fill(_lib.GroupNormParams(), batch=1, positions=1, channels=channels, groups=channels // 64, dtype=_lib.SS2D_BF16,  # noqa: E731
+                                                                              weight_dtype=_lib.SS2D_BF16, eps=1e-5, x=256, out=256, stats=256), dout=256, dx=256, **grads)
+    most = 2 ** 28 - 64
+    assert L.ss2d_group_norm_bwd_workspace_bytes(make(most + 64, **weights)) == L.ss2d_group_norm_bwd(make(most + 64, **weights), HERE, 1 << 62, None) == _lib.SS2D_ENOTSUP
+    assert L.ss2d_group_norm_bwd_workspace_bytes(make(most, **weights)) == 8 * most and L.ss2d_group_norm_bwd_workspace_bytes(make(most + 64)) == 8 * (most + 64)

@@ -746,7 +746,9 @@ extern "C" int ss2d_group_norm_fwd(const ss2d_group_norm_params *params, void *w
     });
 }
 
-static int64_t gn_bwd_plan(const ss2d_group_norm_params *p, GnArgs &a, int &lanes, int &each) {
+static int64_t gn_bwd_plan(const ss2d_group_norm_bwd_params *params, GnArgs &a, int &lanes, int &each) {
+    const ss2d_group_norm_params *p = &params->fwd;
+    if ((params->dweight || params->dbias) && (a.channels + (int64_t)kWave - 1) / kWave > kGnLaunch / 1024) return SS2D_ENOTSUP;       // (more channels than gn_sum_kernel's launch counts)
     const int v = gn_vec(a.cg, gn_size(p->dtype));
     if (a.positions == 1 && gn_unit(a, v, lanes, each)) {
         a.samples = gn_samples(a, lanes);
@@ -762,7 +764,7 @@ extern "C" int64_t ss2d_group_norm_bwd_workspace_bytes(const ss2d_group_norm_bwd
     const int rc = gn_read(params ? &params->fwd : nullptr, a);
     if (rc != SS2D_OK) return rc;
     int lanes, each;
-    return a.batch == 0 || a.positions == 0 ? 0 : gn_bwd_plan(&params->fwd, a, lanes, each);
+    return a.batch == 0 || a.positions == 0 ? 0 : gn_bwd_plan(params, a, lanes, each);
 }
 
 extern "C" int ss2d_group_norm_bwd(const ss2d_group_norm_bwd_params *params, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -788,7 +790,7 @@ extern "C" int ss2d_group_norm_bwd(const ss2d_group_norm_bwd_params *params, voi
     a.dout = params->dout; a.dx = params->dx; a.read_stats = (const float2 *)params->fwd.stats;
     if (!a.x || !a.dout || !a.dx || !a.read_stats) return SS2D_EINVAL;
     int lanes, each;
-    const int64_t need = gn_bwd_plan(&params->fwd, a, lanes, each);
+    const int64_t need = gn_bwd_plan(params, a, lanes, each);
     if (need < 0) return (int)need;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return SS2D_EINVAL;
     if (workspace_bytes < need) return SS2D_ENOMEM;
