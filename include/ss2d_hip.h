@@ -773,7 +773,7 @@ int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *params, void *
  * The recurrence of ss2d_selective_scan_fwd (classification/models/csms6s.py:29-68) for a language model's layout, with states that come in and go out.
  *   u, delta, z (batch, seqlen, dim): dtype, channels dense, other strides in elements; z NULL: no gate.
  *   B, C (batch, seqlen, n_groups, dstate): dtype, states dense; channel d belongs to group d / (dim / n_groups).
- *   A (dim, dstate), D (dim) or NULL (0), delta_bias (dim) or NULL (0): fp32, dense.
+ *   A (dim, dstate), D (dim) or NULL (no such term), delta_bias (dim) or NULL (0): fp32, dense.
  *   cu_seqlens NULL, or n_seqs + 1 ascending places (device memory): sequence i is tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of batch 1.  Places
  *   outside 0 .. seqlen are moved into it; what descending ones leave in the results is not defined (nothing outside the tensors is touched).  Rows of no
  *   sequence get zeros.

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                         step[i] = in ? step[i] : 0.0f;
                         uv[i] = in ? uv[i] : 0.0f;
                     }
-                    extra[r][i] = skip[i] * uv[i];
+                    extra[r][i] = p.D ? skip[i] * uv[i] : 0.0f;      // (without D no term: an infinite u would make 0 u of it)
                     if constexpr (kLocal) sum[i] += step[i];
                 }
                 float *to = s_step + k * L::kPairPitch + 2 * l.at;

@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                     for (int i = 0; i < 4; ++i) {
                         const float4 tok = *reinterpret_cast<const float4 *>(s_tok + k * kRow + 4 * (l.at + i));       // step, s, dy, u
                         uv[i] = tok.w;
-                        u_out[i] = fmaf(skip[i], tok.z, tok.x * tok.y);
+                        u_out[i] = p.D ? fmaf(skip[i], tok.z, tok.x * tok.y) : tok.x * tok.y;
                         d_out[i] = fmaf(kLn2, qv[i], tok.w * tok.y) * slope[r][i];
                         sum_bias[i] += d_out[i];
                         sum_D[i] = fmaf(tok.z, tok.w, sum_D[i]);
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                         const float4 y4 = *reinterpret_cast<const float4 *>(s_y + k * L::kPitch + l.at);
                         const float yv[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) u_out[i] = through[r][i] * fmaf(skip[i], uv[i], yv[i]);
+                        for (int i = 0; i < 4; ++i) u_out[i] = through[r][i] * (p.D ? fmaf(skip[i], uv[i], yv[i]) : yv[i]);
                         ts_store4<T, true>(row_of(dz), mine, whole, u_out);
                     }
                 }

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kBlock) void ts_step_kernel(const TsStepArgs p, uin
             for (int v = 0; v < 3; ++v)
                 if (n + v < p.N) to[n + v] = h[r][v];
         if (lane == 0) {
-            y = fmaf(skip, uv[r], y);
+            y = p.D ? fmaf(skip, uv[r], y) : y;
             ((T *)p.out)[(b0 + r) * p.dim + d] = from_f32<T>(p.z ? y * (zv[r] * ts_sigmoid(zv[r])) : y);
         }
     }
