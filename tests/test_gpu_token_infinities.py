@@ -110,6 +110,29 @@ def compare(args, dout, dfinal, lengths):
     return got, want, size, pieces
 
 
+# (sequence, token, channel) of the infinite value, and tokens: one walk of the token axis, several segments (of 16 channels and fewer from 256 tokens on), packed
+SIDES = {"results": ("out", "final"), "gradients": ("du", "ddelta", "dA", "dB", "dC", "dD", "dz", "ddelta_bias", "dstate")}
+LAYOUTS = {"short": (2, 45, 2, 1, 20, None), "cut": (1, 700, 1, 0, 333, None), "packed": (1, 420, 4, 2, 130, [70, 0, 309, 33])}
+STATES = [1, 3, 12, 16, 20, 50]
+
+
+@pytest.mark.parametrize("side,where", [("results", n) for n in ("u", "delta", "B", "C", "state")])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("N", STATES)
+def test_one_infinite_value(N, layout, side, where):
+    B, T, n_seqs, seq, t, lengths = LAYOUTS[layout]
+    print("CASE infinite", side, where, layout, N, flush=True)
+    dim = 5 if N != 16 else 16                                       # (lanes without channels, and none)
+    args, dout, dfinal = inputs(B, T, dim, N, 1, N, gate=True, extra=N % 2 == 0, state=True, n_seqs=n_seqs)
+    at = (seq if lengths is None else 0, t)
+    {"state": args["state"], "dfinal": dfinal}.get(where, dout if where == "dout" else args.get(where))[(seq, 2, N // 2) if where in ("state", "dfinal") else (*at, 0, N // 2) if where in ("B", "C") else (*at, 2)] = INF
+    got, want, size, pieces = compare(args, dout, dfinal, lengths)
+    assert any(not bool(want[name].isfinite().all()) for name in got if name in SIDES[side])
+    for name in got:
+        if name in SIDES[side]:
+            check(name, got[name], want[name], size[name], args, pieces)
+
+
 @pytest.mark.parametrize("gate", [True, False])
 @pytest.mark.parametrize("dim", [16, 64])
 def test_no_skip_term_is_no_term(dim, gate):

@@ -168,6 +168,12 @@ template <int kSets, int kM> struct TsLane {
 
 __device__ __forceinline__ floatx4_t ts_outer(float row, float col, floatx4_t c) { return __builtin_amdgcn_mfma_f32_4x4x1f32(row, col, c, 0, 0, 0); }
 
+// Values of a lane that stand for no state of a channel: cleared behind what the matrix instruction makes of them, 0 times a step u or a step that may be infinite
+template <int kSets, int kM> __device__ __forceinline__ void ts_clear_others(floatx4_t &v, int m, int N, const TsLane<kSets, kM> &l, bool there) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = there && l.state(m) + i < N ? v[i] : 0.0f;
+}
+
 // A channel's states of a lane from and to [channel][state] memory
 template <int kSets, int kM> __device__ __forceinline__ void ts_read_state(const float *from, int N, const TsLane<kSets, kM> &l, bool there, floatx4_t (&h)[kM]) {
     typedef float here __attribute__((ext_vector_type(4), aligned(4)));
