@@ -133,6 +133,22 @@ def test_one_infinite_value(N, layout, side, where):
             check(name, got[name], want[name], size[name], args, pieces)
 
 
+@pytest.mark.parametrize("side", ["results"])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("N", STATES)
+@pytest.mark.parametrize("dim,G", [(5, 1), (32, 2), (128, 1)], ids=str)
+def test_states_that_forget_at_once(dim, G, N, layout, side):
+    """A of -inf for two states, one of them of a last channel: a decay of 0, in tiles that sequences begin and end in as elsewhere."""
+    B, T, n_seqs, _, _, lengths = LAYOUTS[layout]
+    print("CASE forgets", dim, G, N, layout, flush=True)
+    args, dout, dfinal = inputs(B, T, dim, N, G, N + dim, gate=N != 12, extra=N % 2 == 0, state=True, n_seqs=n_seqs)
+    args["A"][dim // 2, 0] = args["A"][dim - 1, N - 1] = -INF
+    got, want, size, pieces = compare(args, dout, dfinal, lengths)
+    for name in got:
+        if name in SIDES[side]:
+            check(name, got[name], want[name], size[name], args, pieces)
+
+
 @pytest.mark.parametrize("gate", [True, False])
 @pytest.mark.parametrize("dim", [16, 64])
 def test_no_skip_term_is_no_term(dim, gate):
@@ -152,3 +168,17 @@ def test_no_skip_term_of_a_step():
     a["u"][1, 2] = INF
     out = selective_scan_step_fn(*(a[n] for n in ("u", "delta", "A", "B", "C")), a["state"], None, a["z"])
     assert out[1, 2] == INF and int(out.isfinite().sum()) == 11
+
+
+@pytest.mark.parametrize("extra", [True, False])
+@pytest.mark.parametrize("N", [1, 3, 12, 16, 33])
+def test_a_step_is_a_prompt_of_one_token(N, extra):
+    for where in ("u", "delta", "B", "state", "A"):
+        args, dout, _ = inputs(2, 1, 6, N, 2, N, gate=True, extra=extra, state=True, n_seqs=2)
+        args[where][{"u": (1, 0, 2), "delta": (1, 0, 2), "B": (1, 0, 0, 0), "state": (1, 2, 0), "A": (2, N - 1)}[where]] = -INF if where == "A" else INF
+        got, want, size, pieces = compare(args, dout, None, None)
+        state, a = args["state"].clone(), {n: t if t is None or n in ("A", "D", "delta_bias", "state") else t[:, 0] for n, t in args.items()}
+        one = selective_scan_step_fn(*(a[n] for n in ("u", "delta", "A", "B", "C")), state, a["D"], a["z"], a["delta_bias"])
+        for name, t in (("out", one), ("final", state)):
+            check(name, t, want[name].reshape(t.shape), size[name].reshape(t.shape), args, pieces)
+            check(name, got[name], want[name], size[name], args, pieces)
