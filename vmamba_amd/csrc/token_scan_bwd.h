@@ -145,16 +145,21 @@ __global__ __launch_bounds__(kBlock, 3) void ts_left_kernel(const TsBwdArgs q) {
         if (more) request(t - kTsTile, t);
         __builtin_amdgcn_sched_barrier(0);
         wave_lds_sync();
+        auto walk = [&](auto all) {                                  // all: the tile has its 16 tokens (those it has not are not walked, as in the forward)
 #pragma unroll
-        for (int k = kTsTile - 1; k >= 0; --k) {
-            const float2 pair = *reinterpret_cast<const float2 *>(s_step + k * L::kPairPitch + 2 * l.chan);
+            for (int k = kTsTile - 1; k >= 0; --k) {
+                if (!decltype(all)::value && k >= n) continue;
+                const float2 pair = *reinterpret_cast<const float2 *>(s_step + k * L::kPairPitch + 2 * l.chan);
 #pragma unroll
-            for (int m = 0; m < kM; ++m) {
-                const floatx4_t gr = ts_outer(s_C[k * L::kStates + l.state(m) + l.col], pair.y, ga[m]);
+                for (int m = 0; m < kM; ++m) {
+                    const floatx4_t gr = ts_outer(s_C[k * L::kStates + l.state(m) + l.col], pair.y, ga[m]);
 #pragma unroll
-                for (int v = 0; v < 4; ++v) ga[m][v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]) * gr[v];
+                    for (int v = 0; v < 4; ++v) ga[m][v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]) * gr[v];
+                }
             }
-        }
+        };
+        if (n == kTsTile) walk(std::true_type{});
+        else walk(std::false_type{});
         wave_lds_sync();
         if (!more) break;
         e = t;
@@ -206,13 +211,26 @@ static __global__ __launch_bounds__(kBlock) void ts_join_left_kernel(const TsBwd
     }
 }
 
+// Arguments that a piece needs once, read again each time: held in scalar registers with the others, which are more than there are, they would push those out
+typedef const __attribute__((address_space(4))) TsBwdArgs *TsRare;
+__device__ __forceinline__ TsRare ts_rare_args() {
+    TsRare q = (TsRare)__builtin_amdgcn_kernarg_segment_ptr();       // (the kernel's one argument)
+    asm volatile("" : "+s"(q));
+    return q;
+}
+
+enum TsEnds { kTsWhole, kTsLast, kTsPacked };
+
 struct TsPiece { TsSpan sp; int32_t a, e; };                         // tokens a .. e - 1 of one sequence (or of none), from a kept state or a sequence's start on
 
-// kQuick: whole wavefronts of channels, states that fill their lanes, and offsets inside a tile that fit 32 bits.  kPacked: sequences by their places.
-template <typename T, int kSets, int kM, bool kQuick, bool kPacked>
+// kQuick: whole wavefronts of channels, states that fill their lanes, and offsets inside a tile that fit 32 bits.  kEnds: where pieces may begin and end
+// inside eight tokens that are walked together: nowhere, at the last token, anywhere (packed sequences).  Tokens that a piece has not are not walked: their steps of 0 and their
+// products with 0 would be NaN of an A, a state or a gradient that is infinite.
+template <typename T, int kSets, int kM, bool kQuick, TsEnds kEnds>
 __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 : 2) void ts_grad_kernel(const TsBwdArgs q) {
     using L = TsLane<kSets, kM>;
     const TsArgs &p = q.f;
+    constexpr bool kPacked = kEnds == kTsPacked, kRagged = kEnds != kTsWhole;
     constexpr int kWaves = kTsBwdWaves<kM>, kThreads = kWave * kWaves, kRow = 4 * L::kCh + 4, kQuarter = 4 * kSets;
     constexpr int kKeep = kTsTile * kM, kSlots = kKeep / kTsSub;     // (ts_keep); states in LDS of a piece
     constexpr int kSlot = 4 * kWave * kM;                            // floats of a state in LDS, [m][lane][4]; later the sums of its eight tokens, [m][token][state][B, C]
@@ -254,13 +272,13 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
         ga[m] = dA[m] = floatx4_t{0, 0, 0, 0};
     }
     auto of_seq = [&](const float *states, int seq) { return states ? states + ((int64_t)seq * p.dim + d) * N : nullptr; };
-    if (kPacked && q.dinitial && works)                                 // sequences without tokens, dealt out over the segments
+    if (kPacked && ts_rare_args()->dinitial && works)                                 // sequences without tokens, dealt out over the segments
         for (uint32_t i = seg; i < (uint32_t)p.n_seqs; i += p.n_segs) {
             const int lo = min(max(p.cu[i], 0), p.tokens), hi = min(max(p.cu[i + 1], 0), p.tokens);
             if (hi > lo) continue;
             floatx4_t h[kM];
-            ts_read_state<kSets, kM>(of_seq(q.dfinal, (int)i), N, l, there, h);
-            ts_write_state<kSets, kM>(q.dinitial + ((int64_t)i * p.dim + d) * N, N, l, there, h);
+            ts_read_state<kSets, kM>(of_seq(ts_rare_args()->dfinal, (int)i), N, l, there, h);
+            ts_write_state<kSets, kM>(ts_rare_args()->dinitial + ((int64_t)i * p.dim + d) * N, N, l, there, h);
         }
 
     Raw4<T> ru[L::kRounds], rd[L::kRounds], rz[L::kRounds], ro[L::kRounds], rB[L::kBcRounds], rC[L::kBcRounds];
@@ -271,18 +289,18 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
 #pragma unroll
             for (int r = 0; r < L::kRounds; ++r) {
                 const uint32_t k = row_of(r * L::kRows + l.row);
-                ru[r] = ts_load4_at<T>(u + base * p.u_t, (k * (uint32_t)p.u_t + (uint32_t)at) * (uint32_t)sizeof(T));
-                rd[r] = ts_load4_at<T>(dl + base * p.dl_t, (k * (uint32_t)p.dl_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                ru[r] = ts_load4_at<T>(u + (int64_t)base * (int32_t)p.u_t, (k * (uint32_t)(int32_t)p.u_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                rd[r] = ts_load4_at<T>(dl + (int64_t)base * (int32_t)p.dl_t, (k * (uint32_t)(int32_t)p.dl_t + (uint32_t)at) * (uint32_t)sizeof(T));
                 if (second) {
-                    ro[r] = ts_load4_at<T>(dout + base * q.do_t, (k * (uint32_t)q.do_t + (uint32_t)at) * (uint32_t)sizeof(T));
-                    if (z) rz[r] = ts_load4_at<T>(z + base * p.z_t, (k * (uint32_t)p.z_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                    ro[r] = ts_load4_at<T>(dout + (int64_t)base * (int32_t)q.do_t, (k * (uint32_t)(int32_t)q.do_t + (uint32_t)at) * (uint32_t)sizeof(T));
+                    if (z) rz[r] = ts_load4_at<T>(z + (int64_t)base * (int32_t)p.z_t, (k * (uint32_t)(int32_t)p.z_t + (uint32_t)at) * (uint32_t)sizeof(T));
                 }
             }
 #pragma unroll
             for (int r = 0; r < L::kBcRounds; ++r) {
                 const uint32_t k = row_of(r * L::kBcRows + l.bc_row);
-                rB[r] = ts_load4_at<T>(Bp + base * p.B_t, (k * (uint32_t)p.B_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
-                if (second) rC[r] = ts_load4_at<T>(Cp + base * p.C_t, (k * (uint32_t)p.C_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
+                rB[r] = ts_load4_at<T>(Bp + (int64_t)base * (int32_t)p.B_t, (k * (uint32_t)(int32_t)p.B_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
+                if (second) rC[r] = ts_load4_at<T>(Cp + (int64_t)base * (int32_t)p.C_t, (k * (uint32_t)(int32_t)p.C_t + (uint32_t)bc_at) * (uint32_t)sizeof(T));
             }
             return;
         }
@@ -305,16 +323,16 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
     };
     auto piece_before = [&](int e) {
         TsPiece x;
-        x.sp = kPacked ? ts_span_at(p.cu, p.n_seqs, p.tokens, b, e - 1) : TsSpan{b, 0, p.tokens};
+        x.sp = kPacked ? ts_span_at(ts_rare_args()->f.cu, ts_rare_args()->f.n_seqs, p.tokens, b, e - 1) : TsSpan{b, 0, p.tokens};
         x.a = max(max(x.sp.lo, s0), (e - 1) & ~(kKeep - 1));
         x.e = e;
         return x;
     };
     auto tile_of = [](int t) { return t & ~(kTsTile - 1); };
     auto begin = [&](const TsPiece &x) {                             // the first tile of a piece, and the state before it
-        if (!works || (kPacked && x.sp.seq < 0)) return;
+        if (!works) return;
         request(tile_of(x.a), x.a, x.e, tile_of(x.a) == tile_of(x.e - 1));
-        ts_read_state<kSets, kM>(x.a == x.sp.lo ? of_seq(p.initial, x.sp.seq) : p.kept + (((int64_t)b * p.n_kept + x.a / kKeep) * p.dim + d) * N, N, l, there, next_h);
+        ts_read_state<kSets, kM>(x.a == x.sp.lo ? of_seq(ts_rare_args()->f.initial, x.sp.seq) : ts_rare_args()->f.kept + (((int64_t)b * ts_rare_args()->f.n_kept + x.a / kKeep) * p.dim + d) * N, N, l, there, next_h);
     };
     auto put_bc = [&](float *to, const Raw4<T> &raw, int k, bool in) {
         float v[4];
@@ -346,35 +364,47 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
         }
     };
 
-    TsPiece now = piece_before(s1);
-    begin(now);
-    for (int turn = 0;; turn ^= kTurns - 1) {
+    // the memory of a workgroup's sums over channels from token t on
+    auto sums_at = [&](int t) { return ts_rare_args()->pBC + ((((int64_t)wg * p.batch + b) * p.tokens + t) * p.groups + g) * N * 2; };
+    const int64_t bc_row = (int64_t)p.groups * N * 2;
+    auto nothing = [&](int from, int to) {                           // tokens of no sequence: behind the last one and before the first
+        const float zeros[4] = {0, 0, 0, 0};
+        for (int k = from + l.row; works && k < to; k += L::kRows) {
+            ts_store4<T, true>(du + (int64_t)k * p.dim + at, mine, whole, zeros);
+            ts_store4<T, true>(dd + (int64_t)k * p.dim + at, mine, whole, zeros);
+            if (z) ts_store4<T, true>(dz + (int64_t)k * p.dim + at, mine, whole, zeros);
+        }
+        float *sums = sums_at(from);
+        for (int64_t i = threadIdx.x; i < (int64_t)(to - from) * N * 2; i += kThreads) sums[i / (N * 2) * bc_row + i % (N * 2)] = 0.0f;
+    };
+    int rest = s1;                                                   // tokens that are still to be walked, s0 .. rest - 1
+    if (kPacked) {
+        for (TsSpan sp; rest > s0 && (sp = ts_span_at(ts_rare_args()->f.cu, ts_rare_args()->f.n_seqs, p.tokens, b, rest - 1)).seq < 0;) {
+            nothing(max(sp.lo, s0), rest);
+            rest = max(sp.lo, s0);
+        }
+    }
+    TsPiece now;
+    if (rest > s0) {
+        now = piece_before(rest);
+        begin(now);
+    }
+    for (int turn = 0; rest > s0; turn ^= kTurns - 1) {
         const int a = now.a, e = now.e;
         const TsSpan sp = now.sp;
         ts_keep_together(e - s0, s1 - s0);
-        const bool more = a > s0;
+        rest = a;
         TsPiece next = now;
-        if (more) next = piece_before(a);
-        float *s_slot = s_slot_all[turn][wave];
-        float *pBC = q.pBC + ((((int64_t)wg * p.batch + b) * p.tokens + a) * p.groups + g) * N * 2;
-        const int64_t bc_row = (int64_t)p.groups * N * 2;
-        if (kPacked && sp.seq < 0) {
-            const float zeros[4] = {0, 0, 0, 0};
-            if (works)
-                for (int k = a + l.row; k < e; k += L::kRows) {
-                    ts_store4<T, true>(du + (int64_t)k * p.dim + at, mine, whole, zeros);
-                    ts_store4<T, true>(dd + (int64_t)k * p.dim + at, mine, whole, zeros);
-                    if (z) ts_store4<T, true>(dz + (int64_t)k * p.dim + at, mine, whole, zeros);
-                }
-            for (int i = threadIdx.x; i < (e - a) * N * 2; i += kThreads) pBC[i / (N * 2) * bc_row + i % (N * 2)] = 0.0f;
-            if (!more) break;
-            begin(next);
-            now = next;
-            continue;
+        if (rest > s0) next = piece_before(rest);
+        if (kPacked && next.sp.seq < 0) {
+            nothing(s0, rest);
+            rest = s0;
         }
+        const bool more = rest > s0;
+        float *s_slot = s_slot_all[turn][wave];
         if (works) {
-            if (e == sp.hi) ts_read_state<kSets, kM>(of_seq(q.dfinal, sp.seq), N, l, there, ga);
-            else if (e == s1) ts_read_state<kSets, kM>(q.behind + (((int64_t)b * q.slots + seg * q.each) * p.dim + d) * N, N, l, there, ga);
+            if (e == sp.hi) ts_read_state<kSets, kM>(of_seq(ts_rare_args()->dfinal, sp.seq), N, l, there, ga);
+            else if (e == s1) ts_read_state<kSets, kM>(ts_rare_args()->behind + (((int64_t)b * ts_rare_args()->slots + seg * ts_rare_args()->each) * p.dim + d) * N, N, l, there, ga);
             const int low = tile_of(a), high = tile_of(e - 1);
             floatx4_t h[kM];
 #pragma unroll
@@ -411,7 +441,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
 #pragma unroll
                 for (int k = 0; k < kTsTile; ++k) {
                     if (k % kTsSub == 0) keep(base + k);
-                    forwards(k, h);
+                    if (!kPacked || base + k >= a) forwards(k, h);
                 }
                 wave_lds_sync();
             }
@@ -457,7 +487,8 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                     keep(base);
                     if (base + kTsSub < e) {
 #pragma unroll
-                        for (int k = 0; k < kTsSub; ++k) forwards(k, h);
+                        for (int k = 0; k < kTsSub; ++k)
+                            if (!kPacked || base + k >= a) forwards(k, h);
                         keep(base + kTsSub);
                     }
                 }
@@ -472,12 +503,21 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                     float sq[2 * kTsSub];                            // s of the eight tokens, w . A of the eight
 #pragma unroll
                     for (int i = 0; i < 2 * kTsSub; ++i) sq[i] = 0.0f;
+                    auto there_at = [&](int i) { return base + k0 + i >= a && base + k0 + i < e; };
+                    const bool some = kRagged && !(base + k0 >= a && base + k0 + kTsSub <= e);         // of the eight
+                    // Of more than 16 states a branch to a token: those kernels wait for registers, which it leaves free (6007 packed tokens of 64 states 2605 -> 1741 us).  Of 16 and
+                    // fewer it would cost every tile 8 %: states, decays and dA are found again where some are not there, 2041 tokens 407 -> 423 us, 12 011 packed 554 -> 560.
+                    auto in = [&](int i) { return !kRagged || kM == 1 || there_at(i); };
 #pragma unroll
                     for (int m = 0; m < kM; ++m) {
-                        floatx4_t hs[kTsSub + 1], decay[kTsSub];
+                        floatx4_t hs[kTsSub + 1], decay[kTsSub] = {};
                         hs[0] = *reinterpret_cast<const floatx4_t *>(slot + (m * kWave + l.lane) * 4);
 #pragma unroll
                         for (int i = 0; i < kTsSub; ++i) {
+                            if (!in(i)) {
+                                hs[i + 1] = hs[i];
+                                continue;
+                            }
                             const float *row = s_tok + (k0 + i) * kRow + 4 * l.chan;
                             const float2 pair = *reinterpret_cast<const float2 *>(row);
                             floatx4_t kept;
@@ -487,6 +527,35 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                                 kept[v] = decay[i][v] * hs[i][v];
                             }
                             hs[i + 1] = ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept);
+                        }
+                        floatx4_t dA_some = {0, 0, 0, 0};
+                        if (kM == 1 && some) {                       // states, decays and dA again, of its tokens alone
+#pragma unroll
+                            for (int i = 0; i < kTsSub; ++i) {
+                                if (!there_at(i)) {
+                                    hs[i + 1] = hs[i];
+                                    decay[i] = floatx4_t{1, 1, 1, 1};
+                                    continue;
+                                }
+                                const float2 pair = *reinterpret_cast<const float2 *>(s_tok + (k0 + i) * kRow + 4 * l.chan);
+                                floatx4_t kept;
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) kept[v] = decay[i][v] * hs[i][v];
+                                hs[i + 1] = ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept);
+                            }
+                            floatx4_t g_at = ga[m];
+                            dA_some = dA[m];
+#pragma unroll
+                            for (int i = kTsSub - 1; i >= 0; --i) {
+                                if (!there_at(i)) continue;
+                                const float4 tok = *reinterpret_cast<const float4 *>(s_tok + (k0 + i) * kRow + 4 * l.chan);
+                                const floatx4_t gr = ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, g_at);
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) {
+                                    g_at[v] = decay[i][v] * gr[v];
+                                    dA_some[v] = fmaf(g_at[v] * hs[i][v], tok.x, dA_some[v]);
+                                }
+                            }
                         }
                         if (z) {
 #pragma unroll
@@ -501,6 +570,11 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
 #pragma unroll
                             for (int par = 1; par >= 0; --par) {
                                 const int i = 2 * two + par;
+                                if (!in(i)) {
+#pragma unroll
+                                    for (int v = 0; v < 8; ++v) both[8 * par + v] = 0.0f;
+                                    continue;
+                                }
                                 const float4 tok = *reinterpret_cast<const float4 *>(s_tok + (k0 + i) * kRow + 4 * l.chan);
                                 const floatx4_t gr = ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, ga[m]);
                                 const float4 Bv = *reinterpret_cast<const float4 *>(s_B + (k0 + i) * L::kStates + l.state(m));
@@ -519,6 +593,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                             const int par = l.lane >> 5, is_c = l.lane >> 4 & 1, v = l.lane & 3;
                             slot[m * 4 * kWave + ((2 * two + par) * kQuarter + 4 * l.set + v) * 2 + is_c] = total;
                         }
+                        if (kM == 1 && some) dA[m] = dA_some;
                     }
                     wave_lds_sync();
                     ts_sum_sets<kSets>(sq);
@@ -568,10 +643,11 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                 }
                 wave_lds_sync();
             }
-            if (a == sp.lo && q.dinitial) ts_write_state<kSets, kM>(q.dinitial + ((int64_t)sp.seq * p.dim + d) * N, N, l, there, ga);
+            if (a == sp.lo && ts_rare_args()->dinitial) ts_write_state<kSets, kM>(ts_rare_args()->dinitial + ((int64_t)sp.seq * p.dim + d) * N, N, l, there, ga);
         }
         // ---- the piece's dB and dC over the workgroup's channels ---------------------------------------------------------------------
         __syncthreads();
+        float *pBC = sums_at(a);
         for (int i = threadIdx.x; i < (e - a) * L::kStates * 2; i += kThreads) {
             const int k = i / (2 * L::kStates), n = i % (2 * L::kStates) / 2, c = i & 1, t = a + k;
             const int from = t / kTsSub % kSlots * kSlot + n / kQuarter * 4 * kWave + (t % kTsSub * kQuarter + n % kQuarter) * 2 + c;
@@ -580,12 +656,11 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
             if (n < N) pBC[(int64_t)k * bc_row + 2 * n + c] = total;
         }
         if constexpr (kTurns == 1) __syncthreads();                  // (with two, the next piece's barrier comes before these are written again)
-        if (!more) break;
         now = next;
     }
     if (!works) return;
     const int64_t part = (int64_t)b * p.n_segs + seg;
-    ts_write_state<kSets, kM>(q.pA + (part * p.dim + d) * N, N, l, there, dA);
+    ts_write_state<kSets, kM>(ts_rare_args()->pA + (part * p.dim + d) * N, N, l, there, dA);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -594,8 +669,8 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
             sum_bias[i] += __shfl_xor(sum_bias[i], over, kWave);
         }
         if (l.row == 0 && i < mine) {
-            q.pD[part * 2 * p.dim + c0 + at + i] = sum_D[i];
-            q.pD[(part * 2 + 1) * p.dim + c0 + at + i] = sum_bias[i];
+            ts_rare_args()->pD[part * 2 * p.dim + c0 + at + i] = sum_D[i];
+            ts_rare_args()->pD[(part * 2 + 1) * p.dim + c0 + at + i] = sum_bias[i];
         }
     }
 }
@@ -637,9 +712,10 @@ static __global__ __launch_bounds__(kBlock) void ts_sum_rows_kernel(const float 
 template <typename T> int ts_bwd_run(const ss2d_token_scan_bwd_params *p, const TsBwdArgs &q, hipStream_t st) {
     using std::integral_constant;
     const TsArgs &a = q.f;
-    auto run_as = [&](auto sets, auto m, auto quick, auto packed) {
+    auto run_as = [&](auto sets, auto m, auto quick, auto ends) {
         constexpr int kSets = decltype(sets)::value, kM = decltype(m)::value;
-        constexpr bool kQuick = decltype(quick)::value, kPacked = decltype(packed)::value;
+        constexpr bool kQuick = decltype(quick)::value;
+        constexpr TsEnds kEnds = decltype(ends)::value;
         if (a.n_segs > 1) {
             TsBwdArgs left = q;
             left.f.wgs = q.left_wgs;
@@ -648,13 +724,15 @@ template <typename T> int ts_bwd_run(const ss2d_token_scan_bwd_params *p, const 
             const uint32_t per_row = (uint32_t)a.dim * a.N;
             ts_join_left_kernel<<<dim3((per_row + kBlock - 1) / kBlock, a.batch), kBlock, 0, st>>>(q, per_row);
         }
-        ts_grad_kernel<T, kSets, kM, kQuick, kPacked><<<(uint32_t)(a.batch * a.groups * a.wgs * a.n_segs), kWave * kTsBwdWaves<kM>, 0, st>>>(q);
+        ts_grad_kernel<T, kSets, kM, kQuick, kEnds><<<(uint32_t)(a.batch * a.groups * a.wgs * a.n_segs), kWave * kTsBwdWaves<kM>, 0, st>>>(q);
     };
     auto run = [&](auto sets, auto m) {
-        using std::false_type;
-        using std::true_type;
-        if (ts_quick(a)) a.cu ? run_as(sets, m, true_type{}, true_type{}) : run_as(sets, m, true_type{}, false_type{});
-        else a.cu ? run_as(sets, m, false_type{}, true_type{}) : run_as(sets, m, false_type{}, false_type{});
+        auto by_ends = [&](auto quick) {
+            if (a.cu) run_as(sets, m, quick, integral_constant<TsEnds, kTsPacked>{});
+            else if (a.tokens % kTsSub) run_as(sets, m, quick, integral_constant<TsEnds, kTsLast>{});
+            else run_as(sets, m, quick, integral_constant<TsEnds, kTsWhole>{});
+        };
+        ts_quick(a) ? by_ends(std::true_type{}) : by_ends(std::false_type{});
     };
     if (a.N <= 4) run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
     else if (a.N <= 8) run(integral_constant<int, 2>{}, integral_constant<int, 1>{});
