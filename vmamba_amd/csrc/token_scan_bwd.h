@@ -265,10 +265,18 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
         skip[i] = p.D && i < mine ? p.D[c0 + at + i] : 0.0f;
     }
     floatx4_t A2[kM], ga[kM], dA[kM], next_h[kM];
-    ts_read_state<kSets, kM>(p.A + (int64_t)d * N, N, l, works, A2);
+    ts_read_state<kSets, kM>(p.A + (int64_t)d * N, N, l, works && there, A2);
+    // values of a lane that stand for no state, or for none of the group's channels: 0 behind every matrix instruction, which may make NaN of them
+    auto cleared = [&](floatx4_t v, int m) {
+        if constexpr (!kQuick) ts_clear_others<kSets, kM>(v, m, N, l, there);
+        return v;
+    };
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
         A2[m] *= kLog2e;
+        if (!kQuick)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) A2[m][v] = l.state(m) + v < N ? A2[m][v] : -1.0f;            // (a decay that is a number even of an infinite step)
         ga[m] = dA[m] = floatx4_t{0, 0, 0, 0};
     }
     auto of_seq = [&](const float *states, int seq) { return states ? states + ((int64_t)seq * p.dim + d) * N : nullptr; };
@@ -360,7 +368,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
             floatx4_t kept;
 #pragma unroll
             for (int v = 0; v < 4; ++v) kept[v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]) * h[m][v];
-            h[m] = ts_outer(s_B[k * L::kStates + l.state(m) + l.col], pair.y, kept);
+            h[m] = cleared(ts_outer(s_B[k * L::kStates + l.state(m) + l.col], pair.y, kept), m);
         }
     };
 
@@ -526,7 +534,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                                 decay[i][v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]);
                                 kept[v] = decay[i][v] * hs[i][v];
                             }
-                            hs[i + 1] = ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept);
+                            hs[i + 1] = cleared(ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept), m);
                         }
                         floatx4_t dA_some = {0, 0, 0, 0};
                         if (kM == 1 && some) {                       // states, decays and dA again, of its tokens alone
@@ -541,7 +549,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                                 floatx4_t kept;
 #pragma unroll
                                 for (int v = 0; v < 4; ++v) kept[v] = decay[i][v] * hs[i][v];
-                                hs[i + 1] = ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept);
+                                hs[i + 1] = cleared(ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept), m);
                             }
                             floatx4_t g_at = ga[m];
                             dA_some = dA[m];
@@ -549,7 +557,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                             for (int i = kTsSub - 1; i >= 0; --i) {
                                 if (!there_at(i)) continue;
                                 const float4 tok = *reinterpret_cast<const float4 *>(s_tok + (k0 + i) * kRow + 4 * l.chan);
-                                const floatx4_t gr = ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, g_at);
+                                const floatx4_t gr = cleared(ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, g_at), m);
 #pragma unroll
                                 for (int v = 0; v < 4; ++v) {
                                     g_at[v] = decay[i][v] * gr[v];
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                                     continue;
                                 }
                                 const float4 tok = *reinterpret_cast<const float4 *>(s_tok + (k0 + i) * kRow + 4 * l.chan);
-                                const floatx4_t gr = ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, ga[m]);
+                                const floatx4_t gr = cleared(ts_outer(s_C[(k0 + i) * L::kStates + l.state(m) + l.col], tok.z, ga[m]), m);
                                 const float4 Bv = *reinterpret_cast<const float4 *>(s_B + (k0 + i) * L::kStates + l.state(m));
                                 sq[i] = fmaf(gr[3], Bv.w, fmaf(gr[2], Bv.z, fmaf(gr[1], Bv.y, fmaf(gr[0], Bv.x, sq[i]))));
 #pragma unroll
