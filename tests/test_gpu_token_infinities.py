@@ -133,6 +133,26 @@ def test_one_infinite_value(N, layout, side, where):
             check(name, got[name], want[name], size[name], args, pieces)
 
 
+@pytest.mark.parametrize("side,where", [("results", "state"), ("results", "u"), ("gradients", "dfinal"), ("gradients", "dout")])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("N", [3, 16])
+def test_an_infinite_step_forgets_nothing_infinite(N, layout, side, where):
+    """A decay of 0 of an infinite state, or of an infinite gradient of one, is NaN -- from the infinite step on, though a segment before or behind it hands the state on by its steps' sum."""
+    B, T, n_seqs, seq, t, lengths = LAYOUTS[layout]
+    args, dout, dfinal = inputs(B, T, 16, N, 1, N, gate=True, extra=True, state=True, n_seqs=n_seqs)
+    b = seq if lengths is None else 0
+    args["delta"][b, t, 2] = INF
+    if where in ("state", "dfinal"):
+        (args["state"] if where == "state" else dfinal)[seq, 2, N // 2] = INF
+    else:
+        (args["u"] if where == "u" else dout)[b, t + (-15 if where == "u" else 20), 2] = INF
+    got, want, size, pieces = compare(args, dout, dfinal, lengths)
+    assert any(bool(want[name].isnan().any()) for name in got if name in SIDES[side])
+    for name in got:
+        if name in SIDES[side]:
+            check(name, got[name], want[name], size[name], args, pieces)
+
+
 @pytest.mark.parametrize("side", SIDES)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("N", STATES)

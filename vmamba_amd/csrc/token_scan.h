@@ -225,6 +225,14 @@ __device__ __forceinline__ void ts_keep_together(int left, int of) {
     else __builtin_amdgcn_s_setprio(0);
 }
 
+// What a segment hands on of what comes into it, with its own: by its decays' product, exp2(2 A2_half sum), in two halves, so that neither leaves the range of fp32 before the state
+// would.  An infinite state stays what it is by decays that are numbers, however small their product; a decay of 0 (of an infinite step or A) makes NaN of it.
+__device__ __forceinline__ float ts_handed_on(float carry, float A2_half, float sum, float own) {
+    const float of_two = A2_half * sum, half = __builtin_amdgcn_exp2f(of_two);
+    if (fabsf(carry) == __builtin_inff()) return (fabsf(of_two) < __builtin_inff() ? carry : carry * half) + own;
+    return fmaf(carry * half, half, own);
+}
+
 __device__ __forceinline__ float ts_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
 
 }  // namespace ss2d

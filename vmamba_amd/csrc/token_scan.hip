@@ -272,8 +272,7 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
     }
 }
 
-// What enters every segment but the first: a thread per (row, channel, state).  The product of a segment's decays is taken in two halves, so that neither
-// leaves the range of fp32 before the state would.
+// What enters every segment but the first: a thread per (row, channel, state)
 __global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_t per_row) {
     const uint32_t item = blockIdx.x * kBlock + threadIdx.x;
     const int b = (int)blockIdx.y, segs = p.n_segs - 1;
@@ -299,8 +298,7 @@ __global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_
         for (int i = 0; i < kFly; ++i) {
             if (s0 + i >= segs) break;
             if (flag[i] == kTsThrough && carry != 0.0f) {
-                const float half = __builtin_amdgcn_exp2f(A2 * sum[i]);
-                carry = fabsf(carry) == __builtin_inff() ? carry + left[i] : fmaf(carry * half, half, left[i]);
+                carry = ts_handed_on(carry, A2, sum[i], left[i]);
             } else {
                 carry = flag[i] == kTsNothing ? 0.0f : left[i];      // (of nothing, the segment's memory holds nothing)
             }

@@ -201,8 +201,7 @@ static __global__ __launch_bounds__(kBlock) void ts_join_left_kernel(const TsBwd
         for (int i = 0; i < kFly; ++i) {
             if (s0 - i < 0) break;
             if (flag[i] == kTsThrough && carry != 0.0f) {
-                const float half = __builtin_amdgcn_exp2f(A2 * sum[i]);
-                carry = fabsf(carry) == __builtin_inff() ? carry + own[i] : fmaf(carry * half, half, own[i]);
+                carry = ts_handed_on(carry, A2, sum[i], own[i]);
             } else {
                 carry = flag[i] == kTsNothing ? 0.0f : own[i];
             }
