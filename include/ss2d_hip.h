@@ -801,7 +801,7 @@ int ss2d_token_scan_fwd(const ss2d_token_scan_params *params, void *workspace, i
  * Gradients of ss2d_token_scan_fwd, from the inputs again and the states that the forward kept (fwd.kept_states, read only; fwd.out and fwd.final_state are not looked
  * at): dout (batch, seqlen, dim) dtype by its strides, dfinal_state as final_state or NULL.  du, ddelta, dz (not NULL where z is not), dB, dC: dtype, dense, in
  * the shapes of what they are the gradients of; dA (dim, dstate), dD (dim), ddelta_bias (dim), dinitial_state: fp32, any of them NULL.
- * No atomics: the same bits every time.  Rows of no sequence get zeros.
+ * No atomics: the same bits every time.  Rows of no sequence get zeros.  With dim 0 nothing is written (dB and dC, which are then sums of nothing, are the caller's to clear).
  */
 typedef struct ss2d_token_scan_bwd_params {
     ss2d_token_scan_params fwd;

@@ -147,6 +147,8 @@ struct SelectiveScanTokens : torch::autograd::Function<SelectiveScanTokens> {
             const bool want = wanted(saved[i]), always = i < 2 || i == 3 || i == 4 || i == 6;      // (the kernels write these in any case)
             if (saved[i].defined() && (want || always)) result[i] = fresh_like(saved[i]);
         }
+        if (s.u.size(2) == 0)                                        // (without channels no kernel runs, and B and C may have gradients)
+            for (int i : {3, 4}) result[i].zero_();
         p.dout = dout.data_ptr(); p.dfinal_state = (const float *)ptr_of(dfinal);
         p.dout_batch_stride = dout.stride(0); p.dout_token_stride = dout.stride(1);
         p.du = made(result[0]); p.ddelta = made(result[1]); p.dA = (float *)made(result[2]); p.dB = made(result[3]); p.dC = made(result[4]); p.dD = (float *)made(result[5]);

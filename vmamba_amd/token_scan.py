@@ -181,6 +181,8 @@ class SelectiveScanTokensHip(torch.autograd.Function):
         want = ctx.needs_input_grad
         grads = [torch.empty(t.shape, dtype=t.dtype, device=u.device) if t is not None and (always or want[i]) else None
                  for i, (t, always) in enumerate(((u, True), (delta, True), (A, False), (B, True), (C, True), (D, False), (z, True), (delta_bias, False), (initial_state, False)))]
+        if u.shape[2] == 0:                                          # (without channels no kernel runs, and B and C may have gradients)
+            grads[3].zero_(), grads[4].zero_()
         p.dout, p.dfinal_state = dout.data_ptr(), _ptr(dfinal)
         p.dout_batch_stride, p.dout_token_stride = dout.stride()[:2]
         p.du, p.ddelta, p.dA, p.dB, p.dC, p.dD, p.dz, p.ddelta_bias, p.dinitial_state = (_ptr(t) for t in grads)
