@@ -262,9 +262,10 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
                             gt *= sig * fmaf(y, 1.0f - sig, 1.0f);
                         }
                         if (!kAll) gt = now < sp.hi ? gt : 0.0f;
-                        d[i] = w[0][i] * gt;
+                        d[i] = kAll || now < sp.hi ? w[0][i] * gt : 0.0f;
 #pragma unroll
-                        for (int j = 1; j < kW; ++j) d[i] = fmaf(w[j][i], g[kW - 1 - j][i], d[i]);
+                        for (int j = 1; j < kW; ++j)                 // (tokens that are not there: not even 0 times an infinite tap)
+                            if (kAll || now - j < sp.hi) d[i] = fmaf(w[j][i], g[kW - 1 - j][i], d[i]);
 #pragma unroll
                         for (int j = 0; j < kW - 1; ++j) dw[j][i] = own ? fmaf(gt, window[j][i], dw[j][i]) : dw[j][i];
                         dw[kW - 1][i] = own ? fmaf(gt, in, dw[kW - 1][i]) : dw[kW - 1][i];
@@ -282,6 +283,15 @@ template <typename T, int kW, int kV, bool kNear> __global__ __launch_bounds__(k
                         continue;
                     }
                     if (now >= stop || (to < a && (a != sp.lo || !p.dinitial))) continue;
+                    if (to < a) {                                    // a row of the state: of the first tokens' g alone, which are the newest
+#pragma unroll
+                        for (int i = 0; i < kV; ++i) {
+                            d[i] = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < kW - 1; ++j)
+                                if (now - j >= a && now - j < sp.hi) d[i] = fmaf(w[j][i], g[kW - 2 - j][i], d[i]);
+                        }
+                    }
                     const int last = to - (sp.hi - kW + 1);          // its row of the final state, if it is there
                     if (p.dfinal && last >= 0) {
                         const RowPiece<T, kV> f = load_row_piece<T, kV>((const T *)p.dfinal + sp.seq * state + last * (int64_t)p.dim + c.d);
