@@ -3,7 +3,7 @@
 // With g_t = dout_t act'(..):   dx_t = sum_j w_j g_(t + W - 1 - j),   dw_j = sum over t of g_t x_(t - W + 1 + j),   dbias = sum g.
 //
 // Memory bounds it: 8 x 4096 tokens of 2048 channels in bf16 61 us (4.4 TB/s; a strip of 32 tokens 65, of 128 67), their gradients 90 (4.5 TB/s) and 6 for the sums over strips;
-// from the caches, which hold half of it, 46 and 83.
+// from the caches, which hold half of it, 44 and 80.
 // A thread takes the channels of one 16-byte piece (of few tokens: two channels) and walks a strip of tokens with the window in registers; rows are
 // loaded a chunk at a time, all on their way at once.  Threads side by side have neighbouring pieces, strips below each other.  The last
 // piece of a row ends with it, so that it may repeat channels of the one before: both write the same values.
@@ -550,7 +550,8 @@ extern "C" int ss2d_causal_conv_step(const ss2d_causal_conv_step_params *p, void
             kernel<<<(uint32_t)wgs, kBlock, 0, st>>>(a, (T *)p->state, p->state_batch_stride, (uint32_t)blocks, first);
             return launch_status();
         };
-        // several sequences to a thread read the weights once, where there are threads enough
+        // several sequences to a thread read the weights once, where there are threads enough (4096 channels, four sequences to a thread and one: 256 sequences, and 512, from where
+        // on, 6.7 to 7.1 us either way; 1024 9.6 and 11.3)
         const bool many = (int64_t)a.batch * whole >= (1 << 18);
         int rc = whole == 0 ? SS2D_OK : many ? go(cv_step_kernel<T, kW, kV, kRows>, whole, kRows, 0) : go(cv_step_kernel<T, kW, kV, 1>, whole, 1, 0);
         if (rc == SS2D_OK && rest) rc = go(cv_step_kernel<T, kW, 1, 1>, rest, 1, whole * kV);      // (channels behind the last whole piece)

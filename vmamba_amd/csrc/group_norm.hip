@@ -297,7 +297,7 @@ template <int kV, typename F> __device__ __forceinline__ void gn_by_group(const 
 
 constexpr int kGnRows = 8;           // rows of a chunk
 
-// fn(team of lanes) for every group of the bundle: s_out[group] from entries by rows and channels
+// A slice's statistics: of each group of a bundle (or the part of one) the mean and the squares about it
 template <typename T, int kV> __global__ __launch_bounds__(kBlock) void gn_stats_kernel(const GnArgs p) {
     __shared__ float s_mean[kBlock * kV + 2], s_square[kBlock * kV + 2];
     const GnPlace q = gn_place<kV>(p);
@@ -636,7 +636,8 @@ static bool gn_slices(GnArgs &a, int size) {
     return true;
 }
 
-// Slices of whole chunks of a workgroup's rows, as long as there are `enough` workgroups; false: too many
+// Slices of whole chunks of a workgroup's rows, as long as there are `enough` workgroups; false: too many.  768 for the statistics, 1024 for the gradients' sums, 2048 for values and dx: maps of 56 x 56 x 192
+// in fp16, half as many of each and twice as many: 32 of them 26.1 us, 27.7 and 26.1; 64 44.9, 47.6 and 52.8; with gradients 32 81.3, 79.8 and 81.4; 64 123.6, 121.8 and 137.9.
 static bool gn_cut(GnArgs &a, int64_t enough) {
     const int64_t chunk = (int64_t)(kBlock / a.cols) * kGnRows, others = a.batch * a.bundles, chunks = (a.positions + chunk - 1) / chunk;
     int64_t each = chunks * others / enough;

@@ -47,7 +47,8 @@ inline int ts_sets(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }
 // Whole wavefronts of channels, states that fill their lanes, offsets inside a tile that fit 32 bits: the kernels without masks
 inline bool ts_quick(const TsArgs &a) { return a.near && a.per_group % (kWave / ts_sets(a.N)) == 0 && (a.N == 4 || a.N == 8 || a.N == 16 || a.N == 32 || a.N == 64); }
 // Tokens between the states that the forward keeps for the gradients: 4 bytes per token and channel where the states fill their lanes.  (Of 16 states, every 64th token
-// takes a quarter of the memory and the gradients a second walk over every piece: 310 us of their kernel, 4 x 2048 tokens of 2048 channels, where it was 278.)
+// takes a quarter of the memory and the gradients a second walk over every piece: their kernel, before wavefronts kept together, 310 us where it was 278, 4 x 2048 tokens of 2048
+// channels.)
 inline int ts_keep(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 // The gradients' sums have a thread to a value of B, and one to a value of A, D and the bias: launches count them in 32 bits
@@ -216,8 +217,9 @@ template <int kSets> __device__ __forceinline__ void ts_sum_sets(float (&v)[16])
 }
 
 // Wavefronts of a SIMD that walk as far keep together: the oldest would run ahead and leave the last ones a SIMD that they cannot fill.  The nearer the end,
-// the lower the priority: in the first half, to three quarters, seven eighths, behind.  32768 tokens 480 -> 430 us, 4 x 2048 with their gradients 480 -> 452; bounds nearer the end
-// (15/16, 31/32, 63/64) 467, quarters 447, a turn of four priorities every four tiles 437.
+// the lower the priority: in the first half, to three quarters, seven eighths, behind.  32768 tokens 476 -> 418 us, 4 x 2048 with their gradients 447 -> 415 (when 32768 tokens took 430, bounds nearer the
+// end, 15/16, 31/32 and 63/64, 467, quarters 447, a turn of four priorities every four tiles 437).  Beside other work: a scan of 8192 tokens and kernels of another stream end together as soon as
+// without priorities or sooner (0 to 7 %), the others being served later: products of 2048^3 42 us in place of 37 (27 alone), copies of 256 MB 151 and 146 (100), GELUs of 8 MB 9.9 and 9.2 (6).
 __device__ __forceinline__ void ts_keep_together(int left, int of) {
     if (2 * left > of) __builtin_amdgcn_s_setprio(3);
     else if (4 * left > of) __builtin_amdgcn_s_setprio(2);

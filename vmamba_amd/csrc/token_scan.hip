@@ -5,9 +5,9 @@
 // the lanes of the first kind, which add the skip term, apply the gate and store.  The next tile's loads are on their way meanwhile.  A wavefront meets no
 // other: no workgroup barrier.
 //
-// Vector instructions bound it: 416 for a tile of 4096 values of states, 80 of them exponentials and the like of twice the time, 91 % of a SIMD's cycles.  32768 tokens of 2048
-// channels, 16 states, bf16: 257 us, and 190 for what 31 of 32 segments leave (without the sums, gates and outputs, 284 a tile); one pass over the states of the same
-// length, without segments, would keep an eighth of the SIMDs busy.  Where wavefronts run as they come the last ones end alone: 290 and 215 us (ts_keep_together).
+// Vector instructions bound it: 421 for a tile of 4096 values of states, 80 of them exponentials and the like of twice the time; they are issued in 96 % of the CUs' busy cycles.  32768 tokens of 2048
+// channels, 16 states, bf16: 236 us, and 170 for what 31 of 32 segments leave (without the sums, gates and outputs, 286 a tile, 92 %); one pass over the states of the same
+// length, without segments, would keep an eighth of the SIMDs busy.  Where wavefronts run as they come the last ones end alone: 266 and 198 us, 83 % and 79 % (ts_keep_together).
 #include "token_scan.h"
 
 namespace ss2d {
@@ -209,7 +209,8 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                 ts_write_state<kSets, kM>(p.kept + (((int64_t)b * p.n_kept + t / p.keep) * p.dim + d) * N, N, l, there, h);
         }
         float y[kTsTile];
-        // all: every value of a lane is a state's, and the tile has its 16 tokens (those it has not are not walked: a step of 0 is none to an A of -inf)
+        // all: every value of a lane is a state's, and the tile has its 16 tokens (those it has not are not walked: a step of 0 is none to an A of -inf).  One walk of both kinds, and
+        // the states behind it put right, is no faster (32768 tokens 416 us, this 414) and of 64 states 6.4 ms where this is 0.72.
         auto walk = [&](auto all) {
             constexpr bool kAll = decltype(all)::value;
 #pragma unroll
@@ -309,7 +310,8 @@ __global__ __launch_bounds__(kBlock) void ts_join_kernel(const TsArgs p, uint32_
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 // Segments of the token axis.  A cut sequence is walked twice for what goes into the later segments, so it is cut only where its wavefronts are fewer than one and a half to
-// a SIMD, and then into as many as come to four workgroups on every CU: what is between two whole numbers of them waits for the last.
+// a SIMD, and then into as many as come to four workgroups on every CU: what is between two whole numbers of them waits for the last.  Rows of 4096 tokens of 2048 channels, cut and whole: 8 of them 386 and
+// 619 us, 11 637 and 673, 12 (from which on they are left whole) 639 and 673, 14 705 and 679, 16 710 and 680, 24 782 and 781.
 static void ts_cut(TsArgs &a) {
     const int ch = kWave / ts_sets(a.N);
     a.wgs = (int)(((int64_t)a.per_group + ch * kWavesPerWg - 1) / (ch * kWavesPerWg));

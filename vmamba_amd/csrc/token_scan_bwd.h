@@ -9,9 +9,9 @@
 // what a later one hands to an earlier one is found first, from its own tokens (ts_left_kernel), and joined.  Sums over channels: a wavefront's by lane moves, two tokens'
 // dB and dC of a lane's four states at once, a workgroup's four through LDS, all workgroups' from memory in a fixed order.  No atomics.
 //
-// Vector instructions bound it, 1583 a tile of 4096 values of states: 800 for states, decays and products, 256 for sums over channels, 70 over states; they take 77 % of the
-// cycles of two wavefronts to a SIMD, all that 240 registers leave (three spill: 698 us in place of 480 of the whole case).  4 x 2048 tokens of 2048 channels, 16 states,
-// bf16: 264 us, what later segments hand back 42, joins and sums 21, and the forward with kept states 125.
+// Vector instructions bound it, 1603 a tile of 4096 values of states: 800 for states, decays and products, 256 for sums over channels, 70 over states; they are issued in 81 % of the
+// CUs' busy cycles, of two wavefronts to a SIMD, all that 230 registers leave (three spill: 613 us in place of 414 of the whole case).  4 x 2048 tokens of 2048 channels, 16 states,
+// bf16: 242 us, what later segments hand back 38, joins and sums 25, and the forward with kept states 109.
 #pragma once
 #include "token_scan.h"
 

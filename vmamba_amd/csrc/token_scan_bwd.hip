@@ -20,7 +20,7 @@ static int ts_bwd_read(const ss2d_token_scan_bwd_params *p, TsBwdArgs &q) {
     const int ch = kWave / (a.N <= 4 ? 1 : a.N <= 8 ? 2 : 4) * (a.N <= 32 ? kTsBwdWaves<1> : kTsBwdWaves<4>);
     a.wgs = (a.per_group + ch - 1) / ch;
     // Segments: two workgroups to a CU are what the gradients' registers leave room for, so that their rounds are of 512, and what is handed from one segment to the next
-    // costs a fifth of what goes into it.  (4 x 2048 tokens of 2048 channels, 4 segments 482 us with the forward, 6 502, 8 480; 8 x 784 of 768, 8 states: 169, 7 segments; 13: 173.)
+    // costs a fifth of what goes into it.  (4 x 2048 tokens of 2048 channels, forward and gradients: 4 segments 414 us, 6 474, 7 460, 8 422; 8 x 784 of 768, 8 states: 4 205, 6 179, 7 161, 13 166.)
     const int64_t wgs = (int64_t)a.batch * a.groups * a.wgs, most = (a.tokens + (int64_t)kTsGrid - 1) / kTsGrid;
     int64_t n = 1;
     double least = 0;

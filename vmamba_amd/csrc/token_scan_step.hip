@@ -87,6 +87,7 @@ template <typename T, int kLanes> static int ts_step(const TsStepArgs &a, hipStr
         kernel<<<(uint32_t)n, kBlock, 0, st>>>(a, (uint32_t)blocks);
         return launch_status();
     };
+    // (2048 channels of 16 states, four sequences to a workgroup and one: 64 sequences 7.1 to 7.3 us either way, 96 8.0; 128, from where on, 8.9 and 9.3; 256 14.5 and 16.6)
     return blocks * a.batch >= 4096 ? go(ts_step_kernel<T, kLanes, 4>, 4) : go(ts_step_kernel<T, kLanes, 1>, 1);
 }
 
