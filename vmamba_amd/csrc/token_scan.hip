@@ -209,14 +209,14 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                 ts_write_state<kSets, kM>(p.kept + (((int64_t)b * p.n_kept + t / p.keep) * p.dim + d) * N, N, l, there, h);
         }
         float y[kTsTile];
-        // all: every value of a lane is a state's, and the tile has its 16 tokens (those it has not are not walked: a step of 0 is none to an A of -inf).  One walk of both kinds, and
+        // tokens: the tile has its 16 (those it has not are not walked: a step of 0 is none to an A of -inf); states: every value of a lane is one.  One walk of both kinds of tiles, and
         // the states behind it put right, is no faster (32768 tokens 416 us, this 414) and of 64 states 6.4 ms where this is 0.72.
-        auto walk = [&](auto all) {
-            constexpr bool kAll = decltype(all)::value;
+        auto walk = [&](auto tokens, auto states) {
+            constexpr bool kTokens = decltype(tokens)::value, kStates = decltype(states)::value;
 #pragma unroll
             for (int k = 0; k < kTsTile; ++k) {
                 y[k] = 0.0f;
-                if (!kAll && k >= n) continue;                       // (uniform)
+                if (!kTokens && k >= n) continue;                       // (uniform)
                 const float2 pair = *reinterpret_cast<const float2 *>(s_step + k * L::kPairPitch + 2 * l.chan);
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
@@ -225,15 +225,17 @@ __global__ __launch_bounds__(kBlock, kM == 4 ? 2 : 3) void ts_kernel(const TsArg
                     for (int v = 0; v < 4; ++v) kept[v] = __builtin_amdgcn_exp2f(pair.x * A2[m][v]) * h[m][v];
                     h[m] = ts_outer(s_B[k * L::kStates + l.state(m) + l.col], pair.y, kept);
                     if constexpr (!kLocal) {
-                        if constexpr (!kAll && !kQuick) ts_clear_others<kSets, kM>(h[m], m, N, l, true);
+                        if constexpr (!kStates) ts_clear_others<kSets, kM>(h[m], m, N, l, true);
                         const float4 c = *reinterpret_cast<const float4 *>(s_C + k * L::kStates + l.state(m));
                         y[k] = fmaf(c.w, h[m][3], fmaf(c.z, h[m][2], fmaf(c.y, h[m][1], fmaf(c.x, h[m][0], y[k]))));
                     }
                 }
             }
         };
-        if (n == kTsTile && (kQuick || kLocal || bc_whole)) walk(std::true_type{});
-        else walk(std::false_type{});
+        constexpr std::bool_constant<kQuick || kLocal> quick;
+        if (n != kTsTile) walk(std::false_type{}, quick);
+        else if (quick.value || bc_whole) walk(std::true_type{}, std::true_type{});
+        else walk(std::true_type{}, quick);
         wave_lds_sync();
         if constexpr (!kLocal) {
             ts_sum_sets<kSets>(y);
