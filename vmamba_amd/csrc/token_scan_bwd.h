@@ -510,11 +510,13 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                     float sq[2 * kTsSub];                            // s of the eight tokens, w . A of the eight
 #pragma unroll
                     for (int i = 0; i < 2 * kTsSub; ++i) sq[i] = 0.0f;
+                    constexpr bool kRepairs = kM < 4;
                     auto there_at = [&](int i) { return base + k0 + i >= a && base + k0 + i < e; };
                     const bool some = kRagged && !(base + k0 >= a && base + k0 + kTsSub <= e);         // of the eight
-                    // Of more than 16 states a branch to a token: those kernels wait for registers, which it leaves free (6007 packed tokens of 64 states 2605 -> 1741 us).  Of 16 and
-                    // fewer it would cost every tile 8 %: states, decays and dA are found again where some are not there, 2041 tokens 407 -> 423 us, 12 011 packed 554 -> 560.
-                    auto in = [&](int i) { return !kRagged || kM == 1 || there_at(i); };
+                    // Of more than 32 states a branch to a token: that kernel waits for registers, which it leaves free (6007 packed tokens of 64 states 2605 -> 1741 us).  Of fewer it
+                    // would cost every tile 8 to 14 %: states, decays and dA are found again where some are not there, 4 x 2041 tokens 407 -> 423 us, 12 011 packed 554 -> 560, 2 x 2041
+                    // of 32 states 556 -> 587 (637 by branches).
+                    auto in = [&](int i) { return !kRagged || kRepairs || there_at(i); };
 #pragma unroll
                     for (int m = 0; m < kM; ++m) {
                         floatx4_t hs[kTsSub + 1], decay[kTsSub] = {};
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                             hs[i + 1] = cleared(ts_outer(s_B[(k0 + i) * L::kStates + l.state(m) + l.col], pair.y, kept), m);
                         }
                         floatx4_t dA_some = {0, 0, 0, 0};
-                        if (kM == 1 && some) {                       // states, decays and dA again, of its tokens alone
+                        if (kRepairs && some) {                       // states, decays and dA again, of its tokens alone
 #pragma unroll
                             for (int i = 0; i < kTsSub; ++i) {
                                 if (!there_at(i)) {
@@ -600,7 +602,7 @@ __global__ __launch_bounds__(kWave * kTsBwdWaves<kM>, kM > 1 || kSets == 1 ? 1 :
                             const int par = l.lane >> 5, is_c = l.lane >> 4 & 1, v = l.lane & 3;
                             slot[m * 4 * kWave + ((2 * two + par) * kQuarter + 4 * l.set + v) * 2 + is_c] = total;
                         }
-                        if (kM == 1 && some) dA[m] = dA_some;
+                        if (kRepairs && some) dA[m] = dA_some;
                     }
                     wave_lds_sync();
                     ts_sum_sets<kSets>(sq);
