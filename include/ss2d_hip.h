@@ -779,6 +779,7 @@ int ss2d_qk_norm_rotate_bwd(const ss2d_qk_norm_rotate_bwd_params *params, void *
  *   sequence get zeros.
  *   initial_state, final_state (n_seqs or batch, dim, dstate) fp32, dense, either or both NULL; of a sequence without tokens the final state is the initial one.
  *   kept_states NULL or ss2d_token_scan_kept_states(params) floats: the states before every 16th token (dstate to 16; to 32: every 32nd; more: every 64th), which the gradients start from.
+ *   (SS2D_ENOTSUP in their place where there are no gradients: from 2^32 - 255 values of B, or of A, D and the bias twice, on.)
  *   out (batch, seqlen, dim) dtype, dense.
  * dstate up to 64 (SS2D_ENOTSUP beyond).  States and sums are fp32.  workspace: ..._workspace_bytes(params) bytes (or a negative status), 16-byte aligned.
  */
